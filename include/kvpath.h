@@ -363,6 +363,137 @@ int kvp_sample_bf16(const void* logits, int64_t row_stride, int32_t num_rows, in
                     const float* temperatures, const int32_t* seed, int64_t* out,
                     void* workspace, size_t workspace_bytes, void* stream);
 
+/* ------------------------------------------------------------------------------
+ * The quantised paged cache: rows of head_dim values in e4m3 (OCP, with NaN and no
+ * infinity) with one power-of-two scale for each token and head.
+ *
+ * A quantised cache is k_cache / v_cache of bytes, [num_blocks, block_size, num_kv_heads,
+ * head_dim] with strides as above (in elements, that is bytes, multiples of 16), and
+ * k_scale / v_scale, [num_blocks, num_kv_heads, block_size] bytes with strides
+ * (scale_block_stride, scale_head_stride, 1).  Byte e of a row stands for 2^(e - 127),
+ * 1 <= e <= 254, and value q of the row for 2^(e - 127) q.
+ * ------------------------------------------------------------------------------ */
+
+/*
+ * kvp_append_bf16 into a quantised cache.  The row of token i and head h is divided by the
+ * least power of two (2^-126 at least) that brings its largest finite magnitude to 448 or
+ * below, and rounded to nearest even; infinities are stored as NaN.  key and value in bf16,
+ * 16-byte aligned with strides that are multiples of 8 elements; head_dim 64, 128 or 256, any
+ * block_size.  Slots are kvp_append_bf16's: one outside [0, num_cache_slots) is skipped, -1
+ * among them.
+ */
+int kvp_append_fp8(const void* key, int64_t key_tok_stride, int64_t key_head_stride,
+                   const void* value, int64_t value_tok_stride, int64_t value_head_stride,
+                   void* k_cache, void* v_cache,
+                   int64_t cache_block_stride, int64_t cache_slot_stride, int64_t cache_head_stride,
+                   void* k_scale, void* v_scale, int64_t scale_block_stride, int64_t scale_head_stride,
+                   int64_t num_cache_slots, const int32_t* slot_mapping, int32_t num_tokens,
+                   int32_t num_kv_heads, int32_t head_dim, int32_t block_size, void* stream);
+
+/*
+ * Reads sequences of a quantised cache back, packed and in bf16 (exactly: bf16 holds every
+ * product of an e4m3 value and a scale within its range), as dense k / v for
+ * kvp_varlen_prefill_bf16.  Token j of sequence b (0 <= j < cu_seqlens_k[b + 1] - cu_seqlens_k[b])
+ * goes to row cu_seqlens_k[b] + j of k_out / v_out ([total_k, num_kv_heads, head_dim], 16-byte
+ * aligned, strides multiples of 8 elements).  Rows from total_k or cu_seqlens_k[num_seqs] on are
+ * left as they were; a token whose block id is outside [0, num_cache_blocks), or behind the
+ * table's end, is NaN.
+ */
+int kvp_load_fp8(const void* k_cache, const void* v_cache,
+                 int64_t cache_block_stride, int64_t cache_slot_stride, int64_t cache_head_stride,
+                 const void* k_scale, const void* v_scale,
+                 int64_t scale_block_stride, int64_t scale_head_stride, int32_t num_cache_blocks,
+                 const int32_t* block_tables, int64_t block_table_stride, int32_t max_blocks_per_seq,
+                 const int32_t* cu_seqlens_k, int32_t num_seqs, int32_t total_k,
+                 int32_t num_kv_heads, int32_t head_dim, int32_t block_size,
+                 void* k_out, int64_t k_out_tok_stride, int64_t k_out_head_stride,
+                 void* v_out, int64_t v_out_tok_stride, int64_t v_out_head_stride, void* stream);
+
+/*
+ * Bytes of device workspace that kvp_paged_decode_fp8 (max_seqlen_q 1) and kvp_tree_attention
+ * need for up to max_num_seqs sequences of up to max_seqlen_q query tokens, with block tables
+ * max_blocks_per_seq wide: at most 34 MB where a kv head's rows (max_seqlen_q * num_q_heads /
+ * num_kv_heads) are 16 or fewer, 68 MB beyond (more with over 2048 / 32 rows of a head times kv
+ * heads).  256-byte aligned, no initialisation; calls that share it are ordered on one stream.
+ * It grows with every argument.  Returns 0 for arguments the attention does not support.
+ */
+size_t kvp_tree_workspace_bytes(int32_t max_num_seqs, int32_t max_seqlen_q, int32_t num_q_heads,
+                                int32_t num_kv_heads, int32_t head_dim, int32_t max_blocks_per_seq,
+                                int32_t block_size);
+
+/*
+ * kvp_paged_decode_bf16 over a quantised cache, for any GQA ratio up to 16: q and out in bf16,
+ * everything between in 32 bits but the softmax weights, which enter the second product in bf16.
+ * Scale pointers and strides are multiples of 4 bytes.  Rows with context_lens[b] <= 0 are
+ * zeros, rows with an impossible length or a needed block id outside the pool NaN, as there.
+ * head_dim 128; block_size a multiple of 64; block tables of at most 2^24 tokens; cache slot
+ * strides up to 2^24 bytes.
+ */
+int kvp_paged_decode_fp8(const void* q, int64_t q_seq_stride, int64_t q_head_stride,
+                         const void* k_cache, const void* v_cache,
+                         int64_t cache_block_stride, int64_t cache_slot_stride,
+                         int64_t cache_head_stride,
+                         const void* k_scale, const void* v_scale,
+                         int64_t scale_block_stride, int64_t scale_head_stride, int32_t num_cache_blocks,
+                         const int32_t* block_tables, int64_t block_table_stride,
+                         const int32_t* context_lens, int32_t num_seqs,
+                         int32_t num_q_heads, int32_t num_kv_heads, int32_t head_dim,
+                         int32_t block_size, int32_t max_blocks_per_seq, float softmax_scale,
+                         void* out, int64_t out_seq_stride, int64_t out_head_stride,
+                         void* workspace, size_t workspace_bytes, void* stream);
+
+/*
+ * Attention of drafted tokens over a paged cache that holds them behind their contexts.
+ * Sequence b has the query rows [cu_seqlens_q[b], cu_seqlens_q[b + 1]) of q, n_b of them, and a
+ * cache of cache_seqlens[b] tokens, whose last n_b are these tokens (appended before the call).
+ * Query i of b (0-based) sees all cache_seqlens[b] - n_b tokens before them, and draft j where
+ * bit j of tree_mask[cu_seqlens_q[b] + i] is set; bits from n_b on are ignored, and a token does
+ * not see itself unless its own bit says so.  tree_mask NULL: draft j for j <= i (a chain).  A row
+ * that sees nothing is zero; what a masked token holds (infinities, NaN) does not reach it.
+ *   1 <= max_seqlen_q <= 64.  A sequence with more query tokens than max_seqlen_q, with
+ * cache_seqlens[b] below n_b or beyond the table, or with a needed block id outside
+ * [0, num_cache_blocks) gives NaN rows; cache_seqlens[b] <= 0 gives zeros (padding rows of a
+ * captured graph); a sequence whose rows are not within [0, total_q) is skipped.  Rows that no
+ * sequence has are left as they were.
+ *   k_scale and v_scale NULL: caches in bf16, strides in elements, multiples of 8; otherwise a
+ * quantised cache.  GQA ratio up to 16; the other limits are kvp_paged_decode_fp8's (slot strides
+ * up to 2^24 bytes).
+ */
+int kvp_tree_attention(const void* q, int64_t q_tok_stride, int64_t q_head_stride,
+                       const void* k_cache, const void* v_cache,
+                       int64_t cache_block_stride, int64_t cache_slot_stride,
+                       int64_t cache_head_stride,
+                       const void* k_scale, const void* v_scale,
+                       int64_t scale_block_stride, int64_t scale_head_stride, int32_t num_cache_blocks,
+                       const int32_t* block_tables, int64_t block_table_stride,
+                       const int32_t* cu_seqlens_q, const int32_t* cache_seqlens, int32_t num_seqs,
+                       int32_t total_q, int32_t max_seqlen_q, const int64_t* tree_mask,
+                       int32_t num_q_heads, int32_t num_kv_heads, int32_t head_dim,
+                       int32_t block_size, int32_t max_blocks_per_seq, float softmax_scale,
+                       void* out, int64_t out_tok_stride, int64_t out_head_stride,
+                       void* workspace, size_t workspace_bytes, void* stream);
+
+/*
+ * For each row r of [num_rows, vocab] logits, with p = softmax(logits[r]):
+ *   logprobs[r] = ln p[tokens[r]]
+ *   rank[r]     = 1 + the number of logits above that token's
+ *   entropy[r]  = - sum p ln p, in nats
+ *   top_tokens[r, 0 .. top), top_logprobs[r, ...]: the most probable tokens, largest first, the
+ *                 lower index first among equal logits, NaN before all others
+ * logits in bf16 (logits_fp32 0) or fp32 (1), 16-byte aligned, row_stride (elements) a multiple
+ * of 16 bytes; sums in fp32.  0 <= top <= min(64, vocab).  A row with a NaN or +inf, or of -inf
+ * alone, has NaN log probabilities and entropy.  A token outside [0, vocab) has a NaN log
+ * probability and rank 0.  The workspace (16-byte aligned, no initialisation;
+ * kvp_token_logprobs_workspace_bytes, 0 from 512 rows on, 0.5 MB at most) holds the parts of rows
+ * that several workgroups share.
+ */
+size_t kvp_token_logprobs_workspace_bytes(int32_t num_rows);
+int kvp_token_logprobs(const void* logits, int32_t logits_fp32, int64_t row_stride, int32_t num_rows,
+                       int32_t vocab, const int64_t* tokens, int32_t top,
+                       float* logprobs, float* entropy, int64_t* rank,
+                       float* top_logprobs, int64_t* top_tokens,
+                       void* workspace, size_t workspace_bytes, void* stream);
+
 #ifdef __cplusplus
 }
 #endif

@@ -18,7 +18,8 @@ REPO_DIR = PKG_DIR.parent
 CSRC_DIR = PKG_DIR / "csrc"
 INCLUDE_DIR = REPO_DIR / "include"
 LIB_PATH = PKG_DIR / "libkvpath.so"
-SOURCES = ["capi.hip", "kv_append.hip", "paged_decode.hip", "varlen_prefill.hip", "norm_rope.hip"]
+SOURCES = ["capi.hip", "kv_append.hip", "paged_decode.hip", "varlen_prefill.hip", "norm_rope.hip",
+           "kv_quant.hip", "tree_attention.hip", "token_logprobs.hip"]
 ARCH = "gfx950"
 
 HIPCC_FLAGS = [

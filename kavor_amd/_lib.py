@@ -134,6 +134,61 @@ SIGNATURES: dict[str, tuple] = {
         _c_void_p,                        # out (int64)
         _c_void_p, _size_t, _c_void_p,    # workspace, workspace_bytes, stream
     ]),
+    "kvp_append_fp8": (ctypes.c_int, [
+        _c_void_p, _i64, _i64,            # key, key_tok_stride, key_head_stride
+        _c_void_p, _i64, _i64,            # value, value_tok_stride, value_head_stride
+        _c_void_p, _c_void_p,             # k_cache, v_cache
+        _i64, _i64, _i64,                 # cache block/slot/head strides
+        _c_void_p, _c_void_p, _i64, _i64,  # k_scale, v_scale, scale block/head strides
+        _i64, _c_void_p, _i32,            # num_cache_slots, slot_mapping, num_tokens
+        _i32, _i32, _i32,                 # num_kv_heads, head_dim, block_size
+        _c_void_p,                        # stream
+    ]),
+    "kvp_load_fp8": (ctypes.c_int, [
+        _c_void_p, _c_void_p,             # k_cache, v_cache
+        _i64, _i64, _i64,                 # cache block/slot/head strides
+        _c_void_p, _c_void_p, _i64, _i64,  # k_scale, v_scale, scale block/head strides
+        _i32, _c_void_p, _i64, _i32,      # num_cache_blocks, block_tables, block_table_stride, max_blocks_per_seq
+        _c_void_p, _i32, _i32,            # cu_seqlens_k, num_seqs, total_k
+        _i32, _i32, _i32,                 # num_kv_heads, head_dim, block_size
+        _c_void_p, _i64, _i64,            # k_out, k_out_tok_stride, k_out_head_stride
+        _c_void_p, _i64, _i64,            # v_out, v_out_tok_stride, v_out_head_stride
+        _c_void_p,                        # stream
+    ]),
+    "kvp_tree_workspace_bytes": (_size_t, [_i32, _i32, _i32, _i32, _i32, _i32, _i32]),
+    "kvp_paged_decode_fp8": (ctypes.c_int, [
+        _c_void_p, _i64, _i64,            # q, q_seq_stride, q_head_stride
+        _c_void_p, _c_void_p,             # k_cache, v_cache
+        _i64, _i64, _i64,                 # cache block/slot/head strides
+        _c_void_p, _c_void_p, _i64, _i64,  # k_scale, v_scale, scale block/head strides
+        _i32, _c_void_p, _i64,            # num_cache_blocks, block_tables, block_table_stride
+        _c_void_p, _i32,                  # context_lens, num_seqs
+        _i32, _i32, _i32,                 # num_q_heads, num_kv_heads, head_dim
+        _i32, _i32, _f32,                 # block_size, max_blocks_per_seq, softmax_scale
+        _c_void_p, _i64, _i64,            # out, out_seq_stride, out_head_stride
+        _c_void_p, _size_t, _c_void_p,    # workspace, workspace_bytes, stream
+    ]),
+    "kvp_tree_attention": (ctypes.c_int, [
+        _c_void_p, _i64, _i64,            # q, q_tok_stride, q_head_stride
+        _c_void_p, _c_void_p,             # k_cache, v_cache
+        _i64, _i64, _i64,                 # cache block/slot/head strides
+        _c_void_p, _c_void_p, _i64, _i64,  # k_scale, v_scale, scale block/head strides
+        _i32, _c_void_p, _i64,            # num_cache_blocks, block_tables, block_table_stride
+        _c_void_p, _c_void_p, _i32,       # cu_seqlens_q, cache_seqlens, num_seqs
+        _i32, _i32, _c_void_p,            # total_q, max_seqlen_q, tree_mask
+        _i32, _i32, _i32,                 # num_q_heads, num_kv_heads, head_dim
+        _i32, _i32, _f32,                 # block_size, max_blocks_per_seq, softmax_scale
+        _c_void_p, _i64, _i64,            # out, out_tok_stride, out_head_stride
+        _c_void_p, _size_t, _c_void_p,    # workspace, workspace_bytes, stream
+    ]),
+    "kvp_token_logprobs_workspace_bytes": (_size_t, [_i32]),
+    "kvp_token_logprobs": (ctypes.c_int, [
+        _c_void_p, _i32, _i64, _i32, _i32,  # logits, logits_fp32, row_stride, num_rows, vocab
+        _c_void_p, _i32,                  # tokens (int64), top
+        _c_void_p, _c_void_p, _c_void_p,  # logprobs, entropy (fp32), rank (int64)
+        _c_void_p, _c_void_p,             # top_logprobs (fp32), top_tokens (int64)
+        _c_void_p, _size_t, _c_void_p,    # workspace, workspace_bytes, stream
+    ]),
 }
 
 _lock = threading.Lock()

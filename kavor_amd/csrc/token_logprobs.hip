@@ -1,0 +1,454 @@
+// Log probabilities of given tokens, the entropy of their distributions, and the most probable
+// alternatives (kvp_token_logprobs), in one pass over the logits.
+//
+// With c = log2(e) and a reference R near the row's maximum,
+//   s = sum_i 2^(c x_i - R),   w = sum_i 2^(c x_i - R) (c x_i - R)
+// give   log p_t = ln 2 (c x_t - R - log2 s)   and   H = ln 2 (log2 s - w / s).  c x_i - R is one
+// fma; R need not be the maximum (nor a multiple of c), so a wave takes the largest of its first
+// values and changes R only where a value lies 16 binary orders above it.
+//
+// What bounds it: HBM, with the vector ALUs close behind: a bf16 value has to be widened, entered
+// into a maximum, exponentiated (at a quarter of the rate), summed twice and compared (rank).
+//
+// Alternatives, without a comparison more per value: a thread keeps the largest of its own values,
+// which the sums need anyway, and the first chunk that has it.  Values are ordered by (value,
+// index), so the k best of the row lie with the k threads whose own bests are the best: only
+// those threads' chunks are read again, k of 512.
+//
+// A NaN or an infinity among the logits makes what depends on the sum NaN, as log_softmax does;
+// -inf is probability 0.  Beyond 1e38, where c x overflows and neighbouring values are 2^100
+// apart, only values equal to the maximum count.
+#include <math.h>
+
+#include <algorithm>
+#include <type_traits>
+
+#include "common.h"
+
+namespace kvp {
+namespace {
+
+typedef unsigned long long Key;  // (ordered value, ~index): larger is better; 0: none
+
+constexpr int kThreads = 512;
+constexpr int kWaves = kThreads / 64;
+constexpr int kMaxTop = 64;     // one sorted list of alternatives per wave
+constexpr int kMaxSegments = 32;
+constexpr int kBatch = 4;       // chunks in flight per thread
+constexpr int kList = kWaves * 64;
+constexpr float kLog2e = 1.4426950408889634f, kLn2 = 0.6931471805599453f;
+constexpr float kHuge = 1e38f;
+constexpr float kReach = 16.f;  // how far above R a value may lie
+
+struct LogprobParams {
+  const void* logits;
+  int64_t row_stride;  // elements
+  int32_t vocab, top, segments;
+  const int64_t* tokens;
+  float* logprobs;
+  float* entropy;
+  int64_t* rank;
+  float* top_logprobs;  // [rows][top]
+  int64_t* top_tokens;
+  float4* states;  // split rows: [row][segment] (max, s, w, values above the token's)
+  Key* lists;      // [row][segment][kMaxTop]
+};
+
+template <typename T>
+struct Chunk;  // 16 bytes of logits
+template <>
+struct Chunk<uint16_t> {
+  static constexpr int kSize = 8;
+  static __device__ __forceinline__ float one(uint16_t x) { return __uint_as_float(static_cast<u32>(x) << 16); }
+  static __device__ __forceinline__ void widen(uint4 w, float (&f)[8]) { unpack8(w, f); }
+};
+template <>
+struct Chunk<float> {
+  static constexpr int kSize = 4;
+  static __device__ __forceinline__ float one(float x) { return x; }
+  static __device__ __forceinline__ void widen(uint4 w, float (&f)[4]) {
+    f[0] = __uint_as_float(w.x);
+    f[1] = __uint_as_float(w.y);
+    f[2] = __uint_as_float(w.z);
+    f[3] = __uint_as_float(w.w);
+  }
+};
+
+// Monotone map of the values to unsigned numbers; NaN counts as largest, -0 equals 0.
+__device__ __forceinline__ u32 ordered(float x) {
+  if (x != x) return 0xffffffffu;
+  const u32 b = __float_as_uint(x + 0.f);
+  return b & 0x80000000u ? ~b : b | 0x80000000u;
+}
+__device__ __forceinline__ float value_of(Key k) {
+  const u32 o = static_cast<u32>(k >> 32);
+  return o == 0xffffffffu ? __builtin_nanf("") : __uint_as_float(o & 0x80000000u ? o & 0x7fffffffu : ~o);
+}
+__device__ __forceinline__ Key key_of(float x, u32 index) {
+  return static_cast<Key>(ordered(x)) << 32 | (0xffffffffu - index);
+}
+__device__ __forceinline__ u32 index_of(Key k) { return 0xffffffffu - static_cast<u32>(k); }
+
+__device__ __forceinline__ float wave_max(float x) {
+  x = fmaxf(x, dpp_f32<kDppQuadXor1>(x));
+  x = fmaxf(x, dpp_f32<kDppQuadXor2>(x));
+  x = fmaxf(x, dpp_f32<kDppRowHalfMirror>(x));
+  x = fmaxf(x, dpp_f32<kDppRowMirror>(x));
+  return xor32_max(xor16_max(x));
+}
+__device__ __forceinline__ float wave_sum(float x) { return xor32_sum(xor16_sum(row16_sum(x))); }
+
+// Lists of 64 keys, one per lane, largest first.
+__device__ __forceinline__ Key exchange(Key k, int stride, bool keep_max) {
+  const Key o = __shfl_xor(k, stride);
+  return (k > o) == keep_max ? k : o;
+}
+__device__ __forceinline__ Key sort64(Key k) {
+  const int lane = threadIdx.x & 63;
+#pragma unroll
+  for (int size = 2; size <= 64; size *= 2)
+#pragma unroll
+    for (int stride = size / 2; stride > 0; stride /= 2)
+      k = exchange(k, stride, ((lane & size) == 0) == ((lane & stride) == 0));
+  return k;
+}
+// The 64 largest of a list and another one given in reverse order.
+__device__ __forceinline__ Key merge64(Key k, Key reversed) {
+  const int lane = threadIdx.x & 63;
+  k = k > reversed ? k : reversed;
+#pragma unroll
+  for (int stride = 32; stride > 0; stride /= 2) k = exchange(k, stride, (lane & stride) == 0);
+  return k;
+}
+// Wave 0 gets the 64 largest keys of the first `lists` waves' lists.  Every wave calls it.
+__device__ __forceinline__ Key merge_waves(Key k, Key* s_keys, int lists) {
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+  for (int step = 1; step < lists; step *= 2) {
+    __syncthreads();
+    s_keys[threadIdx.x] = k;
+    __syncthreads();
+    if (wave % (2 * step) == 0 && wave + step < lists) k = merge64(k, s_keys[64 * (wave + step) + 63 - lane]);
+  }
+  return k;
+}
+
+// One row's share of the sums; m is the exact maximum.
+struct State {
+  float m, s, w;
+  int above;  // values above the token's
+};
+// R of a maximum.  The product is rounded here: fused into a subtraction, a reference would differ
+// from itself by that rounding.
+__device__ __forceinline__ float reference(float m) {
+#pragma clang fp contract(off)
+  return fminf(fmaxf(m, -kHuge), kHuge) * kLog2e;
+}
+__device__ __forceinline__ void rebase(float& s, float& w, float from, float to) {
+  const float d = from - to, a = fast_exp2(d);
+  w = a * (a == 0.f ? s : fmaf(s, d, w));  // s d may overflow; a NaN stays one
+  s = a * s;
+}
+// The sum of two states, each taken at its own reference(m).
+__device__ __forceinline__ State join(State a, State b) {
+  State r{fmaxf(a.m, b.m), 0.f, 0.f, a.above + b.above};
+  if (fabsf(r.m) > kHuge) {
+    r.s = (a.m == r.m || a.s != a.s ? a.s : 0.f) + (b.m == r.m || b.s != b.s ? b.s : 0.f);
+  } else {
+    const float to = reference(r.m);
+    rebase(a.s, a.w, reference(a.m), to);
+    rebase(b.s, b.w, reference(b.m), to);
+    r.s = a.s + b.s;
+    r.w = a.w + b.w;
+  }
+  return r;
+}
+// ln p of a value, given the row's state; no more than 0.
+__device__ __forceinline__ float log_prob(float x, const State& st) {
+  float lp;
+  if (fabsf(st.m) > kHuge || fabsf(x) > kHuge) lp = st.m - st.m != 0.f ? __builtin_nanf("") : x - st.m - logf(st.s);
+  else lp = kLn2 * (fmaf(x, kLog2e, -reference(st.m)) - log2f(st.s));
+  return lp > 0.f ? 0.f : lp;
+}
+__device__ __forceinline__ float entropy_of(const State& st) {
+  if (fabsf(st.m) > kHuge) return st.m - st.m != 0.f ? __builtin_nanf("") : logf(st.s);
+  return fmaxf(kLn2 * (log2f(st.s) - st.w / st.s), st.s != st.s ? st.s : 0.f);
+}
+template <typename T>
+__device__ __forceinline__ void finish_row(const LogprobParams& p, int r, const State& st, int64_t token, float x) {
+  const bool ok = token >= 0 && token < p.vocab;
+  p.logprobs[r] = ok ? log_prob(x, st) : __builtin_nanf("");
+  p.entropy[r] = entropy_of(st);
+  p.rank[r] = ok ? st.above + 1 : 0;
+}
+__device__ __forceinline__ void write_top(const LogprobParams& p, int r, const State& st, Key k) {
+  const int lane = threadIdx.x & 63;
+  if (lane >= p.top) return;
+  const int64_t at = static_cast<int64_t>(r) * p.top + lane;
+  p.top_logprobs[at] = log_prob(value_of(k), st);
+  p.top_tokens[at] = index_of(k);
+}
+
+// A segment of a row per workgroup: chunks [cbeg, cend), the row's last one maybe not full.
+template <typename T>
+__global__ __launch_bounds__(kThreads) void logprobs_kernel(const LogprobParams p) {
+  constexpr int E = Chunk<T>::kSize;
+  __shared__ Key s_keys[kList];
+  __shared__ State s_state[kWaves];
+  __shared__ int s_count;
+  const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
+  const int r = static_cast<int>(blockIdx.x) / p.segments, seg = static_cast<int>(blockIdx.x) - r * p.segments;
+  const T* row = static_cast<const T*>(p.logits) + r * p.row_stride;
+  const int chunks = (p.vocab + E - 1) / E, full = p.vocab / E;
+  const int per = (chunks + p.segments - 1) / p.segments;
+  const int cbeg = min(seg * per, chunks), cend = min(cbeg + per, chunks);
+  const int64_t token = p.tokens[r];
+  const float mine = token >= 0 && token < p.vocab ? Chunk<T>::one(row[token]) : __builtin_nanf("");
+
+  // The chunk's values; those behind the row's end are -inf.
+  auto values = [&](int c, uint4 w, float (&f)[E]) {
+    if (c < full) {
+      Chunk<T>::widen(w, f);
+    } else {
+#pragma unroll
+      for (int e = 0; e < E; ++e) f[e] = E * c + e < p.vocab ? Chunk<T>::one(row[E * c + e]) : -INFINITY;
+    }
+  };
+  auto load = [&](int c) {  // a whole chunk of the row, whatever c
+    return full > 0 ? *reinterpret_cast<const uint4*>(row + E * static_cast<int64_t>(min(c, full - 1)))
+                    : make_uint4(0, 0, 0, 0);
+  };
+
+  float m = -INFINITY, s = 0.f, w = 0.f, R = 0.f;
+  int best = cbeg + tid, above = 0;
+  bool first = true;
+  for (int c0 = cbeg + (wave << 6); c0 < cend; c0 += kThreads * kBatch) {  // uniform
+    uint4 in[kBatch];
+#pragma unroll
+    for (int u = 0; u < kBatch; ++u) in[u] = load(c0 + u * kThreads + lane);
+#pragma unroll
+    for (int u = 0; u < kBatch; ++u) {
+      const int cw = c0 + u * kThreads, c = cw + lane;
+      if (cw >= cend) break;  // uniform
+      float f[E];
+      if (cw + 64 <= min(full, cend)) {  // uniform: every lane has a whole chunk
+        Chunk<T>::widen(in[u], f);
+      } else if (c < cend) {
+        values(c, in[u], f);
+      } else {
+#pragma unroll
+        for (int e = 0; e < E; ++e) f[e] = -INFINITY;
+      }
+      float top = f[0];
+#pragma unroll
+      for (int e = 1; e < E; ++e) top = fmaxf(top, f[e]);
+      if (first || __any(fmaf(top, kLog2e, -R) > kReach)) {  // uniform
+        const float to = reference(wave_max(top));
+        if (!first) rebase(s, w, R, to);
+        R = to;
+        first = false;
+      }
+      best = top > m ? c : best;
+      m = fmaxf(m, top);
+#pragma unroll
+      for (int e = 0; e < E; ++e) {
+        const float t = fmaf(f[e], kLog2e, -R), x = fast_exp2(t);
+        s += x;
+        // 2^t is 0 long before t is -inf
+        w = fmaf(x, fmaxf(t, -1024.f), w);
+        above += __popcll(__ballot(f[e] > mine));
+      }
+    }
+  }
+
+  // ---- the workgroup's state
+  const bool odd = s != s;  // the thread may have seen a NaN
+  State st{wave_max(m), 0.f, 0.f, above};
+  float ws = wave_sum(s), ww = wave_sum(w);
+  if (fabsf(st.m) <= kHuge) rebase(ws, ww, R, reference(st.m));
+  st.s = ws;
+  st.w = ww;
+  if (lane == 0) s_state[wave] = st;
+  if (tid == 0) s_count = 0;
+  __syncthreads();
+  st = s_state[0];
+#pragma unroll
+  for (int i = 1; i < kWaves; ++i) st = join(st, s_state[i]);
+  if (fabsf(st.m) > kHuge && st.m - st.m == 0.f) {  // uniform: values equal to the maximum
+    float equal = 0.f;
+    for (int c = cbeg + tid; c < cend; c += kThreads) {
+      float f[E];
+      values(c, load(c), f);
+#pragma unroll
+      for (int e = 0; e < E; ++e) equal += f[e] != f[e] ? f[e] : (f[e] == st.m ? 1.f : 0.f);
+    }
+    equal = wave_sum(equal);
+    __syncthreads();
+    if (lane == 0) s_state[wave].s = equal;
+    __syncthreads();
+    st.s = st.w = 0.f;
+#pragma unroll
+    for (int i = 0; i < kWaves; ++i) st.s += s_state[i].s;
+  }
+
+  // ---- alternatives: the threads with the best bests, then the best of their values
+  Key list = 0;
+  if (p.top > 0) {
+    if (odd) {  // NaN counts as largest: look again
+      m = -INFINITY;
+      best = cbeg + tid;
+      u32 most = 0;
+      for (int c = cbeg + tid; c < cend; c += kThreads) {
+        float f[E];
+        values(c, load(c), f);
+#pragma unroll
+        for (int e = 0; e < E; ++e)
+          if (ordered(f[e]) > most) {
+            most = ordered(f[e]);
+            m = f[e];
+            best = c;
+          }
+      }
+    }
+    list = sort64(cbeg + tid < cend ? key_of(m, best) : 0);
+    list = merge_waves(list, s_keys, kWaves);
+    __syncthreads();
+    if (wave == 0) s_keys[lane] = list;
+    __syncthreads();
+    const int threads = min(p.top, min(kThreads, cend - cbeg));  // that hold chunks
+    const Key last = threads > 0 ? s_keys[threads - 1] : 0;
+    const u32 least = threads < p.top ? 0 : static_cast<u32>(last >> 32);  // fewer threads: all of their values
+    const int rounds = (cend - cbeg + kThreads - 1) / kThreads, items = threads * rounds;
+    const Key lanes = s_keys[lane];  // the winners, one per lane
+    __syncthreads();
+    // item i: chunk i / threads of winner i % threads
+    auto chunk_of = [&](int i) {
+      const int j = i / threads;
+      const int winner = static_cast<int>(index_of(__shfl(lanes, i - j * threads)));
+      return cbeg + (winner - cbeg) % kThreads + j * kThreads;
+    };
+    for (int i0 = wave << 6; i0 < items; i0 += kThreads) {  // uniform
+      const int i = i0 + lane, c = chunk_of(min(i, items - 1));
+      if (i < items && c < cend) {
+        float f[E];
+        values(c, load(c), f);
+#pragma unroll
+        for (int e = 0; e < E; ++e)
+          if (ordered(f[e]) >= least && E * c + e < p.vocab) {
+            const int at = atomicAdd(&s_count, 1);
+            if (at < kList) s_keys[at] = key_of(f[e], E * c + e);
+          }
+      }
+    }
+    __syncthreads();
+    const int count = s_count;
+    if (count <= kList) {
+      list = sort64(tid < count ? s_keys[tid] : 0);
+      list = merge_waves(list, s_keys, (count + 63) / 64);
+    } else {  // many equal values: every wave keeps the best of what it sees
+      list = 0;
+      for (int i0 = wave << 6; i0 < items; i0 += kThreads) {
+        const int i = i0 + lane, c = chunk_of(min(i, items - 1));
+        float f[E];
+        values(min(c, cend - 1), load(c), f);
+#pragma unroll 1
+        for (int e = 0; e < E; ++e) {
+          float x = f[0];
+#pragma unroll
+          for (int j = 1; j < E; ++j) x = e == j ? f[j] : x;
+          const bool in = i < items && c < cend && E * c + e < p.vocab;
+          const Key k = sort64(in ? key_of(x, E * c + e) : 0);
+          list = merge64(list, __shfl(k, 63 - lane));
+        }
+      }
+      list = merge_waves(list, s_keys, kWaves);
+    }
+  }
+
+  // ---- out, or to the merge
+  if (p.segments == 1) {
+    if (tid == 0) finish_row<T>(p, r, st, token, mine);
+    if (wave == 0) write_top(p, r, st, list);
+  } else {
+    if (tid == 0) p.states[blockIdx.x] = make_float4(st.m, st.s, st.w, __int_as_float(st.above));
+    if (wave == 0 && p.top > 0) p.lists[static_cast<int64_t>(blockIdx.x) * kMaxTop + lane] = list;
+  }
+}
+
+// A split row's segments, one row per workgroup.
+template <typename T>
+__global__ __launch_bounds__(kThreads) void logprobs_merge_kernel(const LogprobParams p) {
+  __shared__ Key s_keys[kList];
+  const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
+  const int r = static_cast<int>(blockIdx.x);
+  State st{-INFINITY, 0.f, 0.f, 0};
+  for (int i = 0; i < p.segments; ++i) {
+    const float4 x = p.states[static_cast<int64_t>(r) * p.segments + i];
+    st = join(st, State{x.x, x.y, x.z, __float_as_int(x.w)});
+  }
+  if (tid == 0) {
+    const int64_t token = p.tokens[r];
+    const T* row = static_cast<const T*>(p.logits) + r * p.row_stride;
+    finish_row<T>(p, r, st, token, token >= 0 && token < p.vocab ? Chunk<T>::one(row[token]) : 0.f);
+  }
+  if (p.top == 0) return;  // uniform
+  const Key* lists = p.lists + static_cast<int64_t>(r) * p.segments * kMaxTop;
+  Key list = wave < p.segments ? lists[wave * kMaxTop + lane] : 0;
+  for (int i = wave + kWaves; i < p.segments; i += kWaves) list = merge64(list, lists[i * kMaxTop + 63 - lane]);
+  list = merge_waves(list, s_keys, min(kWaves, p.segments));
+  if (wave == 0) write_top(p, r, st, list);
+}
+
+// Segments of a row: enough workgroups to fill the GPU where rows are few.
+int segments_of(int32_t rows) { return rows >= 512 ? 1 : std::min(kMaxSegments, 1024 / std::max(rows, 1)); }
+
+template <typename T>
+int launch(const char* fn, LogprobParams p, int rows, hipStream_t s) {
+  hipLaunchKernelGGL(logprobs_kernel<T>, dim3(static_cast<unsigned>(rows) * p.segments), dim3(kThreads), 0, s, p);
+  if (p.segments > 1)
+    hipLaunchKernelGGL(logprobs_merge_kernel<T>, dim3(static_cast<unsigned>(rows)), dim3(kThreads), 0, s, p);
+  return launch_status(fn);
+}
+
+}  // namespace
+}  // namespace kvp
+
+using namespace kvp;
+
+extern "C" size_t kvp_token_logprobs_workspace_bytes(int32_t num_rows) {
+  if (num_rows <= 0) return 0;
+  const int s = segments_of(num_rows);
+  return s == 1 ? 0 : static_cast<size_t>(num_rows) * s * (sizeof(float4) + kMaxTop * sizeof(Key));
+}
+
+extern "C" int kvp_token_logprobs(const void* logits, int32_t logits_fp32, int64_t row_stride, int32_t num_rows,
+                                  int32_t vocab, const int64_t* tokens, int32_t top, float* logprobs, float* entropy,
+                                  int64_t* rank, float* top_logprobs, int64_t* top_tokens, void* workspace,
+                                  size_t workspace_bytes, void* stream) {
+  static const char fn[] = "kvp_token_logprobs";
+  clear_error();
+  if (num_rows < 0 || vocab < 1) return fail(KVP_EINVAL, "%s: num_rows=%d vocab=%d", fn, num_rows, vocab);
+  if (top < 0 || top > kMaxTop || top > vocab)
+    return fail(KVP_EUNSUPPORTED, "%s: top=%d (supported: 0 to %d, and no more than vocab)", fn, top, kMaxTop);
+  if (num_rows == 0) return KVP_OK;
+  if (!logits || !tokens || !logprobs || !entropy || !rank || (top > 0 && (!top_logprobs || !top_tokens)))
+    return fail(KVP_EINVAL, "%s: null pointer", fn);
+  auto off = [](const void* ptr, unsigned by) { return (reinterpret_cast<uintptr_t>(ptr) & (by - 1)) != 0; };
+  if (!aligned16(logits) || row_stride % (logits_fp32 ? 4 : 8) || row_stride < vocab)
+    return fail(KVP_EINVAL, "%s: logits must be 16-byte aligned with a row stride >= vocab that is a multiple of "
+                "16 bytes", fn);
+  if (off(tokens, 8) || off(logprobs, 4) || off(entropy, 4) || off(rank, 8) || off(top_logprobs, 4) ||
+      off(top_tokens, 8))
+    return fail(KVP_EINVAL, "%s: misaligned tokens or outputs", fn);
+  if (num_rows > INT32_MAX / kMaxSegments) return fail(KVP_EINVAL, "%s: too many rows", fn);
+  const int segments = segments_of(num_rows);
+  const size_t need = kvp_token_logprobs_workspace_bytes(num_rows);
+  if (segments > 1 && (!workspace || workspace_bytes < need))
+    return fail(KVP_EWORKSPACE, "%s: workspace of %zu bytes, %zu needed", fn, workspace_bytes, need);
+  if (!aligned16(workspace)) return fail(KVP_EINVAL, "%s: workspace must be 16-byte aligned", fn);
+  char* ws = static_cast<char*>(workspace);
+  LogprobParams p{logits, row_stride, vocab, top, segments, tokens, logprobs, entropy, rank, top_logprobs, top_tokens,
+                  reinterpret_cast<float4*>(ws),
+                  reinterpret_cast<Key*>(ws + static_cast<size_t>(num_rows) * segments * sizeof(float4))};
+  const auto s = static_cast<hipStream_t>(stream);
+  return logits_fp32 ? launch<float>(fn, p, num_rows, s) : launch<uint16_t>(fn, p, num_rows, s);
+}

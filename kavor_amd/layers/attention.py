@@ -7,7 +7,13 @@ Mirrors kavor/layers/attention/flash_attention_kvcache.py:
 and replaces the two flash-attn calls it makes with
   paged_decode(...)    for flash_attn_with_kvcache(...)           (:80-83)
   varlen_prefill(...)  for flash_attn_varlen_func(...)            (:76-79)
-which keep flash-attn's argument names and meaning.  Every function here only
+which keep flash-attn's argument names and meaning.  Without a counterpart there, and in the
+same manner:
+  store_kvcache_fp8, load_kvcache_fp8   a quantised cache (e4m3, one power-of-two scale for
+                                        each token and head) written, and read back in bf16
+  paged_decode_fp8                      paged_decode over it
+  tree_attention                        drafted tokens over a cache of either kind
+Every function here only
 validates layouts and forwards raw pointers and strides to the C ABI (include/kvpath.h)
 on the current stream; nothing computes on the host and there is no fallback.
 """
@@ -28,6 +34,8 @@ __all__ = [
     "reserve_decode_workspace", "decode_workspace_bytes",
     "reserve_prefill_workspace", "prefill_workspace_bytes",
     "flash_attn_with_kvcache", "flash_attn_varlen_func",
+    "store_kvcache_fp8", "load_kvcache_fp8", "paged_decode_fp8", "tree_attention",
+    "reserve_tree_workspace", "tree_workspace_bytes",
 ]
 
 
@@ -417,6 +425,234 @@ def varlen_prefill(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, max_seqlen
 # flash-attn spellings, so call sites written against flash_attn keep working.
 flash_attn_with_kvcache = paged_decode
 flash_attn_varlen_func = varlen_prefill
+
+
+# ----------------------------------------------------------------------------- quantised cache
+
+def _launch(fn: str, index: int, *args) -> None:
+    """Calls a library function whose tensors are on device `index`, with that device current."""
+    if torch._C._cuda_getDevice() == index:
+        rc = getattr(lib(), fn)(*args)
+    else:
+        with torch.cuda.device(index):
+            rc = getattr(lib(), fn)(*args)
+    check(fn, rc)
+
+
+def _require(name: str, t: torch.Tensor, dtype: torch.dtype, device: torch.device, dim: int) -> None:
+    """A tensor of `dim` dimensions on `device` whose last one is contiguous."""
+    if t.dtype != dtype or t.device != device or t.dim() != dim:
+        raise ValueError(f"{name} must be a {dim}-d {dtype} tensor on {device}, got {t.dim()}-d {t.dtype} on {t.device}")
+    if t.stride(-1) != 1 and t.shape[-1] > 1:
+        raise ValueError(f"{name} must be contiguous in its last dimension")
+
+
+def _quantised(k_cache, v_cache, k_scale, v_scale, device: torch.device):
+    """The shape of a quantised cache, and its pointers and strides as the library takes them."""
+    for name, t in (("k_cache", k_cache), ("v_cache", v_cache)):
+        _require(name, t, torch.float8_e4m3fn, device, 4)
+    for name, t in (("k_scale", k_scale), ("v_scale", v_scale)):
+        _require(name, t, torch.uint8, device, 3)
+    shape, cs, ss = k_cache.shape, k_cache.stride(), k_scale.stride()
+    if shape != v_cache.shape or cs != v_cache.stride():
+        raise ValueError("k_cache and v_cache must share shape and strides")
+    if k_scale.shape != v_scale.shape or ss != v_scale.stride():
+        raise ValueError("k_scale and v_scale must share shape and strides")
+    num_blocks, block_size, heads, _ = shape
+    if k_scale.shape != (num_blocks, heads, block_size):
+        raise ValueError(f"the scales must be [num_blocks, num_kv_heads, block_size] = "
+                         f"{(num_blocks, heads, block_size)}, got {tuple(k_scale.shape)}")
+    return shape, (k_cache.data_ptr(), v_cache.data_ptr(), cs[0], cs[1], cs[2],
+                   k_scale.data_ptr(), v_scale.data_ptr(), ss[0], ss[1])
+
+
+def _table(block_table: torch.Tensor, rows: int, device: torch.device):
+    if block_table.dtype != torch.int32 or block_table.dim() != 2 or block_table.device != device \
+            or (block_table.stride(1) != 1 and block_table.shape[1] > 1):
+        raise ValueError(f"block_table must be an int32 [B, max_blocks] tensor on {device} with contiguous rows")
+    if block_table.shape[0] < rows:
+        raise ValueError("block_table has fewer rows than sequences")
+    width = block_table.shape[1]
+    # a single row may have any stride
+    return block_table.data_ptr(), max(block_table.stride(0), width), width
+
+
+def store_kvcache_fp8(key: torch.Tensor, value: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor,
+                      k_scale: torch.Tensor, v_scale: torch.Tensor, slot_mapping: torch.Tensor) -> None:
+    """store_kvcache into a quantised cache: key[i] / value[i] ([N, num_kv_heads, head_dim] bf16) go to
+    slot slot_mapping[i], each head's row divided by the least power of two that brings it within
+    e4m3's range and rounded to nearest even.
+
+    The caches are [num_blocks, block_size, num_kv_heads, head_dim] in float8_e4m3fn, the scales
+    [num_blocks, num_kv_heads, block_size] in uint8; byte e stands for 2^(e - 127), and value q of
+    its row for 2^(e - 127) q.  Slots outside the cache, -1 among them, are skipped.  An infinity
+    is stored as NaN."""
+    dev = key.device
+    _require_cuda_bf16("key", key)
+    _require("value", value, torch.bfloat16, dev, 3)
+    _require("key", key, torch.bfloat16, dev, 3)
+    if value.shape != key.shape:
+        raise ValueError("key and value must share their shape")
+    (num_blocks, block_size, heads, dim), cache = _quantised(k_cache, v_cache, k_scale, v_scale, dev)
+    N = key.shape[0]
+    if key.shape[1:] != (heads, dim):
+        raise ValueError(f"key and value must be [N, {heads}, {dim}] as the caches, got {tuple(key.shape)}")
+    _require_int32("slot_mapping", slot_mapping, dev)
+    if slot_mapping.numel() != N:
+        raise ValueError("slot_mapping must have one entry per token")
+    _launch("kvp_append_fp8", key.get_device(),
+            key.data_ptr(), key.stride(0), key.stride(1), value.data_ptr(), value.stride(0), value.stride(1),
+            *cache, num_blocks * block_size, slot_mapping.data_ptr(), N, heads, dim, block_size, _stream(key))
+
+
+def load_kvcache_fp8(k_cache: torch.Tensor, v_cache: torch.Tensor, k_scale: torch.Tensor, v_scale: torch.Tensor,
+                     block_table: torch.Tensor, cu_seqlens_k: torch.Tensor, total_k: int,
+                     out: tuple[torch.Tensor, torch.Tensor] | None = None) -> tuple[torch.Tensor, torch.Tensor]:
+    """Reads the sequences of a quantised cache (see store_kvcache_fp8) back as packed bf16 k and v
+    [total_k, num_kv_heads, head_dim], which varlen_prefill takes as dense k / v: token j of
+    sequence b is row cu_seqlens_k[b] + j.  total_k is the host's copy of cu_seqlens_k[-1]; rows
+    of `out` that no sequence has are left as they were.  Tokens of invalid blocks are NaN."""
+    dev = k_cache.device
+    if not k_cache.is_cuda:
+        raise ValueError(f"k_cache must be a CUDA (HIP) tensor, got device {dev}")
+    (num_blocks, block_size, heads, dim), cache = _quantised(k_cache, v_cache, k_scale, v_scale, dev)
+    _require_int32("cu_seqlens_k", cu_seqlens_k, dev)
+    num_seqs, total_k = cu_seqlens_k.numel() - 1, int(total_k)
+    if num_seqs < 0 or total_k < 0:
+        raise ValueError("cu_seqlens_k must have an entry more than sequences, and total_k not be negative")
+    bt, bt_stride, width = _table(block_table, num_seqs, dev)
+    if out is None:
+        out = tuple(torch.empty(total_k, heads, dim, dtype=torch.bfloat16, device=dev) for _ in range(2))
+    k, v = out
+    for name, t in (("out[0]", k), ("out[1]", v)):
+        _require(name, t, torch.bfloat16, dev, 3)
+        if t.shape[0] < total_k or t.shape[1:] != (heads, dim):
+            raise ValueError(f"{name} must be [{total_k} or more, {heads}, {dim}], got {tuple(t.shape)}")
+    _launch("kvp_load_fp8", k_cache.get_device(),
+            *cache, num_blocks, bt, bt_stride, width, cu_seqlens_k.data_ptr(), num_seqs, total_k, heads, dim,
+            block_size, k.data_ptr(), k.stride(0), k.stride(1), v.data_ptr(), v.stride(0), v.stride(1),
+            _stream(k_cache))
+    return k, v
+
+
+# ----------------------------------------------------------------------------- drafted tokens
+
+_tree_pool = Workspaces("tree attention", "reserve_tree_workspace")
+
+
+@lru_cache(maxsize=1024)
+def tree_workspace_bytes(max_num_seqs: int, max_seqlen_q: int, num_q_heads: int, num_kv_heads: int, head_dim: int,
+                         max_blocks_per_seq: int, block_size: int) -> int:
+    return int(lib().kvp_tree_workspace_bytes(max_num_seqs, max_seqlen_q, num_q_heads, num_kv_heads, head_dim,
+                                              max_blocks_per_seq, block_size))
+
+
+def reserve_tree_workspace(max_num_seqs: int, max_seqlen_q: int, num_q_heads: int, num_kv_heads: int, head_dim: int,
+                           max_blocks_per_seq: int, block_size: int,
+                           device: torch.device | str | int) -> torch.Tensor:
+    """Allocates (or grows) the current stream's workspace of tree_attention and, with max_seqlen_q 1,
+    paged_decode_fp8.  Call before graph capture with the largest sizes that a captured graph will
+    use: the capture takes the buffer over.  Eager calls need no reservation."""
+    return _tree_pool.get(device, tree_workspace_bytes(max_num_seqs, max_seqlen_q, num_q_heads, num_kv_heads,
+                                                       head_dim, max_blocks_per_seq, block_size))
+
+
+def _tree_workspace(index, stream, *sizes) -> torch.Tensor:
+    ws = _tree_pool.ready(index, stream, tree_workspace_bytes(*sizes))
+    return ws if ws is not None else reserve_tree_workspace(*sizes, index)
+
+
+def _paged_shape(q, k_cache, v_cache, k_scale, v_scale):
+    """Sizes of q [N, Hq, D] over a cache of either kind, and the cache's pointers and strides."""
+    _require_cuda_bf16("q", q)
+    dev = q.device
+    if k_scale is None:
+        for name, t in (("k_cache", k_cache), ("v_cache", v_cache)):
+            _require(name, t, torch.bfloat16, dev, 4)
+        cs = k_cache.stride()
+        if k_cache.shape != v_cache.shape or cs != v_cache.stride():
+            raise ValueError("k_cache and v_cache must share shape and strides")
+        shape, cache = k_cache.shape, (k_cache.data_ptr(), v_cache.data_ptr(), cs[0], cs[1], cs[2], 0, 0, 0, 0)
+    else:
+        shape, cache = _quantised(k_cache, v_cache, k_scale, v_scale, dev)
+    if q.shape[2] != shape[3] or q.stride(2) != 1:
+        raise ValueError("head_dim mismatch or non-contiguous head_dim")
+    return shape, cache
+
+
+def _like(q: torch.Tensor, out: torch.Tensor | None) -> torch.Tensor:
+    """A bf16 output of q's shape, given or new."""
+    if out is None:
+        return torch.empty(q.shape, dtype=torch.bfloat16, device=q.device)
+    if out.shape != q.shape or out.dtype != torch.bfloat16 or out.device != q.device or out.stride(2) != 1:
+        raise ValueError("out must be a bf16 tensor of q's shape on its device with contiguous head_dim")
+    return out
+
+
+def paged_decode_fp8(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor, k_scale: torch.Tensor,
+                     v_scale: torch.Tensor, cache_seqlens: torch.Tensor, block_table: torch.Tensor,
+                     softmax_scale: float, out: torch.Tensor | None = None) -> torch.Tensor:
+    """paged_decode over a quantised cache (see store_kvcache_fp8): q [B, Hq, D] (or [B, 1, Hq, D]) in
+    bf16, one query token per sequence, at any GQA ratio up to 16."""
+    if q.dim() == 4 and q.shape[1] == 1:
+        if out is not None and out.dim() != 4:
+            raise ValueError("out must have q's shape")
+        return paged_decode_fp8(q[:, 0], k_cache, v_cache, k_scale, v_scale, cache_seqlens, block_table,
+                                softmax_scale, None if out is None else out[:, 0]).unsqueeze(1)
+    if q.dim() != 3:
+        raise ValueError(f"paged_decode_fp8 takes one query token per sequence, got q of shape {tuple(q.shape)}")
+    (num_blocks, block_size, Hkv, D), cache = _paged_shape(q, k_cache, v_cache, k_scale, v_scale)
+    B, Hq, _ = q.shape
+    _require_int32("cache_seqlens", cache_seqlens, q.device)
+    if cache_seqlens.numel() < B:
+        raise ValueError("cache_seqlens has fewer rows than q")
+    bt, bt_stride, width = _table(block_table, B, q.device)
+    out, index, stream = _like(q, out), q.get_device(), _stream(q)
+    ws = _tree_workspace(index, stream, B, 1, Hq, Hkv, D, width, block_size)
+    _launch("kvp_paged_decode_fp8", index, q.data_ptr(), q.stride(0), q.stride(1), *cache, num_blocks, bt, bt_stride,
+            cache_seqlens.data_ptr(), B, Hq, Hkv, D, block_size, width, float(softmax_scale), out.data_ptr(),
+            out.stride(0), out.stride(1), ws.data_ptr(), ws.numel(), stream)
+    return out
+
+
+def tree_attention(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor, cu_seqlens_q: torch.Tensor,
+                   max_seqlen_q: int, cache_seqlens: torch.Tensor, block_table: torch.Tensor, softmax_scale: float,
+                   tree_mask: torch.Tensor | None = None, k_scale: torch.Tensor | None = None,
+                   v_scale: torch.Tensor | None = None, out: torch.Tensor | None = None) -> torch.Tensor:
+    """Attention of drafted tokens over a paged cache that holds them behind their contexts.
+
+    q is [T, Hq, D] bf16; sequence b has rows cu_seqlens_q[b] .. cu_seqlens_q[b + 1] - 1 of it, at most
+    max_seqlen_q <= 64, and cache_seqlens[b] cached tokens, these drafts (appended before) being
+    the last.  A row sees every token before its sequence's drafts, and draft j where bit j of
+    its int64 tree_mask entry is set; without a tree_mask the drafts are a chain (draft j for
+    j <= its own).  Rows that see nothing are zeros, and what a masked token holds reaches no row.
+    The caches are bf16 as paged_decode's or, with k_scale and v_scale, quantised as
+    paged_decode_fp8's; any GQA ratio up to 16.  Rows of q that no sequence has are left as they
+    were in `out`."""
+    if q.dim() != 3:
+        raise ValueError(f"q must be [T, num_q_heads, head_dim], got shape {tuple(q.shape)}")
+    if (k_scale is None) != (v_scale is None):
+        raise ValueError("k_scale and v_scale go together")
+    (num_blocks, block_size, Hkv, D), cache = _paged_shape(q, k_cache, v_cache, k_scale, v_scale)
+    T, Hq, _ = q.shape
+    _require_int32("cu_seqlens_q", cu_seqlens_q, q.device)
+    _require_int32("cache_seqlens", cache_seqlens, q.device)
+    B, max_seqlen_q = cu_seqlens_q.numel() - 1, int(max_seqlen_q)
+    if B < 0 or cache_seqlens.numel() < B:
+        raise ValueError("cu_seqlens_q must have an entry more than sequences, and cache_seqlens one for each")
+    if tree_mask is not None and (tree_mask.dtype != torch.int64 or tree_mask.device != q.device
+                                  or not tree_mask.is_contiguous() or tree_mask.numel() != T):
+        raise ValueError("tree_mask must be a contiguous int64 tensor on q's device with one entry per row of q")
+    bt, bt_stride, width = _table(block_table, B, q.device)
+    out, index, stream = _like(q, out), q.get_device(), _stream(q)
+    if B == 0 or T == 0:
+        return out
+    ws = _tree_workspace(index, stream, B, max_seqlen_q, Hq, Hkv, D, width, block_size)
+    _launch("kvp_tree_attention", index, q.data_ptr(), q.stride(0), q.stride(1), *cache, num_blocks, bt, bt_stride,
+            cu_seqlens_q.data_ptr(), cache_seqlens.data_ptr(), B, T, max_seqlen_q,
+            tree_mask.data_ptr() if tree_mask is not None else 0, Hq, Hkv, D, block_size, width,
+            float(softmax_scale), out.data_ptr(), out.stride(0), out.stride(1), ws.data_ptr(), ws.numel(), stream)
+    return out
 
 
 # ----------------------------------------------------------------------------- module

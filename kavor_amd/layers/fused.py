@@ -6,6 +6,8 @@ These replace the engine-side Triton kernels around the paged KV path:
   qk_norm_rope              q_norm + k_norm + rotary_emb of qwen3.py:85-88 (no append)
   silu_and_mul              kavor/layers/activation.py:6-11
   greedy_argmax             the temperature-0 path of kavor/layers/sampler.py:7-66
+and, without a counterpart there,
+  token_logprobs            log probability and rank of given tokens, entropy, alternatives
 Each function only validates layouts and forwards pointers and strides to the C ABI on
 the current stream; there is no host computation and no fallback.
 """
@@ -18,7 +20,7 @@ from kavor_amd._lib import check, lib
 from kavor_amd.layers.workspace import Workspaces
 
 __all__ = ["rms_norm", "add_rms_norm", "qk_norm_rope_append", "qk_norm_rope", "silu_and_mul",
-           "greedy_argmax"]
+           "greedy_argmax", "sample", "token_logprobs"]
 
 
 def _stream(t: torch.Tensor) -> int:
@@ -244,3 +246,55 @@ def sample(logits: torch.Tensor, temperatures: torch.Tensor, seed: torch.Tensor,
                                seed.data_ptr(), out.data_ptr(), ws.data_ptr(), ws.numel(), stream)
     check("kvp_sample_bf16", rc)
     return out
+
+
+_logprobs_pool = Workspaces("token_logprobs", "reserve_logprobs_workspace")
+_LOGPROBS_WORKSPACE_BYTES = 1 << 20  # more than any batch needs: longer ones do not split their rows
+
+
+def reserve_logprobs_workspace(device: torch.device | str | int) -> torch.Tensor:
+    """Allocates the current stream's workspace of token_logprobs.  Call before graph capture: the
+    capture takes the buffer over.  Eager calls need no reservation."""
+    return _logprobs_pool.get(device, _LOGPROBS_WORKSPACE_BYTES)
+
+
+def token_logprobs(logits: torch.Tensor, tokens: torch.Tensor, top: int = 0):
+    """Log probabilities under softmax(logits) of one token per row, in one pass over the logits.
+
+    logits is [N, vocab] in bf16 or fp32 with a row stride that is a multiple of 16 bytes, tokens
+    int64 [N].  Returns (logprobs fp32 [N], entropy fp32 [N] in nats, rank int64 [N], top_logprobs
+    fp32 [N, top], top_tokens int64 [N, top]): rank is 1 + the number of logits above the token's,
+    and the alternatives are the `top` (at most 64) most probable tokens, the lower index first
+    among equal ones, NaN before all others.  Log probabilities and entropy of a row with a NaN or
+    +inf, or of -inf alone, are NaN; a token outside the vocabulary has a NaN log probability and
+    rank 0."""
+    if not logits.is_cuda or logits.dtype not in (torch.bfloat16, torch.float32) or logits.dim() != 2:
+        raise ValueError(f"logits must be a bf16 or fp32 [N, vocab] GPU tensor (got {logits.dtype} of shape "
+                         f"{tuple(logits.shape)} on {logits.device})")
+    n, vocab = logits.shape
+    if logits.stride(1) != 1 and vocab > 1:
+        raise ValueError("logits must have a contiguous last dimension")
+    if tokens.dtype != torch.int64 or tokens.device != logits.device or not tokens.is_contiguous() \
+            or tokens.numel() != n:
+        raise ValueError("tokens must be a contiguous int64 tensor on the logits' device, one per row")
+    top = int(top)
+    if top < 0:
+        raise ValueError(f"top must not be negative, got {top}")
+    dev, index, stream = logits.device, logits.get_device(), _stream(logits)
+    logprobs, entropy = torch.empty((2, n), dtype=torch.float32, device=dev)
+    rank = torch.empty(n, dtype=torch.int64, device=dev)
+    top_logprobs = torch.empty((n, top), dtype=torch.float32, device=dev)
+    top_tokens = torch.empty((n, top), dtype=torch.int64, device=dev)
+    ws = _logprobs_pool.ready(index, stream, _LOGPROBS_WORKSPACE_BYTES)
+    if ws is None:
+        ws = reserve_logprobs_workspace(index)
+    args = (logits.data_ptr(), logits.dtype == torch.float32, logits.stride(0) if n > 1 else -(-vocab // 8) * 8, n,
+            vocab, tokens.data_ptr(), top, logprobs.data_ptr(), entropy.data_ptr(), rank.data_ptr(),
+            top_logprobs.data_ptr(), top_tokens.data_ptr(), ws.data_ptr(), ws.numel(), stream)
+    if torch._C._cuda_getDevice() == index:
+        rc = lib().kvp_token_logprobs(*args)
+    else:
+        with torch.cuda.device(index):
+            rc = lib().kvp_token_logprobs(*args)
+    check("kvp_token_logprobs", rc)
+    return logprobs, entropy, rank, top_logprobs, top_tokens
