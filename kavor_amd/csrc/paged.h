@@ -1,5 +1,5 @@
-// What the kernels over paged K/V share: metadata reads, the 16-row matrix product, and the
-// reads of bf16 tiles in LDS.
+// What the kernels over paged K/V share: metadata reads, the matrix products, and the reads of
+// bf16 tiles in LDS.
 #pragma once
 
 #include "common.h"
@@ -32,13 +32,40 @@ __device__ __forceinline__ int load_uniform(const int32_t* base, int64_t idx) {
   return ((const __attribute__((address_space(4))) int32_t*)(base))[idx];
 }
 
-typedef __bf16 mfma_bf16x8_t __attribute__((ext_vector_type(8)));
+typedef __bf16 bf16x8_t __attribute__((ext_vector_type(8)));
 typedef float mfma_f32x4_t __attribute__((ext_vector_type(4)));
+typedef float f32x16_t __attribute__((ext_vector_type(16)));
 
 __device__ __forceinline__ mfma_f32x4_t mfma16(u32x4_t a, u32x4_t b, mfma_f32x4_t c) {
-  return __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(mfma_bf16x8_t, a),
-                                                 __builtin_bit_cast(mfma_bf16x8_t, b), c, 0, 0, 0);
+  return __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8_t, a),
+                                                 __builtin_bit_cast(bf16x8_t, b), c, 0, 0, 0);
 }
+typedef short s16x4_t __attribute__((ext_vector_type(4)));
+
+// ds_read_b64_tr_b16: 8 bytes per lane, transposed as 16-bit elements across each
+// 16-lane group (see the V^T operand in the kernel).
+__device__ __forceinline__ uint2 lds_read_tr16(const uint16_t* lds_ptr) {
+  const s16x4_t v = __builtin_amdgcn_ds_read_tr16_b64_v4i16(
+      (__attribute__((address_space(3))) s16x4_t*)(lds_ptr));
+  return __builtin_bit_cast(uint2, v);
+}
+
+// Max / sum of x over lanes l and l ^ 32 (v_permlane32_swap_b32 exchanges the wave halves:
+// the first result holds lanes 0-31 in both halves, the second lanes 32-63).
+__device__ __forceinline__ float half_swap_max(float x) {
+  const auto r = __builtin_amdgcn_permlane32_swap(__float_as_uint(x), __float_as_uint(x), false, false);
+  return fmaxf(__uint_as_float(r[0]), __uint_as_float(r[1]));
+}
+__device__ __forceinline__ float half_swap_sum(float x) {
+  const auto r = __builtin_amdgcn_permlane32_swap(__float_as_uint(x), __float_as_uint(x), false, false);
+  return __uint_as_float(r[0]) + __uint_as_float(r[1]);
+}
+
+__device__ __forceinline__ f32x16_t mfma32(uint4 a, uint4 b, f32x16_t c) {
+  return __builtin_amdgcn_mfma_f32_32x32x16_bf16(__builtin_bit_cast(bf16x8_t, a),
+                                                 __builtin_bit_cast(bf16x8_t, b), c, 0, 0, 0);
+}
+
 // All LDS accesses of the wave are done: what they read may be overwritten.
 __device__ __forceinline__ void wait_lds() { asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory"); }
 

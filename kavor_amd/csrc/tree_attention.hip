@@ -13,23 +13,23 @@
 // every K/V byte is read once for all of them: rows flops to a byte of bf16 cache, twice that
 // quantised.
 //
-// Work decomposition: work is counted in steps, 8 KiB of K and as much of V (32 tokens of bf16, 64
-// quantised), laid end to end over the sequences.  The rows of a kv head are cut into groups of
-// 16 NT; a stream is one such group of one head.  A wave takes one stream over one contiguous
-// range of the steps, all ranges equally long, and meets no barrier behind the prefix sums.
-// Streams of one range are neighbouring waves.  A sequence that lies in one range gets its output
-// from there; of the others every range leaves (max, sum, unnormalised sum of V) in 32 bits, which
+// Work decomposition: the tokens of all sequences are laid end to end in steps of 64 (32 for few rows
+// on a bf16 cache) and cut into equally long ranges, whatever the lengths.  With up to 16 rows per
+// kv head a wave takes one head over one range (tree_few_kernel); with more, a workgroup does, whose
+// four waves share the tiles and take 16 rows each, or 32, and of more than 128 rows blocks of 128
+// run side by side (tree_many_kernel).  A sequence that lies in one range gets its output from
+// there; of the others every range leaves (max, sum, unnormalised sum of V) in 32 bits, which
 // tree_merge_kernel joins.  Only the first and the last sequence of a range can be cut by it, so a
-// range has two places for states whatever the batch: the first for a sequence that it takes up
-// at its own start, the second for one that starts later and goes on behind it.
+// range has two places for states whatever the batch: the first for a sequence that it takes up at
+// its own start, the second for one that starts later and goes on behind it.
 //
 // Layouts are those of the decode kernel (lane l: n = l % 16, q4 = l / 16): S = K Q^T has tokens
 // 4 q4 + j of every 16 in the lane and row n as its column, O^T = V^T P^T takes P from the same
-// registers.  e4m3 is widened to bf16, exactly, on its way from LDS to the matrix cores, K with its
-// scale (the lane's own token); V's scale goes into P, a multiplication by a power of two.  P is
-// rounded to bf16 there: at most 2^-8 of each weight, of either sign, so below the rounding of the
-// bf16 output where the values do not cancel; the sum of the weights is of the unrounded ones, and
-// running maxima, sums and products stay in 32 bits.
+// registers.  e4m3 is widened to bf16, exactly: with few rows on its way from LDS to the matrix
+// cores, K with its scale (the lane's own token), V's scale going into P; with many rows once for
+// all waves, into a bf16 tile.  P is rounded to bf16: at most 2^-8 of each weight, of either sign,
+// so below the rounding of the bf16 output where the values do not cancel; the sum of the weights
+// is of the unrounded ones, and running maxima, sums and products stay in 32 bits.
 #include <math.h>
 
 #include <algorithm>
@@ -51,13 +51,13 @@ constexpr int kSeqsPerLaunch = 2048;  // prefix sums in LDS; more sequences run 
 constexpr int kMaxTokens = 1 << 24;   // per sequence: the steps of a launch fit 32 bits
 constexpr int kHeaderInts = 16;
 constexpr int64_t kHeaderBytes = ((kHeaderInts + kSeqsPerLaunch + 1) * 4 + 255) / 256 * 256;
-constexpr int kMaxWorkgroups = 512;  // bounds the workspace, whatever the device
+constexpr int kMaxFew = 1024, kMaxMany = 512;  // units at once at most: bounds the workspace, whatever the device
 
 template <bool FP8>
 struct Format {
   static constexpr int kRow = FP8 ? kDim : 2 * kDim;  // bytes of a token's row
   static constexpr int kStep = kTile / kRow;          // tokens per step
-  static constexpr int kParts = kStep / 16;           // of 16 tokens
+  static constexpr int kSubs = kStep / 32;            // products of 32 tokens each
   static constexpr int kKOps = FP8 ? 10 : 8;          // vector memory operations of a K tile and both scales
   static constexpr int kVOps = 8;
 };
@@ -83,10 +83,11 @@ struct TreeParams {
   uint16_t* out;
   int64_t o_tok_stride, o_head_stride;
   int32_t* header;  // [0] steps per range, [kHeaderInts ..] step prefix sums
-  float* part_o;    // [range][2][kv head][max rows][128]
-  float* part_ml;   // [range][2][kv head][max rows][2]
-  int32_t streams, ranges, row_groups, max_rows;
-  Divisor div_streams, div_row_groups, div_ranges, div_block, div_group;
+  float* part_o;    // [range][2][kv head][rows][128]
+  float* part_ml;   // [range][2][kv head][rows][2]
+  int32_t ranges, streams, blocks, rows;  // streams: kv heads x blocks of rows; rows: of all blocks
+  u32 q_flip;       // sign bits that turn a negative scale into a positive one
+  Divisor div_streams, div_blocks, div_ranges, div_block, div_group;
 };
 
 // A sequence's query rows and cached tokens; kind says what there is to do.
@@ -106,7 +107,6 @@ __device__ __forceinline__ SeqShape load_shape(const TreeParams& p, int b) {
   return shape_of(p, p.cu_q ? load_uniform(p.cu_q, b) : b, p.cu_q ? load_uniform(p.cu_q, b + 1) : b + 1,
                   load_uniform(p.kv_lens, b));
 }
-
 // s_cum[b] = steps of sequences 0 .. b - 1, built by the whole workgroup.
 template <int STEP>
 __device__ __forceinline__ void build_prefix(const TreeParams& p, int* s_cum, int* s_part) {
@@ -158,24 +158,63 @@ __device__ __forceinline__ void fill_rows(const TreeParams& p, const int* s_cum)
   }
 }
 
-// A wave's place in the steps of its range.
+// A wave-uniform value in scalar registers.
+__device__ __forceinline__ int uniform(int x) { return __builtin_amdgcn_readfirstlane(x); }
+__device__ __forceinline__ int64_t uniform(int64_t x) {
+  return static_cast<int64_t>(uniform(static_cast<int>(x >> 32))) << 32 | static_cast<u32>(uniform(static_cast<int>(x)));
+}
+
+// The range of unit `unit` (stream fastest), or false if it has none.  One workgroup leaves what the
+// merge needs.
+struct Range {
+  int index, S0, S1;  // steps
+  int first;          // the sequence that holds step S0
+  int kvh, block;
+};
+__device__ __forceinline__ bool find_range(const TreeParams& p, const int* s_cum, int unit, Range& r) {
+  const int B = p.num_seqs, total = uniform(s_cum[B]);
+  const int spr = max(1, div_by(total + p.ranges - 1, p.div_ranges));
+  if (blockIdx.x == 0) {
+    if (threadIdx.x == 0) p.header[0] = spr;
+    for (int b = threadIdx.x; b <= B; b += kThreads) p.header[kHeaderInts + b] = s_cum[b];
+  }
+  r.index = div_by(unit, p.div_streams);
+  const int stream = unit - r.index * p.streams;
+  r.kvh = div_by(stream, p.div_blocks);
+  r.block = stream - r.kvh * p.blocks;
+  r.S0 = r.index * spr;
+  r.S1 = min(total, r.S0 + spr);
+  if (r.index >= p.ranges || r.S0 >= r.S1) return false;
+  int lo = 0, hi = B;  // s_cum[lo] <= S0 < s_cum[lo + 1]
+  while (hi - lo > 1) {
+    const int mid = (lo + hi) >> 1;
+    if (s_cum[mid] <= r.S0) lo = mid;
+    else hi = mid;
+  }
+  r.first = uniform(lo);
+  return true;
+}
+
+// A place in the steps of a range.
 struct Cursor {
-  int b, j, nsteps;   // sequence, step within it, its steps
+  int b, j, nsteps;  // sequence, step within it, its steps
   int q0, n, len;
   int lblk, blk, pf_blk;  // logical block, its id, and the id of the next one (-1: not loaded)
-  int active;         // the sequence has rows in the wave's row group
-  int bad;            // a needed block id was out of range
-  int mark;           // vector memory operations issued up to the step's K tile
+  int bad;           // a needed block id was out of range
+  int mark;          // vector memory operations issued up to the step's K tile
 };
+__device__ __forceinline__ int table_entry(const TreeParams& p, int b, int lblk) {
+  return load_uniform(p.block_tables + b * p.bt_stride, lblk);
+}
 __device__ __forceinline__ void enter_block(const TreeParams& p, Cursor& c, int lblk, int blk) {
   const int bad = blk < 0 || blk >= p.num_cache_blocks;
   c.bad |= bad;
   c.blk = bad ? 0 : blk;
   c.lblk = lblk;
-  c.pf_blk = (lblk + 1) * p.block_size < c.len ? load_uniform(p.block_tables + c.b * p.bt_stride, lblk + 1) : -1;
+  c.pf_blk = (lblk + 1) * p.block_size < c.len ? table_entry(p, c.b, lblk + 1) : -1;
 }
 template <int STEP>
-__device__ __forceinline__ void start_seq(const TreeParams& p, Cursor& c, int b, int j, int first_row) {
+__device__ __forceinline__ void start_seq(const TreeParams& p, Cursor& c, int b, int j) {
   const SeqShape s = load_shape(p, b);
   c.b = b;
   c.j = j;
@@ -183,10 +222,23 @@ __device__ __forceinline__ void start_seq(const TreeParams& p, Cursor& c, int b,
   c.n = s.n;
   c.len = s.len;
   c.nsteps = (s.len + STEP - 1) / STEP;
-  c.active = s.n * p.group > first_row;
   c.bad = 0;
   const int lblk = div_by(j * STEP, p.div_block);
-  enter_block(p, c, lblk, load_uniform(p.block_tables + b * p.bt_stride, lblk));
+  enter_block(p, c, lblk, table_entry(p, b, lblk));
+}
+// c: the step behind prev's, which there is.
+template <int STEP>
+__device__ __forceinline__ void next_step(const TreeParams& p, const int* s_cum, const Cursor& prev, Cursor& c) {
+  if (prev.j + 1 < prev.nsteps) {
+    c = prev;
+    c.j = prev.j + 1;
+    const int lblk = div_by(c.j * STEP, p.div_block);
+    if (lblk != c.lblk) enter_block(p, c, lblk, c.pf_blk != -1 ? c.pf_blk : table_entry(p, c.b, lblk));
+  } else {
+    int b = prev.b + 1;
+    while (uniform(s_cum[b + 1]) == uniform(s_cum[b])) ++b;
+    start_seq<STEP>(p, c, b, 0);
+  }
 }
 
 // The lane's part of a tile fill.  Instruction i fills rows R i .. R i + R - 1 of a tile (R = 4 rows
@@ -230,7 +282,7 @@ __device__ __forceinline__ void issue_scales(const TreeParams& p, int64_t base, 
   }
 }
 
-// K of a step in e4m3: the lane's 16 bytes at a[i] of each 16 tokens, k[4 i + part].
+// K of a step in e4m3: the lane's 16 bytes at a0 and a1 of each 16 tokens, k[4 i + part].
 __device__ __forceinline__ void read_k8_tile(u32 a0, u32 a1, u32x4_t (&k)[8]) {
   asm volatile(
       "ds_read_b128 %0, %8\n\tds_read_b128 %1, %8 offset:2048\n\t"
@@ -284,44 +336,189 @@ __device__ __forceinline__ void wait_tiles(int most) {
   else wait_vmem<0>();
 }
 
-template <bool FP8, int NT>
-__global__ __launch_bounds__(kThreads) void tree_attention_kernel(const TreeParams p) {
+// P of two tokens in packed bf16, times their V scales: the exponents are added as integers.  vs:
+// the bytes, shifted into bf16's exponent.  A weight below 2^-126 counts as the scale times 2^-127.
+typedef uint16_t u16x2_t __attribute__((ext_vector_type(2)));
+__device__ __forceinline__ u32 scale_pair(u32 pk, u32 vs) {
+  const u16x2_t one = {127 << 7, 127 << 7};
+  return __builtin_bit_cast(u32, __builtin_elementwise_sub_sat(
+      static_cast<u16x2_t>(__builtin_bit_cast(u16x2_t, pk) + __builtin_bit_cast(u16x2_t, vs)), one));
+}
+
+// Whether a row sees draft d (below 0: a token of the context), given the bits of its drafts.
+__device__ __forceinline__ bool sees(uint64_t seen, int d) {
+  return (d < 0) | ((d < kMaxQ) & static_cast<int>(seen >> (d & (kMaxQ - 1))));
+}
+
+// The 16 rows that a wave works on, and the online softmax over the tokens that they have met.
+template <int NT>
+struct Rows {
+  int tok[NT], head[NT], row[NT];
+  u32x4_t q[NT][4];
+  uint64_t seen[NT];  // the drafts that the column's token sees
+  float m[NT], l[NT];
+  mfma_f32x4_t acc[NT][8];  // dims 16 mt + 4 q4 + j
+
+  __device__ __forceinline__ void place(const TreeParams& p, int kvh, int first, int stride, int n) {
+#pragma unroll
+    for (int nt = 0; nt < NT; ++nt) {
+      row[nt] = first + 16 * stride * nt + n;
+      tok[nt] = div_by(row[nt], p.div_group);
+      head[nt] = kvh * p.group + row[nt] - tok[nt] * p.group;
+    }
+  }
+  __device__ __forceinline__ void reset() {
+#pragma unroll
+    for (int nt = 0; nt < NT; ++nt) {
+      m[nt] = kMaxFloor;
+      l[nt] = 0.f;
+#pragma unroll
+      for (int mt = 0; mt < 8; ++mt) acc[nt][mt] = mfma_f32x4_t{0.f, 0.f, 0.f, 0.f};
+    }
+  }
+  // WIDE: dims in the order of 16-byte reads of an e4m3 row.
+  template <bool WIDE>
+  __device__ __forceinline__ void load_q(const TreeParams& p, const Cursor& c, int q4) {
+#pragma unroll
+    for (int nt = 0; nt < NT; ++nt) {
+      const int i = min(tok[nt], c.n - 1);
+      const uint16_t* src = p.q + (c.q0 + i) * p.q_tok_stride + head[nt] * p.q_head_stride;
+#pragma unroll
+      for (int kk = 0; kk < 4; ++kk)
+        q[nt][kk] = *reinterpret_cast<const u32x4_t*>(
+            src + (WIDE ? 64 * (kk >> 1) + 16 * q4 + 8 * (kk & 1) : 32 * kk + 8 * q4)) ^ p.q_flip;
+      const uint64_t all = ~0ull >> (64 - c.n);
+      const uint64_t bits = p.mask ? static_cast<uint64_t>(p.mask[c.q0 + i]) : ~0ull >> (63 - i);
+      seen[nt] = bits & all;
+      asm volatile("" : "+v"(seen[nt]));  // waited for here, not where its registers are next written
+    }
+  }
+  // Weights of 32 tokens from their scores s0 (tokens 4 q4 + j) and s1 (16 + 4 q4 + j), packed as the
+  // second product's operand; `draft` is the first token's draft, below 0 in the context.  The running
+  // maximum m moves only where a score lies 2^8 above it: weights reach 2^8 at most, and the sums are
+  // rarely multiplied.
+  __device__ __forceinline__ u32x4_t weigh(int nt, mfma_f32x4_t s0, mfma_f32x4_t s1, float scale, bool tail, int draft,
+                                           int q4) {
+    float x[8];
+#pragma unroll
+    for (int e = 0; e < 8; ++e) x[e] = e < 4 ? s0[e] : s1[e - 4];
+    if (tail) {
+#pragma unroll
+      for (int e = 0; e < 8; ++e) {
+        const int d = draft + 16 * (e >> 2) + 4 * q4 + (e & 3);
+        x[e] = sees(seen[nt], d) ? x[e] : -INFINITY;
+      }
+    }
+    float mx = x[0];
+#pragma unroll
+    for (int e = 1; e < 8; ++e) mx = fmaxf(mx, x[e]);
+    mx = xor32_max(xor16_max(mx)) * scale;
+    if (__any(mx > m[nt] + 8.f)) {
+      const float m_new = fmaxf(m[nt], mx);
+      const float alpha = fast_exp2(m[nt] - m_new);
+      m[nt] = m_new;
+      l[nt] *= alpha;
+#pragma unroll
+      for (int mt = 0; mt < 8; ++mt) acc[nt][mt] *= alpha;
+    }
+    u32x4_t pf;
+#pragma unroll
+    for (int e = 0; e < 8; e += 2) {
+      const float w0 = fast_exp2(fmaf(x[e], scale, -m[nt])), w1 = fast_exp2(fmaf(x[e + 1], scale, -m[nt]));
+      l[nt] += w0 + w1;
+      pf[e >> 1] = pack_bf16x2(w0, w1);
+    }
+    return pf;
+  }
+  // The tail's V: a weight of 0 does not undo an infinity or NaN, so tokens behind the last one (from
+  // `left` on) are cleared, and drafts that are not finite leave the product and are added one by one
+  // to the rows that see them.
+  __device__ __forceinline__ void clean(u32x4_t (&vt)[8], const u32x4_t (&pf)[NT], int draft, int left, int q4) {
+    u32x4_t fine;
+    u32 odd = 0;  // bit e: element e (token 4 q4 + e, or 12 + 4 q4 + e for e >= 4) is cached and not finite
+#pragma unroll
+    for (int w = 0; w < 4; ++w) {
+      const int t = 4 * q4 + 16 * (w >> 1) + 2 * (w & 1);
+      fine[w] = (t < left ? 0xffffu : 0u) | (t + 1 < left ? 0xffff0000u : 0u);
+#pragma unroll
+      for (int mt = 0; mt < 8; ++mt) {
+        const u32 v = vt[mt][w] & fine[w];
+        odd |= ((v & 0x7f80u) == 0x7f80u ? 1u : 0u) << (2 * w);
+        odd |= ((v & 0x7f800000u) == 0x7f800000u ? 2u : 0u) << (2 * w);
+      }
+    }
+    if (__any(odd != 0)) {
+#pragma unroll 1
+      for (int i = 0; i < 32; ++i) {  // element e = i % 8 of the lanes of group i / 8
+        const int e = i & 7, g = i >> 3;
+        if (!__any(q4 == g && (odd >> e & 1))) continue;
+        const u32 half = q4 == g ? (e & 1 ? 0xffff0000u : 0xffffu) : 0u;
+        u32x4_t only;
+#pragma unroll
+        for (int w = 0; w < 4; ++w) {
+          only[w] = w == e >> 1 ? half : 0u;
+          fine[w] &= ~only[w];
+        }
+        const int d = draft + 16 * (e >> 2) + 4 * g + (e & 3);
+#pragma unroll
+        for (int nt = 0; nt < NT; ++nt) {
+          const bool mine = sees(seen[nt], d);
+#pragma unroll
+          for (int mt = 0; mt < 8; ++mt) {
+            const mfma_f32x4_t with = mfma16(vt[mt] & only, pf[nt], acc[nt][mt]);
+            if (mine) acc[nt][mt] = with;
+          }
+        }
+      }
+    }
+#pragma unroll
+    for (int mt = 0; mt < 8; ++mt) vt[mt] &= fine;
+  }
+  // The rows' output where a range held all of the sequence, otherwise a partial state at `place`.
+  __device__ __forceinline__ void emit(const TreeParams& p, const Cursor& c, int kvh, bool whole, int place, int q4) {
+#pragma unroll
+    for (int nt = 0; nt < NT; ++nt) {
+      float sum = xor32_sum(xor16_sum(l[nt]));
+      if (c.bad) sum = NAN;
+      if (tok[nt] >= c.n) continue;
+      if (whole) {
+        const float inv = sum == 0.f ? 0.f : 1.f / sum;
+        uint16_t* out = p.out + (c.q0 + tok[nt]) * p.o_tok_stride + head[nt] * p.o_head_stride + 4 * q4;
+#pragma unroll
+        for (int mt = 0; mt < 8; ++mt) {
+          const mfma_f32x4_t o = acc[nt][mt] * inv;
+          *reinterpret_cast<u32x2_t*>(out + 16 * mt) = u32x2_t{pack_bf16x2(o[0], o[1]), pack_bf16x2(o[2], o[3])};
+        }
+      } else {
+        const int64_t at = (static_cast<int64_t>(place) * p.num_kv_heads + kvh) * p.rows + row[nt];
+        float* part = p.part_o + at * kDim + 4 * q4;
+#pragma unroll
+        for (int mt = 0; mt < 8; ++mt) *reinterpret_cast<mfma_f32x4_t*>(part + 16 * mt) = acc[nt][mt];
+        if (q4 == 0) *reinterpret_cast<float2*>(p.part_ml + 2 * at) = make_float2(m[nt], sum);
+      }
+    }
+  }
+};
+
+// Up to 16 rows per kv head: a wave for itself, with the tiles of two steps in flight in its own LDS,
+// so that no wave waits for another.
+template <bool FP8>
+__global__ __launch_bounds__(kThreads) void tree_few_kernel(const TreeParams p) {
   using F = Format<FP8>;
-  constexpr int STEP = F::kStep, PARTS = F::kParts;
+  constexpr int STEP = F::kStep, SUBS = F::kSubs;
   __shared__ __attribute__((aligned(16))) char s_tile[kWaves][2][2 * kTile];
   __shared__ __attribute__((aligned(16))) char s_scale[FP8 ? kWaves : 1][2][128];
   __shared__ int s_cum[kSeqsPerLaunch + 1];
   __shared__ int s_part[kWaves];
 
-  const int tid = threadIdx.x, lane = tid & 63;
-  const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+  const int lane = threadIdx.x & 63, wave = uniform(static_cast<int>(threadIdx.x >> 6));
   const int n = lane & 15, q4 = lane >> 4;
-
   build_prefix<STEP>(p, s_cum, s_part);
   fill_rows(p, s_cum);
-  const int B = p.num_seqs;
-  const int total = __builtin_amdgcn_readfirstlane(s_cum[B]);
-  const int spr = max(1, div_by(total + p.ranges - 1, p.div_ranges));
-  if (blockIdx.x == 0) {  // for the merge
-    if (tid == 0) p.header[0] = spr;
-    for (int b = tid; b <= B; b += kThreads) p.header[kHeaderInts + b] = s_cum[b];
-  }
-  const int unit = static_cast<int>(blockIdx.x) * kWaves + wave;
-  const int range = div_by(unit, p.div_streams), stream = unit - range * p.streams;
-  const int kvh = div_by(stream, p.div_row_groups), rg = stream - kvh * p.row_groups;
-  const int S0 = range * spr, S1 = min(total, S0 + spr);
-  if (range >= p.ranges || S0 >= S1) return;  // no barrier follows
+  Range r;
+  if (!find_range(p, s_cum, static_cast<int>(blockIdx.x) * kWaves + wave, r)) return;  // no barrier follows
 
-  int lo = 0, hi = B;  // s_cum[lo] <= S0 < s_cum[lo + 1]
-  while (hi - lo > 1) {
-    const int mid = (lo + hi) >> 1;
-    if (s_cum[mid] <= S0) lo = mid;
-    else hi = mid;
-  }
-  lo = __builtin_amdgcn_readfirstlane(lo);
-
-  const int first_row = rg * 16 * NT;
-  const int64_t head_off = kvh * p.head_stride, scale_head = kvh * p.scale_head_stride;
+  const int64_t head_off = r.kvh * p.head_stride, scale_head = r.kvh * p.scale_head_stride;
   const TileLane ln = tile_lane<FP8>(p, lane);
   // LDS addresses of the lane's operands in a tile at address 0 (see the swizzles)
   u32 ka[4], va[8];
@@ -338,91 +535,31 @@ __global__ __launch_bounds__(kThreads) void tree_attention_kernel(const TreePara
       va[mt] = kTile + 256 * row + 8 * (n & 3) + 32 * (mt ^ (row & 7));
     }
   }
-  int tok[NT], head[NT];  // the token and query head of the lane's column in each 16 rows
-#pragma unroll
-  for (int nt = 0; nt < NT; ++nt) {
-    const int row = first_row + 16 * nt + n;
-    tok[nt] = div_by(row, p.div_group);
-    head[nt] = kvh * p.group + row - tok[nt] * p.group;
-  }
+  Rows<1> rows;
+  rows.place(p, r.kvh, 0, 1, n);
+  rows.reset();
 
-  u32x4_t qv[NT][4];
-  uint64_t seen[NT];  // the drafts that the column's token sees
-  float m[NT], l[NT];
-  mfma_f32x4_t acc[NT][8];
-  auto reset = [&] {
-#pragma unroll
-    for (int nt = 0; nt < NT; ++nt) {
-      m[nt] = kMaxFloor;
-      l[nt] = 0.f;
-#pragma unroll
-      for (int mt = 0; mt < 8; ++mt) acc[nt][mt] = mfma_f32x4_t{0.f, 0.f, 0.f, 0.f};
-    }
-  };
-  auto load_q = [&](const Cursor& c) {
-#pragma unroll
-    for (int nt = 0; nt < NT; ++nt) {
-      const int i = min(tok[nt], c.n - 1);
-      const uint16_t* src = p.q + (c.q0 + i) * p.q_tok_stride + head[nt] * p.q_head_stride;
-#pragma unroll
-      for (int kk = 0; kk < 4; ++kk)
-        qv[nt][kk] = *reinterpret_cast<const u32x4_t*>(
-            src + (FP8 ? 64 * (kk >> 1) + 16 * q4 + 8 * (kk & 1) : 32 * kk + 8 * q4));
-      const uint64_t all = ~0ull >> (64 - c.n);
-      const uint64_t bits = p.mask ? static_cast<uint64_t>(p.mask[c.q0 + i]) : ~0ull >> (63 - i);
-      seen[nt] = bits & all;
-    }
-  };
-  // The state of the wave's rows of a sequence: its output, or a partial state at `place`.
-  auto emit = [&](const Cursor& c, bool whole, int place) {
-#pragma unroll
-    for (int nt = 0; nt < NT; ++nt) {
-      float sum = xor32_sum(xor16_sum(l[nt]));
-      if (c.bad) sum = NAN;
-      if (tok[nt] >= c.n) continue;
-      if (whole) {
-        const float inv = sum == 0.f ? 0.f : 1.f / sum;
-        uint16_t* out = p.out + (c.q0 + tok[nt]) * p.o_tok_stride + head[nt] * p.o_head_stride + 4 * q4;
-#pragma unroll
-        for (int mt = 0; mt < 8; ++mt) {
-          const mfma_f32x4_t o = acc[nt][mt] * inv;
-          *reinterpret_cast<u32x2_t*>(out + 16 * mt) = u32x2_t{pack_bf16x2(o[0], o[1]), pack_bf16x2(o[2], o[3])};
-        }
-      } else {
-        const int64_t at = (static_cast<int64_t>(place) * p.num_kv_heads + kvh) * p.max_rows + first_row + 16 * nt + n;
-        float* part = p.part_o + at * kDim + 4 * q4;
-#pragma unroll
-        for (int mt = 0; mt < 8; ++mt) *reinterpret_cast<mfma_f32x4_t*>(part + 16 * mt) = acc[nt][mt];
-        if (q4 == 0) *reinterpret_cast<float2*>(p.part_ml + 2 * at) = make_float2(m[nt], sum);
-      }
-    }
-  };
-
-  // The loop.  Iteration S computes step S and issues the tiles of step S + 2, each as soon as its
-  // tile has been read; the first two only issue.  c[i]: the place of step S + i.
+  // Iteration S computes step S and issues the tiles of step S + 2, each as soon as its tile has been
+  // read; the first two only issue.  c[i]: the place of step S + i.
   Cursor c[3] = {};
   Cursor &c0 = c[0], &cn = c[2];
   int issued = 0;
-  reset();
 #pragma unroll 1
-  for (int S = S0 - 2; S < S1; ++S) {
-    const int buf = (S - S0) & 1;
+  for (int S = r.S0 - 2; S < r.S1; ++S) {
+    const int buf = (S - r.S0) & 1;
     char* const tiles = s_tile[wave][buf];
     char* const scales = s_scale[FP8 ? wave : 0][buf];
     const u32 tile = lds_addr(tiles);
-    const bool live = S >= S0 && c0.active, issue = S + 2 < S1;
-    const bool starts = S == S0 || c0.j == 0;
+    const bool live = S >= r.S0, issue = S + 2 < r.S1;
     const int t0 = c0.j * STEP, ctx = c0.len - c0.n;
-    const bool tail = t0 + STEP > ctx;  // the step holds drafts, or ends behind the last token
-    mfma_f32x4_t s[NT][PARTS];
-    u32 vexp[4] = {};
+    // ---- S = K Q^T of the step
+    mfma_f32x4_t s[2 * SUBS];
+    u32 vexp[2 * SUBS] = {};
     if (live) {
-      if (starts) load_q(c0);
+      if (S == r.S0 || c0.j == 0) rows.load_q<FP8>(p, c0, q4);
       wait_tiles<F::kKOps, F::kVOps>(issued - c0.mark);
 #pragma unroll
-      for (int nt = 0; nt < NT; ++nt)
-#pragma unroll
-        for (int h = 0; h < PARTS; ++h) s[nt][h] = mfma_f32x4_t{0.f, 0.f, 0.f, 0.f};
+      for (int h = 0; h < 2 * SUBS; ++h) s[h] = mfma_f32x4_t{0.f, 0.f, 0.f, 0.f};
       u32x4_t k[8];
       if constexpr (FP8) {
         u32 kexp[4];
@@ -430,98 +567,55 @@ __global__ __launch_bounds__(kThreads) void tree_attention_kernel(const TreePara
         read_scales(at + n, at + 64 + 4 * q4, kexp, vexp);
         read_k8_tile(tile + ka[0], tile + ka[1], k);
 #pragma unroll
-        for (int h = 0; h < PARTS; ++h) {
-          const float scale = __uint_as_float(kexp[h] << 23);
+        for (int kk = 0; kk < 4; ++kk)
 #pragma unroll
-          for (int kk = 0; kk < 4; ++kk) {
+          for (int h = 0; h < 4; ++h) {
             const u32x4_t w = k[4 * (kk >> 1) + h];
-            const u32x4_t a = widen8(w[2 * (kk & 1)], w[2 * (kk & 1) + 1], scale);
-#pragma unroll
-            for (int nt = 0; nt < NT; ++nt) s[nt][h] = mfma16(a, qv[nt][kk], s[nt][h]);
+            s[h] = mfma16(widen8(w[2 * (kk & 1)], w[2 * (kk & 1) + 1], __uint_as_float(kexp[h] << 23)), rows.q[0][kk], s[h]);
           }
-        }
       } else {
         const u32 at[4] = {tile + ka[0], tile + ka[1], tile + ka[2], tile + ka[3]};
         read_k_tile(at, k);
 #pragma unroll
-        for (int i = 0; i < 8; ++i)
-#pragma unroll
-          for (int nt = 0; nt < NT; ++nt) s[nt][i & 1] = mfma16(k[i], qv[nt][i >> 1], s[nt][i & 1]);
+        for (int i = 0; i < 8; ++i) s[i & 1] = mfma16(k[i], rows.q[0][i >> 1], s[i & 1]);
       }
     }
     int64_t base = 0;
-    int rows = 0;
+    int left = 0;
     if (issue) {  // K has been read: its tile takes step S + 2
-      const Cursor& prev = c[1];
-      if (S + 2 == S0) {
-        const int cum = __builtin_amdgcn_readfirstlane(s_cum[lo]);
-        start_seq<STEP>(p, cn, lo, S0 - cum, first_row);
-      } else if (prev.j + 1 == prev.nsteps) {
-        int b = prev.b + 1;
-        while (__builtin_amdgcn_readfirstlane(s_cum[b + 1]) == __builtin_amdgcn_readfirstlane(s_cum[b])) ++b;
-        start_seq<STEP>(p, cn, b, 0, first_row);  // a step follows, so a sequence with steps does
-      } else {
-        cn = prev;
-        cn.j = prev.j + 1;
-      }
-      if (cn.active) {
-        const int at = cn.j * STEP, lblk = div_by(at, p.div_block);
-        if (lblk != cn.lblk)
-          enter_block(p, cn, lblk,
-                      cn.pf_blk != -1 ? cn.pf_blk : load_uniform(p.block_tables + cn.b * p.bt_stride, lblk));
-        const int off = at - lblk * p.block_size;
-        rows = min(STEP, cn.len - at);
-        base = cn.blk * p.blk_stride + off * p.slot_stride + head_off;
-        issue_tile<FP8, false>(p, ln, base, rows, tiles);
-        if (FP8) issue_scales(p, cn.blk * p.scale_blk_stride + scale_head + off, lane, scales);
-        issued += F::kKOps;
-        cn.mark = issued;
-      }
+      if (S + 2 == r.S0) start_seq<STEP>(p, cn, r.first, r.S0 - uniform(s_cum[r.first]));
+      else next_step<STEP>(p, s_cum, c[1], cn);
+      const int off = cn.j * STEP - cn.lblk * p.block_size;
+      left = min(STEP, cn.len - cn.j * STEP);
+      base = uniform(cn.blk * p.blk_stride + off * p.slot_stride + head_off);
+      issue_tile<FP8, false>(p, ln, base, left, tiles);
+      if (FP8) issue_scales(p, cn.blk * p.scale_blk_stride + scale_head + off, lane, scales);
+      issued += F::kKOps;
+      cn.mark = issued;
     }
     if (live) {
-      u32 pk[NT][2 * PARTS];
 #pragma unroll
-      for (int nt = 0; nt < NT; ++nt) {
-        float x[4 * PARTS], mx = kMaxFloor;
+      for (int sub = 0; sub < SUBS; ++sub) {  // 32 tokens
+        const int draft = t0 + 32 * sub - ctx;
+        const bool tail = draft > -32;  // drafts among them, or the last token in front of them
+        u32x4_t pf[1] = {rows.weigh(0, s[2 * sub], s[2 * sub + 1], p.scale_log2, tail, draft, q4)};
+        if constexpr (FP8) {
 #pragma unroll
-        for (int e = 0; e < 4 * PARTS; ++e) x[e] = s[nt][e >> 2][e & 3] * p.scale_log2;
-        if (tail) {
-#pragma unroll
-          for (int e = 0; e < 4 * PARTS; ++e) {
-            const int d = t0 + 16 * (e >> 2) + 4 * q4 + (e & 3) - ctx;  // the draft, or below 0
-            if (!(d < 0 || (d < 64 && (seen[nt] >> (d & 63) & 1)))) x[e] = -INFINITY;
+          for (int w = 0; w < 4; ++w) {
+            const u32 bytes = vexp[2 * sub + (w >> 1)];
+            const u32 scaled = scale_pair(pf[0][w], __builtin_amdgcn_perm(0, bytes, w & 1 ? 0x0c030c02 : 0x0c010c00) << 7);
+            // a masked weight is 0 whatever the scale
+            pf[0][w] = !tail ? scaled
+                             : ((pf[0][w] & 0xffffu) ? scaled & 0xffffu : 0u) |
+                                   ((pf[0][w] >> 16) ? scaled & 0xffff0000u : 0u);
           }
         }
-#pragma unroll
-        for (int e = 0; e < 4 * PARTS; ++e) mx = fmaxf(mx, x[e]);
-        mx = xor32_max(xor16_max(mx));
-        const float m_new = fmaxf(m[nt], mx);
-        const float alpha = fast_exp2(m[nt] - m_new);
-        m[nt] = m_new;
-        if (__any(alpha != 1.f)) {
-          l[nt] *= alpha;
-#pragma unroll
-          for (int mt = 0; mt < 8; ++mt) acc[nt][mt] *= alpha;
-        }
-#pragma unroll
-        for (int e = 0; e < 4 * PARTS; e += 2) {
-          float w[2];
-#pragma unroll
-          for (int i = 0; i < 2; ++i) {
-            w[i] = fast_exp2(x[e + i] - m_new);
-            l[nt] += w[i];
-            if (FP8) w[i] = __builtin_amdgcn_ldexpf(w[i], static_cast<int>(vexp[e >> 2] >> (8 * ((e + i) & 3)) & 0xff) - 127);
-          }
-          pk[nt][e >> 1] = pack_bf16x2(w[0], w[1]);
-        }
-      }
-      wait_tiles<F::kKOps, F::kVOps>(issued - c0.mark - F::kVOps);
-#pragma unroll
-      for (int kb = 0; kb < PARTS / 2; ++kb) {  // 32 tokens
+        // ---- O^T += V^T P^T
+        if (sub == 0) wait_tiles<F::kKOps, F::kVOps>(issued - c0.mark - F::kVOps);
         u32x4_t vt[8];
         if constexpr (FP8) {
           u32x2_t v8[8];
-          const u32 at = tile + 4096 * kb;
+          const u32 at = tile + 4096 * sub;
           const u32 a[8] = {at + va[0], at + va[1], at + va[2], at + va[3],
                             at + va[4], at + va[5], at + va[6], at + va[7]};
           read_v8_tile(a, v8);
@@ -535,104 +629,474 @@ __global__ __launch_bounds__(kThreads) void tree_attention_kernel(const TreePara
 #pragma unroll
           for (int mt = 0; mt < 8; ++mt) vt[mt] = u32x4_t{vlo[mt].x, vlo[mt].y, vhi[mt].x, vhi[mt].y};
         }
-        auto pf = [&](int nt) {
-          return u32x4_t{pk[nt][4 * kb], pk[nt][4 * kb + 1], pk[nt][4 * kb + 2], pk[nt][4 * kb + 3]};
-        };
-        if (tail) {
-          // A weight of 0 does not undo an infinity or NaN in V: tokens behind the last one are
-          // cleared, and drafts that are not finite leave the product and are added one by one to
-          // the rows that see them.
-          const int at = t0 + 32 * kb + 4 * q4;  // element e of the lane is token at + e, or at + 12 + e for e >= 4
-          u32x4_t live_w;
-          u32 odd = 0;  // bit e: element e is a cached token that is not finite in some dim
+        if (tail) rows.clean(vt, pf, draft, c0.len - t0 - 32 * sub, q4);
 #pragma unroll
-          for (int w = 0; w < 4; ++w) {
-            const int t = at + 16 * (w >> 1) + 2 * (w & 1);
-            live_w[w] = (t < c0.len ? 0xffffu : 0u) | (t + 1 < c0.len ? 0xffff0000u : 0u);
-#pragma unroll
-            for (int mt = 0; mt < 8; ++mt) {
-              const u32 x = vt[mt][w] & live_w[w];
-              odd |= ((x & 0x7f80u) == 0x7f80u ? 1u : 0u) << (2 * w);
-              odd |= ((x & 0x7f800000u) == 0x7f800000u ? 2u : 0u) << (2 * w);
-            }
-          }
-          u32x4_t fine = live_w;
-          if (__any(odd != 0)) {
-#pragma unroll 1
-            for (int i = 0; i < 32; ++i) {  // element e = i % 8 of the lanes of row group i / 8
-              const int e = i & 7, g = i >> 3;
-              if (!__any(q4 == g && (odd >> e & 1))) continue;
-              const u32 mine = q4 == g ? (e & 1 ? 0xffff0000u : 0xffffu) : 0u;
-              u32x4_t only;
-#pragma unroll
-              for (int w = 0; w < 4; ++w) {
-                only[w] = w == e >> 1 ? mine : 0u;
-                fine[w] &= ~only[w];
-              }
-              const int d = t0 + 32 * kb + 16 * (e >> 2) + 4 * g + (e & 3) - ctx;
-#pragma unroll
-              for (int nt = 0; nt < NT; ++nt) {
-                const bool sees = d < 0 || (seen[nt] >> (d & 63) & 1);
-#pragma unroll
-                for (int mt = 0; mt < 8; ++mt) {
-                  const mfma_f32x4_t with = mfma16(vt[mt] & only, pf(nt), acc[nt][mt]);
-                  if (sees) acc[nt][mt] = with;
-                }
-              }
-            }
-          }
-#pragma unroll
-          for (int mt = 0; mt < 8; ++mt) vt[mt] &= fine;
-        }
-#pragma unroll
-        for (int mt = 0; mt < 8; ++mt)
-#pragma unroll
-          for (int nt = 0; nt < NT; ++nt) acc[nt][mt] = mfma16(vt[mt], pf(nt), acc[nt][mt]);
+        for (int mt = 0; mt < 8; ++mt) rows.acc[0][mt] = mfma16(vt[mt], pf[0], rows.acc[0][mt]);
       }
     }
-    if (issue && cn.active) {
-      issue_tile<FP8, true>(p, ln, base, rows, tiles + kTile);
+    if (issue) {
+      issue_tile<FP8, true>(p, ln, base, left, tiles + kTile);
       issued += F::kVOps;
     }
-    if (live && (c0.j + 1 == c0.nsteps || S + 1 == S1)) {
+    if (live && (c0.j + 1 == c0.nsteps || S + 1 == r.S1)) {
       const int from = S - c0.j, to = from + c0.nsteps;  // the sequence's steps
-      emit(c0, from >= S0 && to <= S1, 2 * range + (from > S0 ? 1 : 0));
-      reset();
+      rows.emit(p, c0, r.kvh, from >= r.S0 && to <= r.S1, 2 * r.index + (from > r.S0 ? 1 : 0), q4);
+      rows.reset();
     }
     c[0] = c[1];
     c[1] = c[2];
   }
 }
 
+// More rows: the four waves of a workgroup share bf16 tiles of 64 tokens, and a wave has 32 rows
+// (v_mfma_f32_32x32x16_bf16; lane l: row l % 32, hf = l / 32).  KW = 1: wave w has rows 32 w .. of a block of
+// 128.  KW = 2, up to 64 rows: waves w and w + 2 have rows 32 (w % 2) .. and 32 tokens of every step each; their
+// states are joined through LDS where the sequence ends.
+//
+// Two workgroups on a CU: one computes while the other waits.  bf16: two tiles, the next one loaded while a tile
+// is used.  e4m3: one bf16 tile, and two of e4m3 behind it, from which every wave widens the 16 tokens that it
+// has loaded itself, with their scales.
+//
+// Tile rows are 256 bytes, 16-byte chunk c of token r at chunk c ^ (r % 16) of K and c ^ 4 (r % 4) of V.  The lane
+// gets the scores of tokens 8 (i / 4) + 4 hf + i % 4 of each 32, and of O^T dims 32 mb + 8 (j / 4) + 4 hf + j % 4.
+constexpr int kManyStep = 64;
+constexpr int kTileElems = kManyStep * kDim;
+// A row's weights of one step sum up to this before its maximum is taken again (see weigh).
+constexpr float kSumLimit = 65536.f;
+
+// All waves' LDS accesses are done, but not their loads.
+__device__ __forceinline__ void tile_barrier() { asm volatile("s_waitcnt lgkmcnt(0)\n\ts_barrier" ::: "memory"); }
+
+template <bool FP8, int KW>
+__global__ __launch_bounds__(kThreads, 2) void tree_many_kernel(const TreeParams p) {
+  constexpr int STEP = kManyStep, BLOCKS = 2 / KW;  // blocks of 32 tokens of a step that a wave takes
+  __shared__ __attribute__((aligned(16))) uint16_t s_k0[kTileElems];
+  __shared__ __attribute__((aligned(16))) uint16_t s_v0[kTileElems];
+  __shared__ __attribute__((aligned(16))) uint16_t s_k1[FP8 ? 8 : kTileElems];
+  __shared__ __attribute__((aligned(16))) uint16_t s_v1[FP8 ? 8 : kTileElems];
+  __shared__ __attribute__((aligned(16))) char s_raw[FP8 ? 2 : 1][FP8 ? 2 * kTile + 128 : 16];
+  __shared__ float2 s_ml[KW == 2 ? 2 : 1][64];
+  __shared__ int s_cum[kSeqsPerLaunch + 1];
+  __shared__ int s_part[kWaves];
+
+  const int lane = threadIdx.x & 63, wave = uniform(static_cast<int>(threadIdx.x >> 6));
+  build_prefix<STEP>(p, s_cum, s_part);
+  fill_rows(p, s_cum);
+  Range r;
+  // Workgroups are dealt out over the 8 XCDs in turn: neighbouring units, which read the same tokens, go to
+  // one XCD, whose L2 then reads them once.
+  const int unit = static_cast<int>(blockIdx.x & 7) * static_cast<int>(gridDim.x >> 3) + static_cast<int>(blockIdx.x >> 3);
+  if (!find_range(p, s_cum, unit, r)) return;  // the whole workgroup
+
+  // ---- loads: the wave fills tokens 16 wave .. + 15, 4 (e4m3: 8) per instruction
+  const int64_t head_off = r.kvh * p.head_stride, scale_head = r.kvh * p.scale_head_stride;
+  const int stride = static_cast<int>(p.slot_stride);
+  // What follows from the lane is derived anew in each step: held over the loop, it would take the registers
+  // that the products need.
+  auto fresh_lane = [&]() __attribute__((always_inline)) {
+    int x = lane;
+    asm volatile("" : "+v"(x));
+    return x;
+  };
+  constexpr int kFills = FP8 ? 2 : 4;               // instructions of a wave for K, and for V
+  constexpr int kOps = 2 * kFills + (FP8 ? 2 : 0);  // and every wave loads the scales
+  auto issue = [&](const Cursor& c, char* k_to, char* v_to, char* scale_to) __attribute__((always_inline)) {
+    const int off = c.j * STEP - c.lblk * p.block_size, last = (min(STEP, c.len - c.j * STEP) - 1) * stride;
+    const int64_t base = uniform(c.blk * p.blk_stride + off * p.slot_stride + head_off);
+    const uint32_t bytes = static_cast<uint32_t>((STEP - 1) * stride + (FP8 ? kDim : 2 * kDim));
+    const int ln = fresh_lane(), lr = FP8 ? ln >> 3 : ln >> 4, lc = FP8 ? ln & 7 : ln & 15;
+    const int row_off = (16 * wave + lr) * stride;
+    const int k_chunk = FP8 ? 16 * lc : 16 * (lc ^ lr), v_chunk = FP8 ? 16 * lc : 16 * (lc ^ (4 * (lr & 3)));
+    const BufferRsrc kr = buffer_rsrc(p.k_cache + base, bytes), vr = buffer_rsrc(p.v_cache + base, bytes);
+    // row 16 wave + 4 i + lr: its K chunks are swizzled by (4 i + lr) % 16
+#pragma unroll
+    for (int i = 0; i < kFills; ++i)
+      raw_buffer_load_lds(kr, (LdsPtr)(k_to + 1024 * (kFills * wave + i)), 16,
+                          min(row_off + (FP8 ? 8 : 4) * i * stride, last) + (FP8 ? k_chunk : k_chunk ^ (64 * i)), 0, 0, 0);
+#pragma unroll
+    for (int i = 0; i < kFills; ++i)
+      raw_buffer_load_lds(vr, (LdsPtr)(v_to + 1024 * (kFills * wave + i)), 16,
+                          min(row_off + (FP8 ? 8 : 4) * i * stride, last) + v_chunk, 0, 0, 0);
+    if (FP8) issue_scales(p, uniform(c.blk * p.scale_blk_stride + scale_head + off), ln, scale_to);
+  };
+  // FP8: the wave's 16 tokens into the bf16 tile.  Lane: token 8 i + lr, dims 16 lc .. + 15.
+  auto widen = [&](int buf) __attribute__((always_inline)) {
+    const u32 raw = lds_addr(s_raw[FP8 ? buf : 0]);
+    const int ln = fresh_lane(), lr = ln >> 3, lc = ln & 7;
+#pragma unroll
+    for (int i = 0; i < 2; ++i) {
+      const int row = 16 * wave + 8 * i + lr;
+      u32x4_t k, v;
+      u32 ke, ve;
+      const u32 at = raw + 128 * row + 16 * lc, scale_at = raw + 2 * kTile + row;
+      asm volatile(
+          "ds_read_b128 %0, %4\n\tds_read_b128 %1, %4 offset:8192\n\tds_read_u8 %2, %5\n\tds_read_u8 %3, %5 offset:64\n\t"
+          "s_waitcnt lgkmcnt(0)"
+          : "=&v"(k), "=&v"(v), "=&v"(ke), "=&v"(ve)
+          : "v"(at), "v"(scale_at)
+          : "memory");
+      const u32 k_to = lds_addr(s_k0) + 256 * row, v_to = lds_addr(s_v0) + 256 * row;
+      const float ks = __uint_as_float(ke << 23), vs = __uint_as_float(ve << 23);
+#pragma unroll
+      for (int h = 0; h < 2; ++h) {
+        const u32x4_t kw = widen8(k[2 * h], k[2 * h + 1], ks), vw = widen8(v[2 * h], v[2 * h + 1], vs);
+        asm volatile("ds_write_b128 %0, %1" ::"v"(k_to + 16 * ((2 * lc + h) ^ (row & 15))), "v"(kw) : "memory");
+        asm volatile("ds_write_b128 %0, %1" ::"v"(v_to + 16 * ((2 * lc + h) ^ (4 * (row & 3)))), "v"(vw) : "memory");
+      }
+    }
+  };
+
+  // ---- the wave's rows
+  const int kw = KW == 2 ? wave >> 1 : 0, rw = KW == 2 ? wave & 1 : wave;
+  const int first_row = r.block * 128 + 32 * rw;
+  auto token_of = [&](int row) __attribute__((always_inline)) { return div_by(row, p.div_group); };
+  uint4 q[8];
+  uint64_t seen = 0;  // the drafts that the row's token sees
+  float m = kMaxFloor, l = 0.f;
+  f32x16_t acc[4];
+  bool fresh = true;  // no step of the sequence has been taken
+  auto start = [&](const Cursor& c) __attribute__((always_inline)) {
+    const int ln = fresh_lane(), row = first_row + (ln & 31), tok = token_of(row);
+    const int i = min(tok, c.n - 1), head = r.kvh * p.group + row - tok * p.group;
+    const uint16_t* src = p.q + (c.q0 + i) * p.q_tok_stride + head * p.q_head_stride + 8 * (ln >> 5);
+#pragma unroll
+    for (int ks = 0; ks < 8; ++ks) {
+      uint4 x = *reinterpret_cast<const uint4*>(src + 16 * ks);
+      q[ks] = make_uint4(x.x ^ p.q_flip, x.y ^ p.q_flip, x.z ^ p.q_flip, x.w ^ p.q_flip);
+    }
+    const uint64_t all = ~0ull >> (64 - c.n);
+    seen = (p.mask ? static_cast<uint64_t>(p.mask[c.q0 + i]) : ~0ull >> (63 - i)) & all;
+    asm volatile("" : "+v"(seen));  // waited for here, not in front of every product that reuses its registers
+    m = kMaxFloor;
+    l = 0.f;
+    fresh = true;
+#pragma unroll
+    for (int mb = 0; mb < 4; ++mb)
+#pragma unroll
+      for (int j = 0; j < 16; ++j) acc[mb][j] = 0.f;
+  };
+
+  auto compute = [&](const Cursor& c, const uint16_t* sk, const uint16_t* sv) __attribute__((always_inline)) {
+    const int t0 = c.j * STEP + 32 * kw, left = c.len - t0;  // the wave's tokens
+    if (left <= 0) return;
+    const int ln = fresh_lane(), n = ln & 31, hf = ln >> 5;
+    const int draft = t0 - (c.len - c.n);        // the first token's draft, below 0 in the context
+    const bool tail = draft + 32 * BLOCKS > 0;  // drafts among the tokens, or the last one in front of them
+    // ---- S = K Q^T: steps (16 dims, block), a ring of four fragments in flight ahead of the products
+    f32x16_t sc[BLOCKS];
+    __builtin_amdgcn_s_setprio(1);
+#pragma unroll
+    for (int mb = 0; mb < BLOCKS; ++mb)
+#pragma unroll
+      for (int j = 0; j < 16; ++j) sc[mb][j] = 0.f;
+    {
+      auto frag = [&](int st) __attribute__((always_inline)) {
+        const int ks = st / BLOCKS, mb = st % BLOCKS;
+        return *reinterpret_cast<const uint4*>(sk + ((32 * (kw + mb) + n) * kDim + 8 * ((2 * ks + hf) ^ (n & 15))));
+      };
+      uint4 ka[4];
+#pragma unroll
+      for (int st = 0; st < 4; ++st) ka[st] = frag(st);
+#pragma unroll
+      for (int st = 0; st < 8 * BLOCKS; ++st) {
+        sc[st % BLOCKS] = mfma32(ka[st & 3], q[st / BLOCKS], sc[st % BLOCKS]);
+        if (st + 4 < 8 * BLOCKS) ka[st & 3] = frag(st + 4);
+      }
+      __builtin_amdgcn_sched_group_barrier(0x100, 4, 0);
+#pragma unroll
+      for (int st = 0; st < 8 * BLOCKS - 4; ++st) {
+        __builtin_amdgcn_sched_group_barrier(0x008, 1, 0);
+        __builtin_amdgcn_sched_group_barrier(0x100, 1, 0);
+      }
+      __builtin_amdgcn_sched_group_barrier(0x008, 4, 0);
+    }
+    __builtin_amdgcn_s_setprio(0);
+    if (tail) {
+#pragma unroll
+      for (int mb = 0; mb < BLOCKS; ++mb)
+#pragma unroll
+        for (int j = 0; j < 16; ++j) {
+          const int d = draft + 32 * mb + 8 * (j >> 2) + 4 * hf + (j & 3);
+          sc[mb][j] = sees(seen, d) ? sc[mb][j] : -INFINITY;
+        }
+    }
+    // ---- weights.  A row's maximum is taken of the first step, and again only where the weights of a
+    // step sum up to more than 2^16: their relative precision does not depend on it.
+    auto step_max = [&]() __attribute__((always_inline)) {
+      float mx = kMaxFloor;
+#pragma unroll
+      for (int mb = 0; mb < BLOCKS; ++mb)
+#pragma unroll
+        for (int j = 0; j < 16; ++j) mx = fmaxf(mx, sc[mb][j]);
+      return half_swap_max(mx) * p.scale_log2;
+    };
+    if (fresh) m = fmaxf(step_max(), kMaxFloor);
+    fresh = false;
+    float sum;
+    u32 pk[BLOCKS][8];  // packed pairs
+    auto weigh = [&]() __attribute__((always_inline)) {
+      sum = 0.f;
+#pragma unroll
+      for (int mb = 0; mb < BLOCKS; ++mb)
+#pragma unroll
+        for (int j = 0; j < 16; j += 2) {
+          const float w0 = fast_exp2(fmaf(sc[mb][j], p.scale_log2, -m));
+          const float w1 = fast_exp2(fmaf(sc[mb][j + 1], p.scale_log2, -m));
+          sum += w0 + w1;
+          pk[mb][j >> 1] = pack_bf16x2(w0, w1);
+        }
+      sum = half_swap_sum(sum);
+    };
+    weigh();
+    if (__any(!(sum <= kSumLimit))) {  // rare
+      const float m_new = fmaxf(m, step_max());
+      const float alpha = fast_exp2(m - m_new);
+      m = m_new;
+      l *= alpha;
+#pragma unroll
+      for (int mb = 0; mb < 4; ++mb)
+#pragma unroll
+        for (int j = 0; j < 16; ++j) acc[mb][j] *= alpha;
+      weigh();
+    }
+    l += sum;
+    // ---- O^T += V^T P^T, 16 tokens at a time
+    auto pf = [&](int kk) __attribute__((always_inline)) {
+      const u32* w = &pk[kk >> 1][4 * (kk & 1)];
+      return make_uint4(w[0], w[1], w[2], w[3]);
+    };
+    // V^T operand (see lds_read_tr16's use in the prefill): the lane addresses token 4 hf + (l % 16) / 4 of 16 at
+    // dims 16 ((l / 16) % 2) + 4 (l % 4) of 32, and gets dim l % 32 of tokens 4 hf + e.
+    const int tr_tok = 4 * hf + ((ln & 15) >> 2);
+    const int tr_chunk = 2 * ((ln >> 4) & 1) + ((ln & 3) >> 1), tr_sub = 4 * (ln & 1);
+    int v_at[4];
+#pragma unroll
+    for (int mb = 0; mb < 4; ++mb) {
+      v_at[mb] = (32 * kw + tr_tok) * kDim + 8 * ((4 * mb + tr_chunk) ^ (4 * (tr_tok & 3))) + tr_sub;
+      // The compiler is not to take the sum apart: behind several additions it no longer knows the array, and
+      // would wait for the next tile in front of the read.
+      asm volatile("" : "+v"(v_at[mb]));
+    }
+    auto read_v = [&](int kk, uint4 (&dst)[4]) __attribute__((always_inline)) {
+#pragma unroll
+      for (int mb = 0; mb < 4; ++mb) {
+        const uint2 lo = lds_read_tr16(sv + (v_at[mb] + 16 * kk * kDim));
+        const uint2 hi = lds_read_tr16(sv + (v_at[mb] + (16 * kk + 8) * kDim));
+        dst[mb] = make_uint4(lo.x, lo.y, hi.x, hi.y);
+      }
+    };
+    if (!tail) {
+      __builtin_amdgcn_s_setprio(1);
+      uint4 vf[2][4];
+      read_v(0, vf[0]);
+#pragma unroll
+      for (int kk = 0; kk < 2 * BLOCKS; ++kk) {
+        if (kk + 1 < 2 * BLOCKS) read_v(kk + 1, vf[(kk + 1) & 1]);
+#pragma unroll
+        for (int mb = 0; mb < 4; ++mb) acc[mb] = mfma32(vf[kk & 1][mb], pf(kk), acc[mb]);
+      }
+      __builtin_amdgcn_sched_group_barrier(0x100, 8, 0);
+#pragma unroll
+      for (int i = 0; i < 4 * (2 * BLOCKS - 1); ++i) {
+        __builtin_amdgcn_sched_group_barrier(0x100, 2, 0);
+        __builtin_amdgcn_sched_group_barrier(0x008, 1, 0);
+      }
+      __builtin_amdgcn_sched_group_barrier(0x008, 4, 0);
+      __builtin_amdgcn_s_setprio(0);
+    } else {
+      // As in Rows::clean: tokens behind the last one are cleared, drafts that are not finite added apart.
+      // Element e of the lane is token 4 hf + e, or 4 + 4 hf + e for e >= 4, of the 16.
+#pragma unroll
+      for (int kk = 0; kk < 2 * BLOCKS; ++kk) {
+        if (16 * kk >= left) break;
+        uint4 vr[4];
+        read_v(kk, vr);
+        u32x4_t vt[4], fine;
+        u32 odd = 0;
+#pragma unroll
+        for (int mb = 0; mb < 4; ++mb) vt[mb] = __builtin_bit_cast(u32x4_t, vr[mb]);
+#pragma unroll
+        for (int w = 0; w < 4; ++w) {
+          const int t = 16 * kk + 4 * hf + 8 * (w >> 1) + 2 * (w & 1);
+          fine[w] = (t < left ? 0xffffu : 0u) | (t + 1 < left ? 0xffff0000u : 0u);
+#pragma unroll
+          for (int mb = 0; mb < 4; ++mb) {
+            const u32 v = vt[mb][w] & fine[w];
+            odd |= ((v & 0x7f80u) == 0x7f80u ? 1u : 0u) << (2 * w);
+            odd |= ((v & 0x7f800000u) == 0x7f800000u ? 2u : 0u) << (2 * w);
+          }
+        }
+        if (__any(odd != 0)) {
+#pragma unroll 1
+          for (int i = 0; i < 16; ++i) {  // element e = i % 8 of the lanes of half i / 8
+            const int e = i & 7, g = i >> 3;
+            if (!__any(hf == g && (odd >> e & 1))) continue;
+            const u32 half = hf == g ? (e & 1 ? 0xffff0000u : 0xffffu) : 0u;
+            u32x4_t only;
+#pragma unroll
+            for (int w = 0; w < 4; ++w) {
+              only[w] = w == e >> 1 ? half : 0u;
+              fine[w] &= ~only[w];
+            }
+            const int d = draft + 16 * kk + 4 * g + (e & 3) + 8 * (e >> 2);
+            const bool mine = sees(seen, d);
+#pragma unroll
+            for (int mb = 0; mb < 4; ++mb) {
+              const f32x16_t with = mfma32(__builtin_bit_cast(uint4, vt[mb] & only), pf(kk), acc[mb]);
+#pragma unroll
+              for (int j = 0; j < 16; ++j) acc[mb][j] = mine ? with[j] : acc[mb][j];
+            }
+          }
+        }
+#pragma unroll
+        for (int mb = 0; mb < 4; ++mb) acc[mb] = mfma32(__builtin_bit_cast(uint4, vt[mb] & fine), pf(kk), acc[mb]);
+      }
+    }
+  };
+
+  // The rows' output where the range held all of the sequence, otherwise a partial state at `place`.
+  auto emit = [&](const Cursor& c, bool whole, int place) __attribute__((always_inline)) {
+    const float sum = c.bad ? NAN : l;
+    const int ln = fresh_lane(), hf = ln >> 5, row = first_row + (ln & 31), tok = token_of(row);
+    const int head = r.kvh * p.group + row - tok * p.group;
+    if (tok >= c.n) return;
+    if (whole) {
+      const float inv = sum == 0.f ? 0.f : 1.f / sum;
+      uint16_t* out = p.out + (c.q0 + tok) * p.o_tok_stride + head * p.o_head_stride + 4 * hf;
+#pragma unroll
+      for (int mb = 0; mb < 4; ++mb)
+#pragma unroll
+        for (int j = 0; j < 16; j += 4)
+          *reinterpret_cast<u32x2_t*>(out + 32 * mb + 2 * j) =
+              u32x2_t{pack_bf16x2(acc[mb][j] * inv, acc[mb][j + 1] * inv), pack_bf16x2(acc[mb][j + 2] * inv, acc[mb][j + 3] * inv)};
+    } else {
+      const int64_t at = (static_cast<int64_t>(place) * p.num_kv_heads + r.kvh) * p.rows + row;
+      float* part = p.part_o + at * kDim + 4 * hf;
+#pragma unroll
+      for (int mb = 0; mb < 4; ++mb)
+#pragma unroll
+        for (int j = 0; j < 16; j += 4)
+          *reinterpret_cast<float4*>(part + 32 * mb + 2 * j) =
+              make_float4(acc[mb][j], acc[mb][j + 1], acc[mb][j + 2], acc[mb][j + 3]);
+      if (hf == 0) *reinterpret_cast<float2*>(p.part_ml + 2 * at) = make_float2(m, sum);
+    }
+  };
+  // KW = 2: wave w takes over the state of wave w + 2, by way of a tile that is done with.
+  auto join = [&](uint16_t* sk, uint16_t* sv) __attribute__((always_inline)) {
+    float* const area = reinterpret_cast<float*>(rw == 0 ? sk : sv) + lane;
+    tile_barrier();  // the tile is done with
+    if (kw == 1) {
+#pragma unroll
+      for (int mb = 0; mb < 4; ++mb)
+#pragma unroll
+        for (int j = 0; j < 16; ++j) area[64 * (16 * mb + j)] = acc[mb][j];
+      s_ml[rw][lane] = make_float2(m, l);
+    }
+    tile_barrier();
+    if (kw == 0) {
+      const float2 o = s_ml[rw][lane];
+      const float m_new = fmaxf(m, o.x), a = fast_exp2(m - m_new), w = fast_exp2(o.x - m_new);
+      m = m_new;
+      l = l * a + o.y * w;
+#pragma unroll
+      for (int mb = 0; mb < 4; ++mb)
+#pragma unroll
+        for (int j = 0; j < 16; ++j) acc[mb][j] = acc[mb][j] * a + area[64 * (16 * mb + j)] * w;
+    }
+  };
+
+  // One step: its place c0, the one behind it c1 and (FP8) c2.
+  Cursor c0{}, c1{}, c2{};
+  auto take = [&](int S, uint16_t* sk, uint16_t* sv) __attribute__((always_inline)) {
+    const bool active = c0.n * p.group > first_row;
+    if (active && (S == r.S0 || c0.j == 0)) start(c0);
+    if (active) compute(c0, sk, sv);
+    if (c0.j + 1 == c0.nsteps || S + 1 == r.S1) {
+      const int from = S - c0.j, to = from + c0.nsteps;  // the sequence's steps
+      if (KW == 2) join(sk, sv);
+      if (active && kw == 0) emit(c0, from >= r.S0 && to <= r.S1, 2 * r.index + (from > r.S0 ? 1 : 0));
+    }
+  };
+  start_seq<STEP>(p, c0, r.first, r.S0 - uniform(s_cum[r.first]));
+  if constexpr (FP8) {
+    issue(c0, s_raw[0], s_raw[0] + kTile, s_raw[0] + 2 * kTile);
+    if (r.S0 + 1 < r.S1) {
+      next_step<STEP>(p, s_cum, c0, c1);
+      issue(c1, s_raw[FP8 ? 1 : 0], s_raw[FP8 ? 1 : 0] + kTile, s_raw[FP8 ? 1 : 0] + 2 * kTile);
+    }
+#pragma unroll 1
+    for (int S = r.S0; S < r.S1; ++S) {
+      const int buf = (S - r.S0) & 1;
+      if (S + 2 < r.S1) next_step<STEP>(p, s_cum, c1, c2);
+      if (S + 1 < r.S1) wait_vmem<kOps>();  // the next step's loads stay in flight
+      else wait_vmem<0>();
+      tile_barrier();  // all waves are done with the tile
+      widen(buf);
+      tile_barrier();
+      if (S + 2 < r.S1) issue(c2, s_raw[buf], s_raw[buf] + kTile, s_raw[buf] + 2 * kTile);
+      take(S, s_k0, s_v0);
+      c0 = c1;
+      c1 = c2;
+    }
+  } else {
+    issue(c0, reinterpret_cast<char*>(s_k0), reinterpret_cast<char*>(s_v0), nullptr);
+    auto step = [&](int S, uint16_t* sk, uint16_t* sv, uint16_t* nk, uint16_t* nv) __attribute__((always_inline)) {
+      const bool more = S + 1 < r.S1;
+      if (more) next_step<STEP>(p, s_cum, c0, c1);
+      wait_vmem<0>();   // the wave's part of the tile
+      __syncthreads();  // the others', and they are done with the tile before.  (The compiler has to see a fence:
+                        // it would wait for the next tile in front of the first read of this one.)
+      if (more) issue(c1, reinterpret_cast<char*>(nk), reinterpret_cast<char*>(nv), nullptr);
+      take(S, sk, sv);
+      c0 = c1;
+    };
+#pragma unroll 1
+    for (int S = r.S0; S < r.S1; S += 2) {
+      step(S, s_k0, s_v0, s_k1, s_v1);
+      if (S + 1 < r.S1) step(S + 1, s_k1, s_v1, s_k0, s_v0);
+    }
+  }
+}
+
 // Joins the states of sequences that several ranges share: one wave for a query token and head.
-// The wave's four 16-lane rows take the sequence's ranges round robin, 8 dims to a lane.
+// The wave's four 16-lane rows take the sequence's ranges round robin, 8 dims to a lane, four of
+// each per round trip.
 __global__ __launch_bounds__(kThreads) void tree_merge_kernel(const TreeParams p) {
-  const int row = blockIdx.x * kWaves + __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);  // token and q head
+  const int row = blockIdx.x * kWaves + uniform(static_cast<int>(threadIdx.x >> 6));  // token and q head
   const int b = blockIdx.y;
   const int cb = load_uniform(p.header, kHeaderInts + b), cb1 = load_uniform(p.header, kHeaderInts + b + 1);
   const int spr = load_uniform(p.header, 0);
-  if (cb1 <= cb) return;  // no steps
+  const SeqShape s = load_shape(p, b);
+  if (cb1 <= cb || row >= s.n * p.num_q_heads) return;  // no steps, or rows
   const int first = cb / spr, np = (cb1 - 1) / spr - first + 1;
   if (np <= 1) return;  // written already
-  const SeqShape s = load_shape(p, b);
-  if (row >= s.n * p.num_q_heads) return;
   const int tok = row / p.num_q_heads, h = row - tok * p.num_q_heads;
-  const int kvh = div_by(h, p.div_group), g = h - kvh * p.group;
+  const int kvh = div_by(h, p.div_group), r = tok * p.group + h - kvh * p.group;  // row of the kv head
   const int r4 = (threadIdx.x >> 4) & 3, d = 8 * (threadIdx.x & 15);
   float m = kMaxFloor, l = 0.f, o[8] = {};
 #pragma unroll 1
-  for (int k = r4; k < np; k += 4) {
-    const int place = 2 * (first + k) + (k == 0 && cb > first * spr ? 1 : 0);
-    const int64_t at = (static_cast<int64_t>(place) * p.num_kv_heads + kvh) * p.max_rows + tok * p.group + g;
-    const float2 st = *reinterpret_cast<const float2*>(p.part_ml + 2 * at);
-    const float4 x = *reinterpret_cast<const float4*>(p.part_o + at * kDim + d);
-    const float4 y = *reinterpret_cast<const float4*>(p.part_o + at * kDim + d + 4);
-    const float m_new = fmaxf(m, st.x), alpha = fast_exp2(m - m_new), w = fast_exp2(st.x - m_new);
-    const float v[8] = {x.x, x.y, x.z, x.w, y.x, y.y, y.z, y.w};
-    m = m_new;
-    l = l * alpha + w * st.y;
+  for (int k0 = r4; k0 - r4 < np; k0 += 16) {
+    float2 st[4];
+    float4 x[4], y[4];
 #pragma unroll
-    for (int j = 0; j < 8; ++j) o[j] = o[j] * alpha + w * v[j];
+    for (int u = 0; u < 4; ++u) {
+      const int k = min(k0 + 4 * u, np - 1);
+      const int place = 2 * (first + k) + (k == 0 && cb > first * spr ? 1 : 0);
+      const int64_t at = (static_cast<int64_t>(place) * p.num_kv_heads + kvh) * p.rows + r;
+      st[u] = *reinterpret_cast<const float2*>(p.part_ml + 2 * at);
+      x[u] = *reinterpret_cast<const float4*>(p.part_o + at * kDim + d);
+      y[u] = *reinterpret_cast<const float4*>(p.part_o + at * kDim + d + 4);
+    }
+#pragma unroll
+    for (int u = 0; u < 4; ++u) {
+      if (k0 + 4 * u >= np) break;
+      const float m_new = fmaxf(m, st[u].x), alpha = fast_exp2(m - m_new), w = fast_exp2(st[u].x - m_new);
+      const float v[8] = {x[u].x, x[u].y, x[u].z, x[u].w, y[u].x, y[u].y, y[u].z, y[u].w};
+      m = m_new;
+      l = l * alpha + w * st[u].y;
+#pragma unroll
+      for (int j = 0; j < 8; ++j) o[j] = o[j] * alpha + w * v[j];
+    }
   }
   const float mm = xor32_max(xor16_max(m));
   const float w = fast_exp2(m - mm);
@@ -643,33 +1107,28 @@ __global__ __launch_bounds__(kThreads) void tree_merge_kernel(const TreeParams p
   if (r4 == 0) *reinterpret_cast<uint4*>(p.out + (s.q0 + tok) * p.o_tok_stride + h * p.o_head_stride + d) = pack8(o);
 }
 
-// Rows of a kv head are taken 16 at a time where they are no more, otherwise 32.
-int row_tiles(int rows) { return rows <= 16 ? 1 : 2; }
-
-// How a batch is cut: the same for the workspace's size and for the launch.
+// How a batch is cut: by its rows per kv head, and into as many ranges as the GPU holds at once.
 struct Plan {
-  int nt, row_groups, streams, ranges;
-  int64_t places() const { return 2ll * ranges; }
+  int waves;   // of 32 rows side by side; 0: tree_few_kernel
+  int blocks;  // of rows
+  int ranges, seqs;  // seqs: per launch
+  int rows() const { return waves ? blocks * 32 * waves : 16; }
+  int64_t bytes(int hkv) const { return kHeaderBytes + 2ll * ranges * hkv * rows() * (kDim + 2) * 4; }
 };
-Plan plan_of(int64_t seqs, int max_q, int hq, int hkv, int64_t max_tokens_per_seq, int step, int workgroups) {
-  Plan pl{};
-  const int rows = max_q * (hq / hkv);
-  pl.nt = row_tiles(rows);
-  pl.row_groups = (rows + 16 * pl.nt - 1) / (16 * pl.nt);
-  pl.streams = hkv * pl.row_groups;
-  const int64_t steps = seqs * ((max_tokens_per_seq + step - 1) / step);
-  pl.ranges = static_cast<int>(
-      std::max<int64_t>(1, std::min<int64_t>(static_cast<int64_t>(workgroups) * kWaves / pl.streams, steps)));
-  return pl;
+void set_rows(Plan& pl, int rows) {
+  pl.waves = rows <= 16 ? 0 : rows <= 64 ? 2 : 4;
+  pl.blocks = pl.waves ? (rows + 32 * pl.waves - 1) / (32 * pl.waves) : 1;
 }
-int64_t workspace_of(const Plan& pl) {
-  return kHeaderBytes + pl.places() * pl.streams * 16 * pl.nt * (kDim + 2) * 4;
+// units: waves of tree_few_kernel, or workgroups of tree_many_kernel, that are resident at once.
+void set_ranges(Plan& pl, int64_t seqs, int hkv, int64_t max_tokens, int step, int units) {
+  const int64_t steps = (max_tokens + step - 1) / step;  // of a sequence
+  pl.seqs = static_cast<int>(std::min<int64_t>(std::min<int64_t>(seqs, kSeqsPerLaunch), (1ll << 30) / steps));
+  pl.ranges = static_cast<int>(std::max<int64_t>(1, std::min<int64_t>(units / (hkv * pl.blocks), pl.seqs * steps)));
 }
 
-// Workgroups of the kernel resident on the current device at once.
-template <bool FP8, int NT>
-int resident() {
-  static std::atomic<int> cached[16];
+// Workgroups of a kernel resident on the current device at once.
+template <typename K>
+int resident(K kernel, std::atomic<int> (&cached)[16]) {
   int dev = 0;
   if (hipGetDevice(&dev) != hipSuccess || dev < 0 || dev >= 16) dev = 0;
   int v = cached[dev].load(std::memory_order_relaxed);
@@ -677,12 +1136,11 @@ int resident() {
   int cus = 0, per_cu = 0;
   bool ok = hipDeviceGetAttribute(&cus, hipDeviceAttributeMultiprocessorCount, dev) == hipSuccess && cus > 0;
   if (!ok) cus = 256;
-  if (hipOccupancyMaxActiveBlocksPerMultiprocessor(&per_cu, tree_attention_kernel<FP8, NT>, kThreads, 0) != hipSuccess ||
-      per_cu <= 0) {
+  if (hipOccupancyMaxActiveBlocksPerMultiprocessor(&per_cu, kernel, kThreads, 0) != hipSuccess || per_cu <= 0) {
     per_cu = 1;
     ok = false;
   }
-  v = std::min(cus * per_cu, kMaxWorkgroups);
+  v = cus * per_cu;
   if (ok) cached[dev].store(v, std::memory_order_relaxed);
   return v;
 }
@@ -763,13 +1221,18 @@ int check_args(const char* fn, const TreeArgs& a) {
   return KVP_OK;
 }
 
-template <bool FP8, int NT>
+template <bool FP8>
 int launch(const char* fn, const TreeArgs& a, hipStream_t stream) {
-  const int most = std::min(a.num_seqs, kSeqsPerLaunch);
+  static std::atomic<int> cached[3][16];
   const int64_t tokens = static_cast<int64_t>(a.max_blocks) * a.block_size;
-  const Plan pl = plan_of(most, a.max_q, a.num_q_heads, a.num_kv_heads, tokens, Format<FP8>::kStep,
-                          resident<FP8, NT>());
-  const size_t need = static_cast<size_t>(workspace_of(pl));
+  Plan pl{};
+  set_rows(pl, a.max_q * (a.num_q_heads / a.num_kv_heads));
+  const int wgs = pl.waves == 0   ? resident(tree_few_kernel<FP8>, cached[0])
+                  : pl.waves == 2 ? resident(tree_many_kernel<FP8, 2>, cached[1])
+                                  : resident(tree_many_kernel<FP8, 1>, cached[2]);
+  const int units = pl.waves == 0 ? std::min(wgs * kWaves, kMaxFew) : std::min(wgs, kMaxMany);
+  set_ranges(pl, a.num_seqs, a.num_kv_heads, tokens, pl.waves ? kManyStep : Format<FP8>::kStep, units);
+  const size_t need = static_cast<size_t>(pl.bytes(a.num_kv_heads));
   if (!a.workspace || a.workspace_bytes < need)
     return fail(KVP_EWORKSPACE, "%s: workspace of %zu bytes, %zu needed", fn, a.workspace_bytes, need);
   const int64_t size = FP8 ? 1 : 2;
@@ -795,25 +1258,27 @@ int launch(const char* fn, const TreeArgs& a, hipStream_t stream) {
   p.num_kv_heads = a.num_kv_heads;
   p.group = a.num_q_heads / a.num_kv_heads;
   p.mask = a.mask;
-  p.scale_log2 = a.softmax_scale * 1.4426950408889634f;
+  p.scale_log2 = fabsf(a.softmax_scale) * 1.4426950408889634f;  // its sign goes into q
+  p.q_flip = a.softmax_scale < 0.f ? 0x80008000u : 0u;
   p.o_tok_stride = a.o_tok_stride;
   p.o_head_stride = a.o_head_stride;
-  p.streams = pl.streams;
   p.ranges = pl.ranges;
-  p.row_groups = pl.row_groups;
-  p.max_rows = pl.row_groups * 16 * pl.nt;
-  p.div_streams = divisor(pl.streams);
-  p.div_row_groups = divisor(pl.row_groups);
+  p.blocks = pl.blocks;
+  p.streams = a.num_kv_heads * pl.blocks;
+  p.rows = pl.rows();
+  p.div_streams = divisor(p.streams);
+  p.div_blocks = divisor(pl.blocks);
   p.div_ranges = divisor(pl.ranges);
   p.div_block = divisor(a.block_size);
   p.div_group = divisor(p.group);
   char* ws = static_cast<char*>(a.workspace);
   p.header = reinterpret_cast<int32_t*>(ws);
   p.part_o = reinterpret_cast<float*>(ws + kHeaderBytes);
-  p.part_ml = p.part_o + pl.places() * a.num_kv_heads * p.max_rows * kDim;
-  const unsigned grid = static_cast<unsigned>((static_cast<int64_t>(pl.ranges) * pl.streams + kWaves - 1) / kWaves);
-  for (int b0 = 0; b0 < a.num_seqs; b0 += kSeqsPerLaunch) {
-    p.num_seqs = std::min(kSeqsPerLaunch, a.num_seqs - b0);
+  p.part_ml = p.part_o + 2ll * pl.ranges * a.num_kv_heads * p.rows * kDim;
+  const int n = pl.ranges * p.streams;
+  const dim3 grid(static_cast<unsigned>(pl.waves ? (n + 7) / 8 * 8 : (n + kWaves - 1) / kWaves)), block(kThreads);
+  for (int b0 = 0; b0 < a.num_seqs; b0 += pl.seqs) {
+    p.num_seqs = std::min(pl.seqs, a.num_seqs - b0);
     p.block_tables = a.block_tables + b0 * a.bt_stride;
     p.kv_lens = a.kv_lens + b0;
     p.cu_q = a.cu_q ? a.cu_q + b0 : nullptr;
@@ -821,10 +1286,12 @@ int launch(const char* fn, const TreeArgs& a, hipStream_t stream) {
     p.q = static_cast<const uint16_t*>(a.q) + row0 * a.q_tok_stride;
     p.out = static_cast<uint16_t*>(a.out) + row0 * a.o_tok_stride;
     p.total_q = a.cu_q ? a.total_q : p.num_seqs;
-    hipLaunchKernelGGL((tree_attention_kernel<FP8, NT>), dim3(grid), dim3(kThreads), 0, stream, p);
+    if (pl.waves == 0) hipLaunchKernelGGL(tree_few_kernel<FP8>, grid, block, 0, stream, p);
+    else if (pl.waves == 2) hipLaunchKernelGGL((tree_many_kernel<FP8, 2>), grid, block, 0, stream, p);
+    else hipLaunchKernelGGL((tree_many_kernel<FP8, 1>), grid, block, 0, stream, p);
     if (pl.ranges > 1)
-      hipLaunchKernelGGL(tree_merge_kernel, dim3((a.max_q * a.num_q_heads + kWaves - 1) / kWaves, p.num_seqs),
-                         dim3(kThreads), 0, stream, p);
+      hipLaunchKernelGGL(tree_merge_kernel, dim3((a.max_q * a.num_q_heads + kWaves - 1) / kWaves, p.num_seqs), block, 0,
+                         stream, p);
     const int rc = launch_status(fn);
     if (rc != KVP_OK) return rc;
   }
@@ -837,9 +1304,7 @@ int enqueue(const char* fn, const TreeArgs& a, void* stream) {
   if (reinterpret_cast<uintptr_t>(a.workspace) & 255u)
     return fail(KVP_EINVAL, "%s: workspace must be 256-byte aligned", fn);
   const auto s = static_cast<hipStream_t>(stream);
-  const bool one = row_tiles(a.max_q * (a.num_q_heads / a.num_kv_heads)) == 1;
-  if (a.fp8) return one ? launch<true, 1>(fn, a, s) : launch<true, 2>(fn, a, s);
-  return one ? launch<false, 1>(fn, a, s) : launch<false, 2>(fn, a, s);
+  return a.fp8 ? launch<true>(fn, a, s) : launch<false>(fn, a, s);
 }
 
 }  // namespace
@@ -853,13 +1318,20 @@ extern "C" size_t kvp_tree_workspace_bytes(int32_t max_num_seqs, int32_t max_seq
   if (max_num_seqs <= 0 ||
       check_shape("", max_seqlen_q, num_q_heads, num_kv_heads, head_dim, block_size, max_blocks_per_seq) != KVP_OK)
     return 0;
-  // ranges x streams of any launch within these sizes, on any device; it grows with each of them
-  Plan pl = plan_of(1, max_seqlen_q, num_q_heads, num_kv_heads, 1, 1, 0);
-  const int64_t steps = static_cast<int64_t>(std::min(max_num_seqs, kSeqsPerLaunch)) *
-                        ((static_cast<int64_t>(max_blocks_per_seq) * block_size + 31) / 32);
-  pl.streams = static_cast<int>(std::min<int64_t>(std::max(kMaxWorkgroups * kWaves, pl.streams), steps * pl.streams));
-  pl.ranges = 1;
-  return static_cast<size_t>(workspace_of(pl));
+  // The most that any launch within these sizes needs, on any device, be its rows few or many: a
+  // launch has as many (range, stream) pairs as units at most, or one range, and no more than steps.
+  const int rows = max_seqlen_q * (num_q_heads / num_kv_heads);
+  const int64_t tokens = static_cast<int64_t>(max_blocks_per_seq) * block_size;
+  int64_t most = 0;
+  for (const int some : {std::min(rows, 16), std::min(rows, 64), rows}) {
+    Plan pl{};
+    set_rows(pl, some);
+    const int step = pl.waves ? kManyStep : Format<false>::kStep;
+    const int64_t streams = num_kv_heads * pl.blocks, steps = max_num_seqs * ((tokens + step - 1) / step);
+    const int64_t pairs = std::min(std::max<int64_t>(pl.waves ? kMaxMany : kMaxFew, streams), steps * streams);
+    most = std::max(most, kHeaderBytes + 2 * pairs * (pl.waves ? 32 * pl.waves : 16) * (kDim + 2) * 4);
+  }
+  return static_cast<size_t>(most);
 }
 
 extern "C" int kvp_paged_decode_fp8(const void* q, int64_t q_seq_stride, int64_t q_head_stride, const void* k_cache,

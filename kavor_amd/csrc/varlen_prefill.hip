@@ -36,7 +36,7 @@
 #include <algorithm>
 #include <atomic>
 
-#include "common.h"
+#include "paged.h"
 
 namespace kvp {
 
@@ -70,9 +70,6 @@ constexpr int kSplitInts = kSplitMergesInt + kUnitInts * kSplitTiles;
 constexpr int kPartFloats = kPrefillRows * (kPrefillHeadDim + 2);  // one partial state: O, then (max, sum) per row
 // A tile's row sum of P above this re-bases the running max (P itself stays <= 2^16).
 constexpr float kSpecSumLimit = 65536.f;
-
-typedef __bf16 bf16x8_t __attribute__((ext_vector_type(8)));
-typedef float f32x16_t __attribute__((ext_vector_type(16)));
 
 struct PrefillParams {
   const uint16_t* q;
@@ -465,32 +462,6 @@ __global__ __launch_bounds__(kPlanThreads) void prefill_split_plan_kernel(const 
     p.split[0] = units * p.num_kv_heads;
     p.split[1] = all_cuts;
   }
-}
-
-typedef short s16x4_t __attribute__((ext_vector_type(4)));
-
-// ds_read_b64_tr_b16: 8 bytes per lane, transposed as 16-bit elements across each
-// 16-lane group (see the V^T operand in the kernel).
-__device__ __forceinline__ uint2 lds_read_tr16(const uint16_t* lds_ptr) {
-  const s16x4_t v = __builtin_amdgcn_ds_read_tr16_b64_v4i16(
-      (__attribute__((address_space(3))) s16x4_t*)(lds_ptr));
-  return __builtin_bit_cast(uint2, v);
-}
-
-// Max / sum of x over lanes l and l ^ 32 (v_permlane32_swap_b32 exchanges the wave halves:
-// the first result holds lanes 0-31 in both halves, the second lanes 32-63).
-__device__ __forceinline__ float half_swap_max(float x) {
-  const auto r = __builtin_amdgcn_permlane32_swap(__float_as_uint(x), __float_as_uint(x), false, false);
-  return fmaxf(__uint_as_float(r[0]), __uint_as_float(r[1]));
-}
-__device__ __forceinline__ float half_swap_sum(float x) {
-  const auto r = __builtin_amdgcn_permlane32_swap(__float_as_uint(x), __float_as_uint(x), false, false);
-  return __uint_as_float(r[0]) + __uint_as_float(r[1]);
-}
-
-__device__ __forceinline__ f32x16_t mfma32(uint4 a, uint4 b, f32x16_t c) {
-  return __builtin_amdgcn_mfma_f32_32x32x16_bf16(__builtin_bit_cast(bf16x8_t, a),
-                                                 __builtin_bit_cast(bf16x8_t, b), c, 0, 0, 0);
 }
 
 // Writes one wave's 32 query rows: O (scaled by inv) through the LDS area `stg` of 32 rows.
