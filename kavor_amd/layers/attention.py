@@ -439,40 +439,61 @@ def _launch(fn: str, index: int, *args) -> None:
     check(fn, rc)
 
 
-def _require(name: str, t: torch.Tensor, dtype: torch.dtype, device: torch.device, dim: int) -> None:
-    """A tensor of `dim` dimensions on `device` whose last one is contiguous."""
-    if t.dtype != dtype or t.device != device or t.dim() != dim:
-        raise ValueError(f"{name} must be a {dim}-d {dtype} tensor on {device}, got {t.dim()}-d {t.dtype} on {t.device}")
-    if t.stride(-1) != 1 and t.shape[-1] > 1:
-        raise ValueError(f"{name} must be contiguous in its last dimension")
+_FP8 = torch.float8_e4m3fn
 
 
-def _quantised(k_cache, v_cache, k_scale, v_scale, device: torch.device):
+# Checks of small calls cost as much as their kernels: what is right passes in one expression, and only
+# what is not is looked at again for its message.
+
+def _is(t: torch.Tensor, dtype: torch.dtype, index: int, dim: int) -> bool:
+    """Whether t has these, with a contiguous last dimension."""
+    return t.dtype is dtype and t.get_device() == index and t.dim() == dim and (t.stride(-1) == 1 or t.shape[-1] <= 1)
+
+
+def _refuse(name: str, t: torch.Tensor, dtype: torch.dtype, dim: int, device: torch.device) -> None:
+    raise ValueError(f"{name} must be a {dim}-d {dtype} tensor on {device} whose last dimension is contiguous, got "
+                     f"{t.dim()}-d {t.dtype} on {t.device} with strides {tuple(t.stride())}")
+
+
+def _require(name: str, t: torch.Tensor, dtype: torch.dtype, like: torch.Tensor, dim: int) -> None:
+    if not _is(t, dtype, like.get_device(), dim):
+        _refuse(name, t, dtype, dim, like.device)
+
+
+def _paired(k: torch.Tensor, v: torch.Tensor, k_name: str, dtype: torch.dtype, like: torch.Tensor, dim: int):
+    """Shape and strides of a K tensor that its V tensor shares."""
+    shape, strides = k.shape, k.stride()
+    index = like.get_device()
+    if not (_is(k, dtype, index, dim) and _is(v, dtype, index, dim) and shape == v.shape and strides == v.stride()):
+        v_name = k_name.replace("k", "v", 1)
+        _require(k_name, k, dtype, like, dim)
+        _require(v_name, v, dtype, like, dim)
+        raise ValueError(f"{k_name} and {v_name} must share shape and strides")
+    return shape, strides
+
+
+def _quantised(k_cache, v_cache, k_scale, v_scale, like: torch.Tensor):
     """The shape of a quantised cache, and its pointers and strides as the library takes them."""
-    for name, t in (("k_cache", k_cache), ("v_cache", v_cache)):
-        _require(name, t, torch.float8_e4m3fn, device, 4)
-    for name, t in (("k_scale", k_scale), ("v_scale", v_scale)):
-        _require(name, t, torch.uint8, device, 3)
-    shape, cs, ss = k_cache.shape, k_cache.stride(), k_scale.stride()
-    if shape != v_cache.shape or cs != v_cache.stride():
-        raise ValueError("k_cache and v_cache must share shape and strides")
-    if k_scale.shape != v_scale.shape or ss != v_scale.stride():
-        raise ValueError("k_scale and v_scale must share shape and strides")
-    num_blocks, block_size, heads, _ = shape
-    if k_scale.shape != (num_blocks, heads, block_size):
+    shape, cs = _paired(k_cache, v_cache, "k_cache", _FP8, like, 4)
+    scales, ss = _paired(k_scale, v_scale, "k_scale", torch.uint8, like, 3)
+    if scales != (shape[0], shape[2], shape[1]):
         raise ValueError(f"the scales must be [num_blocks, num_kv_heads, block_size] = "
-                         f"{(num_blocks, heads, block_size)}, got {tuple(k_scale.shape)}")
+                         f"{(shape[0], shape[2], shape[1])}, got {tuple(scales)}")
     return shape, (k_cache.data_ptr(), v_cache.data_ptr(), cs[0], cs[1], cs[2],
                    k_scale.data_ptr(), v_scale.data_ptr(), ss[0], ss[1])
 
 
-def _table(block_table: torch.Tensor, rows: int, device: torch.device):
-    if block_table.dtype != torch.int32 or block_table.dim() != 2 or block_table.device != device \
-            or (block_table.stride(1) != 1 and block_table.shape[1] > 1):
-        raise ValueError(f"block_table must be an int32 [B, max_blocks] tensor on {device} with contiguous rows")
-    if block_table.shape[0] < rows:
+def _ints(name: str, t: torch.Tensor, like: torch.Tensor) -> None:
+    if not (t.dtype is torch.int32 and t.get_device() == like.get_device() and t.is_contiguous()):
+        _require_int32(name, t, like.device)
+
+
+def _table(block_table: torch.Tensor, rows: int, like: torch.Tensor):
+    if not _is(block_table, torch.int32, like.get_device(), 2):
+        _refuse("block_table", block_table, torch.int32, 2, like.device)
+    n, width = block_table.shape
+    if n < rows:
         raise ValueError("block_table has fewer rows than sequences")
-    width = block_table.shape[1]
     # a single row may have any stride
     return block_table.data_ptr(), max(block_table.stride(0), width), width
 
@@ -487,22 +508,24 @@ def store_kvcache_fp8(key: torch.Tensor, value: torch.Tensor, k_cache: torch.Ten
     [num_blocks, num_kv_heads, block_size] in uint8; byte e stands for 2^(e - 127), and value q of
     its row for 2^(e - 127) q.  Slots outside the cache, -1 among them, are skipped.  An infinity
     is stored as NaN."""
-    dev = key.device
-    _require_cuda_bf16("key", key)
-    _require("value", value, torch.bfloat16, dev, 3)
-    _require("key", key, torch.bfloat16, dev, 3)
-    if value.shape != key.shape:
+    index = key.get_device()
+    if not (index >= 0 and _is(key, torch.bfloat16, index, 3) and _is(value, torch.bfloat16, index, 3)):
+        _require_cuda_bf16("key", key)
+        _require("key", key, torch.bfloat16, key, 3)
+        _require("value", value, torch.bfloat16, key, 3)
+    (num_blocks, block_size, heads, dim), cache = _quantised(k_cache, v_cache, k_scale, v_scale, key)
+    shape, ks, vs = key.shape, key.stride(), value.stride()
+    N = shape[0]
+    if value.shape != shape:
         raise ValueError("key and value must share their shape")
-    (num_blocks, block_size, heads, dim), cache = _quantised(k_cache, v_cache, k_scale, v_scale, dev)
-    N = key.shape[0]
-    if key.shape[1:] != (heads, dim):
-        raise ValueError(f"key and value must be [N, {heads}, {dim}] as the caches, got {tuple(key.shape)}")
-    _require_int32("slot_mapping", slot_mapping, dev)
+    if shape[1] != heads or shape[2] != dim:
+        raise ValueError(f"key and value must be [N, {heads}, {dim}] as the caches, got {tuple(shape)}")
+    _ints("slot_mapping", slot_mapping, key)
     if slot_mapping.numel() != N:
         raise ValueError("slot_mapping must have one entry per token")
-    _launch("kvp_append_fp8", key.get_device(),
-            key.data_ptr(), key.stride(0), key.stride(1), value.data_ptr(), value.stride(0), value.stride(1),
-            *cache, num_blocks * block_size, slot_mapping.data_ptr(), N, heads, dim, block_size, _stream(key))
+    _launch("kvp_append_fp8", index, key.data_ptr(), ks[0], ks[1], value.data_ptr(), vs[0], vs[1], *cache,
+            num_blocks * block_size, slot_mapping.data_ptr(), N, heads, dim, block_size,
+            torch._C._cuda_getCurrentRawStream(index))
 
 
 def load_kvcache_fp8(k_cache: torch.Tensor, v_cache: torch.Tensor, k_scale: torch.Tensor, v_scale: torch.Tensor,
@@ -512,20 +535,19 @@ def load_kvcache_fp8(k_cache: torch.Tensor, v_cache: torch.Tensor, k_scale: torc
     [total_k, num_kv_heads, head_dim], which varlen_prefill takes as dense k / v: token j of
     sequence b is row cu_seqlens_k[b] + j.  total_k is the host's copy of cu_seqlens_k[-1]; rows
     of `out` that no sequence has are left as they were.  Tokens of invalid blocks are NaN."""
-    dev = k_cache.device
     if not k_cache.is_cuda:
-        raise ValueError(f"k_cache must be a CUDA (HIP) tensor, got device {dev}")
-    (num_blocks, block_size, heads, dim), cache = _quantised(k_cache, v_cache, k_scale, v_scale, dev)
-    _require_int32("cu_seqlens_k", cu_seqlens_k, dev)
+        raise ValueError(f"k_cache must be a CUDA (HIP) tensor, got device {k_cache.device}")
+    (num_blocks, block_size, heads, dim), cache = _quantised(k_cache, v_cache, k_scale, v_scale, k_cache)
+    _ints("cu_seqlens_k", cu_seqlens_k, k_cache)
     num_seqs, total_k = cu_seqlens_k.numel() - 1, int(total_k)
     if num_seqs < 0 or total_k < 0:
         raise ValueError("cu_seqlens_k must have an entry more than sequences, and total_k not be negative")
-    bt, bt_stride, width = _table(block_table, num_seqs, dev)
+    bt, bt_stride, width = _table(block_table, num_seqs, k_cache)
     if out is None:
-        out = tuple(torch.empty(total_k, heads, dim, dtype=torch.bfloat16, device=dev) for _ in range(2))
+        out = tuple(torch.empty((total_k, heads, dim), dtype=torch.bfloat16, device=k_cache.device) for _ in range(2))
     k, v = out
     for name, t in (("out[0]", k), ("out[1]", v)):
-        _require(name, t, torch.bfloat16, dev, 3)
+        _require(name, t, torch.bfloat16, k_cache, 3)
         if t.shape[0] < total_k or t.shape[1:] != (heads, dim):
             raise ValueError(f"{name} must be [{total_k} or more, {heads}, {dim}], got {tuple(t.shape)}")
     _launch("kvp_load_fp8", k_cache.get_device(),
@@ -564,17 +586,13 @@ def _tree_workspace(index, stream, *sizes) -> torch.Tensor:
 
 def _paged_shape(q, k_cache, v_cache, k_scale, v_scale):
     """Sizes of q [N, Hq, D] over a cache of either kind, and the cache's pointers and strides."""
-    _require_cuda_bf16("q", q)
-    dev = q.device
+    if not (q.is_cuda and q.dtype is torch.bfloat16):
+        _require_cuda_bf16("q", q)
     if k_scale is None:
-        for name, t in (("k_cache", k_cache), ("v_cache", v_cache)):
-            _require(name, t, torch.bfloat16, dev, 4)
-        cs = k_cache.stride()
-        if k_cache.shape != v_cache.shape or cs != v_cache.stride():
-            raise ValueError("k_cache and v_cache must share shape and strides")
-        shape, cache = k_cache.shape, (k_cache.data_ptr(), v_cache.data_ptr(), cs[0], cs[1], cs[2], 0, 0, 0, 0)
+        shape, cs = _paired(k_cache, v_cache, "k_cache", torch.bfloat16, q, 4)
+        cache = (k_cache.data_ptr(), v_cache.data_ptr(), cs[0], cs[1], cs[2], 0, 0, 0, 0)
     else:
-        shape, cache = _quantised(k_cache, v_cache, k_scale, v_scale, dev)
+        shape, cache = _quantised(k_cache, v_cache, k_scale, v_scale, q)
     if q.shape[2] != shape[3] or q.stride(2) != 1:
         raise ValueError("head_dim mismatch or non-contiguous head_dim")
     return shape, cache
@@ -583,7 +601,7 @@ def _paged_shape(q, k_cache, v_cache, k_scale, v_scale):
 def _like(q: torch.Tensor, out: torch.Tensor | None) -> torch.Tensor:
     """A bf16 output of q's shape, given or new."""
     if out is None:
-        return torch.empty(q.shape, dtype=torch.bfloat16, device=q.device)
+        return q.new_empty(q.shape)
     if out.shape != q.shape or out.dtype != torch.bfloat16 or out.device != q.device or out.stride(2) != 1:
         raise ValueError("out must be a bf16 tensor of q's shape on its device with contiguous head_dim")
     return out
@@ -603,15 +621,16 @@ def paged_decode_fp8(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tens
         raise ValueError(f"paged_decode_fp8 takes one query token per sequence, got q of shape {tuple(q.shape)}")
     (num_blocks, block_size, Hkv, D), cache = _paged_shape(q, k_cache, v_cache, k_scale, v_scale)
     B, Hq, _ = q.shape
-    _require_int32("cache_seqlens", cache_seqlens, q.device)
+    _ints("cache_seqlens", cache_seqlens, q)
     if cache_seqlens.numel() < B:
         raise ValueError("cache_seqlens has fewer rows than q")
-    bt, bt_stride, width = _table(block_table, B, q.device)
+    bt, bt_stride, width = _table(block_table, B, q)
     out, index, stream = _like(q, out), q.get_device(), _stream(q)
     ws = _tree_workspace(index, stream, B, 1, Hq, Hkv, D, width, block_size)
-    _launch("kvp_paged_decode_fp8", index, q.data_ptr(), q.stride(0), q.stride(1), *cache, num_blocks, bt, bt_stride,
-            cache_seqlens.data_ptr(), B, Hq, Hkv, D, block_size, width, float(softmax_scale), out.data_ptr(),
-            out.stride(0), out.stride(1), ws.data_ptr(), ws.numel(), stream)
+    qs, os = q.stride(), out.stride()
+    _launch("kvp_paged_decode_fp8", index, q.data_ptr(), qs[0], qs[1], *cache, num_blocks, bt, bt_stride,
+            cache_seqlens.data_ptr(), B, Hq, Hkv, D, block_size, width, softmax_scale, out.data_ptr(), os[0], os[1],
+            ws.data_ptr(), ws.numel(), stream)
     return out
 
 
@@ -635,23 +654,25 @@ def tree_attention(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor
         raise ValueError("k_scale and v_scale go together")
     (num_blocks, block_size, Hkv, D), cache = _paged_shape(q, k_cache, v_cache, k_scale, v_scale)
     T, Hq, _ = q.shape
-    _require_int32("cu_seqlens_q", cu_seqlens_q, q.device)
-    _require_int32("cache_seqlens", cache_seqlens, q.device)
+    _ints("cu_seqlens_q", cu_seqlens_q, q)
+    _ints("cache_seqlens", cache_seqlens, q)
     B, max_seqlen_q = cu_seqlens_q.numel() - 1, int(max_seqlen_q)
     if B < 0 or cache_seqlens.numel() < B:
         raise ValueError("cu_seqlens_q must have an entry more than sequences, and cache_seqlens one for each")
-    if tree_mask is not None and (tree_mask.dtype != torch.int64 or tree_mask.device != q.device
-                                  or not tree_mask.is_contiguous() or tree_mask.numel() != T):
+    index = q.get_device()
+    if tree_mask is not None and not (tree_mask.dtype is torch.int64 and tree_mask.get_device() == index
+                                      and tree_mask.is_contiguous() and tree_mask.numel() == T):
         raise ValueError("tree_mask must be a contiguous int64 tensor on q's device with one entry per row of q")
-    bt, bt_stride, width = _table(block_table, B, q.device)
-    out, index, stream = _like(q, out), q.get_device(), _stream(q)
+    bt, bt_stride, width = _table(block_table, B, q)
+    out, stream = _like(q, out), _stream(q)
     if B == 0 or T == 0:
         return out
     ws = _tree_workspace(index, stream, B, max_seqlen_q, Hq, Hkv, D, width, block_size)
-    _launch("kvp_tree_attention", index, q.data_ptr(), q.stride(0), q.stride(1), *cache, num_blocks, bt, bt_stride,
+    qs, os = q.stride(), out.stride()
+    _launch("kvp_tree_attention", index, q.data_ptr(), qs[0], qs[1], *cache, num_blocks, bt, bt_stride,
             cu_seqlens_q.data_ptr(), cache_seqlens.data_ptr(), B, T, max_seqlen_q,
             tree_mask.data_ptr() if tree_mask is not None else 0, Hq, Hkv, D, block_size, width,
-            float(softmax_scale), out.data_ptr(), out.stride(0), out.stride(1), ws.data_ptr(), ws.numel(), stream)
+            softmax_scale, out.data_ptr(), os[0], os[1], ws.data_ptr(), ws.numel(), stream)
     return out
 
 

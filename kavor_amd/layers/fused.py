@@ -268,27 +268,29 @@ def token_logprobs(logits: torch.Tensor, tokens: torch.Tensor, top: int = 0):
     among equal ones, NaN before all others.  Log probabilities and entropy of a row with a NaN or
     +inf, or of -inf alone, are NaN; a token outside the vocabulary has a NaN log probability and
     rank 0."""
-    if not logits.is_cuda or logits.dtype not in (torch.bfloat16, torch.float32) or logits.dim() != 2:
-        raise ValueError(f"logits must be a bf16 or fp32 [N, vocab] GPU tensor (got {logits.dtype} of shape "
+    index, dtype = logits.get_device(), logits.dtype
+    if index < 0 or (dtype is not torch.bfloat16 and dtype is not torch.float32) or logits.dim() != 2:
+        raise ValueError(f"logits must be a bf16 or fp32 [N, vocab] GPU tensor (got {dtype} of shape "
                          f"{tuple(logits.shape)} on {logits.device})")
     n, vocab = logits.shape
     if logits.stride(1) != 1 and vocab > 1:
         raise ValueError("logits must have a contiguous last dimension")
-    if tokens.dtype != torch.int64 or tokens.device != logits.device or not tokens.is_contiguous() \
-            or tokens.numel() != n:
+    if not (tokens.dtype is torch.int64 and tokens.get_device() == index and tokens.is_contiguous()
+            and tokens.numel() == n):
         raise ValueError("tokens must be a contiguous int64 tensor on the logits' device, one per row")
     top = int(top)
     if top < 0:
         raise ValueError(f"top must not be negative, got {top}")
-    dev, index, stream = logits.device, logits.get_device(), _stream(logits)
-    logprobs, entropy = torch.empty((2, n), dtype=torch.float32, device=dev)
-    rank = torch.empty(n, dtype=torch.int64, device=dev)
-    top_logprobs = torch.empty((n, top), dtype=torch.float32, device=dev)
-    top_tokens = torch.empty((n, top), dtype=torch.int64, device=dev)
+    stream = _stream(logits)
+    logprobs = logits.new_empty((n,), dtype=torch.float32)
+    entropy = logits.new_empty((n,), dtype=torch.float32)
+    rank = tokens.new_empty((n,))
+    top_logprobs = logits.new_empty((n, top), dtype=torch.float32)
+    top_tokens = tokens.new_empty((n, top))
     ws = _logprobs_pool.ready(index, stream, _LOGPROBS_WORKSPACE_BYTES)
     if ws is None:
         ws = reserve_logprobs_workspace(index)
-    args = (logits.data_ptr(), logits.dtype == torch.float32, logits.stride(0) if n > 1 else -(-vocab // 8) * 8, n,
+    args = (logits.data_ptr(), dtype is torch.float32, logits.stride(0) if n > 1 else -(-vocab // 8) * 8, n,
             vocab, tokens.data_ptr(), top, logprobs.data_ptr(), entropy.data_ptr(), rank.data_ptr(),
             top_logprobs.data_ptr(), top_tokens.data_ptr(), ws.data_ptr(), ws.numel(), stream)
     if torch._C._cuda_getDevice() == index:
