@@ -76,6 +76,14 @@ __device__ __forceinline__ float xor32_max(float x) {
   return fmaxf(__uint_as_float(r[0]), __uint_as_float(r[1]));
 }
 
+// max(a, b, c) in one instruction; a NaN loses against a number.  (fmaxf costs up to three: the compiler
+// quiets each operand that could be a signalling NaN first.)
+__device__ __forceinline__ float max3(float a, float b, float c) {
+  float r;
+  asm("v_max3_f32 %0, %1, %2, %3" : "=v"(r) : "v"(a), "v"(b), "v"(c));
+  return r;
+}
+
 __device__ __forceinline__ float fast_exp2(float x) { return __builtin_amdgcn_exp2f(x); }
 
 // Inclusive prefix sum over the 64 lanes of a wave (all lanes active): DPP right shifts by

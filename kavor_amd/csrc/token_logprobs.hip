@@ -8,12 +8,12 @@
 // values and changes R only where a value lies 16 binary orders above it.
 //
 // What bounds it: HBM, with the vector ALUs close behind: a bf16 value has to be widened, entered
-// into a maximum, exponentiated (at a quarter of the rate), summed twice and compared (rank).
+// into a maximum, exponentiated (at less than the full rate) and summed twice.
 //
 // Alternatives, without a comparison more per value: a thread keeps the largest of its own values,
-// which the sums need anyway, and the first chunk that has it.  Values are ordered by (value,
-// index), so the k best of the row lie with the k threads whose own bests are the best: only
-// those threads' chunks are read again, k of 512.
+// which it needs anyway, so the k-th largest of the threads' maxima is a lower bound of the row's k-th
+// largest value, and the values that reach it lie with the few threads whose maxima do.  Only those
+// threads' chunks are read again (about k of 512), and what reaches the bound is sorted by value and index.
 //
 // A NaN or an infinity among the logits makes what depends on the sum NaN, as log_softmax does;
 // -inf is probability 0.  Beyond 1e38, where c x overflows and neighbouring values are 2^100
@@ -34,7 +34,6 @@ constexpr int kThreads = 512;
 constexpr int kWaves = kThreads / 64;
 constexpr int kMaxTop = 64;     // one sorted list of alternatives per wave
 constexpr int kMaxSegments = 32;
-constexpr int kBatch = 4;       // chunks in flight per thread
 constexpr int kList = kWaves * 64;
 constexpr float kLog2e = 1.4426950408889634f, kLn2 = 0.6931471805599453f;
 constexpr float kHuge = 1e38f;
@@ -59,12 +58,14 @@ struct Chunk;  // 16 bytes of logits
 template <>
 struct Chunk<uint16_t> {
   static constexpr int kSize = 8;
+  static constexpr int kLowest = 16;  // lowest bit of an ordered value that can be set
   static __device__ __forceinline__ float one(uint16_t x) { return __uint_as_float(static_cast<u32>(x) << 16); }
   static __device__ __forceinline__ void widen(uint4 w, float (&f)[8]) { unpack8(w, f); }
 };
 template <>
 struct Chunk<float> {
   static constexpr int kSize = 4;
+  static constexpr int kLowest = 0;
   static __device__ __forceinline__ float one(float x) { return x; }
   static __device__ __forceinline__ void widen(uint4 w, float (&f)[4]) {
     f[0] = __uint_as_float(w.x);
@@ -98,38 +99,66 @@ __device__ __forceinline__ float wave_max(float x) {
 }
 __device__ __forceinline__ float wave_sum(float x) { return xor32_sum(xor16_sum(row16_sum(x))); }
 
+// x of lane ^ S, on the vector ALU (through LDS a sort of 64 keys waits 21 times for two round trips).
+template <int S>
+__device__ __forceinline__ u32 across(u32 x) {
+  const int v = static_cast<int>(x), lane = threadIdx.x & 63;
+  if constexpr (S == 1) return __builtin_amdgcn_update_dpp(0, v, kDppQuadXor1, 0xf, 0xf, false);
+  if constexpr (S == 2) return __builtin_amdgcn_update_dpp(0, v, kDppQuadXor2, 0xf, 0xf, false);
+  if constexpr (S == 4)  // groups 0 and 2 of four lanes from 4 up, 1 and 3 from 4 down
+    return __builtin_amdgcn_update_dpp(__builtin_amdgcn_update_dpp(v, v, 0x104, 0xf, 0x5, false), v, 0x114, 0xf, 0xa, false);
+  if constexpr (S == 8) return __builtin_amdgcn_update_dpp(0, v, 0x128, 0xf, 0xf, false);  // row_ror:8
+  if constexpr (S == 16) {
+    const auto r = __builtin_amdgcn_permlane16_swap(x, x, false, false);
+    return lane & 16 ? r[0] : r[1];
+  }
+  const auto r = __builtin_amdgcn_permlane32_swap(x, x, false, false);
+  return lane & 32 ? r[0] : r[1];
+}
+template <int S>
+__device__ __forceinline__ float across_f(float x) {
+  return __uint_as_float(across<S>(__float_as_uint(x)));
+}
 // Lists of 64 keys, one per lane, largest first.
-__device__ __forceinline__ Key exchange(Key k, int stride, bool keep_max) {
-  const Key o = __shfl_xor(k, stride);
+template <int S>
+__device__ __forceinline__ Key exchange(Key k, bool keep_max) {
+  const Key o = static_cast<Key>(across<S>(static_cast<u32>(k >> 32))) << 32 | across<S>(static_cast<u32>(k));
   return (k > o) == keep_max ? k : o;
+}
+// Bitonic stages of strides S, S / 2, .. 1, in falling order where `falls`.
+template <int S>
+__device__ __forceinline__ Key stages(Key k, bool falls) {
+  k = exchange<S>(k, falls == ((threadIdx.x & S) == 0));
+  if constexpr (S > 1) k = stages<S / 2>(k, falls);
+  return k;
 }
 __device__ __forceinline__ Key sort64(Key k) {
   const int lane = threadIdx.x & 63;
-#pragma unroll
-  for (int size = 2; size <= 64; size *= 2)
-#pragma unroll
-    for (int stride = size / 2; stride > 0; stride /= 2)
-      k = exchange(k, stride, ((lane & size) == 0) == ((lane & stride) == 0));
-  return k;
+  k = stages<1>(k, (lane & 2) == 0);
+  k = stages<2>(k, (lane & 4) == 0);
+  k = stages<4>(k, (lane & 8) == 0);
+  k = stages<8>(k, (lane & 16) == 0);
+  k = stages<16>(k, (lane & 32) == 0);
+  return stages<32>(k, true);
+}
+__device__ __forceinline__ Key reversed64(Key k) {
+  const int lane = threadIdx.x & 63;
+  return static_cast<Key>(static_cast<u32>(__builtin_amdgcn_ds_bpermute(4 * (63 - lane), static_cast<int>(k >> 32)))) << 32 |
+         static_cast<u32>(__builtin_amdgcn_ds_bpermute(4 * (63 - lane), static_cast<int>(k)));
 }
 // The 64 largest of a list and another one given in reverse order.
-__device__ __forceinline__ Key merge64(Key k, Key reversed) {
+__device__ __forceinline__ Key merge64(Key k, Key reversed) { return stages<32>(k > reversed ? k : reversed, true); }
+// The 64 largest of `count` keys in LDS, by one wave.
+__device__ __forceinline__ Key best64(const Key* s_keys, int count) {
   const int lane = threadIdx.x & 63;
-  k = k > reversed ? k : reversed;
-#pragma unroll
-  for (int stride = 32; stride > 0; stride /= 2) k = exchange(k, stride, (lane & stride) == 0);
-  return k;
-}
-// Wave 0 gets the 64 largest keys of the first `lists` waves' lists.  Every wave calls it.
-__device__ __forceinline__ Key merge_waves(Key k, Key* s_keys, int lists) {
-  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-  for (int step = 1; step < lists; step *= 2) {
-    __syncthreads();
-    s_keys[threadIdx.x] = k;
-    __syncthreads();
-    if (wave % (2 * step) == 0 && wave + step < lists) k = merge64(k, s_keys[64 * (wave + step) + 63 - lane]);
+  Key list = 0;
+#pragma unroll 1
+  for (int i = 0; i < count; i += 64) {
+    const int at = i + lane;
+    const Key k = sort64(at < count ? s_keys[at] : 0);
+    list = i == 0 ? k : merge64(list, reversed64(k));
   }
-  return k;
+  return list;
 }
 
 // One row's share of the sums; m is the exact maximum.
@@ -171,7 +200,8 @@ __device__ __forceinline__ float log_prob(float x, const State& st) {
 }
 __device__ __forceinline__ float entropy_of(const State& st) {
   if (fabsf(st.m) > kHuge) return st.m - st.m != 0.f ? __builtin_nanf("") : logf(st.s);
-  return fmaxf(kLn2 * (log2f(st.s) - st.w / st.s), st.s != st.s ? st.s : 0.f);
+  const float h = kLn2 * (log2f(st.s) - st.w / st.s);
+  return h < 0.f ? 0.f : h;
 }
 template <typename T>
 __device__ __forceinline__ void finish_row(const LogprobParams& p, int r, const State& st, int64_t token, float x) {
@@ -194,16 +224,15 @@ __global__ __launch_bounds__(kThreads) void logprobs_kernel(const LogprobParams 
   constexpr int E = Chunk<T>::kSize;
   __shared__ Key s_keys[kList];
   __shared__ State s_state[kWaves];
-  __shared__ int s_count;
+  __shared__ u32 s_bound[kThreads], s_least;
+  __shared__ uint16_t s_winner[kThreads];
+  __shared__ int s_count[2];
   const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
   const int r = static_cast<int>(blockIdx.x) / p.segments, seg = static_cast<int>(blockIdx.x) - r * p.segments;
   const T* row = static_cast<const T*>(p.logits) + r * p.row_stride;
   const int chunks = (p.vocab + E - 1) / E, full = p.vocab / E;
   const int per = (chunks + p.segments - 1) / p.segments;
   const int cbeg = min(seg * per, chunks), cend = min(cbeg + per, chunks);
-  const int64_t token = p.tokens[r];
-  const float mine = token >= 0 && token < p.vocab ? Chunk<T>::one(row[token]) : __builtin_nanf("");
-
   // The chunk's values; those behind the row's end are -inf.
   auto values = [&](int c, uint4 w, float (&f)[E]) {
     if (c < full) {
@@ -218,46 +247,79 @@ __global__ __launch_bounds__(kThreads) void logprobs_kernel(const LogprobParams 
                     : make_uint4(0, 0, 0, 0);
   };
 
-  float m = -INFINITY, s = 0.f, w = 0.f, R = 0.f;
-  int best = cbeg + tid, above = 0;
-  bool first = true;
-  for (int c0 = cbeg + (wave << 6); c0 < cend; c0 += kThreads * kBatch) {  // uniform
-    uint4 in[kBatch];
+  // Batches of 32 values per thread, the next one in flight while one is taken; what is left of the
+  // segment behind them chunk by chunk.
+  constexpr int kBatch = 32 / E;
+  const int whole = min(full, cend);  // chunks up to here are whole
+  uint4 in[kBatch];
+  auto load_batch = [&](int c0) {
 #pragma unroll
     for (int u = 0; u < kBatch; ++u) in[u] = load(c0 + u * kThreads + lane);
+  };
+  int c0 = cbeg + (wave << 6);
+  load_batch(c0);  // before the token, whose logit is two round trips away
+  const int64_t token = p.tokens[r];
+  const float mine = token >= 0 && token < p.vocab ? Chunk<T>::one(row[token]) : __builtin_nanf("");
+
+  float m = -INFINITY, s = 0.f, w = 0.f, R = 0.f;
+  int above = 0;
+  bool first = true;
+  auto take = [&](auto count, const float* f) __attribute__((always_inline)) {  // the lane's values
+    constexpr int N = decltype(count)::value;
+    float most = max3(f[0], f[1], f[2]);
 #pragma unroll
-    for (int u = 0; u < kBatch; ++u) {
-      const int cw = c0 + u * kThreads, c = cw + lane;
-      if (cw >= cend) break;  // uniform
-      float f[E];
-      if (cw + 64 <= min(full, cend)) {  // uniform: every lane has a whole chunk
-        Chunk<T>::widen(in[u], f);
-      } else if (c < cend) {
-        values(c, in[u], f);
-      } else {
+    for (int e = 3; e < N; e += 2) most = max3(most, f[e], f[min(e + 1, N - 1)]);
+    if (first || __any(fmaf(most, kLog2e, -R) > kReach)) {  // uniform
+      const float to = reference(wave_max(most));
+      if (!first) rebase(s, w, R, to);
+      R = to;
+      first = false;
+    }
+    m = max3(m, most, most);
+    if (__any(most > mine)) {  // of a likely token's row few batches have one
 #pragma unroll
-        for (int e = 0; e < E; ++e) f[e] = -INFINITY;
-      }
-      float top = f[0];
+      for (int e = 0; e < N; ++e) above += __popcll(__ballot(f[e] > mine));
+    }
+    const float s0 = s, w0 = w;
 #pragma unroll
-      for (int e = 1; e < E; ++e) top = fmaxf(top, f[e]);
-      if (first || __any(fmaf(top, kLog2e, -R) > kReach)) {  // uniform
-        const float to = reference(wave_max(top));
-        if (!first) rebase(s, w, R, to);
-        R = to;
-        first = false;
-      }
-      best = top > m ? c : best;
-      m = fmaxf(m, top);
+    for (int e = 0; e < N; ++e) {
+      const float t = fmaf(f[e], kLog2e, -R), x = fast_exp2(t);
+      s += x;
+      w = fmaf(x, t, w);
+    }
+    if (__any(w != w)) {  // 0 times -inf (or a NaN): once more; 2^t is 0 long before t is -inf
+      s = s0;
+      w = w0;
+      float again = R;
+      asm volatile("" : "+v"(again));  // or the compiler makes one loop of the two and every batch pays for both
 #pragma unroll
-      for (int e = 0; e < E; ++e) {
-        const float t = fmaf(f[e], kLog2e, -R), x = fast_exp2(t);
+      for (int e = 0; e < N; ++e) {
+        const float t = fmaf(f[e], kLog2e, -again), x = fast_exp2(t);
         s += x;
-        // 2^t is 0 long before t is -inf
         w = fmaf(x, fmaxf(t, -1024.f), w);
-        above += __popcll(__ballot(f[e] > mine));
       }
     }
+  };
+  constexpr int kStride = kThreads * kBatch, kSpan = kThreads * (kBatch - 1) + 64;
+#pragma unroll 1
+  for (; c0 + kSpan <= whole; c0 += kStride) {  // uniform
+    float f[kBatch * E];
+#pragma unroll
+    for (int u = 0; u < kBatch; ++u) Chunk<T>::widen(in[u], *reinterpret_cast<float(*)[E]>(f + u * E));
+    if (c0 + kStride + kSpan <= whole) load_batch(c0 + kStride);
+    take(std::integral_constant<int, kBatch * E>{}, f);
+  }
+#pragma unroll 1
+  for (; c0 < cend; c0 += kThreads) {  // uniform
+    const int c = c0 + lane;
+    float f[E];
+    if (c < cend) {
+      values(c, load(c), f);
+    } else {
+#pragma unroll
+      for (int e = 0; e < E; ++e) f[e] = -INFINITY;
+    }
+    take(std::integral_constant<int, E>{}, f);
   }
 
   // ---- the workgroup's state
@@ -268,84 +330,89 @@ __global__ __launch_bounds__(kThreads) void logprobs_kernel(const LogprobParams 
   st.s = ws;
   st.w = ww;
   if (lane == 0) s_state[wave] = st;
-  if (tid == 0) s_count = 0;
-  __syncthreads();
-  st = s_state[0];
+  // ... and every thread's maximum, ordered, NaN above all
+  u32 bound = ordered(m);
+  if (p.top > 0) {
+    if (odd) {
+      for (int c = cbeg + tid; c < cend; c += kThreads) {
+        float f[E];
+        values(c, load(c), f);
 #pragma unroll
-  for (int i = 1; i < kWaves; ++i) st = join(st, s_state[i]);
-  if (fabsf(st.m) > kHuge && st.m - st.m == 0.f) {  // uniform: values equal to the maximum
+        for (int e = 0; e < E; ++e) bound = max(bound, ordered(f[e]));
+      }
+    }
+    s_bound[tid] = cbeg + tid < cend ? bound : 0;
+  }
+  if (tid == 0) s_count[0] = s_count[1] = 0;
+  __syncthreads();
+  float top_m = s_state[0].m;
+#pragma unroll
+  for (int i = 1; i < kWaves; ++i) top_m = fmaxf(top_m, s_state[i].m);
+  if (fabsf(top_m) > kHuge && top_m - top_m == 0.f) {  // uniform: values equal to the maximum
     float equal = 0.f;
     for (int c = cbeg + tid; c < cend; c += kThreads) {
       float f[E];
       values(c, load(c), f);
 #pragma unroll
-      for (int e = 0; e < E; ++e) equal += f[e] != f[e] ? f[e] : (f[e] == st.m ? 1.f : 0.f);
+      for (int e = 0; e < E; ++e) equal += f[e] != f[e] ? f[e] : (f[e] == top_m ? 1.f : 0.f);
     }
     equal = wave_sum(equal);
     __syncthreads();
-    if (lane == 0) s_state[wave].s = equal;
+    if (lane == 0) s_state[wave] = State{top_m, equal, 0.f, above};
     __syncthreads();
-    st.s = st.w = 0.f;
+  }
+  if (wave == 0) {
+    st = s_state[0];
 #pragma unroll
-    for (int i = 0; i < kWaves; ++i) st.s += s_state[i].s;
+    for (int i = 1; i < kWaves; ++i) st = join(st, s_state[i]);
   }
 
-  // ---- alternatives: the threads with the best bests, then the best of their values
+  // ---- alternatives
   Key list = 0;
   if (p.top > 0) {
-    if (odd) {  // NaN counts as largest: look again
-      m = -INFINITY;
-      best = cbeg + tid;
-      u32 most = 0;
-      for (int c = cbeg + tid; c < cend; c += kThreads) {
-        float f[E];
-        values(c, load(c), f);
+    if (wave == 0) {  // the top-th largest of the maxima, bit by bit; 0 if there are fewer
+      u32 mine8[kWaves], least = 0;
 #pragma unroll
-        for (int e = 0; e < E; ++e)
-          if (ordered(f[e]) > most) {
-            most = ordered(f[e]);
-            m = f[e];
-            best = c;
-          }
+      for (int i = 0; i < kWaves; ++i) mine8[i] = s_bound[64 * i + lane];
+#pragma unroll 1
+      for (int bit = 31; bit >= Chunk<T>::kLowest; --bit) {
+        const u32 with = least | 1u << bit;
+        int reach = 0;
+#pragma unroll
+        for (int i = 0; i < kWaves; ++i) reach += __popcll(__ballot(mine8[i] >= with));
+        if (reach >= p.top) least = with;
       }
+      if (lane == 0) s_least = least;
     }
-    list = sort64(cbeg + tid < cend ? key_of(m, best) : 0);
-    list = merge_waves(list, s_keys, kWaves);
     __syncthreads();
-    if (wave == 0) s_keys[lane] = list;
+    const u32 least = s_least;
+    // the threads whose maxima reach it
+    const bool wins = s_bound[tid] >= max(least, 1u);
+    if (wins) s_winner[atomicAdd(&s_count[0], 1)] = static_cast<uint16_t>(tid);
     __syncthreads();
-    const int threads = min(p.top, min(kThreads, cend - cbeg));  // that hold chunks
-    const Key last = threads > 0 ? s_keys[threads - 1] : 0;
-    const u32 least = threads < p.top ? 0 : static_cast<u32>(last >> 32);  // fewer threads: all of their values
-    const int rounds = (cend - cbeg + kThreads - 1) / kThreads, items = threads * rounds;
-    const Key lanes = s_keys[lane];  // the winners, one per lane
-    __syncthreads();
-    // item i: chunk i / threads of winner i % threads
+    const int winners = s_count[0], rounds = (cend - cbeg + kThreads - 1) / kThreads, items = winners * rounds;
+    // item i: chunk i / winners of winner i % winners
     auto chunk_of = [&](int i) {
-      const int j = i / threads;
-      const int winner = static_cast<int>(index_of(__shfl(lanes, i - j * threads)));
-      return cbeg + (winner - cbeg) % kThreads + j * kThreads;
+      const int j = i / winners;
+      return cbeg + s_winner[i - j * winners] + j * kThreads;
     };
-    for (int i0 = wave << 6; i0 < items; i0 += kThreads) {  // uniform
-      const int i = i0 + lane, c = chunk_of(min(i, items - 1));
-      if (i < items && c < cend) {
-        float f[E];
-        values(c, load(c), f);
+    for (int i = tid; i < items; i += kThreads) {
+      const int c = chunk_of(i);
+      if (c >= cend) continue;
+      float f[E];
+      values(c, load(c), f);
 #pragma unroll
-        for (int e = 0; e < E; ++e)
-          if (ordered(f[e]) >= least && E * c + e < p.vocab) {
-            const int at = atomicAdd(&s_count, 1);
-            if (at < kList) s_keys[at] = key_of(f[e], E * c + e);
-          }
-      }
+      for (int e = 0; e < E; ++e)
+        if (ordered(f[e]) >= least && E * c + e < p.vocab) {
+          const int at = atomicAdd(&s_count[1], 1);
+          if (at < kList) s_keys[at] = key_of(f[e], E * c + e);
+        }
     }
     __syncthreads();
-    const int count = s_count;
-    if (count <= kList) {
-      list = sort64(tid < count ? s_keys[tid] : 0);
-      list = merge_waves(list, s_keys, (count + 63) / 64);
-    } else {  // many equal values: every wave keeps the best of what it sees
-      list = 0;
+    int count = s_count[1];
+    if (count > kList) {  // many equal values: every wave keeps the best of what it sees
+      Key last = 0;       // its top-th best
+#pragma unroll 1
       for (int i0 = wave << 6; i0 < items; i0 += kThreads) {
         const int i = i0 + lane, c = chunk_of(min(i, items - 1));
         float f[E];
@@ -355,13 +422,17 @@ __global__ __launch_bounds__(kThreads) void logprobs_kernel(const LogprobParams 
           float x = f[0];
 #pragma unroll
           for (int j = 1; j < E; ++j) x = e == j ? f[j] : x;
-          const bool in = i < items && c < cend && E * c + e < p.vocab;
-          const Key k = sort64(in ? key_of(x, E * c + e) : 0);
-          list = merge64(list, __shfl(k, 63 - lane));
+          const Key k = i < items && c < cend && E * c + e < p.vocab ? key_of(x, E * c + e) : 0;
+          if (!__any(k > last)) continue;
+          list = merge64(list, reversed64(sort64(k)));
+          last = __shfl(list, p.top - 1);
         }
       }
-      list = merge_waves(list, s_keys, kWaves);
+      s_keys[tid] = list;
+      count = kList;
+      __syncthreads();
     }
+    if (wave == 0) list = best64(s_keys, count);
   }
 
   // ---- out, or to the merge
@@ -370,7 +441,7 @@ __global__ __launch_bounds__(kThreads) void logprobs_kernel(const LogprobParams 
     if (wave == 0) write_top(p, r, st, list);
   } else {
     if (tid == 0) p.states[blockIdx.x] = make_float4(st.m, st.s, st.w, __int_as_float(st.above));
-    if (wave == 0 && p.top > 0) p.lists[static_cast<int64_t>(blockIdx.x) * kMaxTop + lane] = list;
+    if (wave == 0 && lane < p.top) p.lists[static_cast<int64_t>(blockIdx.x) * p.top + lane] = list;
   }
 }
 
@@ -380,22 +451,44 @@ __global__ __launch_bounds__(kThreads) void logprobs_merge_kernel(const LogprobP
   __shared__ Key s_keys[kList];
   const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
   const int r = static_cast<int>(blockIdx.x);
-  State st{-INFINITY, 0.f, 0.f, 0};
-  for (int i = 0; i < p.segments; ++i) {
-    const float4 x = p.states[static_cast<int64_t>(r) * p.segments + i];
-    st = join(st, State{x.x, x.y, x.z, __float_as_int(x.w)});
-  }
+  // the segments' alternatives side by side, 64 to a wave and round
+  const int keys = p.segments * p.top;
+  const Key* lists = p.lists + static_cast<int64_t>(r) * keys;
+  constexpr int kRounds = kMaxSegments * kMaxTop / kThreads;
+  Key key[kRounds];
+#pragma unroll
+  for (int i = 0; i < kRounds; ++i) key[i] = tid + i * kThreads < keys ? lists[tid + i * kThreads] : 0;
+  // every wave joins all segments' states, one per lane
+  const float4 x = p.states[static_cast<int64_t>(r) * p.segments + min(lane, p.segments - 1)];
+  State st = lane < p.segments ? State{x.x, x.y, x.z, __float_as_int(x.w)} : State{-INFINITY, 0.f, 0.f, 0};
+  auto with = [&](auto stride) {
+    constexpr int S = decltype(stride)::value;
+    st = join(st, State{across_f<S>(st.m), across_f<S>(st.s), across_f<S>(st.w), static_cast<int>(across<S>(st.above))});
+  };
+  with(std::integral_constant<int, 1>{});
+  with(std::integral_constant<int, 2>{});
+  with(std::integral_constant<int, 4>{});
+  with(std::integral_constant<int, 8>{});
+  with(std::integral_constant<int, 16>{});
+  with(std::integral_constant<int, 32>{});
   if (tid == 0) {
     const int64_t token = p.tokens[r];
     const T* row = static_cast<const T*>(p.logits) + r * p.row_stride;
     finish_row<T>(p, r, st, token, token >= 0 && token < p.vocab ? Chunk<T>::one(row[token]) : 0.f);
   }
   if (p.top == 0) return;  // uniform
-  const Key* lists = p.lists + static_cast<int64_t>(r) * p.segments * kMaxTop;
-  Key list = wave < p.segments ? lists[wave * kMaxTop + lane] : 0;
-  for (int i = wave + kWaves; i < p.segments; i += kWaves) list = merge64(list, lists[i * kMaxTop + 63 - lane]);
-  list = merge_waves(list, s_keys, min(kWaves, p.segments));
-  if (wave == 0) write_top(p, r, st, list);
+  Key list = 0;
+#pragma unroll
+  for (int i = 0; i < kRounds; ++i)
+    if (64 * wave + i * kThreads < keys) list = i == 0 ? sort64(key[0]) : merge64(list, reversed64(sort64(key[i])));
+  s_keys[tid] = list;
+  __syncthreads();
+  if (wave == 0) {
+    const int waves = min(kWaves, (keys + 63) / 64);
+#pragma unroll 1
+    for (int i = 1; i < waves; ++i) list = merge64(list, s_keys[64 * i + 63 - lane]);
+    write_top(p, r, st, list);
+  }
 }
 
 // Segments of a row: enough workgroups to fill the GPU where rows are few.
