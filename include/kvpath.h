@@ -484,7 +484,7 @@ int kvp_tree_attention(const void* q, int64_t q_tok_stride, int64_t q_head_strid
  * of 16 bytes; sums in fp32.  0 <= top <= min(64, vocab).  A row with a NaN or +inf, or of -inf
  * alone, has NaN log probabilities and entropy.  A token outside [0, vocab) has a NaN log
  * probability and rank 0.  The workspace (16-byte aligned, no initialisation;
- * kvp_token_logprobs_workspace_bytes, 0 from 512 rows on, 0.5 MB at most) holds the parts of rows
+ * kvp_token_logprobs_workspace_bytes, 0 from 256 rows on, 0.3 MB at most) holds the parts of rows
  * that several workgroups share.
  */
 size_t kvp_token_logprobs_workspace_bytes(int32_t num_rows);

@@ -33,7 +33,7 @@ typedef unsigned long long Key;  // (ordered value, ~index): larger is better; 0
 constexpr int kThreads = 512;
 constexpr int kWaves = kThreads / 64;
 constexpr int kMaxTop = 64;     // one sorted list of alternatives per wave
-constexpr int kMaxSegments = 32;
+constexpr int kMaxSegments = 16;
 constexpr int kList = kWaves * 64;
 constexpr float kLog2e = 1.4426950408889634f, kLn2 = 0.6931471805599453f;
 constexpr float kHuge = 1e38f;
@@ -491,8 +491,11 @@ __global__ __launch_bounds__(kThreads) void logprobs_merge_kernel(const LogprobP
   }
 }
 
-// Segments of a row: enough workgroups to fill the GPU where rows are few.
-int segments_of(int32_t rows) { return rows >= 512 ? 1 : std::min(kMaxSegments, 1024 / std::max(rows, 1)); }
+// Segments of a row: no more workgroups than are resident at once (two per CU), since every segment
+// pays for its alternatives anew and a second round of workgroups for a second time: 64 fp32 rows of
+// 151936 take 20 us in 8 segments, 33 in 16.  From one row per CU on splitting is not worth its join
+// (256 rows: 33 us whole, 39 in halves), and behind 16 segments only the join grows.
+int segments_of(int32_t rows) { return rows >= 256 ? 1 : std::min(kMaxSegments, 512 / std::max(rows, 1)); }
 
 template <typename T>
 int launch(const char* fn, LogprobParams p, int rows, hipStream_t s) {
