@@ -25,9 +25,8 @@
 //
 // Layouts are those of the decode kernel (lane l: n = l % 16, q4 = l / 16): S = K Q^T has tokens
 // 4 q4 + j of every 16 in the lane and row n as its column, O^T = V^T P^T takes P from the same
-// registers.  e4m3 is widened to bf16, exactly: with few rows on its way from LDS to the matrix
-// cores, K with its scale (the lane's own token), V's scale going into P; with many rows once for
-// all waves, into a bf16 tile.  P is rounded to bf16: at most 2^-8 of each weight, of either sign,
+// registers.  e4m3 is widened to bf16, exactly, on its way from LDS to the matrix cores, K with its
+// scale (the lane's own token), V's scale going into P.  P is rounded to bf16: at most 2^-8 of each weight, of either sign,
 // so below the rounding of the bf16 output where the values do not cancel; the sum of the weights
 // is of the unrounded ones, and running maxima, sums and products stay in 32 bits.
 #include <math.h>
@@ -336,13 +335,16 @@ __device__ __forceinline__ void wait_tiles(int most) {
   else wait_vmem<0>();
 }
 
-// P of two tokens in packed bf16, times their V scales: the exponents are added as integers.  vs:
-// the bytes, shifted into bf16's exponent.  A weight below 2^-126 counts as the scale times 2^-127.
+// P of two tokens in packed bf16, times their V scales, bytes 0 and 1 of `bytes`, or 2 and 3: the
+// exponents are added as integers.  A weight below 2^-126 counts as the scale times 2^-127; a masked
+// one (`tail`: there may be some) is 0 whatever the scale.
 typedef uint16_t u16x2_t __attribute__((ext_vector_type(2)));
-__device__ __forceinline__ u32 scale_pair(u32 pk, u32 vs) {
+__device__ __forceinline__ u32 scale_weights(u32 pk, u32 bytes, bool upper, bool tail) {
+  const u32 vs = __builtin_amdgcn_perm(0, bytes, upper ? 0x0c030c02 : 0x0c010c00) << 7;
   const u16x2_t one = {127 << 7, 127 << 7};
-  return __builtin_bit_cast(u32, __builtin_elementwise_sub_sat(
+  const u32 scaled = __builtin_bit_cast(u32, __builtin_elementwise_sub_sat(
       static_cast<u16x2_t>(__builtin_bit_cast(u16x2_t, pk) + __builtin_bit_cast(u16x2_t, vs)), one));
+  return !tail ? scaled : ((pk & 0xffffu) ? scaled & 0xffffu : 0u) | ((pk >> 16) ? scaled & 0xffff0000u : 0u);
 }
 
 // Whether a row sees draft d (below 0: a token of the context), given the bits of its drafts.
@@ -601,14 +603,7 @@ __global__ __launch_bounds__(kThreads) void tree_few_kernel(const TreeParams p) 
         u32x4_t pf[1] = {rows.weigh(0, s[2 * sub], s[2 * sub + 1], p.scale_log2, tail, draft, q4)};
         if constexpr (FP8) {
 #pragma unroll
-          for (int w = 0; w < 4; ++w) {
-            const u32 bytes = vexp[2 * sub + (w >> 1)];
-            const u32 scaled = scale_pair(pf[0][w], __builtin_amdgcn_perm(0, bytes, w & 1 ? 0x0c030c02 : 0x0c010c00) << 7);
-            // a masked weight is 0 whatever the scale
-            pf[0][w] = !tail ? scaled
-                             : ((pf[0][w] & 0xffffu) ? scaled & 0xffffu : 0u) |
-                                   ((pf[0][w] >> 16) ? scaled & 0xffff0000u : 0u);
-          }
+          for (int w = 0; w < 4; ++w) pf[0][w] = scale_weights(pf[0][w], vexp[2 * sub + (w >> 1)], w & 1, tail);
         }
         // ---- O^T += V^T P^T
         if (sub == 0) wait_tiles<F::kKOps, F::kVOps>(issued - c0.mark - F::kVOps);
@@ -648,21 +643,62 @@ __global__ __launch_bounds__(kThreads) void tree_few_kernel(const TreeParams p) 
   }
 }
 
-// More rows: the four waves of a workgroup share bf16 tiles of 64 tokens, and a wave has 32 rows
+// More rows: the four waves of a workgroup share tiles of 64 tokens, and a wave has 32 rows
 // (v_mfma_f32_32x32x16_bf16; lane l: row l % 32, hf = l / 32).  KW = 1: wave w has rows 32 w .. of a block of
 // 128.  KW = 2, up to 64 rows: waves w and w + 2 have rows 32 (w % 2) .. and 32 tokens of every step each; their
 // states are joined through LDS where the sequence ends.
 //
 // Two workgroups on a CU: one computes while the other waits.  bf16: two tiles, the next one loaded while a tile
-// is used.  e4m3: one bf16 tile, and two of e4m3 behind it, from which every wave widens the 16 tokens that it
-// has loaded itself, with their scales.
+// is used.  e4m3: four, three of them being loaded, and every wave widens what it reads.
 //
-// Tile rows are 256 bytes, 16-byte chunk c of token r at chunk c ^ (r % 16) of K and c ^ 4 (r % 4) of V.  The lane
+// Tile rows are 256 bytes, 16-byte chunk c of token r at chunk c ^ (r % 16) of K and c ^ 4 (r % 4) of V; in
+// e4m3 128 bytes, c ^ ((r / 2) % 8) and c ^ ((r & 2) + (r & 8) / 2).  The lane
 // gets the scores of tokens 8 (i / 4) + 4 hf + i % 4 of each 32, and of O^T dims 32 mb + 8 (j / 4) + 4 hf + j % 4.
 constexpr int kManyStep = 64;
 constexpr int kTileElems = kManyStep * kDim;
+constexpr int kRawTiles = 4, kRawBytes = 2 * kTile + 2 * kManyStep;
 // A row's weights of one step sum up to this before its maximum is taken again (see weigh).
 constexpr float kSumLimit = 65536.f;
+constexpr float kSumLimitScaled = 256.f;  // e4m3: and times a scale they are to fit bf16
+
+// One or two blocks of 32 tokens (4096 bytes each) in e4m3: K from the lane's four addresses in the first, its
+// exponent byte at `ka`, those of V's tokens 8 i + 0 .. 3 at `va` + 8 i.
+template <int BLOCKS>
+__device__ __forceinline__ void read_k8_blocks(const u32 (&at)[4], u32 ka, u32 va, u32x4_t (&k)[BLOCKS][4],
+                                               u32 (&kexp)[BLOCKS], u32 (&vexp)[BLOCKS][4]) {
+#pragma unroll
+  for (int b = 0; b < BLOCKS; ++b)
+    asm volatile(
+        "ds_read_u8 %4, %13\n\t"
+        "ds_read_b128 %0, %9\n\tds_read_b128 %1, %10\n\tds_read_b128 %2, %11\n\tds_read_b128 %3, %12\n\t"
+        "ds_read_b32 %5, %14\n\tds_read_b32 %6, %14 offset:8\n\tds_read_b32 %7, %14 offset:16\n\t"
+        "ds_read_b32 %8, %14 offset:24\n\ts_waitcnt lgkmcnt(0)"
+        : "=&v"(k[b][0]), "=&v"(k[b][1]), "=&v"(k[b][2]), "=&v"(k[b][3]), "=&v"(kexp[b]), "=&v"(vexp[b][0]),
+          "=&v"(vexp[b][1]), "=&v"(vexp[b][2]), "=&v"(vexp[b][3])
+        : "v"(at[0] + 4096 * b), "v"(at[1] + 4096 * b), "v"(at[2] + 4096 * b), "v"(at[3] + 4096 * b), "v"(ka + 32 * b),
+          "v"(va + 32 * b)
+        : "memory");
+}
+// V of 16 or 32 tokens in e4m3, transposed: 8 bytes at a[mb] + off, and 2048 further.
+__device__ __forceinline__ void read_v8_16(const int (&a)[4], int off, u32x2_t (&v)[4]) {
+  asm volatile(
+      "ds_read_b64_tr_b8 %0, %4\n\tds_read_b64_tr_b8 %1, %5\n\t"
+      "ds_read_b64_tr_b8 %2, %6\n\tds_read_b64_tr_b8 %3, %7\n\ts_waitcnt lgkmcnt(0)"
+      : "=&v"(v[0]), "=&v"(v[1]), "=&v"(v[2]), "=&v"(v[3])
+      : "v"(a[0] + off), "v"(a[1] + off), "v"(a[2] + off), "v"(a[3] + off)
+      : "memory");
+}
+__device__ __forceinline__ void read_v8_32(const int (&a)[4], int off, u32x2_t (&v)[2][4]) {
+  asm volatile(
+      "ds_read_b64_tr_b8 %0, %8\n\tds_read_b64_tr_b8 %1, %9\n\t"
+      "ds_read_b64_tr_b8 %2, %10\n\tds_read_b64_tr_b8 %3, %11\n\t"
+      "ds_read_b64_tr_b8 %4, %8 offset:2048\n\tds_read_b64_tr_b8 %5, %9 offset:2048\n\t"
+      "ds_read_b64_tr_b8 %6, %10 offset:2048\n\tds_read_b64_tr_b8 %7, %11 offset:2048\n\ts_waitcnt lgkmcnt(0)"
+      : "=&v"(v[0][0]), "=&v"(v[0][1]), "=&v"(v[0][2]), "=&v"(v[0][3]), "=&v"(v[1][0]), "=&v"(v[1][1]), "=&v"(v[1][2]),
+        "=&v"(v[1][3])
+      : "v"(a[0] + off), "v"(a[1] + off), "v"(a[2] + off), "v"(a[3] + off)
+      : "memory");
+}
 
 // All waves' LDS accesses are done, but not their loads.
 __device__ __forceinline__ void tile_barrier() { asm volatile("s_waitcnt lgkmcnt(0)\n\ts_barrier" ::: "memory"); }
@@ -670,11 +706,13 @@ __device__ __forceinline__ void tile_barrier() { asm volatile("s_waitcnt lgkmcnt
 template <bool FP8, int KW>
 __global__ __launch_bounds__(kThreads, 2) void tree_many_kernel(const TreeParams p) {
   constexpr int STEP = kManyStep, BLOCKS = 2 / KW;  // blocks of 32 tokens of a step that a wave takes
-  __shared__ __attribute__((aligned(16))) uint16_t s_k0[kTileElems];
-  __shared__ __attribute__((aligned(16))) uint16_t s_v0[kTileElems];
+  // bf16: the compiler has to tell the tile that is read from the one that is loaded
+  __shared__ __attribute__((aligned(16))) uint16_t s_k0[FP8 ? 8 : kTileElems];
+  __shared__ __attribute__((aligned(16))) uint16_t s_v0[FP8 ? 8 : kTileElems];
   __shared__ __attribute__((aligned(16))) uint16_t s_k1[FP8 ? 8 : kTileElems];
   __shared__ __attribute__((aligned(16))) uint16_t s_v1[FP8 ? 8 : kTileElems];
-  __shared__ __attribute__((aligned(16))) char s_raw[FP8 ? 2 : 1][FP8 ? 2 * kTile + 128 : 16];
+  // e4m3: K, V, K's scales, V's scales
+  __shared__ __attribute__((aligned(16))) char s_raw[FP8 ? kRawTiles : 1][FP8 ? kRawBytes : 16];
   __shared__ float2 s_ml[KW == 2 ? 2 : 1][64];
   __shared__ int s_cum[kSeqsPerLaunch + 1];
   __shared__ int s_part[kWaves];
@@ -706,46 +744,19 @@ __global__ __launch_bounds__(kThreads, 2) void tree_many_kernel(const TreeParams
     const uint32_t bytes = static_cast<uint32_t>((STEP - 1) * stride + (FP8 ? kDim : 2 * kDim));
     const int ln = fresh_lane(), lr = FP8 ? ln >> 3 : ln >> 4, lc = FP8 ? ln & 7 : ln & 15;
     const int row_off = (16 * wave + lr) * stride;
-    const int k_chunk = FP8 ? 16 * lc : 16 * (lc ^ lr), v_chunk = FP8 ? 16 * lc : 16 * (lc ^ (4 * (lr & 3)));
+    const int k_chunk = 16 * (FP8 ? lc ^ (lr >> 1) : lc ^ lr), v_chunk = 16 * (FP8 ? lc ^ (lr & 2) : lc ^ (4 * (lr & 3)));
     const BufferRsrc kr = buffer_rsrc(p.k_cache + base, bytes), vr = buffer_rsrc(p.v_cache + base, bytes);
-    // row 16 wave + 4 i + lr: its K chunks are swizzled by (4 i + lr) % 16
+    // row 16 wave + 4 i + lr (e4m3: 8 i): the part of i in the swizzle is 4 i chunks, but none in bf16's V
 #pragma unroll
     for (int i = 0; i < kFills; ++i)
       raw_buffer_load_lds(kr, (LdsPtr)(k_to + 1024 * (kFills * wave + i)), 16,
-                          min(row_off + (FP8 ? 8 : 4) * i * stride, last) + (FP8 ? k_chunk : k_chunk ^ (64 * i)), 0, 0, 0);
+                          min(row_off + (FP8 ? 8 : 4) * i * stride, last) + (k_chunk ^ (64 * i)), 0, 0, 0);
 #pragma unroll
     for (int i = 0; i < kFills; ++i)
       raw_buffer_load_lds(vr, (LdsPtr)(v_to + 1024 * (kFills * wave + i)), 16,
-                          min(row_off + (FP8 ? 8 : 4) * i * stride, last) + v_chunk, 0, 0, 0);
+                          min(row_off + (FP8 ? 8 : 4) * i * stride, last) + (FP8 ? v_chunk ^ (64 * i) : v_chunk), 0, 0, 0);
     if (FP8) issue_scales(p, uniform(c.blk * p.scale_blk_stride + scale_head + off), ln, scale_to);
   };
-  // FP8: the wave's 16 tokens into the bf16 tile.  Lane: token 8 i + lr, dims 16 lc .. + 15.
-  auto widen = [&](int buf) __attribute__((always_inline)) {
-    const u32 raw = lds_addr(s_raw[FP8 ? buf : 0]);
-    const int ln = fresh_lane(), lr = ln >> 3, lc = ln & 7;
-#pragma unroll
-    for (int i = 0; i < 2; ++i) {
-      const int row = 16 * wave + 8 * i + lr;
-      u32x4_t k, v;
-      u32 ke, ve;
-      const u32 at = raw + 128 * row + 16 * lc, scale_at = raw + 2 * kTile + row;
-      asm volatile(
-          "ds_read_b128 %0, %4\n\tds_read_b128 %1, %4 offset:8192\n\tds_read_u8 %2, %5\n\tds_read_u8 %3, %5 offset:64\n\t"
-          "s_waitcnt lgkmcnt(0)"
-          : "=&v"(k), "=&v"(v), "=&v"(ke), "=&v"(ve)
-          : "v"(at), "v"(scale_at)
-          : "memory");
-      const u32 k_to = lds_addr(s_k0) + 256 * row, v_to = lds_addr(s_v0) + 256 * row;
-      const float ks = __uint_as_float(ke << 23), vs = __uint_as_float(ve << 23);
-#pragma unroll
-      for (int h = 0; h < 2; ++h) {
-        const u32x4_t kw = widen8(k[2 * h], k[2 * h + 1], ks), vw = widen8(v[2 * h], v[2 * h + 1], vs);
-        asm volatile("ds_write_b128 %0, %1" ::"v"(k_to + 16 * ((2 * lc + h) ^ (row & 15))), "v"(kw) : "memory");
-        asm volatile("ds_write_b128 %0, %1" ::"v"(v_to + 16 * ((2 * lc + h) ^ (4 * (row & 3)))), "v"(vw) : "memory");
-      }
-    }
-  };
-
   // ---- the wave's rows
   const int kw = KW == 2 ? wave >> 1 : 0, rw = KW == 2 ? wave & 1 : wave;
   const int first_row = r.block * 128 + 32 * rw;
@@ -758,10 +769,10 @@ __global__ __launch_bounds__(kThreads, 2) void tree_many_kernel(const TreeParams
   auto start = [&](const Cursor& c) __attribute__((always_inline)) {
     const int ln = fresh_lane(), row = first_row + (ln & 31), tok = token_of(row);
     const int i = min(tok, c.n - 1), head = r.kvh * p.group + row - tok * p.group;
-    const uint16_t* src = p.q + (c.q0 + i) * p.q_tok_stride + head * p.q_head_stride + 8 * (ln >> 5);
+    const uint16_t* src = p.q + (c.q0 + i) * p.q_tok_stride + head * p.q_head_stride + (FP8 ? 16 : 8) * (ln >> 5);
 #pragma unroll
     for (int ks = 0; ks < 8; ++ks) {
-      uint4 x = *reinterpret_cast<const uint4*>(src + 16 * ks);
+      uint4 x = *reinterpret_cast<const uint4*>(src + (FP8 ? 32 * (ks >> 1) + 8 * (ks & 1) : 16 * ks));
       q[ks] = make_uint4(x.x ^ p.q_flip, x.y ^ p.q_flip, x.z ^ p.q_flip, x.w ^ p.q_flip);
     }
     const uint64_t all = ~0ull >> (64 - c.n);
@@ -776,20 +787,36 @@ __global__ __launch_bounds__(kThreads, 2) void tree_many_kernel(const TreeParams
       for (int j = 0; j < 16; ++j) acc[mb][j] = 0.f;
   };
 
-  auto compute = [&](const Cursor& c, const uint16_t* sk, const uint16_t* sv) __attribute__((always_inline)) {
+  // The step's tiles: sk and sv, or in e4m3 at LDS address `raw`.
+  auto compute = [&](const Cursor& c, const uint16_t* sk, const uint16_t* sv, u32 raw) __attribute__((always_inline)) {
     const int t0 = c.j * STEP + 32 * kw, left = c.len - t0;  // the wave's tokens
     if (left <= 0) return;
     const int ln = fresh_lane(), n = ln & 31, hf = ln >> 5;
     const int draft = t0 - (c.len - c.n);        // the first token's draft, below 0 in the context
     const bool tail = draft + 32 * BLOCKS > 0;  // drafts among the tokens, or the last one in front of them
-    // ---- S = K Q^T: steps (16 dims, block), a ring of four fragments in flight ahead of the products
+    // ---- S = K Q^T
     f32x16_t sc[BLOCKS];
     __builtin_amdgcn_s_setprio(1);
 #pragma unroll
     for (int mb = 0; mb < BLOCKS; ++mb)
 #pragma unroll
       for (int j = 0; j < 16; ++j) sc[mb][j] = 0.f;
-    {
+    u32 vexp[BLOCKS][4];  // V's scales of tokens 8 i + 4 hf + 0 .. 3, one a byte
+    if constexpr (FP8) {
+      u32x4_t k[BLOCKS][4];  // dims 32 i + 16 hf .. + 15
+      u32 kexp[BLOCKS];
+      const u32 row = raw + 128 * (32 * kw + n), f = (n >> 1) & 7;
+      const u32 at[4] = {row + 16 * (hf ^ f), row + 16 * ((2 + hf) ^ f), row + 16 * ((4 + hf) ^ f), row + 16 * ((6 + hf) ^ f)};
+      read_k8_blocks(at, raw + 2 * kTile + 32 * kw + n, raw + 2 * kTile + kManyStep + 32 * kw + 4 * hf, k, kexp, vexp);
+#pragma unroll
+      for (int ks = 0; ks < 8; ++ks)
+#pragma unroll
+        for (int mb = 0; mb < BLOCKS; ++mb) {
+          const u32x4_t w = k[mb][ks >> 1];
+          sc[mb] = mfma32(__builtin_bit_cast(uint4, widen8(w[2 * (ks & 1)], w[2 * (ks & 1) + 1], __uint_as_float(kexp[mb] << 23))),
+                          q[ks], sc[mb]);
+        }
+    } else {  // steps (16 dims, block), a ring of four fragments in flight ahead of the products
       auto frag = [&](int st) __attribute__((always_inline)) {
         const int ks = st / BLOCKS, mb = st % BLOCKS;
         return *reinterpret_cast<const uint4*>(sk + ((32 * (kw + mb) + n) * kDim + 8 * ((2 * ks + hf) ^ (n & 15))));
@@ -848,7 +875,7 @@ __global__ __launch_bounds__(kThreads, 2) void tree_many_kernel(const TreeParams
       sum = half_swap_sum(sum);
     };
     weigh();
-    if (__any(!(sum <= kSumLimit))) {  // rare
+    if (__any(!(sum <= (FP8 ? kSumLimitScaled : kSumLimit)))) {  // rare
       const float m_new = fmaxf(m, step_max());
       const float alpha = fast_exp2(m - m_new);
       m = m_new;
@@ -860,24 +887,43 @@ __global__ __launch_bounds__(kThreads, 2) void tree_many_kernel(const TreeParams
       weigh();
     }
     l += sum;
+    if constexpr (FP8) {
+#pragma unroll
+      for (int mb = 0; mb < BLOCKS; ++mb)
+#pragma unroll
+        for (int i = 0; i < 8; ++i) pk[mb][i] = scale_weights(pk[mb][i], vexp[mb][i >> 1], i & 1, tail);
+    }
     // ---- O^T += V^T P^T, 16 tokens at a time
     auto pf = [&](int kk) __attribute__((always_inline)) {
       const u32* w = &pk[kk >> 1][4 * (kk & 1)];
       return make_uint4(w[0], w[1], w[2], w[3]);
     };
     // V^T operand (see lds_read_tr16's use in the prefill): the lane addresses token 4 hf + (l % 16) / 4 of 16 at
-    // dims 16 ((l / 16) % 2) + 4 (l % 4) of 32, and gets dim l % 32 of tokens 4 hf + e.
-    const int tr_tok = 4 * hf + ((ln & 15) >> 2);
+    // dims 16 ((l / 16) % 2) + 4 (l % 4) of 32, and gets dim l % 32 of tokens 4 hf + e.  e4m3: it addresses token
+    // 8 (e / 4) + 4 hf + e % 4, e = (l % 16) / 2, at dims 16 ((l / 16) % 2) + 8 (l % 2), and gets all 8.
+    const int tr_tok = FP8 ? 4 * hf + ((ln & 8) | ((ln & 7) >> 1)) : 4 * hf + ((ln & 15) >> 2);
     const int tr_chunk = 2 * ((ln >> 4) & 1) + ((ln & 3) >> 1), tr_sub = 4 * (ln & 1);
     int v_at[4];
 #pragma unroll
     for (int mb = 0; mb < 4; ++mb) {
+      if (FP8) {
+        v_at[mb] = static_cast<int>(raw) + kTile + 128 * (32 * kw + tr_tok) +
+                   16 * ((2 * mb + ((ln >> 4) & 1)) ^ ((tr_tok & 2) | (tr_tok & 8) >> 1)) + 8 * (ln & 1);
+        continue;
+      }
       v_at[mb] = (32 * kw + tr_tok) * kDim + 8 * ((4 * mb + tr_chunk) ^ (4 * (tr_tok & 3))) + tr_sub;
       // The compiler is not to take the sum apart: behind several additions it no longer knows the array, and
       // would wait for the next tile in front of the read.
       asm volatile("" : "+v"(v_at[mb]));
     }
     auto read_v = [&](int kk, uint4 (&dst)[4]) __attribute__((always_inline)) {
+      if constexpr (FP8) {
+        u32x2_t v[4];
+        read_v8_16(v_at, 2048 * kk, v);
+#pragma unroll
+        for (int mb = 0; mb < 4; ++mb) dst[mb] = __builtin_bit_cast(uint4, widen8(v[mb].x, v[mb].y, 1.f));
+        return;
+      }
 #pragma unroll
       for (int mb = 0; mb < 4; ++mb) {
         const uint2 lo = lds_read_tr16(sv + (v_at[mb] + 16 * kk * kDim));
@@ -885,7 +931,20 @@ __global__ __launch_bounds__(kThreads, 2) void tree_many_kernel(const TreeParams
         dst[mb] = make_uint4(lo.x, lo.y, hi.x, hi.y);
       }
     };
-    if (!tail) {
+    if (FP8 && !tail) {
+      __builtin_amdgcn_s_setprio(1);
+#pragma unroll
+      for (int h = 0; h < BLOCKS; ++h) {
+        u32x2_t v[2][4];
+        read_v8_32(v_at, 4096 * h, v);
+#pragma unroll
+        for (int kk = 0; kk < 2; ++kk)
+#pragma unroll
+          for (int mb = 0; mb < 4; ++mb)
+            acc[mb] = mfma32(__builtin_bit_cast(uint4, widen8(v[kk][mb].x, v[kk][mb].y, 1.f)), pf(2 * h + kk), acc[mb]);
+      }
+      __builtin_amdgcn_s_setprio(0);
+    } else if (!tail) {
       __builtin_amdgcn_s_setprio(1);
       uint4 vf[2][4];
       read_v(0, vf[0]);
@@ -981,62 +1040,79 @@ __global__ __launch_bounds__(kThreads, 2) void tree_many_kernel(const TreeParams
       if (hf == 0) *reinterpret_cast<float2*>(p.part_ml + 2 * at) = make_float2(m, sum);
     }
   };
-  // KW = 2: wave w takes over the state of wave w + 2, by way of a tile that is done with.
-  auto join = [&](uint16_t* sk, uint16_t* sv) __attribute__((always_inline)) {
-    float* const area = reinterpret_cast<float*>(rw == 0 ? sk : sv) + lane;
-    tile_barrier();  // the tile is done with
-    if (kw == 1) {
+  // KW = 2: wave w takes over the state of wave w + 2, by way of the step's tile (in e4m3 it is half as large).
+  auto join = [&](uint16_t* sk, uint16_t* sv, u32 buf) __attribute__((always_inline)) {
+    constexpr int kRounds = FP8 ? 2 : 1, MB = 4 / kRounds;
+    float* const area = (FP8 ? reinterpret_cast<float*>(s_raw[FP8 ? buf : 0] + (FP8 ? kTile * rw : 0))
+                             : reinterpret_cast<float*>(rw == 0 ? sk : sv)) + lane;
+    float a = 0.f, w = 0.f;
 #pragma unroll
-      for (int mb = 0; mb < 4; ++mb)
+    for (int round = 0; round < kRounds; ++round) {
+      tile_barrier();  // the tile is done with
+      if (kw == 1) {
 #pragma unroll
-        for (int j = 0; j < 16; ++j) area[64 * (16 * mb + j)] = acc[mb][j];
-      s_ml[rw][lane] = make_float2(m, l);
-    }
-    tile_barrier();
-    if (kw == 0) {
-      const float2 o = s_ml[rw][lane];
-      const float m_new = fmaxf(m, o.x), a = fast_exp2(m - m_new), w = fast_exp2(o.x - m_new);
-      m = m_new;
-      l = l * a + o.y * w;
+        for (int mb = 0; mb < MB; ++mb)
 #pragma unroll
-      for (int mb = 0; mb < 4; ++mb)
+          for (int j = 0; j < 16; ++j) area[64 * (16 * mb + j)] = acc[MB * round + mb][j];
+        if (round == 0) s_ml[rw][lane] = make_float2(m, l);
+      }
+      tile_barrier();
+      if (kw == 0) {
+        if (round == 0) {
+          const float2 o = s_ml[rw][lane];
+          const float m_new = fmaxf(m, o.x);
+          a = fast_exp2(m - m_new), w = fast_exp2(o.x - m_new);
+          m = m_new;
+          l = l * a + o.y * w;
+        }
 #pragma unroll
-        for (int j = 0; j < 16; ++j) acc[mb][j] = acc[mb][j] * a + area[64 * (16 * mb + j)] * w;
+        for (int mb = 0; mb < MB; ++mb)
+#pragma unroll
+          for (int j = 0; j < 16; ++j)
+            acc[MB * round + mb][j] = acc[MB * round + mb][j] * a + area[64 * (16 * mb + j)] * w;
+      }
     }
   };
 
-  // One step: its place c0, the one behind it c1 and (FP8) c2.
-  Cursor c0{}, c1{}, c2{};
-  auto take = [&](int S, uint16_t* sk, uint16_t* sv) __attribute__((always_inline)) {
+  // One step: its place c0, and those behind it (bf16 uses one).
+  Cursor c0{}, c1{}, c2{}, c3{};
+  auto take = [&](int S, uint16_t* sk, uint16_t* sv, u32 buf) __attribute__((always_inline)) {
     const bool active = c0.n * p.group > first_row;
     if (active && (S == r.S0 || c0.j == 0)) start(c0);
-    if (active) compute(c0, sk, sv);
+    if (active) compute(c0, sk, sv, lds_addr(s_raw[FP8 ? buf : 0]));
     if (c0.j + 1 == c0.nsteps || S + 1 == r.S1) {
       const int from = S - c0.j, to = from + c0.nsteps;  // the sequence's steps
-      if (KW == 2) join(sk, sv);
+      if (KW == 2) join(sk, sv, buf);
       if (active && kw == 0) emit(c0, from >= r.S0 && to <= r.S1, 2 * r.index + (from > r.S0 ? 1 : 0));
     }
   };
   start_seq<STEP>(p, c0, r.first, r.S0 - uniform(s_cum[r.first]));
   if constexpr (FP8) {
-    issue(c0, s_raw[0], s_raw[0] + kTile, s_raw[0] + 2 * kTile);
+    auto issue_to = [&](const Cursor& c, int buf) __attribute__((always_inline)) {
+      issue(c, s_raw[buf], s_raw[buf] + kTile, s_raw[buf] + 2 * kTile);
+    };
+    issue_to(c0, 0);
     if (r.S0 + 1 < r.S1) {
       next_step<STEP>(p, s_cum, c0, c1);
-      issue(c1, s_raw[FP8 ? 1 : 0], s_raw[FP8 ? 1 : 0] + kTile, s_raw[FP8 ? 1 : 0] + 2 * kTile);
+      issue_to(c1, FP8 ? 1 : 0);
+    }
+    if (r.S0 + 2 < r.S1) {
+      next_step<STEP>(p, s_cum, c1, c2);
+      issue_to(c2, FP8 ? 2 : 0);
     }
 #pragma unroll 1
     for (int S = r.S0; S < r.S1; ++S) {
-      const int buf = (S - r.S0) & 1;
-      if (S + 2 < r.S1) next_step<STEP>(p, s_cum, c1, c2);
-      if (S + 1 < r.S1) wait_vmem<kOps>();  // the next step's loads stay in flight
+      const int buf = (S - r.S0) & (kRawTiles - 1);
+      if (S + 3 < r.S1) next_step<STEP>(p, s_cum, c2, c3);
+      if (S + 2 < r.S1) wait_vmem<2 * kOps>();  // later steps' loads stay in flight
+      else if (S + 1 < r.S1) wait_vmem<kOps>();
       else wait_vmem<0>();
-      tile_barrier();  // all waves are done with the tile
-      widen(buf);
-      tile_barrier();
-      if (S + 2 < r.S1) issue(c2, s_raw[buf], s_raw[buf] + kTile, s_raw[buf] + 2 * kTile);
-      take(S, s_k0, s_v0);
+      tile_barrier();  // the other waves' part of the tile, and they are done with the one before
+      if (S + 3 < r.S1) issue_to(c3, (buf + 3) & (kRawTiles - 1));
+      take(S, s_k0, s_v0, buf);
       c0 = c1;
       c1 = c2;
+      c2 = c3;
     }
   } else {
     issue(c0, reinterpret_cast<char*>(s_k0), reinterpret_cast<char*>(s_v0), nullptr);
@@ -1047,7 +1123,7 @@ __global__ __launch_bounds__(kThreads, 2) void tree_many_kernel(const TreeParams
       __syncthreads();  // the others', and they are done with the tile before.  (The compiler has to see a fence:
                         // it would wait for the next tile in front of the first read of this one.)
       if (more) issue(c1, reinterpret_cast<char*>(nk), reinterpret_cast<char*>(nv), nullptr);
-      take(S, sk, sv);
+      take(S, sk, sv, 0);
       c0 = c1;
     };
 #pragma unroll 1
@@ -1058,11 +1134,15 @@ __global__ __launch_bounds__(kThreads, 2) void tree_many_kernel(const TreeParams
   }
 }
 
-// Joins the states of sequences that several ranges share: one wave for a query token and head.
-// The wave's four 16-lane rows take the sequence's ranges round robin, 8 dims to a lane, four of
-// each per round trip.
+// Joins the states of sequences that several ranges share, 8 dims to a lane, four ranges per round
+// trip.  SPLIT: one wave for a query token and head, whose four 16-lane rows take the ranges round
+// robin; otherwise each of them has a token and head of its own.
+template <bool SPLIT>
 __global__ __launch_bounds__(kThreads) void tree_merge_kernel(const TreeParams p) {
-  const int row = blockIdx.x * kWaves + uniform(static_cast<int>(threadIdx.x >> 6));  // token and q head
+  constexpr int SPAN = SPLIT ? 4 : 1;
+  const int r4 = (threadIdx.x >> 4) & 3, d = 8 * (threadIdx.x & 15);
+  const int wave = blockIdx.x * kWaves + uniform(static_cast<int>(threadIdx.x >> 6));
+  const int row = SPLIT ? wave : 4 * wave + r4;  // token and q head
   const int b = blockIdx.y;
   const int cb = load_uniform(p.header, kHeaderInts + b), cb1 = load_uniform(p.header, kHeaderInts + b + 1);
   const int spr = load_uniform(p.header, 0);
@@ -1072,15 +1152,15 @@ __global__ __launch_bounds__(kThreads) void tree_merge_kernel(const TreeParams p
   if (np <= 1) return;  // written already
   const int tok = row / p.num_q_heads, h = row - tok * p.num_q_heads;
   const int kvh = div_by(h, p.div_group), r = tok * p.group + h - kvh * p.group;  // row of the kv head
-  const int r4 = (threadIdx.x >> 4) & 3, d = 8 * (threadIdx.x & 15);
+  const int k_first = SPLIT ? r4 : 0;
   float m = kMaxFloor, l = 0.f, o[8] = {};
 #pragma unroll 1
-  for (int k0 = r4; k0 - r4 < np; k0 += 16) {
+  for (int k0 = k_first; k0 - k_first < np; k0 += 4 * SPAN) {
     float2 st[4];
     float4 x[4], y[4];
 #pragma unroll
     for (int u = 0; u < 4; ++u) {
-      const int k = min(k0 + 4 * u, np - 1);
+      const int k = min(k0 + SPAN * u, np - 1);
       const int place = 2 * (first + k) + (k == 0 && cb > first * spr ? 1 : 0);
       const int64_t at = (static_cast<int64_t>(place) * p.num_kv_heads + kvh) * p.rows + r;
       st[u] = *reinterpret_cast<const float2*>(p.part_ml + 2 * at);
@@ -1089,7 +1169,7 @@ __global__ __launch_bounds__(kThreads) void tree_merge_kernel(const TreeParams p
     }
 #pragma unroll
     for (int u = 0; u < 4; ++u) {
-      if (k0 + 4 * u >= np) break;
+      if (k0 + SPAN * u >= np) break;
       const float m_new = fmaxf(m, st[u].x), alpha = fast_exp2(m - m_new), w = fast_exp2(st[u].x - m_new);
       const float v[8] = {x[u].x, x[u].y, x[u].z, x[u].w, y[u].x, y[u].y, y[u].z, y[u].w};
       m = m_new;
@@ -1098,13 +1178,17 @@ __global__ __launch_bounds__(kThreads) void tree_merge_kernel(const TreeParams p
       for (int j = 0; j < 8; ++j) o[j] = o[j] * alpha + w * v[j];
     }
   }
-  const float mm = xor32_max(xor16_max(m));
-  const float w = fast_exp2(m - mm);
-  const float sum = xor32_sum(xor16_sum(l * w));
-  const float inv = sum == 0.f ? 0.f : 1.f / sum;
+  if constexpr (SPLIT) {
+    const float mm = xor32_max(xor16_max(m));
+    const float w = fast_exp2(m - mm);
+    l = xor32_sum(xor16_sum(l * w));
 #pragma unroll
-  for (int j = 0; j < 8; ++j) o[j] = xor32_sum(xor16_sum(o[j] * w)) * inv;
-  if (r4 == 0) *reinterpret_cast<uint4*>(p.out + (s.q0 + tok) * p.o_tok_stride + h * p.o_head_stride + d) = pack8(o);
+    for (int j = 0; j < 8; ++j) o[j] = xor32_sum(xor16_sum(o[j] * w));
+  }
+  const float inv = l == 0.f ? 0.f : 1.f / l;
+#pragma unroll
+  for (int j = 0; j < 8; ++j) o[j] *= inv;
+  if (!SPLIT || r4 == 0) *reinterpret_cast<uint4*>(p.out + (s.q0 + tok) * p.o_tok_stride + h * p.o_head_stride + d) = pack8(o);
 }
 
 // How a batch is cut: by its rows per kv head, and into as many ranges as the GPU holds at once.
@@ -1289,9 +1373,16 @@ int launch(const char* fn, const TreeArgs& a, hipStream_t stream) {
     if (pl.waves == 0) hipLaunchKernelGGL(tree_few_kernel<FP8>, grid, block, 0, stream, p);
     else if (pl.waves == 2) hipLaunchKernelGGL((tree_many_kernel<FP8, 2>), grid, block, 0, stream, p);
     else hipLaunchKernelGGL((tree_many_kernel<FP8, 1>), grid, block, 0, stream, p);
-    if (pl.ranges > 1)
-      hipLaunchKernelGGL(tree_merge_kernel, dim3((a.max_q * a.num_q_heads + kWaves - 1) / kWaves, p.num_seqs), block, 0,
-                         stream, p);
+    if (pl.ranges > 1) {
+      // A wave for every row while they fit the GPU at once (32 to a CU): rows are few then, and of many
+      // ranges each.
+      const int rows = a.max_q * a.num_q_heads;
+      const bool split = static_cast<int64_t>(rows) * p.num_seqs <= 8192;
+      const int per = split ? kWaves : 4 * kWaves;
+      const dim3 rows_grid(static_cast<unsigned>((rows + per - 1) / per), static_cast<unsigned>(p.num_seqs));
+      if (split) hipLaunchKernelGGL(tree_merge_kernel<true>, rows_grid, block, 0, stream, p);
+      else hipLaunchKernelGGL(tree_merge_kernel<false>, rows_grid, block, 0, stream, p);
+    }
     const int rc = launch_status(fn);
     if (rc != KVP_OK) return rc;
   }

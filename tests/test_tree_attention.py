@@ -413,3 +413,13 @@ def test_wrappers_check_types_shapes_and_devices(cuda_device):
                 dict(k_scale=None), dict(cache_seqlens=y.ctx), dict(out=y.q.cuda().float())):
         with pytest.raises((ValueError, AttributeError)):
             decode(y, **bad)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("quantised", [False, True])
+def test_many_rows_of_sequences_that_ranges_cut(cuda_device, quantised):
+    """More rows than are joined a wave each: 24 sequences of up to 12 drafts at 32 heads."""
+    rng = random.Random(9)
+    x = Batch([rng.randint(0, 400) for _ in range(23)] + [1500], [rng.randint(1, 12) for _ in range(23)] + [12], 32, 8, 64,
+              quantised)
+    x.check(x.run())
