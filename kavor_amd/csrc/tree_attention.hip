@@ -26,9 +26,9 @@
 // Layouts are those of the decode kernel (lane l: n = l % 16, q4 = l / 16): S = K Q^T has tokens
 // 4 q4 + j of every 16 in the lane and row n as its column, O^T = V^T P^T takes P from the same
 // registers.  e4m3 is widened to bf16, exactly, on its way from LDS to the matrix cores, K with its
-// scale (the lane's own token), V's scale going into P.  P is rounded to bf16: at most 2^-8 of each weight, of either sign,
-// so below the rounding of the bf16 output where the values do not cancel; the sum of the weights
-// is of the unrounded ones, and running maxima, sums and products stay in 32 bits.
+// scale (the lane's own token), V's scale going into P.  P is rounded to bf16: at most 2^-8 of each
+// weight, of either sign, so below the rounding of the bf16 output where the values do not cancel; the
+// sum of the weights is of the unrounded ones, and running maxima, sums and products stay in 32 bits.
 #include <math.h>
 
 #include <algorithm>
@@ -397,8 +397,8 @@ struct Rows {
   }
   // Weights of 32 tokens from their scores s0 (tokens 4 q4 + j) and s1 (16 + 4 q4 + j), packed as the
   // second product's operand; `draft` is the first token's draft, below 0 in the context.  The running
-  // maximum m moves only where a score lies 2^8 above it: weights reach 2^8 at most, and the sums are
-  // rarely multiplied.
+  // maximum m moves only where a score lies 7 above it: weights reach 2^7 at most (which times a scale
+  // of 2^120 bf16 still holds), and the sums are rarely multiplied.
   __device__ __forceinline__ u32x4_t weigh(int nt, mfma_f32x4_t s0, mfma_f32x4_t s1, float scale, bool tail, int draft,
                                            int q4) {
     float x[8];
@@ -415,7 +415,7 @@ struct Rows {
 #pragma unroll
     for (int e = 1; e < 8; ++e) mx = fmaxf(mx, x[e]);
     mx = xor32_max(xor16_max(mx)) * scale;
-    if (__any(mx > m[nt] + 8.f)) {
+    if (__any(mx > m[nt] + 7.f)) {
       const float m_new = fmaxf(m[nt], mx);
       const float alpha = fast_exp2(m[nt] - m_new);
       m[nt] = m_new;
@@ -503,7 +503,9 @@ struct Rows {
 };
 
 // Up to 16 rows per kv head: a wave for itself, with the tiles of two steps in flight in its own LDS,
-// so that no wave waits for another.
+// so that no wave waits for another.  One query token and e4m3, 8 kv heads: 256 sequences of 100 to
+// 2048 tokens take 107 us (5.3 TB/s), 128 of 1024 to 32768 727 us (6.1 TB/s), one of 611 7.2 us (a chain
+// of dependent loads).
 template <bool FP8>
 __global__ __launch_bounds__(kThreads) void tree_few_kernel(const TreeParams p) {
   using F = Format<FP8>;
@@ -651,6 +653,11 @@ __global__ __launch_bounds__(kThreads) void tree_few_kernel(const TreeParams p) 
 // Two workgroups on a CU: one computes while the other waits.  bf16: two tiles, the next one loaded while a tile
 // is used.  e4m3: four, three of them being loaded, and every wave widens what it reads.
 //
+// Matrix and vector instructions bound it, and they add up (64 tokens of a wave with 32 rows: 1024 cycles of
+// products, 275 vector instructions in bf16, 487 in e4m3).  24 sequences of 1000 to 9000 tokens with 61 to 64
+// drafts at 64 heads take 323 us (766 TFLOP/s); a call of 32 of 8192 with 8, 16 and 25 drafts at 32 heads in e4m3 125,
+// 160 and 235 us (KW = 2, 2, 1), with tiles that are widened once for all waves through LDS 146, 168 and 235.
+//
 // Tile rows are 256 bytes, 16-byte chunk c of token r at chunk c ^ (r % 16) of K and c ^ 4 (r % 4) of V; in
 // e4m3 128 bytes, c ^ ((r / 2) % 8) and c ^ ((r & 2) + (r & 8) / 2).  The lane
 // gets the scores of tokens 8 (i / 4) + 4 hf + i % 4 of each 32, and of O^T dims 32 mb + 8 (j / 4) + 4 hf + j % 4.
@@ -659,7 +666,7 @@ constexpr int kTileElems = kManyStep * kDim;
 constexpr int kRawTiles = 4, kRawBytes = 2 * kTile + 2 * kManyStep;
 // A row's weights of one step sum up to this before its maximum is taken again (see weigh).
 constexpr float kSumLimit = 65536.f;
-constexpr float kSumLimitScaled = 256.f;  // e4m3: and times a scale they are to fit bf16
+constexpr float kSumLimitScaled = 128.f;  // e4m3: and times a scale (2^120 at most) they are to fit bf16
 
 // One or two blocks of 32 tokens (4096 bytes each) in e4m3: K from the lane's four addresses in the first, its
 // exponent byte at `ka`, those of V's tokens 8 i + 0 .. 3 at `va` + 8 i.
