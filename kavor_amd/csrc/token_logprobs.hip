@@ -9,8 +9,8 @@
 //
 // What bounds it: HBM, with the vector ALUs close behind: a bf16 value has to be widened, entered
 // into a maximum, exponentiated (at less than the full rate) and summed twice.  4096 bf16 rows of
-// 151936 take 226 us (5.5 TB/s, the ALUs 80% busy), with 64 alternatives 300; 256 fp32 rows of
-// 151643 35 us (4.5 TB/s: finding the alternatives takes the last 5).
+// 151936 take 211 us (5.9 TB/s, the ALUs 80% busy), with 64 alternatives 290; 256 fp32 rows of
+// 151643 32 us (4.9 TB/s: finding the alternatives takes the last 5).
 //
 // Alternatives, without a comparison more per value: a thread keeps the largest of its own values,
 // which it needs anyway, so the k-th largest of the threads' maxima is a lower bound of the row's k-th
@@ -245,8 +245,7 @@ __global__ __launch_bounds__(kThreads) void logprobs_kernel(const LogprobParams 
     }
   };
   auto load = [&](int c) {  // a whole chunk of the row, whatever c
-    return full > 0 ? *reinterpret_cast<const uint4*>(row + E * static_cast<int64_t>(min(c, full - 1)))
-                    : make_uint4(0, 0, 0, 0);
+    return full > 0 ? load16_nt(row + E * static_cast<int64_t>(min(c, full - 1))) : make_uint4(0, 0, 0, 0);
   };
 
   // Batches of 32 values per thread, the next one in flight while one is taken; what is left of the

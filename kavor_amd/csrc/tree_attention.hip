@@ -269,9 +269,9 @@ __device__ __forceinline__ void issue_tile(const TreeParams& p, const TileLane& 
                                       static_cast<uint32_t>((Format<FP8>::kStep - 1) * stride + Format<FP8>::kRow));
   const int last = (rows - 1) * stride;
 #pragma unroll
-  for (int i = 0; i < 8; ++i)
+  for (int i = 0; i < 8; ++i)  // nontemporal: every row is read once
     raw_buffer_load_lds(rsrc, (LdsPtr)(tile + 1024 * i), 16,
-                        min(t.row_off + kPer * i * stride, last) + (V ? t.v_chunk[i & 1] : t.k_chunk[i & 3]), 0, 0, 0);
+                        min(t.row_off + kPer * i * stride, last) + (V ? t.v_chunk[i & 1] : t.k_chunk[i & 3]), 0, 0, 2);
 }
 // The scales of a step's 64 tokens: K's bytes, then V's.
 __device__ __forceinline__ void issue_scales(const TreeParams& p, int64_t base, int lane, char* to) {
@@ -504,8 +504,8 @@ struct Rows {
 
 // Up to 16 rows per kv head: a wave for itself, with the tiles of two steps in flight in its own LDS,
 // so that no wave waits for another.  One query token and e4m3, 8 kv heads: 256 sequences of 100 to
-// 2048 tokens take 107 us (5.3 TB/s), 128 of 1024 to 32768 727 us (6.1 TB/s), one of 611 7.2 us (a chain
-// of dependent loads).
+// 2048 tokens take 93 us (6.1 TB/s), 128 of 1024 to 32768 648 us (6.9 TB/s; 727 with loads that are not
+// nontemporal), one of 611 7.2 us (a chain of dependent loads).
 template <bool FP8>
 __global__ __launch_bounds__(kThreads) void tree_few_kernel(const TreeParams p) {
   using F = Format<FP8>;
@@ -655,8 +655,8 @@ __global__ __launch_bounds__(kThreads) void tree_few_kernel(const TreeParams p) 
 //
 // Matrix and vector instructions bound it, and they add up (64 tokens of a wave with 32 rows: 1024 cycles of
 // products, 275 vector instructions in bf16, 487 in e4m3).  24 sequences of 1000 to 9000 tokens with 61 to 64
-// drafts at 64 heads take 323 us (766 TFLOP/s); a call of 32 of 8192 with 8, 16 and 25 drafts at 32 heads in e4m3 125,
-// 160 and 235 us (KW = 2, 2, 1), with tiles that are widened once for all waves through LDS 146, 168 and 235.
+// drafts at 64 heads take 323 us (766 TFLOP/s); a call of 32 of 8192 with 8, 16 and 25 drafts at 32 heads in e4m3 121,
+// 154 and 235 us (KW = 2, 2, 1), with tiles that are widened once for all waves through LDS 146, 168 and 235.
 //
 // Tile rows are 256 bytes, 16-byte chunk c of token r at chunk c ^ (r % 16) of K and c ^ 4 (r % 4) of V; in
 // e4m3 128 bytes, c ^ ((r / 2) % 8) and c ^ ((r & 2) + (r & 8) / 2).  The lane
@@ -753,15 +753,18 @@ __global__ __launch_bounds__(kThreads, 2) void tree_many_kernel(const TreeParams
     const int row_off = (16 * wave + lr) * stride;
     const int k_chunk = 16 * (FP8 ? lc ^ (lr >> 1) : lc ^ lr), v_chunk = 16 * (FP8 ? lc ^ (lr & 2) : lc ^ (4 * (lr & 3)));
     const BufferRsrc kr = buffer_rsrc(p.k_cache + base, bytes), vr = buffer_rsrc(p.v_cache + base, bytes);
+    // Nontemporal where rows are read once: 32 sequences of 8192, 16 drafts at 32 heads in bf16 188 us against 212.
+    // Blocks of 128 rows read them again (8 heads to a kv head: 394 us against 368).
+    constexpr int kNt = KW == 2 ? 2 : 0;
     // row 16 wave + 4 i + lr (e4m3: 8 i): the part of i in the swizzle is 4 i chunks, but none in bf16's V
 #pragma unroll
     for (int i = 0; i < kFills; ++i)
       raw_buffer_load_lds(kr, (LdsPtr)(k_to + 1024 * (kFills * wave + i)), 16,
-                          min(row_off + (FP8 ? 8 : 4) * i * stride, last) + (k_chunk ^ (64 * i)), 0, 0, 0);
+                          min(row_off + (FP8 ? 8 : 4) * i * stride, last) + (k_chunk ^ (64 * i)), 0, 0, kNt);
 #pragma unroll
     for (int i = 0; i < kFills; ++i)
       raw_buffer_load_lds(vr, (LdsPtr)(v_to + 1024 * (kFills * wave + i)), 16,
-                          min(row_off + (FP8 ? 8 : 4) * i * stride, last) + (FP8 ? v_chunk ^ (64 * i) : v_chunk), 0, 0, 0);
+                          min(row_off + (FP8 ? 8 : 4) * i * stride, last) + (FP8 ? v_chunk ^ (64 * i) : v_chunk), 0, 0, kNt);
     if (FP8) issue_scales(p, uniform(c.blk * p.scale_blk_stride + scale_head + off), ln, scale_to);
   };
   // ---- the wave's rows
