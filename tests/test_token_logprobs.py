@@ -174,3 +174,14 @@ def test_wrapper_checks_types_and_shapes(cuda_device):
     for bad in ((x, t, 65), (torch.zeros(4, 65, device=cuda_device), t)):
         with pytest.raises(_lib.KVPathError):
             fused.token_logprobs(*bad)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+@pytest.mark.parametrize("rows,vocab,top", [(1, 1, 1), (3, 5, 5), (2, 63, 63), (255, 70, 64), (256, 70, 64), (16, 40, 33),
+                                            (1, 200003, 64)])
+def test_small_vocabularies_and_the_bounds_of_the_split(cuda_device, dtype, rows, vocab, top):
+    g = gen(7 * rows + vocab)
+    logits = (torch.randn(rows, vocab, generator=g) * 3).to(dtype)
+    tokens = torch.randint(0, vocab, (rows,), generator=g)
+    check(run(logits, tokens, top), logits, tokens, top)

@@ -423,3 +423,27 @@ def test_many_rows_of_sequences_that_ranges_cut(cuda_device, quantised):
     x = Batch([rng.randint(0, 400) for _ in range(23)] + [1500], [rng.randint(1, 12) for _ in range(23)] + [12], 32, 8, 64,
               quantised)
     x.check(x.run())
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("quantised", [False, True])
+@pytest.mark.parametrize("case", [
+    ([5, 70], [2, 3], 256, 256, 64), ([300, 10], [64, 40], 16, 1, 64), ([0, 1000], [64, 64], 32, 2, 128),
+    ([200, 77], [22, 30], 9, 3, 64), ([5000, 10, 20], [20, 1, 3], 8, 2, 64)], ids=lambda c: f"n{c[1]}h{c[2]}x{c[3]}")
+def test_the_ends_of_the_limits(cuda_device, case, quantised):
+    """256 kv heads, 1024 rows of one kv head in blocks, three query heads to one, a long sequence among short ones."""
+    x = Batch(*case, quantised)
+    x.check(x.run())
+
+
+@pytest.mark.gpu
+def test_weights_times_the_largest_scale_stay_finite(cuda_device):
+    """Rows of zeros at the largest scale, 2^120: the scale goes into the weights, and an infinite product
+    of the two would make NaN of the zeros."""
+    for drafts in (1, 30):
+        x = Batch([200], [drafts], 2, 1, 64, True)
+        k, v, ks, vs = x.dev
+        vs.fill_(247)
+        v.view(torch.uint8).zero_()
+        got = x.run().cpu()
+        assert torch.equal(got, torch.zeros_like(got))
