@@ -494,8 +494,8 @@ def _table(block_table: torch.Tensor, rows: int, like: torch.Tensor):
     n, width = block_table.shape
     if n < rows:
         raise ValueError("block_table has fewer rows than sequences")
-    # a single row may have any stride
-    return block_table.data_ptr(), max(block_table.stride(0), width), width
+    # a single row may have any stride; the library refuses rows that overlap
+    return block_table.data_ptr(), block_table.stride(0) if n > 1 else width, width
 
 
 def store_kvcache_fp8(key: torch.Tensor, value: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor,

@@ -447,3 +447,21 @@ def test_weights_times_the_largest_scale_stay_finite(cuda_device):
         v.view(torch.uint8).zero_()
         got = x.run().cpu()
         assert torch.equal(got, torch.zeros_like(got))
+
+
+@pytest.mark.gpu
+def test_block_tables_whose_rows_overlap_are_refused(cuda_device):
+    """An expanded table is one row in memory: with another stride the rows behind it would be read from
+    beyond its end."""
+    x = Batch([100, 90], [2, 3], 4, 2, 64, True)
+    k, v, ks, vs = x.dev
+    q, cu, ctx, bt = (t.to(cuda_device) for t in (x.q, x.cu, x.ctx, x.bt))
+    shared = bt[:1].expand(2, -1)
+    with pytest.raises((ValueError, _lib.KVPathError)):
+        attention.tree_attention(q, k, v, cu, 3, ctx, shared, SCALE, k_scale=ks, v_scale=vs)
+    with pytest.raises((ValueError, _lib.KVPathError)):
+        attention.paged_decode_fp8(q[:2], k, v, ks, vs, ctx, shared, SCALE)
+    with pytest.raises((ValueError, _lib.KVPathError)):
+        attention.load_kvcache_fp8(k, v, ks, vs, shared, cu, 5)
+    one = torch.empty_strided((1, bt.shape[1]), (1, 1), dtype=torch.int32, device=cuda_device).copy_(bt[:1])
+    attention.load_kvcache_fp8(k, v, ks, vs, one, cu[:2], 2)
