@@ -123,3 +123,42 @@ def test_the_loop_captured_into_a_graph(cuda_device):
         eager = loop.step()
         torch.cuda.synchronize()
         assert all(bits_equal(a, b) for a, b in zip(got[:2], eager[:2]))
+
+
+def far_apart(x: torch.Tensor, stride: int) -> torch.Tensor:
+    """x with its first dimension at another stride, on the GPU."""
+    room = torch.empty((x.shape[0] - 1) * stride + x[0].numel(), dtype=x.dtype, device="cuda")
+    y = room.as_strided(x.shape, (stride,) + x.stride()[1:])
+    return y.copy_(x) if x.dtype != torch.float8_e4m3fn else (y.view(torch.uint8).copy_(x.view(torch.uint8)), y)[1]
+
+
+@pytest.mark.gpu
+def test_offsets_beyond_32_bits(cuda_device):
+    """Pages and rows of logits more than 2^32 bytes from the first one: the same bits as close together."""
+    g = gen(2)
+    pool = quantised_pool(3, BLOCK, HKV, D, g).to(cuda_device)
+    near = tuple(t.contiguous() for t in pool_views(pool, BLOCK, HKV, D))
+    far = tuple(far_apart(t, (5 << 29) + 64) for t in near)
+    bt = torch.tensor([[2, 0, 1]], dtype=torch.int32, device=cuda_device)
+    cu, ctx = (torch.tensor(t, dtype=torch.int32, device=cuda_device) for t in ([0, 5], [170]))
+    slots = torch.tensor([2 * BLOCK + 3, BLOCK + 9], dtype=torch.int32, device=cuda_device)
+    new = randn_bf16((2, HKV, D), g).to(cuda_device)
+    for hq in (H, 16 * HKV):  # few rows per kv head, and many
+        q = randn_bf16((5, hq, D), g).to(cuda_device)
+        got = []
+        for k, v, ks, vs in (near, far):
+            attention.store_kvcache_fp8(new, new, k, v, ks, vs, slots)
+            read = attention.load_kvcache_fp8(k, v, ks, vs, bt, torch.tensor([0, 170], dtype=torch.int32, device="cuda"), 170)
+            got.append((*read, attention.paged_decode_fp8(q[:1], k, v, ks, vs, ctx, bt, SCALE),
+                        attention.tree_attention(q, k, v, cu, 5, ctx, bt, SCALE, k_scale=ks, v_scale=vs)))
+        assert all(bits_equal(a, b) for a, b in zip(*got))
+        wide = [attention.load_kvcache_fp8(*near, torch.tensor([[0, 1, 2]], dtype=torch.int32, device="cuda"),
+                                           torch.tensor([0, 3 * BLOCK], dtype=torch.int32, device="cuda"), 3 * BLOCK)][0]
+        k, v = (t.view(3, BLOCK, HKV, D) for t in wide)
+        a = attention.tree_attention(q, k, v, cu, 5, ctx, bt, SCALE)
+        b = attention.tree_attention(q, far_apart(k, (5 << 28) + 64), far_apart(v, (5 << 28) + 64), cu, 5, ctx, bt, SCALE)
+        assert bits_equal(a, b)
+    logits = torch.randn(3, VOCAB + 3, generator=g).to(cuda_device)
+    ids = torch.tensor([1, 2, 3], device=cuda_device)
+    for a, b in zip(fused.token_logprobs(logits, ids, 4), fused.token_logprobs(far_apart(logits, 3 << 28), ids, 4)):
+        assert torch.equal(a, b)
