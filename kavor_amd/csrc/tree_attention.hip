@@ -404,12 +404,13 @@ struct Rows {
     float x[8];
 #pragma unroll
     for (int e = 0; e < 8; ++e) x[e] = e < 4 ? s0[e] : s1[e - 4];
-    if (tail) {
+    if (tail) {  // hidden behind the scale: at 0 the product would be NaN
 #pragma unroll
       for (int e = 0; e < 8; ++e) {
         const int d = draft + 16 * (e >> 2) + 4 * q4 + (e & 3);
-        x[e] = sees(seen[nt], d) ? x[e] : -INFINITY;
+        x[e] = sees(seen[nt], d) ? x[e] * scale : -INFINITY;
       }
+      scale = 1.f;
     }
     float mx = x[0];
 #pragma unroll
@@ -848,14 +849,16 @@ __global__ __launch_bounds__(kThreads, 2) void tree_many_kernel(const TreeParams
       __builtin_amdgcn_sched_group_barrier(0x008, 4, 0);
     }
     __builtin_amdgcn_s_setprio(0);
-    if (tail) {
+    float scale = p.scale_log2;
+    if (tail) {  // hidden behind the scale: at 0 the product would be NaN
 #pragma unroll
       for (int mb = 0; mb < BLOCKS; ++mb)
 #pragma unroll
         for (int j = 0; j < 16; ++j) {
           const int d = draft + 32 * mb + 8 * (j >> 2) + 4 * hf + (j & 3);
-          sc[mb][j] = sees(seen, d) ? sc[mb][j] : -INFINITY;
+          sc[mb][j] = sees(seen, d) ? sc[mb][j] * scale : -INFINITY;
         }
+      scale = 1.f;
     }
     // ---- weights.  A row's maximum is taken of the first step, and again only where the weights of a
     // step sum up to more than 2^16: their relative precision does not depend on it.
@@ -865,7 +868,7 @@ __global__ __launch_bounds__(kThreads, 2) void tree_many_kernel(const TreeParams
       for (int mb = 0; mb < BLOCKS; ++mb)
 #pragma unroll
         for (int j = 0; j < 16; ++j) mx = fmaxf(mx, sc[mb][j]);
-      return half_swap_max(mx) * p.scale_log2;
+      return half_swap_max(mx) * scale;
     };
     if (fresh) m = fmaxf(step_max(), kMaxFloor);
     fresh = false;
@@ -877,8 +880,8 @@ __global__ __launch_bounds__(kThreads, 2) void tree_many_kernel(const TreeParams
       for (int mb = 0; mb < BLOCKS; ++mb)
 #pragma unroll
         for (int j = 0; j < 16; j += 2) {
-          const float w0 = fast_exp2(fmaf(sc[mb][j], p.scale_log2, -m));
-          const float w1 = fast_exp2(fmaf(sc[mb][j + 1], p.scale_log2, -m));
+          const float w0 = fast_exp2(fmaf(sc[mb][j], scale, -m));
+          const float w1 = fast_exp2(fmaf(sc[mb][j + 1], scale, -m));
           sum += w0 + w1;
           pk[mb][j >> 1] = pack_bf16x2(w0, w1);
         }
