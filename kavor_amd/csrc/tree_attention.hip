@@ -404,13 +404,12 @@ struct Rows {
     float x[8];
 #pragma unroll
     for (int e = 0; e < 8; ++e) x[e] = e < 4 ? s0[e] : s1[e - 4];
-    if (tail) {  // hidden behind the scale: at 0 the product would be NaN
+    if (tail) {
 #pragma unroll
       for (int e = 0; e < 8; ++e) {
         const int d = draft + 16 * (e >> 2) + 4 * q4 + (e & 3);
-        x[e] = sees(seen[nt], d) ? x[e] * scale : -INFINITY;
+        x[e] = sees(seen[nt], d) ? x[e] : -INFINITY;
       }
-      scale = 1.f;
     }
     float mx = x[0];
 #pragma unroll
@@ -849,16 +848,14 @@ __global__ __launch_bounds__(kThreads, 2) void tree_many_kernel(const TreeParams
       __builtin_amdgcn_sched_group_barrier(0x008, 4, 0);
     }
     __builtin_amdgcn_s_setprio(0);
-    float scale = p.scale_log2;
-    if (tail) {  // hidden behind the scale: at 0 the product would be NaN
+    if (tail) {
 #pragma unroll
       for (int mb = 0; mb < BLOCKS; ++mb)
 #pragma unroll
         for (int j = 0; j < 16; ++j) {
           const int d = draft + 32 * mb + 8 * (j >> 2) + 4 * hf + (j & 3);
-          sc[mb][j] = sees(seen, d) ? sc[mb][j] * scale : -INFINITY;
+          sc[mb][j] = sees(seen, d) ? sc[mb][j] : -INFINITY;
         }
-      scale = 1.f;
     }
     // ---- weights.  A row's maximum is taken of the first step, and again only where the weights of a
     // step sum up to more than 2^16: their relative precision does not depend on it.
@@ -868,7 +865,7 @@ __global__ __launch_bounds__(kThreads, 2) void tree_many_kernel(const TreeParams
       for (int mb = 0; mb < BLOCKS; ++mb)
 #pragma unroll
         for (int j = 0; j < 16; ++j) mx = fmaxf(mx, sc[mb][j]);
-      return half_swap_max(mx) * scale;
+      return half_swap_max(mx) * p.scale_log2;
     };
     if (fresh) m = fmaxf(step_max(), kMaxFloor);
     fresh = false;
@@ -880,8 +877,8 @@ __global__ __launch_bounds__(kThreads, 2) void tree_many_kernel(const TreeParams
       for (int mb = 0; mb < BLOCKS; ++mb)
 #pragma unroll
         for (int j = 0; j < 16; j += 2) {
-          const float w0 = fast_exp2(fmaf(sc[mb][j], scale, -m));
-          const float w1 = fast_exp2(fmaf(sc[mb][j + 1], scale, -m));
+          const float w0 = fast_exp2(fmaf(sc[mb][j], p.scale_log2, -m));
+          const float w1 = fast_exp2(fmaf(sc[mb][j + 1], p.scale_log2, -m));
           sum += w0 + w1;
           pk[mb][j >> 1] = pack_bf16x2(w0, w1);
         }
@@ -1355,7 +1352,10 @@ int launch(const char* fn, const TreeArgs& a, hipStream_t stream) {
   p.num_kv_heads = a.num_kv_heads;
   p.group = a.num_q_heads / a.num_kv_heads;
   p.mask = a.mask;
-  p.scale_log2 = fabsf(a.softmax_scale) * 1.4426950408889634f;  // its sign goes into q
+  // The kernels hide a score as -inf and scale it afterwards, which asks for a positive scale: its sign goes into q,
+  // and 0 counts as 2^-149, which moves no score that is finite in 32 bits by more than 2^-21.
+  p.scale_log2 = fabsf(a.softmax_scale) * 1.4426950408889634f;
+  if (p.scale_log2 == 0.f) p.scale_log2 = __FLT_DENORM_MIN__;
   p.q_flip = a.softmax_scale < 0.f ? 0x80008000u : 0u;
   p.o_tok_stride = a.o_tok_stride;
   p.o_head_stride = a.o_head_stride;
