@@ -424,6 +424,8 @@ size_t kvp_tree_workspace_bytes(int32_t max_num_seqs, int32_t max_seqlen_q, int3
 /*
  * kvp_paged_decode_bf16 over a quantised cache, for any GQA ratio up to 16: q and out in bf16,
  * everything between in 32 bits but the softmax weights, which enter the second product in bf16.
+ * The sums of V have weights up to 1 on the way and are divided at the end: a sequence's tokens, in
+ * whole 64s, times the largest |V| have to stay below 2^128, or infinities and NaN appear.
  * Scale pointers and strides are multiples of 4 bytes.  Rows with context_lens[b] <= 0 are
  * zeros, rows with an impossible length or a needed block id outside the pool NaN, as there.
  * head_dim 128; block_size a multiple of 64; block tables of at most 2^24 tokens; cache slot
@@ -457,7 +459,7 @@ int kvp_paged_decode_fp8(const void* q, int64_t q_seq_stride, int64_t q_head_str
  * sequence has are left as they were.
  *   k_scale and v_scale NULL: caches in bf16, strides in elements, multiples of 8; otherwise a
  * quantised cache.  GQA ratio up to 16; the other limits are kvp_paged_decode_fp8's (slot strides
- * up to 2^24 bytes).
+ * up to 2^24 bytes, and those of |V|).
  */
 int kvp_tree_attention(const void* q, int64_t q_tok_stride, int64_t q_head_stride,
                        const void* k_cache, const void* v_cache,

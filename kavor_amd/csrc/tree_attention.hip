@@ -397,8 +397,8 @@ struct Rows {
   }
   // Weights of 32 tokens from their scores s0 (tokens 4 q4 + j) and s1 (16 + 4 q4 + j), packed as the
   // second product's operand; `draft` is the first token's draft, below 0 in the context.  The running
-  // maximum m moves only where a score lies 7 above it: weights reach 2^7 at most (which times a scale
-  // of 2^120 bf16 still holds), and the sums are rarely multiplied.
+  // maximum m follows every score above it: weights are 1 at most, so sums stay within the number of tokens
+  // times the largest V.  The loop waits for memory, and the multiplications of the sums cost no time.
   __device__ __forceinline__ u32x4_t weigh(int nt, mfma_f32x4_t s0, mfma_f32x4_t s1, float scale, bool tail, int draft,
                                            int q4) {
     float x[8];
@@ -415,7 +415,7 @@ struct Rows {
 #pragma unroll
     for (int e = 1; e < 8; ++e) mx = fmaxf(mx, x[e]);
     mx = xor32_max(xor16_max(mx)) * scale;
-    if (__any(mx > m[nt] + 7.f)) {
+    if (__any(mx > m[nt])) {
       const float m_new = fmaxf(m[nt], mx);
       const float alpha = fast_exp2(m[nt] - m_new);
       m[nt] = m_new;
@@ -664,9 +664,6 @@ __global__ __launch_bounds__(kThreads) void tree_few_kernel(const TreeParams p) 
 constexpr int kManyStep = 64;
 constexpr int kTileElems = kManyStep * kDim;
 constexpr int kRawTiles = 4, kRawBytes = 2 * kTile + 2 * kManyStep;
-// A row's weights of one step sum up to this before its maximum is taken again (see weigh).
-constexpr float kSumLimit = 65536.f;
-constexpr float kSumLimitScaled = 128.f;  // e4m3: and times a scale (2^120 at most) they are to fit bf16
 
 // One or two blocks of 32 tokens (4096 bytes each) in e4m3: K from the lane's four addresses in the first, its
 // exponent byte at `ka`, those of V's tokens 8 i + 0 .. 3 at `va` + 8 i.
@@ -857,8 +854,8 @@ __global__ __launch_bounds__(kThreads, 2) void tree_many_kernel(const TreeParams
           sc[mb][j] = sees(seen, d) ? sc[mb][j] : -INFINITY;
         }
     }
-    // ---- weights.  A row's maximum is taken of the first step, and again only where the weights of a
-    // step sum up to more than 2^16: their relative precision does not depend on it.
+    // ---- weights.  A row's maximum is taken of the first step, and again only where the weights of a step sum up to
+    // more than its tokens, so that no sum over a row's tokens is larger than their number times the largest V.
     auto step_max = [&]() __attribute__((always_inline)) {
       float mx = kMaxFloor;
 #pragma unroll
@@ -885,7 +882,7 @@ __global__ __launch_bounds__(kThreads, 2) void tree_many_kernel(const TreeParams
       sum = half_swap_sum(sum);
     };
     weigh();
-    if (__any(!(sum <= (FP8 ? kSumLimitScaled : kSumLimit)))) {  // rare
+    if (__any(!(sum <= 32.f * BLOCKS))) {  // rare
       const float m_new = fmaxf(m, step_max());
       const float alpha = fast_exp2(m - m_new);
       m = m_new;
