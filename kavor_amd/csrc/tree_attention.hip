@@ -335,16 +335,13 @@ __device__ __forceinline__ void wait_tiles(int most) {
   else wait_vmem<0>();
 }
 
-// P of two tokens in packed bf16, times their V scales, bytes 0 and 1 of `bytes`, or 2 and 3: the
-// exponents are added as integers.  A weight below 2^-126 counts as the scale times 2^-127; a masked
-// one (`tail`: there may be some) is 0 whatever the scale.
-typedef uint16_t u16x2_t __attribute__((ext_vector_type(2)));
-__device__ __forceinline__ u32 scale_weights(u32 pk, u32 bytes, bool upper, bool tail) {
-  const u32 vs = __builtin_amdgcn_perm(0, bytes, upper ? 0x0c030c02 : 0x0c010c00) << 7;
-  const u16x2_t one = {127 << 7, 127 << 7};
-  const u32 scaled = __builtin_bit_cast(u32, __builtin_elementwise_sub_sat(
-      static_cast<u16x2_t>(__builtin_bit_cast(u16x2_t, pk) + __builtin_bit_cast(u16x2_t, vs)), one));
-  return !tail ? scaled : ((pk & 0xffffu) ? scaled & 0xffffu : 0u) | ((pk >> 16) ? scaled & 0xffff0000u : 0u);
+// A weight times its token's V scale, byte `i` of `bytes`: exact down to 2^-126, and 0 stays 0 whatever the byte (those
+// behind the last token can be anything).  Two instructions, one of which picks the byte; -127 is held in a vector
+// register, since scalar ones are short (32 sequences of 8192, 8 drafts: 123 us against 129).
+__device__ __forceinline__ float scale_weight(float w, u32 bytes, int i) {
+  int less = -127;
+  asm("" : "+v"(less));
+  return __builtin_ldexpf(w, static_cast<int>(bytes >> (8 * i) & 0xffu) + less);
 }
 
 // Whether a row sees draft d (below 0: a token of the context), given the bits of its drafts.
@@ -399,8 +396,10 @@ struct Rows {
   // second product's operand; `draft` is the first token's draft, below 0 in the context.  The running
   // maximum m follows every score above it: weights are 1 at most, so sums stay within the number of tokens
   // times the largest V.  The loop waits for memory, and the multiplications of the sums cost no time.
-  __device__ __forceinline__ u32x4_t weigh(int nt, mfma_f32x4_t s0, mfma_f32x4_t s1, float scale, bool tail, int draft,
-                                           int q4) {
+  // SCALED: each is multiplied by its V scale, the bytes of v0 and v1.
+  template <bool SCALED>
+  __device__ __forceinline__ u32x4_t weigh(int nt, mfma_f32x4_t s0, mfma_f32x4_t s1, u32 v0, u32 v1, float scale,
+                                           bool tail, int draft, int q4) {
     float x[8];
 #pragma unroll
     for (int e = 0; e < 8; ++e) x[e] = e < 4 ? s0[e] : s1[e - 4];
@@ -426,8 +425,12 @@ struct Rows {
     u32x4_t pf;
 #pragma unroll
     for (int e = 0; e < 8; e += 2) {
-      const float w0 = fast_exp2(fmaf(x[e], scale, -m[nt])), w1 = fast_exp2(fmaf(x[e + 1], scale, -m[nt]));
+      float w0 = fast_exp2(fmaf(x[e], scale, -m[nt])), w1 = fast_exp2(fmaf(x[e + 1], scale, -m[nt]));
       l[nt] += w0 + w1;
+      if (SCALED) {
+        w0 = scale_weight(w0, e < 4 ? v0 : v1, e & 3);
+        w1 = scale_weight(w1, e < 4 ? v0 : v1, (e & 3) + 1);
+      }
       pf[e >> 1] = pack_bf16x2(w0, w1);
     }
     return pf;
@@ -602,11 +605,8 @@ __global__ __launch_bounds__(kThreads) void tree_few_kernel(const TreeParams p) 
       for (int sub = 0; sub < SUBS; ++sub) {  // 32 tokens
         const int draft = t0 + 32 * sub - ctx;
         const bool tail = draft > -32;  // drafts among them, or the last token in front of them
-        u32x4_t pf[1] = {rows.weigh(0, s[2 * sub], s[2 * sub + 1], p.scale_log2, tail, draft, q4)};
-        if constexpr (FP8) {
-#pragma unroll
-          for (int w = 0; w < 4; ++w) pf[0][w] = scale_weights(pf[0][w], vexp[2 * sub + (w >> 1)], w & 1, tail);
-        }
+        const u32x4_t pf[1] = {rows.template weigh<FP8>(0, s[2 * sub], s[2 * sub + 1], vexp[2 * sub], vexp[2 * sub + 1],
+                                                        p.scale_log2, tail, draft, q4)};
         // ---- O^T += V^T P^T
         if (sub == 0) wait_tiles<F::kKOps, F::kVOps>(issued - c0.mark - F::kVOps);
         u32x4_t vt[8];
@@ -874,9 +874,13 @@ __global__ __launch_bounds__(kThreads, 2) void tree_many_kernel(const TreeParams
       for (int mb = 0; mb < BLOCKS; ++mb)
 #pragma unroll
         for (int j = 0; j < 16; j += 2) {
-          const float w0 = fast_exp2(fmaf(sc[mb][j], p.scale_log2, -m));
-          const float w1 = fast_exp2(fmaf(sc[mb][j + 1], p.scale_log2, -m));
+          float w0 = fast_exp2(fmaf(sc[mb][j], p.scale_log2, -m));
+          float w1 = fast_exp2(fmaf(sc[mb][j + 1], p.scale_log2, -m));
           sum += w0 + w1;
+          if (FP8) {
+            w0 = scale_weight(w0, vexp[mb][j >> 2], j & 3);
+            w1 = scale_weight(w1, vexp[mb][j >> 2], (j & 3) + 1);
+          }
           pk[mb][j >> 1] = pack_bf16x2(w0, w1);
         }
       sum = half_swap_sum(sum);
@@ -894,12 +898,6 @@ __global__ __launch_bounds__(kThreads, 2) void tree_many_kernel(const TreeParams
       weigh();
     }
     l += sum;
-    if constexpr (FP8) {
-#pragma unroll
-      for (int mb = 0; mb < BLOCKS; ++mb)
-#pragma unroll
-        for (int i = 0; i < 8; ++i) pk[mb][i] = scale_weights(pk[mb][i], vexp[mb][i >> 1], i & 1, tail);
-    }
     // ---- O^T += V^T P^T, 16 tokens at a time
     auto pf = [&](int kk) __attribute__((always_inline)) {
       const u32* w = &pk[kk >> 1][4 * (kk & 1)];

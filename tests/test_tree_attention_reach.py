@@ -60,3 +60,16 @@ def test_large_values_do_not_overflow_the_sums(cuda_device, rows, quantised):
     got = x.run(mask=None)
     assert got.isfinite().all()
     check(x, got)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("rows", ROWS)
+def test_a_weight_of_zero_takes_no_part_whatever_its_scale(cuda_device, rows):
+    """All tokens but the first 64 lie 200 binary orders and more below these and hold V of 2^121 at most, whose sums
+    fit 32 bits; what they add, less than 700 * 2^-200 * 2^121, is nothing beside values around 2^-6."""
+    x = slopes(rows, True, -200, -6)
+    vs = x.dev[3]
+    for b, n in enumerate(x.lens):
+        for page in x.bt[b, 1:-(-n // 64)].tolist():
+            vs[page] = 243
+    check(x, x.run(mask=None))
