@@ -205,7 +205,6 @@ __device__ __forceinline__ float entropy_of(const State& st) {
   const float h = kLn2 * (log2f(st.s) - st.w / st.s);
   return h < 0.f ? 0.f : h;
 }
-template <typename T>
 __device__ __forceinline__ void finish_row(const LogprobParams& p, int r, const State& st, int64_t token, float x) {
   const bool ok = token >= 0 && token < p.vocab;
   p.logprobs[r] = ok ? log_prob(x, st) : __builtin_nanf("");
@@ -438,7 +437,7 @@ __global__ __launch_bounds__(kThreads) void logprobs_kernel(const LogprobParams 
 
   // ---- out, or to the merge
   if (p.segments == 1) {
-    if (tid == 0) finish_row<T>(p, r, st, token, mine);
+    if (tid == 0) finish_row(p, r, st, token, mine);
     if (wave == 0) write_top(p, r, st, list);
   } else {
     if (tid == 0) p.states[blockIdx.x] = make_float4(st.m, st.s, st.w, __int_as_float(st.above));
@@ -475,7 +474,7 @@ __global__ __launch_bounds__(kThreads) void logprobs_merge_kernel(const LogprobP
   if (tid == 0) {
     const int64_t token = p.tokens[r];
     const T* row = static_cast<const T*>(p.logits) + r * p.row_stride;
-    finish_row<T>(p, r, st, token, token >= 0 && token < p.vocab ? Chunk<T>::one(row[token]) : 0.f);
+    finish_row(p, r, st, token, token >= 0 && token < p.vocab ? Chunk<T>::one(row[token]) : 0.f);
   }
   if (p.top == 0) return;  // uniform
   Key list = 0;

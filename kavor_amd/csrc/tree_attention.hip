@@ -350,47 +350,37 @@ __device__ __forceinline__ bool sees(uint64_t seen, int d) {
 }
 
 // The 16 rows that a wave works on, and the online softmax over the tokens that they have met.
-template <int NT>
 struct Rows {
-  int tok[NT], head[NT], row[NT];
-  u32x4_t q[NT][4];
-  uint64_t seen[NT];  // the drafts that the column's token sees
-  float m[NT], l[NT];
-  mfma_f32x4_t acc[NT][8];  // dims 16 mt + 4 q4 + j
+  int row, tok, head;  // of the lane's column
+  u32x4_t q[4];
+  uint64_t seen;  // the drafts that the column's token sees
+  float m, l;
+  mfma_f32x4_t acc[8];  // dims 16 mt + 4 q4 + j
 
-  __device__ __forceinline__ void place(const TreeParams& p, int kvh, int first, int stride, int n) {
-#pragma unroll
-    for (int nt = 0; nt < NT; ++nt) {
-      row[nt] = first + 16 * stride * nt + n;
-      tok[nt] = div_by(row[nt], p.div_group);
-      head[nt] = kvh * p.group + row[nt] - tok[nt] * p.group;
-    }
+  __device__ __forceinline__ void place(const TreeParams& p, int kvh, int n) {
+    row = n;
+    tok = div_by(row, p.div_group);
+    head = kvh * p.group + row - tok * p.group;
   }
   __device__ __forceinline__ void reset() {
+    m = kMaxFloor;
+    l = 0.f;
 #pragma unroll
-    for (int nt = 0; nt < NT; ++nt) {
-      m[nt] = kMaxFloor;
-      l[nt] = 0.f;
-#pragma unroll
-      for (int mt = 0; mt < 8; ++mt) acc[nt][mt] = mfma_f32x4_t{0.f, 0.f, 0.f, 0.f};
-    }
+    for (int mt = 0; mt < 8; ++mt) acc[mt] = mfma_f32x4_t{0.f, 0.f, 0.f, 0.f};
   }
   // WIDE: dims in the order of 16-byte reads of an e4m3 row.
   template <bool WIDE>
   __device__ __forceinline__ void load_q(const TreeParams& p, const Cursor& c, int q4) {
+    const int i = min(tok, c.n - 1);
+    const uint16_t* src = p.q + (c.q0 + i) * p.q_tok_stride + head * p.q_head_stride;
 #pragma unroll
-    for (int nt = 0; nt < NT; ++nt) {
-      const int i = min(tok[nt], c.n - 1);
-      const uint16_t* src = p.q + (c.q0 + i) * p.q_tok_stride + head[nt] * p.q_head_stride;
-#pragma unroll
-      for (int kk = 0; kk < 4; ++kk)
-        q[nt][kk] = *reinterpret_cast<const u32x4_t*>(
-            src + (WIDE ? 64 * (kk >> 1) + 16 * q4 + 8 * (kk & 1) : 32 * kk + 8 * q4)) ^ p.q_flip;
-      const uint64_t all = ~0ull >> (64 - c.n);
-      const uint64_t bits = p.mask ? static_cast<uint64_t>(p.mask[c.q0 + i]) : ~0ull >> (63 - i);
-      seen[nt] = bits & all;
-      asm volatile("" : "+v"(seen[nt]));  // waited for here, not where its registers are next written
-    }
+    for (int kk = 0; kk < 4; ++kk)
+      q[kk] = *reinterpret_cast<const u32x4_t*>(
+          src + (WIDE ? 64 * (kk >> 1) + 16 * q4 + 8 * (kk & 1) : 32 * kk + 8 * q4)) ^ p.q_flip;
+    const uint64_t all = ~0ull >> (64 - c.n);
+    const uint64_t bits = p.mask ? static_cast<uint64_t>(p.mask[c.q0 + i]) : ~0ull >> (63 - i);
+    seen = bits & all;
+    asm volatile("" : "+v"(seen));  // waited for here, not where its registers are next written
   }
   // Weights of 32 tokens from their scores s0 (tokens 4 q4 + j) and s1 (16 + 4 q4 + j), packed as the
   // second product's operand; `draft` is the first token's draft, below 0 in the context.  The running
@@ -398,7 +388,7 @@ struct Rows {
   // times the largest V.  The loop waits for memory, and the multiplications of the sums cost no time.
   // SCALED: each is multiplied by its V scale, the bytes of v0 and v1.
   template <bool SCALED>
-  __device__ __forceinline__ u32x4_t weigh(int nt, mfma_f32x4_t s0, mfma_f32x4_t s1, u32 v0, u32 v1, float scale,
+  __device__ __forceinline__ u32x4_t weigh(mfma_f32x4_t s0, mfma_f32x4_t s1, u32 v0, u32 v1, float scale,
                                            bool tail, int draft, int q4) {
     float x[8];
 #pragma unroll
@@ -407,26 +397,26 @@ struct Rows {
 #pragma unroll
       for (int e = 0; e < 8; ++e) {
         const int d = draft + 16 * (e >> 2) + 4 * q4 + (e & 3);
-        x[e] = sees(seen[nt], d) ? x[e] : -INFINITY;
+        x[e] = sees(seen, d) ? x[e] : -INFINITY;
       }
     }
     float mx = x[0];
 #pragma unroll
     for (int e = 1; e < 8; ++e) mx = fmaxf(mx, x[e]);
     mx = xor32_max(xor16_max(mx)) * scale;
-    if (__any(mx > m[nt])) {
-      const float m_new = fmaxf(m[nt], mx);
-      const float alpha = fast_exp2(m[nt] - m_new);
-      m[nt] = m_new;
-      l[nt] *= alpha;
+    if (__any(mx > m)) {
+      const float m_new = fmaxf(m, mx);
+      const float alpha = fast_exp2(m - m_new);
+      m = m_new;
+      l *= alpha;
 #pragma unroll
-      for (int mt = 0; mt < 8; ++mt) acc[nt][mt] *= alpha;
+      for (int mt = 0; mt < 8; ++mt) acc[mt] *= alpha;
     }
     u32x4_t pf;
 #pragma unroll
     for (int e = 0; e < 8; e += 2) {
-      float w0 = fast_exp2(fmaf(x[e], scale, -m[nt])), w1 = fast_exp2(fmaf(x[e + 1], scale, -m[nt]));
-      l[nt] += w0 + w1;
+      float w0 = fast_exp2(fmaf(x[e], scale, -m)), w1 = fast_exp2(fmaf(x[e + 1], scale, -m));
+      l += w0 + w1;
       if (SCALED) {
         w0 = scale_weight(w0, e < 4 ? v0 : v1, e & 3);
         w1 = scale_weight(w1, e < 4 ? v0 : v1, (e & 3) + 1);
@@ -438,7 +428,7 @@ struct Rows {
   // The tail's V: a weight of 0 does not undo an infinity or NaN, so tokens behind the last one (from
   // `left` on) are cleared, and drafts that are not finite leave the product and are added one by one
   // to the rows that see them.
-  __device__ __forceinline__ void clean(u32x4_t (&vt)[8], const u32x4_t (&pf)[NT], int draft, int left, int q4) {
+  __device__ __forceinline__ void clean(u32x4_t (&vt)[8], u32x4_t pf, int draft, int left, int q4) {
     u32x4_t fine;
     u32 odd = 0;  // bit e: element e (token 4 q4 + e, or 12 + 4 q4 + e for e >= 4) is cached and not finite
 #pragma unroll
@@ -465,14 +455,11 @@ struct Rows {
           fine[w] &= ~only[w];
         }
         const int d = draft + 16 * (e >> 2) + 4 * g + (e & 3);
+        const bool mine = sees(seen, d);
 #pragma unroll
-        for (int nt = 0; nt < NT; ++nt) {
-          const bool mine = sees(seen[nt], d);
-#pragma unroll
-          for (int mt = 0; mt < 8; ++mt) {
-            const mfma_f32x4_t with = mfma16(vt[mt] & only, pf[nt], acc[nt][mt]);
-            if (mine) acc[nt][mt] = with;
-          }
+        for (int mt = 0; mt < 8; ++mt) {
+          const mfma_f32x4_t with = mfma16(vt[mt] & only, pf, acc[mt]);
+          if (mine) acc[mt] = with;
         }
       }
     }
@@ -481,26 +468,23 @@ struct Rows {
   }
   // The rows' output where a range held all of the sequence, otherwise a partial state at `place`.
   __device__ __forceinline__ void emit(const TreeParams& p, const Cursor& c, int kvh, bool whole, int place, int q4) {
+    float sum = xor32_sum(xor16_sum(l));
+    if (c.bad) sum = NAN;
+    if (tok >= c.n) return;
+    if (whole) {
+      const float inv = sum == 0.f ? 0.f : 1.f / sum;
+      uint16_t* out = p.out + (c.q0 + tok) * p.o_tok_stride + head * p.o_head_stride + 4 * q4;
 #pragma unroll
-    for (int nt = 0; nt < NT; ++nt) {
-      float sum = xor32_sum(xor16_sum(l[nt]));
-      if (c.bad) sum = NAN;
-      if (tok[nt] >= c.n) continue;
-      if (whole) {
-        const float inv = sum == 0.f ? 0.f : 1.f / sum;
-        uint16_t* out = p.out + (c.q0 + tok[nt]) * p.o_tok_stride + head[nt] * p.o_head_stride + 4 * q4;
-#pragma unroll
-        for (int mt = 0; mt < 8; ++mt) {
-          const mfma_f32x4_t o = acc[nt][mt] * inv;
-          *reinterpret_cast<u32x2_t*>(out + 16 * mt) = u32x2_t{pack_bf16x2(o[0], o[1]), pack_bf16x2(o[2], o[3])};
-        }
-      } else {
-        const int64_t at = (static_cast<int64_t>(place) * p.num_kv_heads + kvh) * p.rows + row[nt];
-        float* part = p.part_o + at * kDim + 4 * q4;
-#pragma unroll
-        for (int mt = 0; mt < 8; ++mt) *reinterpret_cast<mfma_f32x4_t*>(part + 16 * mt) = acc[nt][mt];
-        if (q4 == 0) *reinterpret_cast<float2*>(p.part_ml + 2 * at) = make_float2(m[nt], sum);
+      for (int mt = 0; mt < 8; ++mt) {
+        const mfma_f32x4_t o = acc[mt] * inv;
+        *reinterpret_cast<u32x2_t*>(out + 16 * mt) = u32x2_t{pack_bf16x2(o[0], o[1]), pack_bf16x2(o[2], o[3])};
       }
+    } else {
+      const int64_t at = (static_cast<int64_t>(place) * p.num_kv_heads + kvh) * p.rows + row;
+      float* part = p.part_o + at * kDim + 4 * q4;
+#pragma unroll
+      for (int mt = 0; mt < 8; ++mt) *reinterpret_cast<mfma_f32x4_t*>(part + 16 * mt) = acc[mt];
+      if (q4 == 0) *reinterpret_cast<float2*>(p.part_ml + 2 * at) = make_float2(m, sum);
     }
   }
 };
@@ -542,8 +526,8 @@ __global__ __launch_bounds__(kThreads) void tree_few_kernel(const TreeParams p) 
       va[mt] = kTile + 256 * row + 8 * (n & 3) + 32 * (mt ^ (row & 7));
     }
   }
-  Rows<1> rows;
-  rows.place(p, r.kvh, 0, 1, n);
+  Rows rows;
+  rows.place(p, r.kvh, n);
   rows.reset();
 
   // Iteration S computes step S and issues the tiles of step S + 2, each as soon as its tile has been
@@ -578,13 +562,13 @@ __global__ __launch_bounds__(kThreads) void tree_few_kernel(const TreeParams p) 
 #pragma unroll
           for (int h = 0; h < 4; ++h) {
             const u32x4_t w = k[4 * (kk >> 1) + h];
-            s[h] = mfma16(widen8(w[2 * (kk & 1)], w[2 * (kk & 1) + 1], __uint_as_float(kexp[h] << 23)), rows.q[0][kk], s[h]);
+            s[h] = mfma16(widen8(w[2 * (kk & 1)], w[2 * (kk & 1) + 1], __uint_as_float(kexp[h] << 23)), rows.q[kk], s[h]);
           }
       } else {
         const u32 at[4] = {tile + ka[0], tile + ka[1], tile + ka[2], tile + ka[3]};
         read_k_tile(at, k);
 #pragma unroll
-        for (int i = 0; i < 8; ++i) s[i & 1] = mfma16(k[i], rows.q[0][i >> 1], s[i & 1]);
+        for (int i = 0; i < 8; ++i) s[i & 1] = mfma16(k[i], rows.q[i >> 1], s[i & 1]);
       }
     }
     int64_t base = 0;
@@ -605,8 +589,8 @@ __global__ __launch_bounds__(kThreads) void tree_few_kernel(const TreeParams p) 
       for (int sub = 0; sub < SUBS; ++sub) {  // 32 tokens
         const int draft = t0 + 32 * sub - ctx;
         const bool tail = draft > -32;  // drafts among them, or the last token in front of them
-        const u32x4_t pf[1] = {rows.template weigh<FP8>(0, s[2 * sub], s[2 * sub + 1], vexp[2 * sub], vexp[2 * sub + 1],
-                                                        p.scale_log2, tail, draft, q4)};
+        const u32x4_t pf = rows.template weigh<FP8>(s[2 * sub], s[2 * sub + 1], vexp[2 * sub], vexp[2 * sub + 1],
+                                                    p.scale_log2, tail, draft, q4);
         // ---- O^T += V^T P^T
         if (sub == 0) wait_tiles<F::kKOps, F::kVOps>(issued - c0.mark - F::kVOps);
         u32x4_t vt[8];
@@ -628,7 +612,7 @@ __global__ __launch_bounds__(kThreads) void tree_few_kernel(const TreeParams p) 
         }
         if (tail) rows.clean(vt, pf, draft, c0.len - t0 - 32 * sub, q4);
 #pragma unroll
-        for (int mt = 0; mt < 8; ++mt) rows.acc[0][mt] = mfma16(vt[mt], pf[0], rows.acc[0][mt]);
+        for (int mt = 0; mt < 8; ++mt) rows.acc[mt] = mfma16(vt[mt], pf, rows.acc[mt]);
       }
     }
     if (issue) {
