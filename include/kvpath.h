@@ -423,7 +423,8 @@ size_t kvp_tree_workspace_bytes(int32_t max_num_seqs, int32_t max_seqlen_q, int3
 
 /*
  * kvp_paged_decode_bf16 over a quantised cache, for any GQA ratio up to 16: q and out in bf16,
- * everything between in 32 bits but the softmax weights, which enter the second product in bf16.
+ * everything between in 32 bits but the softmax weights, which enter the second product as two bf16
+ * parts, off by 2^-15 of each weight.
  * The sums of V have weights up to 1 on the way and are divided at the end: a sequence's tokens, in
  * whole 64s, times the largest |V| have to stay below 2^128, or infinities and NaN appear.
  * Scale pointers and strides are multiples of 4 bytes.  Rows with context_lens[b] <= 0 are
@@ -457,6 +458,8 @@ int kvp_paged_decode_fp8(const void* q, int64_t q_seq_stride, int64_t q_head_str
  * [0, num_cache_blocks) gives NaN rows; cache_seqlens[b] <= 0 gives zeros (padding rows of a
  * captured graph); a sequence whose rows are not within [0, total_q) is skipped.  Rows that no
  * sequence has are left as they were.
+ *   The softmax weights enter the second product as two bf16 parts (off by 2^-15 of each weight) where
+ * max_seqlen_q * num_q_heads / num_kv_heads is 16 or less, as one (off by 2^-8 of it) beyond.
  *   k_scale and v_scale NULL: caches in bf16, strides in elements, multiples of 8; otherwise a
  * quantised cache.  GQA ratio up to 16; the other limits are kvp_paged_decode_fp8's (slot strides
  * up to 2^24 bytes, and those of |V|).

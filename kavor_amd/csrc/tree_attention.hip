@@ -1,5 +1,5 @@
 // Attention of a few query tokens per sequence over its paged KV cache, in bf16 or quantised:
-// the drafted tokens of a speculative step (kvp_tree_attention_*), and the one token of a decode
+// the drafted tokens of a speculative step (kvp_tree_attention), and the one token of a decode
 // step over the quantised cache (kvp_paged_decode_fp8).
 //
 // Sequence b has n_b query tokens (at most 64) and a cache of len_b tokens, the last n_b of which
@@ -26,8 +26,10 @@
 // Layouts are those of the decode kernel (lane l: n = l % 16, q4 = l / 16): S = K Q^T has tokens
 // 4 q4 + j of every 16 in the lane and row n as its column, O^T = V^T P^T takes P from the same
 // registers.  e4m3 is widened to bf16, exactly, on its way from LDS to the matrix cores, K with its
-// scale (the lane's own token), V's scale going into P.  P is rounded to bf16: at most 2^-8 of each
-// weight, of either sign, so below the rounding of the bf16 output where the values do not cancel; the
+// scale (the lane's own token), V's scale going into P.  Up to 16 rows, where the matrix cores wait for
+// memory, P enters its product as two bf16 parts, off by 2^-15 of each weight (one part alone was no
+// faster); beyond, where they bound it, P is rounded to bf16 as in the prefill: at most 2^-8 of each
+// weight, of either sign, so below the rounding of the bf16 output where the values do not cancel.  The
 // sum of the weights is of the unrounded ones, and running maxima, sums and products stay in 32 bits.
 #include <math.h>
 
@@ -349,6 +351,21 @@ __device__ __forceinline__ bool sees(uint64_t seen, int d) {
   return (d < 0) | ((d < kMaxQ) & static_cast<int>(seen >> (d & (kMaxQ - 1))));
 }
 
+// Weights of two tokens as bf16 parts that sum up to them, but for 2^-15 of each: `hi` is cut off just below the weight,
+// so that the rest is above 0 even of a weight that bf16 holds (0 times an infinity of V would be NaN).
+__device__ __forceinline__ void split_weights(float w0, float w1, u32& hi, u32& lo) {
+  const u32 h0 = __builtin_elementwise_sub_sat(__float_as_uint(w0), 1u) & 0xffff0000u;
+  const u32 h1 = __builtin_elementwise_sub_sat(__float_as_uint(w1), 1u) & 0xffff0000u;
+  hi = h0 >> 16 | h1;
+  lo = pack_bf16x2(w0 - __uint_as_float(h0), w1 - __uint_as_float(h1));
+}
+struct Split {
+  u32x4_t hi, lo;
+};
+__device__ __forceinline__ mfma_f32x4_t mfma16_split(u32x4_t a, const Split& b, mfma_f32x4_t c) {
+  return mfma16(a, b.lo, mfma16(a, b.hi, c));
+}
+
 // The 16 rows that a wave works on, and the online softmax over the tokens that they have met.
 struct Rows {
   int row, tok, head;  // of the lane's column
@@ -382,14 +399,15 @@ struct Rows {
     seen = bits & all;
     asm volatile("" : "+v"(seen));  // waited for here, not where its registers are next written
   }
-  // Weights of 32 tokens from their scores s0 (tokens 4 q4 + j) and s1 (16 + 4 q4 + j), packed as the
-  // second product's operand; `draft` is the first token's draft, below 0 in the context.  The running
-  // maximum m follows every score above it: weights are 1 at most, so sums stay within the number of tokens
-  // times the largest V.  The loop waits for memory, and the multiplications of the sums cost no time.
+  // Weights of 32 tokens from their scores s0 (tokens 4 q4 + j) and s1 (16 + 4 q4 + j), split as the second
+  // product's operands; `draft` is the first token's draft, below 0 in the context.  The running maximum m
+  // follows every score above it: weights are 1 at most, so sums stay within the number of tokens times the
+  // largest V.  The loop waits for memory, and neither the multiplications of the sums nor the second part's
+  // products cost time.
   // SCALED: each is multiplied by its V scale, the bytes of v0 and v1.
   template <bool SCALED>
-  __device__ __forceinline__ u32x4_t weigh(mfma_f32x4_t s0, mfma_f32x4_t s1, u32 v0, u32 v1, float scale,
-                                           bool tail, int draft, int q4) {
+  __device__ __forceinline__ Split weigh(mfma_f32x4_t s0, mfma_f32x4_t s1, u32 v0, u32 v1, float scale, bool tail,
+                                         int draft, int q4) {
     float x[8];
 #pragma unroll
     for (int e = 0; e < 8; ++e) x[e] = e < 4 ? s0[e] : s1[e - 4];
@@ -412,7 +430,7 @@ struct Rows {
 #pragma unroll
       for (int mt = 0; mt < 8; ++mt) acc[mt] *= alpha;
     }
-    u32x4_t pf;
+    Split pf;
 #pragma unroll
     for (int e = 0; e < 8; e += 2) {
       float w0 = fast_exp2(fmaf(x[e], scale, -m)), w1 = fast_exp2(fmaf(x[e + 1], scale, -m));
@@ -421,14 +439,17 @@ struct Rows {
         w0 = scale_weight(w0, e < 4 ? v0 : v1, e & 3);
         w1 = scale_weight(w1, e < 4 ? v0 : v1, (e & 3) + 1);
       }
-      pf[e >> 1] = pack_bf16x2(w0, w1);
+      u32 hi, lo;
+      split_weights(w0, w1, hi, lo);
+      pf.hi[e >> 1] = hi;
+      pf.lo[e >> 1] = lo;
     }
     return pf;
   }
   // The tail's V: a weight of 0 does not undo an infinity or NaN, so tokens behind the last one (from
   // `left` on) are cleared, and drafts that are not finite leave the product and are added one by one
   // to the rows that see them.
-  __device__ __forceinline__ void clean(u32x4_t (&vt)[8], u32x4_t pf, int draft, int left, int q4) {
+  __device__ __forceinline__ void clean(u32x4_t (&vt)[8], const Split& pf, int draft, int left, int q4) {
     u32x4_t fine;
     u32 odd = 0;  // bit e: element e (token 4 q4 + e, or 12 + 4 q4 + e for e >= 4) is cached and not finite
 #pragma unroll
@@ -458,7 +479,7 @@ struct Rows {
         const bool mine = sees(seen, d);
 #pragma unroll
         for (int mt = 0; mt < 8; ++mt) {
-          const mfma_f32x4_t with = mfma16(vt[mt] & only, pf, acc[mt]);
+          const mfma_f32x4_t with = mfma16_split(vt[mt] & only, pf, acc[mt]);
           if (mine) acc[mt] = with;
         }
       }
@@ -589,8 +610,8 @@ __global__ __launch_bounds__(kThreads) void tree_few_kernel(const TreeParams p) 
       for (int sub = 0; sub < SUBS; ++sub) {  // 32 tokens
         const int draft = t0 + 32 * sub - ctx;
         const bool tail = draft > -32;  // drafts among them, or the last token in front of them
-        const u32x4_t pf = rows.template weigh<FP8>(s[2 * sub], s[2 * sub + 1], vexp[2 * sub], vexp[2 * sub + 1],
-                                                    p.scale_log2, tail, draft, q4);
+        const Split pf = rows.template weigh<FP8>(s[2 * sub], s[2 * sub + 1], vexp[2 * sub], vexp[2 * sub + 1],
+                                                  p.scale_log2, tail, draft, q4);
         // ---- O^T += V^T P^T
         if (sub == 0) wait_tiles<F::kKOps, F::kVOps>(issued - c0.mark - F::kVOps);
         u32x4_t vt[8];
@@ -612,7 +633,7 @@ __global__ __launch_bounds__(kThreads) void tree_few_kernel(const TreeParams p) 
         }
         if (tail) rows.clean(vt, pf, draft, c0.len - t0 - 32 * sub, q4);
 #pragma unroll
-        for (int mt = 0; mt < 8; ++mt) rows.acc[mt] = mfma16(vt[mt], pf, rows.acc[mt]);
+        for (int mt = 0; mt < 8; ++mt) rows.acc[mt] = mfma16_split(vt[mt], pf, rows.acc[mt]);
       }
     }
     if (issue) {
