@@ -412,10 +412,11 @@ int kvp_load_fp8(const void* k_cache, const void* v_cache,
 /*
  * Bytes of device workspace that kvp_paged_decode_fp8 (max_seqlen_q 1) and kvp_tree_attention
  * need for up to max_num_seqs sequences of up to max_seqlen_q query tokens, with block tables
- * max_blocks_per_seq wide: at most 17 MB where a kv head's rows (max_seqlen_q * num_q_heads /
- * num_kv_heads) are 16 or fewer, 34 MB up to 64, 68 MB beyond (more where kv heads times blocks of
- * 128 rows exceed 512).  256-byte aligned, no initialisation; calls that share it are ordered on
- * one stream.  It falls with no argument that grows.  Returns 0 for arguments the attention does not support.
+ * max_blocks_per_seq wide: at most 17 MB where max_seqlen_q * min(16, num_q_heads) is 16 or less,
+ * 34 MB up to 64, 68 MB beyond (more where kv heads times blocks of 128 rows exceed 512).  256-byte
+ * aligned, no initialisation; calls that share it are ordered on one stream.  It falls with no argument
+ * that grows, so the largest sizes serve all smaller ones (fewer kv heads, with more rows each, among
+ * them).  Returns 0 for arguments the attention does not support.
  */
 size_t kvp_tree_workspace_bytes(int32_t max_num_seqs, int32_t max_seqlen_q, int32_t num_q_heads,
                                 int32_t num_kv_heads, int32_t head_dim, int32_t max_blocks_per_seq,

@@ -1422,18 +1422,21 @@ extern "C" size_t kvp_tree_workspace_bytes(int32_t max_num_seqs, int32_t max_seq
   if (max_num_seqs <= 0 ||
       check_shape("", max_seqlen_q, num_q_heads, num_kv_heads, head_dim, block_size, max_blocks_per_seq) != KVP_OK)
     return 0;
-  // The most that any launch within these sizes needs, on any device, be its rows few or many: a
-  // launch has as many (range, stream) pairs as units at most, or one range, and no more than steps.
-  const int rows = max_seqlen_q * (num_q_heads / num_kv_heads);
+  // The most that any launch within these sizes needs, on any device, be its rows few or many (fewer kv
+  // heads have more rows each): a launch has as many (range, stream) pairs as units at most, or one range,
+  // and no more than steps.
   const int64_t tokens = static_cast<int64_t>(max_blocks_per_seq) * block_size;
   int64_t most = 0;
-  for (const int some : {std::min(rows, 16), std::min(rows, 64), rows}) {
-    Plan pl{};
-    set_rows(pl, some);
-    const int step = pl.waves ? kManyStep : Format<false>::kStep;
-    const int64_t streams = num_kv_heads * pl.blocks, steps = max_num_seqs * ((tokens + step - 1) / step);
-    const int64_t pairs = std::min(std::max<int64_t>(pl.waves ? kMaxMany : kMaxFew, streams), steps * streams);
-    most = std::max(most, kHeaderBytes + 2 * pairs * (pl.waves ? 32 * pl.waves : 16) * (kDim + 2) * 4);
+  for (int hkv = 1; hkv <= num_kv_heads; ++hkv) {
+    const int rows = max_seqlen_q * std::min(kMaxGroup, num_q_heads / hkv);
+    for (const int some : {std::min(rows, 16), std::min(rows, 64), rows}) {
+      Plan pl{};
+      set_rows(pl, some);
+      const int step = pl.waves ? kManyStep : Format<false>::kStep;
+      const int64_t streams = hkv * pl.blocks, steps = max_num_seqs * ((tokens + step - 1) / step);
+      const int64_t pairs = std::min(std::max<int64_t>(pl.waves ? kMaxMany : kMaxFew, streams), steps * streams);
+      most = std::max(most, kHeaderBytes + 2 * pairs * (pl.waves ? 32 * pl.waves : 16) * (kDim + 2) * 4);
+    }
   }
   return static_cast<size_t>(most);
 }
