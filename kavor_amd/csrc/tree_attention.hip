@@ -149,12 +149,14 @@ __device__ __forceinline__ void fill_rows(const TreeParams& p, const int* s_cum)
     const SeqShape s = load_shape(p, b);
     if (s.kind == kNone) continue;
     const u32 w = s.kind == kZeros ? 0u : 0x7fc07fc0u;
-    const int chunks = s.n * p.num_q_heads * (kDim / 8);
+    const int per = p.num_q_heads * (kDim / 8);  // 16-byte chunks of a row; a sequence's may pass 32 bits
+    int tok = 0;
 #pragma unroll 1
-    for (int i = threadIdx.x; i < chunks; i += kThreads) {
-      const int row = i / (kDim / 8), tok = row / p.num_q_heads, h = row - tok * p.num_q_heads;
-      *reinterpret_cast<uint4*>(p.out + (s.q0 + tok) * p.o_tok_stride + h * p.o_head_stride + i % (kDim / 8) * 8) =
-          make_uint4(w, w, w, w);
+    for (int i = threadIdx.x;; i += kThreads) {
+      while (i >= per) i -= per, ++tok;
+      if (tok >= s.n) break;
+      *reinterpret_cast<uint4*>(p.out + (s.q0 + tok) * p.o_tok_stride + i / (kDim / 8) * p.o_head_stride +
+                                i % (kDim / 8) * 8) = make_uint4(w, w, w, w);
     }
   }
 }

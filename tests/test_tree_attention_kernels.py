@@ -7,6 +7,7 @@ import random
 import pytest
 import torch
 
+from kavor_amd.layers import attention
 from tests.test_tree_attention import SCALE, Batch, signed
 from tests.test_tree_attention_reach import HKV, ROWS, check
 from tests.helpers import bits_equal
@@ -92,3 +93,16 @@ def test_maxima_that_lie_apart(cuda_device, rows, unit, quantised):
         x.dev = (x.plain[0].cuda(), x.dev[1], None, None)
     assert x.plain[0].shape[2] == HKV
     check(x, x.run(mask=None))
+
+
+@pytest.mark.gpu
+def test_nan_rows_beyond_32_bit_counts(cuda_device):
+    """One sequence of 40000 rows of 4096 heads, where two were said: 2^31.3 chunks of 16 bytes become NaN (all in the
+    place of one row, whose stride is 0)."""
+    T, hq = 40_000, 4096
+    k, v = (torch.zeros(1, 64, 256, 128, dtype=torch.bfloat16, device=cuda_device) for _ in range(2))
+    out = torch.zeros(1, hq, 128, dtype=torch.bfloat16, device=cuda_device)
+    cu, ctx = (torch.tensor(t, dtype=torch.int32, device=cuda_device) for t in ([0, T], [64]))
+    attention.tree_attention(out.expand(T, -1, -1), k, v, cu, 2, ctx, torch.zeros(1, 1, dtype=torch.int32, device=cuda_device),
+                             SCALE, out=out.expand(T, -1, -1))
+    assert out.isnan().all()
