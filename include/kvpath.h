@@ -380,7 +380,9 @@ int kvp_sample_bf16(const void* logits, int64_t row_stride, int32_t num_rows, in
  * below, and rounded to nearest even; infinities are stored as NaN.  key and value in bf16,
  * 16-byte aligned with strides that are multiples of 8 elements; head_dim 64, 128 or 256, any
  * block_size.  Slots are kvp_append_bf16's: one outside [0, num_cache_slots) is skipped, -1
- * among them.
+ * among them.  Of duplicate slots (a padded graph's) every 16 bytes of a row and its scale are some
+ * writer's, not all of the same one: what such a slot stands for is no token's row, and is not to be
+ * attended to.
  */
 int kvp_append_fp8(const void* key, int64_t key_tok_stride, int64_t key_head_stride,
                    const void* value, int64_t value_tok_stride, int64_t value_head_stride,

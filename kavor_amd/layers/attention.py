@@ -506,8 +506,9 @@ def store_kvcache_fp8(key: torch.Tensor, value: torch.Tensor, k_cache: torch.Ten
 
     The caches are [num_blocks, block_size, num_kv_heads, head_dim] in float8_e4m3fn, the scales
     [num_blocks, num_kv_heads, block_size] in uint8; byte e stands for 2^(e - 127), and value q of
-    its row for 2^(e - 127) q.  Slots outside the cache, -1 among them, are skipped.  An infinity
-    is stored as NaN."""
+    its row for 2^(e - 127) q.  Slots outside the cache, -1 among them, are skipped; a slot that
+    several tokens name is left with bytes of one and perhaps the scale of another.  An infinity is
+    stored as NaN."""
     index = key.get_device()
     if not (index >= 0 and _is(key, torch.bfloat16, index, 3) and _is(value, torch.bfloat16, index, 3)):
         _require_cuda_bf16("key", key)
