@@ -209,6 +209,7 @@ int kvp_paged_decode_bf16_noalloc(const void* q, int64_t q_seq_stride, int64_t q
  *                         that start with the same block are scheduled together).
  * q, k, v and out are 16-byte aligned, head_dim is contiguous and every other stride is a
  * multiple of 8 elements (KVP_EINVAL otherwise).
+ * softmax_scale is not negative.
  * max_seqlen_q only sizes the work list: a sequence longer than it is still computed in
  * full (its extra query tiles are taken by the workgroups that own its first ones), so
  * an understated max_seqlen_q costs time, never rows.  The workspace (size from

@@ -1237,6 +1237,8 @@ extern "C" int kvp_varlen_prefill_bf16(const void* q, int64_t q_tok_stride, int6
   p.pair_slots = static_cast<int32_t>(pair_slots);
   p.num_kv_heads = num_kv_heads;
   p.scale_log2 = softmax_scale * 1.4426950408889634f;
+  // hidden scores are -inf and scaled afterwards: 0 counts as 2^-149, which moves no finite score by more than 2^-21
+  if (p.scale_log2 == 0.f) p.scale_log2 = __FLT_DENORM_MIN__;
   p.out = static_cast<uint16_t*>(out);
   p.o_tok_stride = out_tok_stride;
   p.o_head_stride = out_head_stride;
