@@ -27,6 +27,8 @@
  *   - Work is enqueued on `stream` (a hipStream_t; pass the current torch stream).
  *     Nothing is allocated, freed or synchronised, so every entry point may be
  *     captured into a hipGraph; all per-step metadata is read from device memory.
+ *   - Calls may come from several threads.  Those that share a workspace are on one stream,
+ *     where a call's kernels follow each other without another call's between them.
  *   - Return value: 0 on success, a negative KVP_E* code when the arguments are
  *     rejected on the host (nothing was launched), or a positive hipError_t when a
  *     launch failed.  kvp_last_error() describes the last failure on this thread.

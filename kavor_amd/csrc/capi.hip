@@ -2,6 +2,8 @@
 #include <stdarg.h>
 #include <stdio.h>
 
+#include <mutex>
+
 #include "common.h"
 
 namespace kvp {
@@ -26,6 +28,10 @@ int launch_status(const char* what) {
   }
   return KVP_OK;
 }
+
+static std::mutex g_launch_order;
+LaunchOrder::LaunchOrder() { g_launch_order.lock(); }
+LaunchOrder::~LaunchOrder() { g_launch_order.unlock(); }
 
 }  // namespace kvp
 

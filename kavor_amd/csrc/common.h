@@ -19,6 +19,14 @@ void clear_error();
 // Converts a launch status into the exported return convention.
 int launch_status(const char* what);
 
+// Held while a call enqueues kernels that hand data to each other in a workspace: another thread's call on the
+// same stream and workspace comes before or after all of them.
+struct LaunchOrder {
+  LaunchOrder();
+  ~LaunchOrder();
+  LaunchOrder(const LaunchOrder&) = delete;
+};
+
 inline bool aligned16(const void* ptr) { return (reinterpret_cast<uintptr_t>(ptr) & 15u) == 0; }
 inline bool mult8(int64_t stride) { return (stride & 7) == 0; }
 

@@ -814,6 +814,7 @@ static int launch_argmax(ArgmaxParams p, int32_t num_rows, void* workspace, size
   // Split rows need the caller's workspace; without one (or too small) rows stay whole.
   if (p.segments > 1 && workspace && workspace_bytes >= kvp_argmax_workspace_bytes(num_rows)) {
     const int per = (p.vocab / 8 + p.segments - 1) / p.segments;  // chunks per segment
+    const LaunchOrder order;
     if (per > 5 * kArgmaxSplitThreads)
       hipLaunchKernelGGL((argmax_kernel<kArgmaxSplitThreads, 10, true, SAMPLE>), dim3(num_rows * p.segments),
                          dim3(kArgmaxSplitThreads), 0, s, p);

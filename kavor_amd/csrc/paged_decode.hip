@@ -1078,6 +1078,7 @@ static int enqueue_decode(const char* fn, const DecodeArgs& a, int64_t ranges, c
                           const DecodeParams* fused = nullptr) {
   const int g = a.num_q_heads / a.num_kv_heads;
   const int most = seqs_per_launch(g, FUSED, steps_ahead(g, a.num_seqs));
+  const LaunchOrder order;
   for (int b0 = 0; b0 < a.num_seqs; b0 += most) {
     const int nb = std::min(most, a.num_seqs - b0);
     DecodeParams p = fused ? *fused : DecodeParams{};

@@ -499,6 +499,7 @@ int segments_of(int32_t rows) { return rows >= 256 ? 1 : std::min(kMaxSegments, 
 
 template <typename T>
 int launch(const char* fn, LogprobParams p, int rows, hipStream_t s) {
+  const LaunchOrder order;
   hipLaunchKernelGGL(logprobs_kernel<T>, dim3(static_cast<unsigned>(rows) * p.segments), dim3(kThreads), 0, s, p);
   if (p.segments > 1)
     hipLaunchKernelGGL(logprobs_merge_kernel<T>, dim3(static_cast<unsigned>(rows)), dim3(kThreads), 0, s, p);

@@ -1376,6 +1376,7 @@ int launch(const char* fn, const TreeArgs& a, hipStream_t stream) {
   p.part_ml = p.part_o + 2ll * pl.ranges * a.num_kv_heads * p.rows * kDim;
   const int n = pl.ranges * p.streams;
   const dim3 grid(static_cast<unsigned>(pl.waves ? (n + 7) / 8 * 8 : (n + kWaves - 1) / kWaves)), block(kThreads);
+  const LaunchOrder order;
   for (int b0 = 0; b0 < a.num_seqs; b0 += pl.seqs) {
     p.num_seqs = std::min(pl.seqs, a.num_seqs - b0);
     p.block_tables = a.block_tables + b0 * a.bt_stride;

@@ -1267,6 +1267,7 @@ extern "C" int kvp_varlen_prefill_bf16(const void* q, int64_t q_tok_stride, int6
   // cu_seqlens hold absolute offsets, so a launch over sequences [s0, s0 + n) reads
   // the same q/k/out rows through the offset pointers.  Consecutive launches share the
   // workspace: each one's plan kernel runs after the previous attention kernel.
+  const LaunchOrder order;
   for (int s0 = 0; s0 < num_seqs; s0 += kMaxPrefillSeqs) {
     const int n = std::min(kMaxPrefillSeqs, num_seqs - s0);
     p.cu_q = cu_seqlens_q + s0;
