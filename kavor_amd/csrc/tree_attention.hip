@@ -16,8 +16,8 @@
 // Work decomposition: the tokens of all sequences are laid end to end in steps of 64 (32 for few rows
 // on a bf16 cache) and cut into equally long ranges, whatever the lengths.  With up to 16 rows per
 // kv head a wave takes one head over one range (tree_few_kernel); with more, a workgroup does, whose
-// four waves share the tiles and take 16 rows each, or 32, and of more than 128 rows blocks of 128
-// run side by side (tree_many_kernel).  A sequence that lies in one range gets its output from
+// four waves share the tiles and take 32 rows each, and of more than 128 rows blocks of 128 run side
+// by side (tree_many_kernel).  A sequence that lies in one range gets its output from
 // there; of the others every range leaves (max, sum, unnormalised sum of V) in 32 bits, which
 // tree_merge_kernel joins.  Only the first and the last sequence of a range can be cut by it, so a
 // range has two places for states whatever the batch: the first for a sequence that it takes up at
@@ -514,8 +514,9 @@ struct Rows {
 
 // Up to 16 rows per kv head: a wave for itself, with the tiles of two steps in flight in its own LDS,
 // so that no wave waits for another.  One query token and e4m3, 8 kv heads: 256 sequences of 100 to
-// 2048 tokens take 93 us (6.1 TB/s), 128 of 1024 to 32768 648 us (6.9 TB/s; 727 with loads that are not
-// nontemporal), one of 611 7.2 us (a chain of dependent loads).
+// 2048 tokens take 95 us (6.0 TB/s), 128 of 1024 to 32768 643 us (6.9 TB/s; with loads that are not
+// nontemporal 80 more), one of 611 7.5 us (a chain of dependent loads).  Four drafts of 32 sequences of
+// 8192 at four query heads to a kv head: 162 us in bf16 (6.6 TB/s), 91 in e4m3 (6.0 TB/s).
 template <bool FP8>
 __global__ __launch_bounds__(kThreads) void tree_few_kernel(const TreeParams p) {
   using F = Format<FP8>;
@@ -660,10 +661,12 @@ __global__ __launch_bounds__(kThreads) void tree_few_kernel(const TreeParams p) 
 // Two workgroups on a CU: one computes while the other waits.  bf16: two tiles, the next one loaded while a tile
 // is used.  e4m3: four, three of them being loaded, and every wave widens what it reads.
 //
-// Matrix and vector instructions bound it, and they add up (64 tokens of a wave with 32 rows: 1024 cycles of
-// products, 275 vector instructions in bf16, 487 in e4m3).  24 sequences of 1000 to 9000 tokens with 61 to 64
-// drafts at 64 heads take 323 us (766 TFLOP/s); a call of 32 of 8192 with 8, 16 and 25 drafts at 32 heads in e4m3 121,
-// 154 and 235 us (KW = 2, 2, 1), with tiles that are widened once for all waves through LDS 146, 168 and 235.
+// Matrix and vector instructions take most of the time, and they add up: 64 tokens of a wave with 32 rows are 1024
+// cycles of products and 281 vector instructions in bf16, 501 in e4m3 (whole launches, counted).  End to end they
+// would fill 72% of the first call below and 82% of the last; what is left is a step's chain of LDS reads,
+// products and softmax, which the other workgroup covers in part.  24 sequences of 1000 to 9000 tokens with 61 to 64
+// drafts at 64 heads take 320 us (775 TFLOP/s); a call of 32 of 8192 with 8, 16 and 25 drafts at 32 heads in e4m3 121,
+// 151 and 210 us (KW = 2, 2, 1), with tiles that are widened once for all waves through LDS 146, 168 and 235.
 //
 // Tile rows are 256 bytes, 16-byte chunk c of token r at chunk c ^ (r % 16) of K and c ^ 4 (r % 4) of V; in
 // e4m3 128 bytes, c ^ ((r / 2) % 8) and c ^ ((r & 2) + (r & 8) / 2).  The lane
