@@ -865,7 +865,8 @@ __global__ __launch_bounds__(kThreads, 2) void tree_many_kernel(const TreeParams
         }
     }
     // ---- weights.  A row's maximum is taken of the first step, and again only where the weights of a step sum up to
-    // more than its tokens, so that no sum over a row's tokens is larger than their number times the largest V.
+    // more than its tokens (equal scores can lie above their maximum by its rounding), so that no sum over a row's tokens
+    // is larger than their number times the largest V, but for these 2%.
     auto step_max = [&]() __attribute__((always_inline)) {
       float mx = kMaxFloor;
 #pragma unroll
@@ -896,7 +897,7 @@ __global__ __launch_bounds__(kThreads, 2) void tree_many_kernel(const TreeParams
       sum = half_swap_sum(sum);
     };
     weigh();
-    if (__any(!(sum <= 32.f * BLOCKS))) {  // rare
+    if (__any(!(sum <= 32.5f * BLOCKS))) {  // rare
       const float m_new = fmaxf(m, step_max());
       const float alpha = fast_exp2(m - m_new);
       m = m_new;
