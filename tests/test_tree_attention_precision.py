@@ -1,5 +1,5 @@
-"""Up to 16 rows of a kv head the softmax weights enter the second product in two bf16 parts, as precise as
-paged_decode's: decode over the quantised cache and small trees over both kinds, where the values of V cancel.
+"""Up to 16 rows of a kv head the softmax weights enter the second product in two bf16 parts (paged_decode: three):
+decode over the quantised cache and small trees over both kinds, where the values of V cancel.
 
 Tolerance: the output is rounded to bf16 once (2^-8 of it).  A weight's first part leaves less than 2^-7 of it, of
 which the second part keeps all but 2^-8: 2^-15.  Scores of q.k are off by less than 2^-24 * 128 * |q||k| scale,
