@@ -505,6 +505,84 @@ int kvp_token_logprobs(const void* logits, int32_t logits_fp32, int64_t row_stri
                        float* top_logprobs, int64_t* top_tokens,
                        void* workspace, size_t workspace_bytes, void* stream);
 
+/* ------------------------------------------------------------------------------
+ * The end of a step with drafted tokens, and pages copied.
+ * ------------------------------------------------------------------------------ */
+
+/*
+ * Which drafts stay, and the token that follows them.  Sequence b has the rows [cu_seqlens_q[b],
+ * cu_seqlens_q[b + 1]) of logits, tokens and uniforms, at most max_seqlen_q <= 64: row 0 is its last
+ * token, the others are drafts.  logits[r] are the target's for the token behind row r's.  Bit j of
+ * tree_mask[r] says that row r sees row j of its sequence (kvp_tree_attention's masks: a row's
+ * ancestors; its own bit and those above are ignored), so the highest one below it is its parent.
+ * tree_mask NULL: a chain.
+ *   With T = temperatures[b] > 0, p = softmax(logits[r] / T) and u the draft's own uniform number,
+ * in [0, 1), a draft x behind row r stays
+ *   - with draft_logits (a chain whose drafts were sampled from q = softmax(draft_logits[r] / T))
+ *     where u q(x) < p(x); behind a refused one the next token follows max(p - q, 0);
+ *   - without (drafts that were chosen, in a chain or a tree), its siblings taken in order of their
+ *     rows, where u (1 - p of the siblings refused before) < p(x); a token that a sibling had is refused.
+ *     Behind refused ones the next token follows p without their tokens.
+ * Where nothing is left to follow, it follows p.  Greedy otherwise (T <= 0 or NaN): a draft stays if it
+ * is kvp_argmax_bf16's index of logits[r], and the next token is that index.
+ *   The next token is the least index whose running sum of weights exceeds row 0's uniform number times
+ * their sum; weights and sums are in 64 bits.  Sums that decide about drafts are in 32 bits.
+ * accepted[b]: the number of drafts that stay; path[b, 0 .. accepted): their rows in the sequence,
+ * rising; out_tokens[b, 0 .. accepted): their tokens, and the next token behind them; the rest of
+ * both [num_seqs, max_seqlen_q] is -1.
+ *   A row of logits with a NaN or +inf, or of -inf alone, keeps no draft at T > 0, and its next token is
+ * the greedy one; such a row of draft_logits keeps none either, and the next token follows p.  A draft
+ * outside [0, vocab) is refused.  Rows of draft_logits without a draft behind them are not read.  A
+ * sequence without rows, with more than max_seqlen_q, or with rows outside [0, total_q) has
+ * accepted 0 and -1 alone.
+ *   logits and draft_logits in bf16 (logits_fp32 0) or fp32 (1), 16-byte aligned, row strides
+ * (elements) multiples of 16 bytes.  The workspace is 16-byte aligned and needs no initialisation;
+ * its size falls with no argument that grows.
+ */
+size_t kvp_verify_workspace_bytes(int32_t max_num_seqs, int32_t max_seqlen_q, int32_t vocab);
+int kvp_verify_drafts(const void* logits, int32_t logits_fp32, int64_t row_stride, int32_t total_q,
+                      int32_t vocab, const void* draft_logits, int64_t draft_row_stride,
+                      const int64_t* tokens, const float* uniforms, const float* temperatures,
+                      const int32_t* cu_seqlens_q, int32_t num_seqs, int32_t max_seqlen_q,
+                      const int64_t* tree_mask, int32_t* accepted, int32_t* path, int64_t* out_tokens,
+                      void* workspace, size_t workspace_bytes, void* stream);
+
+/*
+ * The keys and values of drafts that stay, moved next to their context in every layer: sequence b
+ * has cache_seqlens[b] cached tokens of which the last n_b = cu_seqlens_q[b + 1] - cu_seqlens_q[b] are
+ * its rows; row path[b, j] (kvp_verify_drafts) becomes row j + 1, for j < accepted[b].
+ * new_seqlens[b] = cache_seqlens[b] - n_b + 1 + accepted[b], what a cache holds of row 0 and the drafts
+ * that stay.  Rows behind them keep what they hold.
+ *   A path rises, and its entries lie in [1, n_b): the moves end before the first one that does not,
+ * or whose block id (its own or its destination's) is outside [0, num_cache_blocks) or behind the table.
+ * A sequence with n_b <= 0, n_b > cache_seqlens[b] or accepted[b] outside [0, min(n_b - 1, path_width)]
+ * is left alone, with new_seqlens[b] = cache_seqlens[b].  Pages that hold rows of a sequence belong
+ * to it alone.
+ *   Caches are kvp_append_bf16's or, with k_scale and v_scale, quantised ones, in num_layers layers that
+ * lie cache_layer_stride (scale_layer_stride) apart; any block_size.  path_width <= 64.
+ */
+int kvp_keep_drafts(void* k_cache, void* v_cache, int64_t cache_layer_stride, int64_t cache_block_stride,
+                    int64_t cache_slot_stride, int64_t cache_head_stride,
+                    void* k_scale, void* v_scale, int64_t scale_layer_stride,
+                    int64_t scale_block_stride, int64_t scale_head_stride,
+                    int32_t num_layers, int32_t num_cache_blocks,
+                    const int32_t* block_tables, int64_t block_table_stride,
+                    const int32_t* path, int64_t path_stride, int32_t path_width,
+                    const int32_t* accepted, const int32_t* cu_seqlens_q, const int32_t* cache_seqlens,
+                    int32_t num_seqs, int32_t num_kv_heads, int32_t head_dim, int32_t block_size,
+                    int32_t max_blocks_per_seq, int32_t* new_seqlens, void* stream);
+
+/*
+ * Page src[i] copied to page dst[i] in each of num_layers layers, as if all pages were read before any is
+ * written: pages may change places.  src and dst are HOST memory, read before the call returns; ids
+ * outside [0, num_pages) and a page that is written twice are refused.  A page is page_bytes
+ * bytes of anything, at pages + layer * layer_stride + id * page_stride (all in bytes, multiples
+ * of 16).  No temporary page is needed.  A captured call copies the same pages on every replay.
+ */
+int kvp_copy_pages(void* pages, int64_t layer_stride, int64_t page_stride, int32_t num_layers,
+                   int32_t num_pages, int64_t page_bytes, const int32_t* src, const int32_t* dst,
+                   int32_t num_pairs, void* stream);
+
 #ifdef __cplusplus
 }
 #endif

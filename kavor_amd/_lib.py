@@ -189,6 +189,31 @@ SIGNATURES: dict[str, tuple] = {
         _c_void_p, _c_void_p,             # top_logprobs (fp32), top_tokens (int64)
         _c_void_p, _size_t, _c_void_p,    # workspace, workspace_bytes, stream
     ]),
+    "kvp_keep_drafts": (ctypes.c_int, [
+        _c_void_p, _c_void_p,             # k_cache, v_cache
+        _i64, _i64, _i64, _i64,           # cache layer/block/slot/head strides
+        _c_void_p, _c_void_p, _i64, _i64, _i64,  # k_scale, v_scale, scale layer/block/head strides
+        _i32, _i32, _c_void_p, _i64,      # num_layers, num_cache_blocks, block_tables, block_table_stride
+        _c_void_p, _i64, _i32, _c_void_p,  # path, path_stride, path_width, accepted
+        _c_void_p, _c_void_p, _i32,       # cu_seqlens_q, cache_seqlens, num_seqs
+        _i32, _i32, _i32, _i32,           # num_kv_heads, head_dim, block_size, max_blocks_per_seq
+        _c_void_p, _c_void_p,             # new_seqlens, stream
+    ]),
+    "kvp_copy_pages": (ctypes.c_int, [
+        _c_void_p, _i64, _i64,            # pages, layer_stride, page_stride (bytes)
+        _i32, _i32, _i64,                 # num_layers, num_pages, page_bytes
+        _c_void_p, _c_void_p, _i32,       # src, dst (host), num_pairs
+        _c_void_p,                        # stream
+    ]),
+    "kvp_verify_workspace_bytes": (_size_t, [_i32, _i32, _i32]),
+    "kvp_verify_drafts": (ctypes.c_int, [
+        _c_void_p, _i32, _i64, _i32, _i32,  # logits, logits_fp32, row_stride, total_q, vocab
+        _c_void_p, _i64,                  # draft_logits, draft_row_stride
+        _c_void_p, _c_void_p, _c_void_p,  # tokens (int64), uniforms, temperatures (fp32)
+        _c_void_p, _i32, _i32, _c_void_p,  # cu_seqlens_q, num_seqs, max_seqlen_q, tree_mask
+        _c_void_p, _c_void_p, _c_void_p,  # accepted, path (int32), out_tokens (int64)
+        _c_void_p, _size_t, _c_void_p,    # workspace, workspace_bytes, stream
+    ]),
 }
 
 _lock = threading.Lock()

@@ -22,6 +22,8 @@ from dataclasses import dataclass
 
 import torch
 
+from kavor_amd.layers.attention import copy_pages
+
 
 @dataclass(frozen=True)
 class CacheLayout:
@@ -106,6 +108,11 @@ class CachePool:
             return
         if len(src_ids) != len(dst_ids):
             raise ValueError("src_ids and dst_ids differ in length")
+        if self.pools.is_cuda and self.page_bytes % 16 == 0:
+            n = self.pools.shape[1]  # ids as an index takes them: from the end below 0, the last one where two write
+            pairs = {d + n if d < 0 else d: s + n if s < 0 else s for s, d in zip(src_ids, dst_ids)}
+            copy_pages(self.pools, list(pairs.values()), list(pairs))
+            return
         dev = self.pools.device
         src = torch.tensor(src_ids, dtype=torch.int64, device=dev)
         dst = torch.tensor(dst_ids, dtype=torch.int64, device=dev)

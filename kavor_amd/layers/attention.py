@@ -13,6 +13,8 @@ same manner:
                                         each token and head) written, and read back in bf16
   paged_decode_fp8                      paged_decode over it
   tree_attention                        drafted tokens over a cache of either kind
+  keep_drafts                           those that stay, moved next to their context in every layer
+  copy_pages                            whole pages copied in every layer
 Every function here only
 validates layouts and forwards raw pointers and strides to the C ABI (include/kvpath.h)
 on the current stream; nothing computes on the host and there is no fallback.
@@ -20,6 +22,7 @@ on the current stream; nothing computes on the host and there is no fallback.
 
 from __future__ import annotations
 
+from array import array
 from functools import lru_cache
 
 import torch
@@ -35,6 +38,7 @@ __all__ = [
     "reserve_prefill_workspace", "prefill_workspace_bytes",
     "flash_attn_with_kvcache", "flash_attn_varlen_func",
     "store_kvcache_fp8", "load_kvcache_fp8", "paged_decode_fp8", "tree_attention",
+    "keep_drafts", "copy_pages",
     "reserve_tree_workspace", "tree_workspace_bytes",
 ]
 
@@ -675,6 +679,81 @@ def tree_attention(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor
             tree_mask.data_ptr() if tree_mask is not None else 0, Hq, Hkv, D, block_size, width,
             softmax_scale, out.data_ptr(), os[0], os[1], ws.data_ptr(), ws.numel(), stream)
     return out
+
+
+def keep_drafts(k_cache: torch.Tensor, v_cache: torch.Tensor, path: torch.Tensor, accepted: torch.Tensor,
+                cu_seqlens_q: torch.Tensor, cache_seqlens: torch.Tensor, block_table: torch.Tensor,
+                k_scale: torch.Tensor | None = None, v_scale: torch.Tensor | None = None) -> torch.Tensor:
+    """Moves the keys and values of the drafts that stay (verify_drafts' path and accepted) next to their
+    context, in every layer: row path[b, j] of sequence b becomes row j + 1, for j < accepted[b].
+
+    cu_seqlens_q, cache_seqlens and block_table as tree_attention had them.  The caches are
+    [layers, num_blocks, block_size, num_kv_heads, head_dim] (or one layer's, without the first dimension) in
+    bf16 or, with k_scale and v_scale [layers, num_blocks, num_kv_heads, block_size], quantised as
+    store_kvcache_fp8's.  Returns the sequences' new lengths, int32 [B]: the context, row 0 and what
+    stays.  Pages that hold a sequence's rows must belong to it alone; what lies behind the new length is
+    left as it is.  A path that does not rise, or leaves the sequence's rows or pages, ends there."""
+    if not k_cache.is_cuda:
+        raise ValueError(f"k_cache must be a CUDA (HIP) tensor, got device {k_cache.device}")
+    if (k_scale is None) != (v_scale is None):
+        raise ValueError("k_scale and v_scale go together")
+    dim = k_cache.dim()
+    if dim != 4 and dim != 5:
+        raise ValueError(f"k_cache must be [layers, num_blocks, block_size, num_kv_heads, head_dim] or one layer's, got "
+                         f"shape {tuple(k_cache.shape)}")
+    shape, cs = _paired(k_cache, v_cache, "k_cache", torch.bfloat16 if k_scale is None else _FP8, k_cache, dim)
+    layers, (num_blocks, block_size, heads, head_dim) = (1 if dim == 4 else shape[0]), shape[-4:]
+    scale = (0, 0, 0, 0, 0)
+    if k_scale is not None:
+        scales, ss = _paired(k_scale, v_scale, "k_scale", torch.uint8, k_cache, dim - 1)
+        if scales != (*shape[:-3], heads, block_size):
+            raise ValueError(f"the scales must be {(*shape[:-3], heads, block_size)}, got {tuple(scales)}")
+        scale = (k_scale.data_ptr(), v_scale.data_ptr(), ss[0] if dim == 5 else 0, ss[-3], ss[-2])
+    for name, t in (("cu_seqlens_q", cu_seqlens_q), ("cache_seqlens", cache_seqlens), ("accepted", accepted)):
+        _ints(name, t, k_cache)
+    _require("path", path, torch.int32, k_cache, 2)
+    batch = cu_seqlens_q.numel() - 1
+    if batch < 0 or cache_seqlens.numel() < batch or accepted.numel() < batch or path.shape[0] < batch:
+        raise ValueError("cu_seqlens_q must have an entry more than sequences, and cache_seqlens, accepted and path one "
+                         "for each")
+    bt, bt_stride, width = _table(block_table, batch, k_cache)
+    new_lens = cache_seqlens.new_empty((batch,))
+    if layers == 0:
+        raise ValueError("the caches have no layers")
+    _launch("kvp_keep_drafts", k_cache.get_device(), k_cache.data_ptr(), v_cache.data_ptr(), cs[0] if dim == 5 else 0,
+            cs[-4], cs[-3], cs[-2], *scale, layers, num_blocks, bt, bt_stride, path.data_ptr(),
+            path.stride(0) if path.shape[0] > 1 else path.shape[1], path.shape[1], accepted.data_ptr(),
+            cu_seqlens_q.data_ptr(), cache_seqlens.data_ptr(), batch, heads, head_dim, block_size, width,
+            new_lens.data_ptr(), _stream(k_cache))
+    return new_lens
+
+
+# ----------------------------------------------------------------------------- pages
+
+def copy_pages(pages: torch.Tensor, src: list[int], dst: list[int]) -> None:
+    """Copies page src[i] to page dst[i] in every layer, as if all pages were read before any is written.
+
+    pages is [layers, num_pages, page] of any type with contiguous pages of a multiple of 16 bytes (a
+    page pool of either kind of cache).  src and dst are host lists; a page may be copied to several, pages may
+    change places, and a page that is written twice is refused.  Nothing is copied to the GPU for it, and
+    no temporary page is used.  A captured call copies the same pages on every replay."""
+    if not pages.is_cuda:
+        raise ValueError(f"pages must be a CUDA (HIP) tensor, got device {pages.device}")
+    if pages.dim() != 3 or (pages.stride(2) != 1 and pages.shape[2] > 1):
+        raise ValueError(f"pages must be [layers, num_pages, page] with contiguous pages, got shape {tuple(pages.shape)} "
+                         f"with strides {tuple(pages.stride())}")
+    count = len(src)
+    if len(dst) != count:
+        raise ValueError("src and dst differ in length")
+    try:
+        ids = array("i", src) + array("i", dst)
+    except (TypeError, OverflowError) as e:
+        raise ValueError(f"src and dst must be lists of page ids: {e}") from None
+    layers, num_pages, size = pages.shape
+    item = pages.element_size()
+    at = ids.buffer_info()[0]
+    _launch("kvp_copy_pages", pages.get_device(), pages.data_ptr(), pages.stride(0) * item, pages.stride(1) * item,
+            layers, num_pages, size * item, at, at + 4 * count, count, _stream(pages))
 
 
 # ----------------------------------------------------------------------------- module

@@ -8,11 +8,14 @@ These replace the engine-side Triton kernels around the paged KV path:
   greedy_argmax             the temperature-0 path of kavor/layers/sampler.py:7-66
 and, without a counterpart there,
   token_logprobs            log probability and rank of given tokens, entropy, alternatives
+  verify_drafts             drafted tokens kept or refused, and the token that follows them
 Each function only validates layouts and forwards pointers and strides to the C ABI on
 the current stream; there is no host computation and no fallback.
 """
 
 from __future__ import annotations
+
+from functools import lru_cache
 
 import torch
 
@@ -20,7 +23,7 @@ from kavor_amd._lib import check, lib
 from kavor_amd.layers.workspace import Workspaces
 
 __all__ = ["rms_norm", "add_rms_norm", "qk_norm_rope_append", "qk_norm_rope", "silu_and_mul",
-           "greedy_argmax", "sample", "token_logprobs"]
+           "greedy_argmax", "sample", "token_logprobs", "verify_drafts"]
 
 
 def _stream(t: torch.Tensor) -> int:
@@ -300,3 +303,90 @@ def token_logprobs(logits: torch.Tensor, tokens: torch.Tensor, top: int = 0):
             rc = lib().kvp_token_logprobs(*args)
     check("kvp_token_logprobs", rc)
     return logprobs, entropy, rank, top_logprobs, top_tokens
+
+
+_verify_pool = Workspaces("verify_drafts", "reserve_verify_workspace")
+
+
+@lru_cache(maxsize=1024)
+def verify_workspace_bytes(max_num_seqs: int, max_seqlen_q: int, vocab: int) -> int:
+    return int(lib().kvp_verify_workspace_bytes(max_num_seqs, max_seqlen_q, vocab))
+
+
+def reserve_verify_workspace(max_num_seqs: int, max_seqlen_q: int, vocab: int,
+                             device: torch.device | str | int) -> torch.Tensor:
+    """Allocates (or grows) the current stream's workspace of verify_drafts.  Call before graph capture
+    with the largest sizes that a captured graph will use: the capture takes the buffer over.  Eager
+    calls need no reservation."""
+    return _verify_pool.get(device, verify_workspace_bytes(max_num_seqs, max_seqlen_q, vocab))
+
+
+def verify_drafts(logits: torch.Tensor, tokens: torch.Tensor, uniforms: torch.Tensor, temperatures: torch.Tensor,
+                  cu_seqlens_q: torch.Tensor, max_seqlen_q: int, tree_mask: torch.Tensor | None = None,
+                  draft_logits: torch.Tensor | None = None) -> tuple[torch.Tensor, torch.Tensor, torch.Tensor]:
+    """Which drafted tokens stay, so that the output is distributed as the target's, and the next token.
+
+    Sequence b has rows cu_seqlens_q[b] .. cu_seqlens_q[b + 1] - 1, at most max_seqlen_q <= 64, of logits
+    [T, vocab] (bf16 or fp32, rows at a stride of 16 bytes), tokens int64 [T] and uniforms fp32 [T]
+    (numbers in [0, 1)): row 0 is its last token, the others its drafts; logits[r] are the target's for the
+    token behind row r's.  Bit j of the int64 tree_mask[r] says that row r sees row j (tree_attention's
+    masks; without them the rows are a chain).  temperatures fp32 [B]; T <= 0 is greedy.
+
+    With p = softmax(logits / T) of its parent's row, a draft x with the number u stays
+      - in a chain with draft_logits (like logits; its drafts were sampled from
+        q = softmax(draft_logits / T) of the rows before them) where u q(x) < p(x), and behind a refused
+        one the next token follows max(p - q, 0);
+      - otherwise where u (1 - p of its siblings refused before) < p(x), and behind refused ones the
+        next token follows p without them.
+    The next token is the least index whose running sum of weights, in 64 bits, exceeds row 0's number
+    times their sum.  Returns (accepted int32 [B], path int32 [B, max_seqlen_q]: the rows that stay,
+    out_tokens int64 [B, max_seqlen_q]: their tokens and the next one), -1 behind these.  A row of logits with a NaN or
+    +inf, or of -inf alone, keeps no draft and gives the greedy token (NaN counts as largest)."""
+    index, dtype = logits.get_device(), logits.dtype
+    if index < 0 or (dtype is not torch.bfloat16 and dtype is not torch.float32) or logits.dim() != 2:
+        raise ValueError(f"logits must be a bf16 or fp32 [T, vocab] GPU tensor (got {dtype} of shape "
+                         f"{tuple(logits.shape)} on {logits.device})")
+    n, vocab = logits.shape
+    if logits.stride(1) != 1 and vocab > 1:
+        raise ValueError("logits must have a contiguous last dimension")
+    for name, t, kind, count in (("tokens", tokens, torch.int64, n), ("uniforms", uniforms, torch.float32, n)):
+        if not (t.dtype is kind and t.get_device() == index and t.is_contiguous() and t.numel() == count):
+            raise ValueError(f"{name} must be a contiguous {kind} tensor on the logits' device, one per row")
+    if not (cu_seqlens_q.dtype is torch.int32 and cu_seqlens_q.get_device() == index and cu_seqlens_q.is_contiguous()
+            and cu_seqlens_q.numel() > 0):
+        raise ValueError("cu_seqlens_q must be a contiguous int32 tensor on the logits' device with an entry more "
+                         "than sequences")
+    batch, rows = cu_seqlens_q.numel() - 1, int(max_seqlen_q)
+    if not (temperatures.dtype is torch.float32 and temperatures.get_device() == index and temperatures.is_contiguous()
+            and temperatures.numel() >= batch):
+        raise ValueError("temperatures must be a contiguous fp32 tensor on the logits' device, one per sequence")
+    if tree_mask is not None and not (tree_mask.dtype is torch.int64 and tree_mask.get_device() == index
+                                      and tree_mask.is_contiguous() and tree_mask.numel() == n):
+        raise ValueError("tree_mask must be a contiguous int64 tensor on the logits' device, one per row")
+    draft, draft_stride = 0, 0
+    if draft_logits is not None:
+        if tree_mask is not None:
+            raise ValueError("draft_logits go with a chain, not with a tree_mask")
+        if not (draft_logits.dtype is dtype and draft_logits.get_device() == index and draft_logits.shape == logits.shape
+                and (draft_logits.stride(1) == 1 or vocab <= 1)):
+            raise ValueError("draft_logits must have the logits' type, shape and device and a contiguous last dimension")
+        draft, draft_stride = draft_logits.data_ptr(), draft_logits.stride(0) if n > 1 else -(-vocab // 8) * 8
+    accepted = cu_seqlens_q.new_empty((batch,))
+    path = cu_seqlens_q.new_empty((batch, max(rows, 0)))
+    out = tokens.new_empty((batch, max(rows, 0)))
+    stream = _stream(logits)
+    need = verify_workspace_bytes(batch, rows, vocab)
+    ws = _verify_pool.ready(index, stream, need)
+    if ws is None:
+        ws = reserve_verify_workspace(batch, rows, vocab, index)
+    args = (logits.data_ptr(), dtype is torch.float32, logits.stride(0) if n > 1 else -(-vocab // 8) * 8, n, vocab,
+            draft, draft_stride, tokens.data_ptr(), uniforms.data_ptr(), temperatures.data_ptr(),
+            cu_seqlens_q.data_ptr(), batch, rows, tree_mask.data_ptr() if tree_mask is not None else 0,
+            accepted.data_ptr(), path.data_ptr(), out.data_ptr(), ws.data_ptr(), ws.numel(), stream)
+    if torch._C._cuda_getDevice() == index:
+        rc = lib().kvp_verify_drafts(*args)
+    else:
+        with torch.cuda.device(index):
+            rc = lib().kvp_verify_drafts(*args)
+    check("kvp_verify_drafts", rc)
+    return accepted, path, out

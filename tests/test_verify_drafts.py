@@ -1,0 +1,377 @@
+"""Verification of drafted tokens against the 64-bit oracle: equal counts, paths and tokens.
+
+Sums that decide about drafts are in 32 bits.  The exponent of 2^t is rounded to 2^-24 of itself, three times, the exponential is
+off by 2^-23, and a thread adds at most vocab / 512 + 8 values one after the other before a tree of twelve additions: a
+row's sum is off by at most (vocab / 512 + 24 + 3 |t|) 2^-24 of itself, with |t| <= 40 wherever 2^t matters, so a
+decision is the oracle's where its two sides are further apart than twice that.  Next tokens come from 64-bit
+sums, off by less than 1e-12 of the whole.  Inputs nearer than that to a border are no test (the oracle says how near
+they are, and the seeds are such that none are).
+"""
+
+import math
+import random
+
+import pytest
+import torch
+
+from kavor_amd import _lib
+from kavor_amd.layers import fused
+from oracle import drafts_oracle as oracle
+from tests.helpers import gen
+
+BELOW_ONE = 1 - 2.0 ** -24
+
+
+def reach(vocab):
+    return 2 * (vocab / 512 + 24 + 120) * 2.0 ** -24
+
+
+def trees(lens, rng):
+    """Masks of a random tree for each sequence, and each row's parent."""
+    masks, parents = [], []
+    for n in lens:
+        own = []
+        for i in range(n):
+            parent = rng.randint(max(0, i - 4), i - 1) if i else -1
+            own.append((own[parent] if i else 0) | 1 << i)
+            parents.append(parent)
+        masks += own
+    return torch.tensor([m - (1 << 64) if m >> 63 else m for m in masks], dtype=torch.int64), parents
+
+
+class Batch:
+    """Drafts that have a fair chance: sampled from a distribution near the target's, or from its best tokens."""
+
+    def __init__(self, lens, vocab, dtype, form, seed=0, greedy=0.3, width=6.0):
+        g, rng = gen(seed), random.Random(seed)
+        T = sum(lens)
+        self.cu = torch.tensor([sum(lens[:i]) for i in range(len(lens) + 1)], dtype=torch.int32)
+        self.max_q = max(lens + [1])
+        self.logits = (torch.randn(T, vocab, generator=g) * torch.rand(T, 1, generator=g) * width).to(dtype)
+        self.temps = torch.rand(len(lens), generator=g) + 0.4
+        self.temps[torch.rand(len(lens), generator=g) < greedy] = 0.0
+        self.uniforms = torch.rand(T, generator=g)
+        self.draft = self.mask = None
+        if form == "tree":
+            self.mask, parents = trees(lens, rng)
+        else:
+            parents = [i - 1 for n in lens for i in range(n)]
+        near = self.logits.float() + 0.5 * torch.randn(T, vocab, generator=g)
+        if form == "sampled":
+            self.draft = near.to(dtype)
+        first = [q for q, n in zip(self.cu.tolist(), lens) for _ in range(n)]
+        above = torch.tensor([f + max(p, 0) for f, p in zip(first, parents)], dtype=torch.int64)
+        seq = [b for b, n in enumerate(lens) for _ in range(n)]
+        self.tokens = torch.zeros(T, dtype=torch.int64)
+        for r in range(T):
+            up, temp = int(above[r]), float(self.temps[seq[r]])
+            if form == "sampled":
+                p = oracle.softmax(self.draft[up], temp) if temp > 0 else None
+                self.tokens[r] = int(torch.multinomial(p, 1, generator=g)) if p is not None else oracle.greedy(self.draft[up])
+            else:
+                best = near[up].topk(min(3, vocab)).indices
+                self.tokens[r] = int(best[rng.randrange(len(best))])
+
+    def args(self):
+        return dict(logits=self.logits, tokens=self.tokens, uniforms=self.uniforms, temperatures=self.temps,
+                    cu_seqlens_q=self.cu, max_seqlen_q=self.max_q, tree_mask=self.mask, draft_logits=self.draft)
+
+    def on_gpu(self):
+        """Rows padded to a multiple of 8 whose padding is not to be read."""
+        a = {k: v.cuda() if isinstance(v, torch.Tensor) else v for k, v in self.args().items()}
+        for name in ("logits", "draft_logits"):
+            if a[name] is not None:
+                n, vocab = a[name].shape
+                room = torch.full((n, -(-vocab // 8) * 8 + 8), math.nan, dtype=a[name].dtype, device="cuda")
+                room[:, :vocab] = a[name]
+                a[name] = room[:, :vocab]
+        return a
+
+    def want(self):
+        *want, margin = oracle.verify_drafts(**self.args())
+        assert margin > 1e-11
+        return want, margin
+
+
+def same(got, want):
+    for name, x, y in zip(("accepted", "path", "out_tokens"), got, want):
+        x = x.cpu()
+        assert x.dtype == y.dtype and torch.equal(x, y), f"{name}:\n{x}\n{y}"
+
+
+def check(batch):
+    want, _ = batch.want()
+    same(fused.verify_drafts(**batch.on_gpu()), want)
+    return want
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+@pytest.mark.parametrize("form", ["sampled", "chosen", "tree"])
+@pytest.mark.parametrize("lens,vocab", [
+    ([1], 1), ([2], 1), ([3, 1], 2), ([5], 7), ([2, 0, 4], 8), ([8] * 9, 100), ([1, 9, 3, 0, 0], 513), ([16, 5, 7], 1013),
+    ([64], 300), ([64, 63, 1, 33], 4099), ([4] * 33, 4096), ([6, 2], 32_003), ([5], 151_936)])
+def test_batches_match_the_oracle(cuda_device, dtype, form, lens, vocab):
+    check(Batch(lens, vocab, dtype, form, seed=len(lens) + vocab, greedy=0.3 if len(lens) > 1 else 0.0))
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("form", ["sampled", "chosen", "tree"])
+@pytest.mark.parametrize("seqs,rows", [(300, 4), (40, 30), (700, 2)])
+def test_many_rows_match_the_oracle(cuda_device, form, seqs, rows):
+    lens = [random.Random(i).randint(0, rows) for i in range(seqs)]
+    want = check(Batch(lens, 700, torch.bfloat16, form, seed=seqs, width=9.0))
+    # with 0 to 2 rows a third of the sequences have a draft, and one of the three best tokens, not the best one, passes
+    # about one time in four: a twelfth of the sequences keep one
+    assert want[0].sum() > seqs / 16
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("form", ["sampled", "chosen", "tree"])
+def test_the_output_is_distributed_as_the_target(cuda_device, form):
+    """50,000 sequences with the same rows and drafts drawn anew: the first token's frequencies against p, by the
+    chi-squared statistic over 11 degrees of freedom (48 is passed once in 1e6)."""
+    n, vocab, g = 50_000, 12, gen(4)
+    z, y = torch.randn(vocab, generator=g) * 1.5, torch.randn(vocab, generator=g) * 1.5
+    p, q = torch.softmax(z.bfloat16().double() / 0.8, 0), torch.softmax(y.bfloat16().double() / 0.8, 0)
+    rows = {"sampled": 2, "chosen": 2, "tree": 4}[form]
+    logits = torch.zeros(n, rows, 16, dtype=torch.bfloat16)
+    logits[:, :, :vocab] = z.bfloat16()
+    logits = logits.view(-1, 16).cuda()[:, :vocab]
+    draft = torch.zeros(n * rows, 16, dtype=torch.bfloat16, device="cuda")
+    draft[:, :vocab] = y.bfloat16().cuda()
+    tokens = torch.zeros(n, rows, dtype=torch.int64)
+    if form == "sampled":
+        tokens[:, 1] = torch.multinomial(q, n, replacement=True, generator=g)
+    else:
+        tokens[:, 1:] = torch.topk(p, 3).indices[torch.randint(0, 3, (n, rows - 1), generator=g)]
+    cu = torch.arange(0, n * rows + 1, rows, dtype=torch.int32).cuda()
+    mask = torch.tensor([1, 3, 5, 9]).repeat(n).cuda() if form == "tree" else None
+    _, _, out = fused.verify_drafts(logits, tokens.view(-1).cuda(), torch.rand(n * rows, generator=g).cuda(),
+                                    torch.full((n,), 0.8).cuda(), cu, rows, mask, draft[:, :vocab] if form == "sampled" else None)
+    seen = torch.bincount(out[:, 0].cpu(), minlength=vocab).double()
+    assert float(((seen - n * p) ** 2 / (n * p)).sum()) < 48
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+@pytest.mark.parametrize("form", ["sampled", "chosen", "tree"])
+def test_rows_without_a_softmax_and_hidden_tokens(cuda_device, dtype, form):
+    x = Batch([4] * 12, 3000, dtype, form, seed=2, greedy=0.0)
+    low = torch.finfo(dtype).min
+    x.logits[0, 77] = math.nan
+    x.logits[4] = -math.inf
+    x.logits[8, [5, 2000]] = math.inf
+    x.logits[12, 10:] = -math.inf
+    x.logits[16] = low
+    x.logits[20, 1:] = low
+    x.logits[24] = math.nan
+    x.logits[28, 100] = torch.finfo(dtype).max
+    x.temps[7] = 0.0                  # row 28: greedy
+    x.logits[32, 2999], x.logits[32, 3] = math.inf, math.nan
+    x.tokens[13], x.tokens[33] = 11, 3
+    if form == "sampled":
+        x.draft[36, 9] = math.nan
+        x.draft[40] = -math.inf
+        x.draft[44, 20:] = -math.inf
+        x.tokens[45] = 30             # q(x) = 0: kept if p(x) > 0
+        x.draft[3::4] = math.nan      # no draft behind these
+    check(x)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("form", ["sampled", "chosen", "tree"])
+def test_temperatures_and_numbers_at_their_ends(cuda_device, form):
+    x = Batch([3] * 16, 500, torch.float32, form, seed=5, greedy=0.0)
+    x.temps[:8] = torch.tensor([0.0, -1.0, math.nan, math.inf, 1e-30, 1e30, 1e-42, 0.02])
+    x.logits[18, 40] = x.logits[18].max()  # at a temperature near 0: the first of two equal ones, or both
+    x.uniforms[24:36] = 0.0
+    x.uniforms[36:48] = BELOW_ONE
+    *want, _ = oracle.verify_drafts(**x.args())
+    same(fused.verify_drafts(**x.on_gpu()), want)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+def test_a_draft_model_that_is_the_target_keeps_everything(cuda_device, dtype):
+    x = Batch([8] * 20, 5003, dtype, "sampled", seed=3, greedy=0.0)
+    x.draft = x.logits.clone()
+    for r in range(len(x.tokens)):
+        if r % 8:
+            p = oracle.softmax(x.draft[r - 1], float(x.temps[r // 8]))
+            x.tokens[r] = int(torch.multinomial(p, 1, generator=gen(r)))
+    x.uniforms.view(20, 8)[:, 1:] = BELOW_ONE
+    got = fused.verify_drafts(**x.on_gpu())
+    assert (got[0] == 7).all()
+    same(got, oracle.verify_drafts(**x.args())[:3])
+
+
+@pytest.mark.gpu
+def test_siblings_and_what_is_left_of_them(cuda_device):
+    """Siblings with one token, siblings that have nearly all of p, a row that sees no row, masks with bits above."""
+    x = Batch([6, 6, 6, 6, 3], 64, torch.float32, "tree", seed=8, greedy=0.0)
+    star = torch.tensor([1] + [1 | 1 << i for i in range(1, 6)])
+    x.mask[:24] = star.repeat(4)
+    x.tokens[:6] = torch.tensor([0, 9, 9, 9, 4, 9])          # twins: the later ones never pass
+    x.logits[6] = torch.where(torch.arange(64) < 5, 10.0, -20.0)
+    x.tokens[6:12] = torch.tensor([0, 0, 1, 2, 3, 4])
+    x.uniforms[6:12] = torch.tensor([0.5] + [BELOW_ONE] * 5)  # 1e-13 of p is left behind them
+    x.logits[12] = -math.inf
+    x.logits[12, 7] = 1.0                                    # p is one token, refused as none has it
+    x.tokens[12:18] = torch.tensor([0, 1, 2, 3, 4, 5])
+    x.mask[19] = 0                                           # sees nothing: not kept, nobody's child
+    x.mask[20] |= 1 << 40
+    x.tokens[20] = x.logits[18].argmax()
+    x.uniforms[20] = 0.0
+    x.temps[4] = 0.0
+    x.mask[24:27] = torch.tensor([1, 3, 7])
+    x.tokens[25], x.tokens[26] = x.logits[24].argmax(), x.logits[25].argmax()
+    want = check(x)
+    assert want[1][3, 0] == 2 and want[0][4] == 2
+
+
+@pytest.mark.gpu
+def test_tokens_outside_the_vocabulary_are_refused(cuda_device):
+    for form in ("sampled", "chosen", "tree"):
+        x = Batch([3] * 6, 1000, torch.bfloat16, form, seed=1)
+        x.tokens[1::3] = torch.tensor([-1, 1000, 1 << 40, -(1 << 60), (1 << 32) + 5, 5])
+        check(x)
+
+
+@pytest.mark.gpu
+def test_sequences_that_are_no_batch(cuda_device):
+    """More rows than announced, rows outside the tensor, falling offsets: nothing kept, no token; the others as ever."""
+    x = Batch([3, 5, 2, 4], 200, torch.bfloat16, "chosen", seed=6)
+    x.max_q = 4
+    want, _ = x.want()
+    assert want[0][1] == 0 and (want[2][1] == -1).all()
+    same(fused.verify_drafts(**x.on_gpu()), want)
+    for ends in ([0, 3, 3, 20, 14], [-2, 3, 8, 10, 14], [0, 8, 3, 10, 14]):
+        x.cu = torch.tensor(ends, dtype=torch.int32)
+        same(fused.verify_drafts(**x.on_gpu()), oracle.verify_drafts(**x.args())[:3])
+    a = x.on_gpu()
+    empty = {k: v[:0].contiguous() if isinstance(v, torch.Tensor) else v for k, v in a.items()}
+    empty["cu_seqlens_q"] = a["cu_seqlens_q"][:1] * 0
+    assert [t.shape for t in fused.verify_drafts(**empty)] == [(0,), (0, 4), (0, 4)]
+    empty["cu_seqlens_q"], empty["temperatures"] = torch.zeros(3, dtype=torch.int32, device="cuda"), torch.ones(2, device="cuda")
+    got = fused.verify_drafts(**empty)
+    assert (got[0] == 0).all() and (got[1] == -1).all() and (got[2] == -1).all()
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("form", ["sampled", "tree"])
+def test_rows_far_apart(cuda_device, form):
+    """Rows more than 2^32 bytes from the first one."""
+    x = Batch([3], 400, torch.bfloat16, form, seed=4, greedy=0.0)
+    want, _ = x.want()
+    a = x.on_gpu()
+    stride = (5 << 28) + 64
+    for name in ("logits", "draft_logits"):
+        if a[name] is not None:
+            room = torch.empty(2 * stride + 400, dtype=torch.bfloat16, device="cuda")
+            a[name] = room.as_strided((3, 400), (stride, 1)).copy_(a[name])
+    same(fused.verify_drafts(**a), want)
+
+
+@pytest.mark.gpu
+def test_other_streams_and_captured_graphs(cuda_device):
+    first, second = (Batch([5, 0, 9, 2], 3001, torch.bfloat16, "sampled", seed=s) for s in (1, 2))
+    second.cu = first.cu
+    wants = [b.want()[0] for b in (first, second)]
+    side = torch.cuda.Stream()
+    a = first.on_gpu()
+    torch.cuda.synchronize()
+    with torch.cuda.stream(side):
+        got = fused.verify_drafts(**a)
+    side.synchronize()
+    same(got, wants[0])
+    fused.reserve_verify_workspace(4, 9, 3001, cuda_device)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        got = fused.verify_drafts(**a)
+    for batch, want in ((second, wants[1]), (first, wants[0]), (second, wants[1])):
+        for k, v in batch.on_gpu().items():
+            if isinstance(v, torch.Tensor):
+                a[k].copy_(v)
+        graph.replay()
+        torch.cuda.synchronize()
+        same(got, want)
+        same(fused.verify_drafts(**a), want)  # eager calls in between have a buffer of their own
+
+
+@pytest.mark.gpu
+def test_two_graphs_in_turn(cuda_device):
+    """Graphs of different sizes share the captured workspace; replays in turn keep their results."""
+    batches = [Batch([4, 2], 2000, torch.float32, "sampled", seed=1), Batch([64, 9, 1], 900, torch.bfloat16, "tree", seed=2)]
+    fused.reserve_verify_workspace(4, 64, 2000, cuda_device)
+    made = []
+    for b in batches:
+        a, graph = b.on_gpu(), torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph):
+            got = fused.verify_drafts(**a)
+        made.append((graph, a, got, b.want()[0]))
+    for _ in range(3):
+        for graph, _, got, want in made:
+            for t in got:
+                t.fill_(-7)
+            graph.replay()
+            torch.cuda.synchronize()
+            same(got, want)
+
+
+def test_refusals_on_the_host():
+    lib = _lib.lib()
+    args = dict(logits=16, fp32=0, rs=1000, total=10, vocab=1000, draft=None, drs=0, tokens=16, uniforms=16, temps=16,
+                cu=16, seqs=2, max_q=8, mask=None, accepted=16, path=16, out=16, ws=16, wsb=1 << 30, stream=None)
+
+    def call(**over):
+        return lib.kvp_verify_drafts(*dict(args, **over).values())
+
+    assert call(seqs=0) == _lib.KVP_OK
+    for bad in (dict(seqs=-1), dict(total=-1), dict(vocab=0), dict(logits=None), dict(tokens=None), dict(uniforms=None),
+                dict(temps=None), dict(cu=None), dict(accepted=None), dict(path=None), dict(out=None), dict(logits=24),
+                dict(rs=996), dict(rs=1004), dict(fp32=1, rs=1001), dict(draft=16, drs=992), dict(draft=8, drs=1000),
+                dict(tokens=12), dict(uniforms=18), dict(cu=18), dict(mask=20), dict(out=20), dict(ws=24)):
+        assert call(**bad) == _lib.KVP_EINVAL, bad
+    for bad in (dict(max_q=0), dict(max_q=65), dict(seqs=65536), dict(vocab=(1 << 30) + 1, rs=1 << 31),
+                dict(draft=16, drs=1000, mask=16)):
+        assert call(**bad) == _lib.KVP_EUNSUPPORTED, bad
+    assert call(wsb=64) == _lib.KVP_EWORKSPACE and call(ws=None) == _lib.KVP_EWORKSPACE
+    assert b"kvp_verify_drafts" in lib.kvp_last_error()
+
+
+def test_workspace_sizes_grow_with_every_argument():
+    size = _lib.lib().kvp_verify_workspace_bytes
+    grid = [(b, n, v) for b in (1, 2, 7, 64, 300) for n in (1, 5, 64) for v in (1, 1000, 151_936)]
+    for small in grid:
+        for large in grid:
+            if all(x <= y for x, y in zip(small, large)):
+                assert size(*small) <= size(*large)
+    assert size(0, 1, 1) == size(1, 65, 1) == size(65536, 1, 1) == size(1, 1, 0) == 0
+
+
+def test_refusals_of_the_python_layer():
+    logits, ids = torch.zeros(3, 8), torch.zeros(3, dtype=torch.int64)
+    with pytest.raises(ValueError, match="GPU"):
+        fused.verify_drafts(logits, ids, torch.zeros(3), torch.ones(1), torch.tensor([0, 3], dtype=torch.int32), 3)
+
+
+@pytest.mark.gpu
+def test_refusals_of_wrong_tensors(cuda_device):
+    good = Batch([3, 2], 64, torch.bfloat16, "sampled", seed=1).on_gpu()
+    for name, value, match in (
+            ("logits", good["logits"].half(), "bf16"), ("logits", good["logits"].t(), "contiguous|tokens"),
+            ("tokens", good["tokens"].int(), "tokens"), ("tokens", good["tokens"][:4], "tokens"),
+            ("tokens", good["tokens"].cpu(), "tokens"), ("uniforms", good["uniforms"].double(), "uniforms"),
+            ("uniforms", good["uniforms"][::2], "uniforms"), ("temperatures", good["temperatures"][:1], "temperatures"),
+            ("cu_seqlens_q", good["cu_seqlens_q"].long(), "cu_seqlens_q"), ("cu_seqlens_q", good["cu_seqlens_q"][:0], "cu_seqlens_q"),
+            ("draft_logits", good["draft_logits"].float(), "draft_logits"), ("draft_logits", good["draft_logits"][:3], "draft_logits"),
+            ("tree_mask", torch.ones(5, dtype=torch.int64, device="cuda"), "chain")):
+        with pytest.raises(ValueError, match=match):
+            fused.verify_drafts(**{**good, name: value})
+    for mask in (torch.ones(5, dtype=torch.int32, device="cuda"), torch.ones(4, dtype=torch.int64, device="cuda")):
+        with pytest.raises(ValueError, match="tree_mask"):
+            fused.verify_drafts(**{**good, "draft_logits": None, "tree_mask": mask})
+    for rows in (0, 65, -1):
+        with pytest.raises(_lib.KVPathError, match="max_seqlen_q"):
+            fused.verify_drafts(**{**good, "max_seqlen_q": rows})
