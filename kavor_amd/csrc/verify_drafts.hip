@@ -17,6 +17,7 @@
 #include <math.h>
 
 #include <algorithm>
+#include <type_traits>
 
 #include "paged.h"
 
@@ -27,11 +28,18 @@ typedef unsigned long long u64;
 
 constexpr int kThreads = 512;
 constexpr int kWaves = kThreads / 64;
+constexpr int kWalkThreads = 1024;
+constexpr int kWalkWaves = kWalkThreads / 64;
 constexpr int kMaxRows = 64;  // rows of a sequence, as in kvp_tree_attention: one per lane
-constexpr int kMaxSegments = 16;
-constexpr int kRangeChunks = 512;  // chunks of a range, at most: one per thread where it is taken again
+constexpr int kMaxSegments = 16;   // of a row: one per lane of a 16-lane row where they are joined
+constexpr int kMaxRange = 512;     // chunks of a range, at most: one per thread where it is taken again
+constexpr int kMostRanges = 512;   // of a row, unless they would be longer than that
+constexpr int kBatch = 4;          // chunks in flight per lane
 constexpr float kReach = 16.f;     // binary orders that a value may lie above the reference
 constexpr float kHuge = 3.4028234e38f;
+// Weights relative to a row's largest: a single one below kTiny counts as 0.  Sums take them as 2^-1000 at least, so up to
+// 2^30 hidden values add up to less than kNothing, and one of the 2^12 of a range that has more is no less than kTiny.
+constexpr double kTiny = 0x1p-985, kNothing = 0x1p-969;
 
 // What a sequence has left to draw.
 enum Mode : int32_t { kDone = 0, kAll = 1, kRest = 2, kWithout = 3, kUndefined = 4 };
@@ -41,7 +49,7 @@ struct Record {   // of a sequence
   int32_t mode;
   double scale;   // log2(e) / T
   double top_p, top_q;  // the rows' maxima
-  double lambda;  // sum of exp(p's logits) over that of q's, in 32 bits
+  double lambda;  // sum of exp(p's logits) over that of q's, from 32-bit sums
   u64 gone;       // kWithout: the sequence's rows whose tokens are refused
 };
 
@@ -64,7 +72,7 @@ struct VerifyParams {
   int64_t* out;     // [num_seqs][max_rows]
   int32_t segments; // of a row in the first pass
   int32_t range_chunks, ranges;
-  float4* stats;    // [sequence][row][p, q][segment]: maximum, sum, index of the maximum
+  float4* stats;    // [sequence][row][p, q][segment]: maximum and sum, or the greedy key
   Record* records;
   Sums* sums;       // [sequence][range]
 };
@@ -89,17 +97,27 @@ struct Chunk<float> {
   }
 };
 
-// A row's chunk c; values behind the row's end are -inf, weights of 0.
+// A row of logits.  Values behind its end are -inf, weights of 0.
 template <typename T>
-__device__ __forceinline__ void load_chunk(const T* row, int c, int vocab, float (&f)[Chunk<T>::kSize]) {
-  constexpr int E = Chunk<T>::kSize;
-  if (E * (c + 1) <= vocab) {
-    Chunk<T>::widen(*reinterpret_cast<const uint4*>(row + static_cast<int64_t>(E) * c), f);
-  } else {
-#pragma unroll
-    for (int e = 0; e < E; ++e) f[e] = E * c + e < vocab ? Chunk<T>::one(row[E * c + e]) : -INFINITY;
+struct Row {
+  static constexpr int E = Chunk<T>::kSize;
+  const T* at;
+  int vocab, full;  // full chunks
+  __device__ __forceinline__ Row(const T* base, int vocab) : at(base), vocab(vocab), full(vocab / E) {}
+  __device__ __forceinline__ int chunks() const { return (vocab + E - 1) / E; }
+  __device__ __forceinline__ uint4 load(int c) const {  // of a whole chunk; another one if c is none
+    return full > 0 ? *reinterpret_cast<const uint4*>(at + static_cast<int64_t>(E) * min(c, full - 1)) : make_uint4(0, 0, 0, 0);
   }
-}
+  // Chunk c, of which load() gave w.
+  __device__ __forceinline__ void values(int c, uint4 w, float (&f)[E]) const {
+    if (c < full) {
+      Chunk<T>::widen(w, f);
+    } else {
+#pragma unroll
+      for (int e = 0; e < E; ++e) f[e] = E * c + e < vocab ? Chunk<T>::one(at[E * c + e]) : -INFINITY;
+    }
+  }
+};
 
 __device__ __forceinline__ float clamped(float m) { return fminf(fmaxf(m, -kHuge), kHuge); }
 
@@ -108,28 +126,35 @@ __device__ __forceinline__ float clamped(float m) { return fminf(fmaxf(m, -kHuge
 __device__ __forceinline__ double scale_of(float temp) {
   return temp > 0.f ? fmax(1.4426950408889634 / static_cast<double>(temp), 1e-30) : 0.0;
 }
+__device__ __forceinline__ float scale32(double scale) { return fminf(static_cast<float>(scale), 3e38f); }
 
-// 2^t for t <= 0, to 1e-14 of it: the Taylor series of e^x over |x| <= ln(2) / 2, its exponent added.  0 below 2^-1000.
-__device__ __forceinline__ double exp2_64(double t) {
-  const double k = rint(t), x = (t - k) * 0.6931471805599453;
-  double y = 1.0 / 39916800;
-  y = fma(y, x, 1.0 / 3628800);
-  y = fma(y, x, 1.0 / 362880);
-  y = fma(y, x, 1.0 / 40320);
-  y = fma(y, x, 1.0 / 5040);
-  y = fma(y, x, 1.0 / 720);
-  y = fma(y, x, 1.0 / 120);
-  y = fma(y, x, 1.0 / 24);
-  y = fma(y, x, 1.0 / 6);
-  y = fma(y, x, 0.5);
-  y = fma(y, x, 1.0);
-  y = fma(y, x, 1.0);
-  const int shift = static_cast<int>(fmax(k, -1001.0));
-  const double r = __longlong_as_double(__double_as_longlong(y) + (static_cast<long long>(shift) << 52));
-  return k < -1000.0 ? 0.0 : r;
+// 2^((x - top) scale) for x <= top, to 2e-13 of it and not below 2^-1000: t - k for the nearest integer k, which the
+// addition of 1.5 * 2^52 leaves in the low bits, the Taylor series of 2^f over |f| <= 1/2, and k added to the
+// exponent.  Twenty instructions at the full rate of 64-bit ones (those that round, convert to integers or scale
+// are slower).
+__device__ __forceinline__ double weight_floor(float x, double top, double scale) {
+  const double t = fmax((static_cast<double>(x) - top) * scale, -1000.0);
+  const double magic = 6755399441055744.0, r = t + magic, f = t - (r - magic);
+  double y = 7.054911620801121e-9;  // ln(2)^n / n!
+  y = fma(y, f, 1.0178086009239696e-7);
+  y = fma(y, f, 1.3215486790144305e-6);
+  y = fma(y, f, 1.5252733804059838e-5);
+  y = fma(y, f, 1.5403530393381606e-4);
+  y = fma(y, f, 1.3333558146428441e-3);
+  y = fma(y, f, 9.618129107628477e-3);
+  y = fma(y, f, 5.5504108664821576e-2);
+  y = fma(y, f, 0.2402265069591007);
+  y = fma(y, f, 0.6931471805599453);
+  y = fma(y, f, 1.0);
+  const u32 k = static_cast<u32>(__double_as_longlong(r));
+  const long long bits = __double_as_longlong(y);
+  return __longlong_as_double(static_cast<long long>(static_cast<u64>(static_cast<u32>(bits >> 32) + (k << 20)) << 32 |
+                                                     static_cast<u32>(bits)));
 }
+// The same, and 0 below 2^-985.
 __device__ __forceinline__ double weight(float x, double top, double scale) {
-  return exp2_64((static_cast<double>(x) - top) * scale);
+  const double w = weight_floor(x, top, scale);
+  return w < kTiny ? 0.0 : w;
 }
 
 // Order of the greedy token: NaN above all, the lower index first among equals.
@@ -138,33 +163,69 @@ __device__ __forceinline__ u64 greedy_key(float x, u32 index) {
   const u32 o = x != x ? 0xffffffffu : (b & 0x80000000u ? ~b : b | 0x80000000u);
   return static_cast<u64>(o) << 32 | (0xffffffffu - index);
 }
-__device__ __forceinline__ u64 shfl_key(u64 k, int from) {
-  return static_cast<u64>(__shfl(static_cast<u32>(k >> 32), from)) << 32 | __shfl(static_cast<u32>(k), from);
-}
-__device__ __forceinline__ u64 wave_max_key(u64 k) {
-#pragma unroll
-  for (int s = 32; s; s >>= 1) {
-    const u64 o = shfl_key(k, (threadIdx.x & 63) ^ s);
-    k = o > k ? o : k;
+__device__ __forceinline__ int64_t token_of(u64 key) { return 0xffffffffu - static_cast<u32>(key); }
+
+// ---- across the lanes of a wave
+
+// x of lane ^ S.
+template <int S>
+__device__ __forceinline__ u32 across(u32 x) {
+  const int v = static_cast<int>(x), lane = threadIdx.x & 63;
+  if constexpr (S == 1) return __builtin_amdgcn_update_dpp(0, v, kDppQuadXor1, 0xf, 0xf, false);
+  if constexpr (S == 2) return __builtin_amdgcn_update_dpp(0, v, kDppQuadXor2, 0xf, 0xf, false);
+  if constexpr (S == 4)  // of a half row in which the lanes of a quad are equal, as combine() leaves them
+    return __builtin_amdgcn_update_dpp(0, v, kDppRowHalfMirror, 0xf, 0xf, false);
+  if constexpr (S == 8)  // of a row in which half rows are
+    return __builtin_amdgcn_update_dpp(0, v, kDppRowMirror, 0xf, 0xf, false);
+  if constexpr (S == 16) {
+    const auto r = __builtin_amdgcn_permlane16_swap(x, x, false, false);
+    return lane & 16 ? r[0] : r[1];
   }
-  return k;
+  const auto r = __builtin_amdgcn_permlane32_swap(x, x, false, false);
+  return lane & 32 ? r[0] : r[1];
 }
-__device__ __forceinline__ double shfl_f64(double x, int from) {
-  return __longlong_as_double(static_cast<long long>(shfl_key(static_cast<u64>(__double_as_longlong(x)), from)));
+template <int S>
+__device__ __forceinline__ float across(float x) {
+  return __uint_as_float(across<S>(__float_as_uint(x)));
 }
-// x of one lane, the same for all.
-__device__ __forceinline__ double lane_f64(double x, int lane) {
-  const long long v = __double_as_longlong(x);
-  const u32 lo = __builtin_amdgcn_readlane(static_cast<int>(v), lane), hi = __builtin_amdgcn_readlane(static_cast<int>(v >> 32), lane);
-  return __longlong_as_double(static_cast<long long>(static_cast<u64>(hi) << 32 | lo));
+template <int S>
+__device__ __forceinline__ u64 across(u64 x) {
+  return static_cast<u64>(across<S>(static_cast<u32>(x >> 32))) << 32 | across<S>(static_cast<u32>(x));
 }
-__device__ __forceinline__ double wave_sum_f64(double x) {
-#pragma unroll
-  for (int s = 32; s; s >>= 1) x += shfl_f64(x, (threadIdx.x & 63) ^ s);
+template <int S>
+__device__ __forceinline__ double across(double x) {
+  return __longlong_as_double(static_cast<long long>(across<S>(static_cast<u64>(__double_as_longlong(x)))));
+}
+// x combined over LANES lanes (a power of two), the same in all of them; `op` is commutative.
+template <int LANES, typename V, typename F>
+__device__ __forceinline__ V combine(V x, F op) {
+  x = op(x, across<1>(x));
+  x = op(x, across<2>(x));
+  x = op(x, across<4>(x));
+  x = op(x, across<8>(x));
+  if constexpr (LANES > 16) x = op(x, across<16>(x));
+  if constexpr (LANES > 32) x = op(x, across<32>(x));
   return x;
 }
+template <int LANES = 64>
+__device__ __forceinline__ float max_of(float x) {
+  return combine<LANES>(x, [](float a, float b) { return fmaxf(a, b); });
+}
+template <int LANES = 64, typename V>
+__device__ __forceinline__ V sum_of(V x) {
+  return combine<LANES>(x, [](V a, V b) { return a + b; });
+}
+template <int LANES = 64>
+__device__ __forceinline__ u64 best_of(u64 x) {
+  return combine<LANES>(x, [](u64 a, u64 b) { return a > b ? a : b; });
+}
+__device__ __forceinline__ double shfl_f64(double x, int from) {
+  const u64 v = static_cast<u64>(__double_as_longlong(x));
+  return __longlong_as_double(static_cast<long long>(static_cast<u64>(__shfl(static_cast<u32>(v >> 32), from)) << 32 |
+                                                     __shfl(static_cast<u32>(v), from)));
+}
 // Sum of x over the lanes up to this one.
-__device__ __forceinline__ double wave_scan_f64(double x) {
+__device__ __forceinline__ double scan_f64(double x) {
   const int lane = threadIdx.x & 63;
 #pragma unroll
   for (int s = 1; s < 64; s <<= 1) {
@@ -173,221 +234,364 @@ __device__ __forceinline__ double wave_scan_f64(double x) {
   }
   return x;
 }
-__device__ __forceinline__ float wave_max(float x) {
-#pragma unroll
-  for (int s = 32; s; s >>= 1) x = fmaxf(x, __shfl_xor(x, s));
-  return x;
+// x of one lane, the same for all.
+__device__ __forceinline__ float lane_of(float x, int lane) {
+  return __uint_as_float(__builtin_amdgcn_readlane(static_cast<int>(__float_as_uint(x)), lane));
 }
-__device__ __forceinline__ float wave_sum(float x) {
-#pragma unroll
-  for (int s = 32; s; s >>= 1) x += __shfl_xor(x, s);
-  return x;
+__device__ __forceinline__ u64 lane_of(u64 x, int lane) {
+  return static_cast<u64>(static_cast<u32>(__builtin_amdgcn_readlane(static_cast<int>(x >> 32), lane))) << 32 |
+         static_cast<u32>(__builtin_amdgcn_readlane(static_cast<int>(x), lane));
+}
+__device__ __forceinline__ double lane_of(double x, int lane) {
+  return __longlong_as_double(static_cast<long long>(lane_of(static_cast<u64>(__double_as_longlong(x)), lane)));
 }
 
-// ---------------------------------------------------------------- maximum and sum of every row
+// ---------------------------------------------------------------- maximum and sum of a row
 
-// A segment of a row per workgroup: maximum m and sum of 2^((x - m) scale), or the greedy key.
+struct Part {  // of a row: maximum and sum of 2^((x - clamped(max)) scale); a NaN makes the sum NaN
+  float max, sum;
+};
+__device__ __forceinline__ float rebased(const Part& part, float to, float scale) {
+  return part.sum * fast_exp2((clamped(part.max) - to) * scale);
+}
+
+// The chunks from c0 on that the waves of a group of `waves` take, 64 at a time, up to cend; c0 is the wave's own first one.
+template <typename T>
+__device__ __forceinline__ Part part_of(const Row<T>& row, int c0, int waves, int cend, float scale) {
+  constexpr int E = Chunk<T>::kSize;
+  const int lane = threadIdx.x & 63, step = 64 * waves;
+  const int whole = min(cend, row.full);
+  float m = -INFINITY, s = 0.f, ref = -kHuge;
+  auto take = [&](auto count, const float* f) __attribute__((always_inline)) {
+    constexpr int N = decltype(count)::value;
+    float most = max3(f[0], f[1], f[2]);
+#pragma unroll
+    for (int e = 3; e < N; e += 2) most = max3(most, f[e], f[min(e + 1, N - 1)]);
+    if (__any((most - ref) * scale > kReach)) {  // uniform
+      const float to = clamped(max_of(most));
+      s *= fast_exp2((ref - to) * scale);
+      ref = to;
+    }
+    m = max3(m, most, most);
+#pragma unroll
+    for (int e = 0; e < N; ++e) s += fast_exp2((f[e] - ref) * scale);
+  };
+  uint4 in[kBatch];
+  auto load_batch = [&](int c) {
+#pragma unroll
+    for (int u = 0; u < kBatch; ++u) in[u] = row.load(c + u * step + lane);
+  };
+  load_batch(c0);
+#pragma unroll 1
+  for (; c0 + (kBatch - 1) * step + 64 <= whole; c0 += kBatch * step) {  // uniform
+    float f[kBatch * E];
+#pragma unroll
+    for (int u = 0; u < kBatch; ++u) Chunk<T>::widen(in[u], *reinterpret_cast<float(*)[E]>(f + u * E));
+    load_batch(c0 + kBatch * step);
+    take(std::integral_constant<int, kBatch * E>{}, f);
+  }
+#pragma unroll
+  for (int u = 0; u < kBatch; ++u) {  // what is left is in flight
+    const int c = c0 + u * step + lane;
+    if (c0 + u * step < cend) {  // uniform
+      float f[E];
+#pragma unroll
+      for (int e = 0; e < E; ++e) f[e] = -INFINITY;
+      if (c < cend) row.values(c, in[u], f);
+      take(std::integral_constant<int, E>{}, f);
+    }
+  }
+  const float top = max_of(m);
+  return {top, sum_of(s) * fast_exp2((ref - clamped(top)) * scale)};
+}
+
+// The greedy key of the same chunks.
+template <typename T>
+__device__ __forceinline__ u64 key_of(const Row<T>& row, int c0, int waves, int cend) {
+  constexpr int E = Chunk<T>::kSize;
+  const int lane = threadIdx.x & 63, step = 64 * waves;
+  u64 key = 0;
+  float best = -INFINITY;  // of the lane
+  bool any = false, nan = false;
+  uint4 in[kBatch];
+  auto load_batch = [&](int c) {
+#pragma unroll
+    for (int u = 0; u < kBatch; ++u) in[u] = row.load(c + u * step + lane);
+  };
+  load_batch(c0);
+#pragma unroll 1
+  for (; c0 < cend; c0 += kBatch * step) {
+    uint4 now[kBatch];
+#pragma unroll
+    for (int u = 0; u < kBatch; ++u) now[u] = in[u];
+    load_batch(c0 + kBatch * step);
+#pragma unroll
+    for (int u = 0; u < kBatch; ++u) {
+      const int c = c0 + u * step + lane;
+      if (c >= cend) continue;
+      float f[E];
+      row.values(c, now[u], f);
+      float most = f[0];
+      bool odd = f[0] != f[0];
+#pragma unroll
+      for (int e = 1; e < E; ++e) {
+        most = fmaxf(most, f[e]);
+        odd |= f[e] != f[e];
+      }
+      if (nan || (any && !odd && !(most > best))) continue;  // a lane's first NaN is its last key
+      any = true;
+      nan = odd;
+      best = most;
+#pragma unroll
+      for (int e = 0; e < E; ++e) {
+        const u64 k = greedy_key(f[e], E * c + e);
+        if (E * c + e < row.vocab && k > key) key = k;
+      }
+    }
+  }
+  return best_of(key);
+}
+
+// A segment of a row per workgroup.
 template <typename T>
 __global__ __launch_bounds__(kThreads) void row_stats_kernel(const VerifyParams p) {
-  constexpr int E = Chunk<T>::kSize;
-  __shared__ float s_max[kWaves], s_sum[kWaves];
+  __shared__ Part s_part[kWaves];
   __shared__ u64 s_key[kWaves];
   const int seg = static_cast<int>(blockIdx.x), i = blockIdx.y >> (p.draft ? 1 : 0), b = blockIdx.z;
   const bool of_draft = p.draft && (blockIdx.y & 1);
   const int q0 = p.cu[b], n = p.cu[b + 1] - q0;
   if (n > p.max_rows || q0 < 0 || q0 + n > p.total || i >= n - (of_draft ? 1 : 0)) return;
-  const float temp = p.temps[b];
-  const double scale64 = scale_of(temp);
-  if (of_draft && scale64 == 0) return;
-  const T* row = of_draft ? static_cast<const T*>(p.draft) + (q0 + i) * p.draft_stride
-                          : static_cast<const T*>(p.logits) + (q0 + i) * p.row_stride;
-  const int chunks = (p.vocab + E - 1) / E, per = (chunks + p.segments - 1) / p.segments;
+  const double scale = scale_of(p.temps[b]);
+  if (of_draft && scale == 0) return;
+  const Row<T> row(of_draft ? static_cast<const T*>(p.draft) + (q0 + i) * p.draft_stride
+                            : static_cast<const T*>(p.logits) + (q0 + i) * p.row_stride, p.vocab);
+  const int chunks = row.chunks(), per = (chunks + p.segments - 1) / p.segments;
   const int cbeg = min(seg * per, chunks), cend = min(cbeg + per, chunks);
-  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-  float m = -INFINITY, s = 0.f;
-  u64 key = 0;
-  if (scale64 == 0) {
-    for (int c = cbeg + threadIdx.x; c < cend; c += kThreads) {
-      float f[E];
-      load_chunk(row, c, p.vocab, f);
-#pragma unroll
-      for (int e = 0; e < E; ++e) {
-        const u64 k = greedy_key(f[e], E * c + e);
-        if (E * c + e < p.vocab && k > key) key = k;
-      }
-    }
-    key = wave_max_key(key);
-    if (lane == 0) s_key[wave] = key;
-  } else {
-    const float scale = fminf(static_cast<float>(scale64), 3e38f);
-    float ref = -kHuge;
-    for (int c0 = cbeg + (wave << 6); c0 < cend; c0 += kThreads) {  // uniform in a wave
-      const int c = c0 + lane;
-      float f[E];
-#pragma unroll
-      for (int e = 0; e < E; ++e) f[e] = -INFINITY;
-      if (c < cend) load_chunk(row, c, p.vocab, f);
-      float most = f[0];
-#pragma unroll
-      for (int e = 1; e < E; ++e) most = fmaxf(most, f[e]);
-      if (__any((most - ref) * scale > kReach)) {
-        const float to = clamped(wave_max(most));
-        s *= fast_exp2((ref - to) * scale);
-        ref = to;
-      }
-      m = fmaxf(m, most);
-#pragma unroll
-      for (int e = 0; e < E; ++e) s += fast_exp2((f[e] - ref) * scale);
-    }
-    m = wave_max(m);
-    s = wave_sum(s) * fast_exp2((ref - clamped(m)) * scale);
-    if (lane == 0) {
-      s_max[wave] = m;
-      s_sum[wave] = s;
-    }
-  }
-  __syncthreads();
-  if (threadIdx.x) return;
+  const int wave = threadIdx.x >> 6, lane = threadIdx.x & 63;
   float4& out = p.stats[(((static_cast<int64_t>(b) * p.max_rows + i) << 1) + of_draft) * p.segments + seg];
-  if (scale64 == 0) {
-    for (int w = 1; w < kWaves; ++w) key = s_key[w] > key ? s_key[w] : key;
-    out = make_float4(__uint_as_float(static_cast<u32>(key)), __uint_as_float(static_cast<u32>(key >> 32)), 0.f, 0.f);
+  if (scale == 0) {  // uniform
+    const u64 key = key_of(row, cbeg + 64 * wave, kWaves, cend);
+    if (lane == 0) s_key[wave] = key;
+    __syncthreads();
+    if (wave != 0) return;
+    const u64 best = best_of<16>(s_key[lane & (kWaves - 1)]);
+    if (lane == 0) out = make_float4(__uint_as_float(static_cast<u32>(best)), __uint_as_float(static_cast<u32>(best >> 32)), 0.f, 0.f);
     return;
   }
-  const float scale = fminf(static_cast<float>(scale64), 3e38f);
-  for (int w = 1; w < kWaves; ++w) m = fmaxf(m, s_max[w]);
-  float sum = 0.f;
-  for (int w = 0; w < kWaves; ++w) sum += s_sum[w] * fast_exp2((clamped(s_max[w]) - clamped(m)) * scale);
-  out = make_float4(m, sum, 0.f, 0.f);
+  const Part part = part_of(row, cbeg + 64 * wave, kWaves, cend, scale32(scale));
+  if (lane == 0) s_part[wave] = part;
+  __syncthreads();
+  if (wave != 0) return;
+  Part mine = s_part[lane & (kWaves - 1)];
+  const float top = max_of<16>(mine.max);
+  const float sum = sum_of<16>(lane < kWaves ? rebased(mine, clamped(top), scale32(scale)) : 0.f);
+  if (lane == 0) out = make_float4(top, sum, 0.f, 0.f);
 }
 
+// ---------------------------------------------------------------- the way through the drafts
+
+// What a row's parts come to.
 struct RowStats {
-  double top, sum;
+  float top;
+  double sum;
   bool ok;  // the softmax exists: no NaN, no +inf, not -inf alone
+  u64 key;  // greedy
 };
-__device__ __forceinline__ RowStats join(const float4* seg, int segments, double scale) {
-  float m = -INFINITY;
-  for (int k = 0; k < segments; ++k) m = fmaxf(m, seg[k].x);
-  const float top = clamped(m), sc = fminf(static_cast<float>(scale), 3e38f);
-  double s = 0;
-  for (int k = 0; k < segments; ++k) s += static_cast<double>(seg[k].y) * fast_exp2((clamped(seg[k].x) - top) * sc);
-  return {top, s, s > 0 && s < 1e300 && fabsf(m) <= kHuge};
+__device__ __forceinline__ RowStats stats_of(float max, double sum) {
+  return {clamped(max), sum, sum > 0 && sum < 1e300 && fabsf(max) <= kHuge, 0};
 }
 
-// ---------------------------------------------------------------- drafts kept
-
-// A wave per sequence, a row per lane.
+// A row of the sequence per lane.
+struct Draft {
+  int64_t token;
+  double u;
+  int parent;    // -1: none
+  bool inside;   // a draft with a parent and a token of the vocabulary
+  float z, y;    // its logits in its parent's rows
+};
 template <typename T>
-__global__ __launch_bounds__(64) void keep_kernel(const VerifyParams p) {
-  const int b = blockIdx.x, i = threadIdx.x;
-  const int q0 = p.cu[b], n = p.cu[b + 1] - q0;
-  int32_t* path = p.path + static_cast<int64_t>(b) * p.max_rows;
-  int64_t* out = p.out + static_cast<int64_t>(b) * p.max_rows;
-  Record& rec = p.records[b];
-  if (n <= 0 || n > p.max_rows || q0 < 0 || q0 + n > p.total) {
-    if (i < p.max_rows) {
+__device__ __forceinline__ Draft draft_of(const VerifyParams& p, int q0, int n) {
+  const int i = threadIdx.x & 63;
+  Draft d{-1, 0.0, -1, false, 0.f, 0.f};
+  if (i < n) {
+    d.token = p.tokens[q0 + i];
+    d.u = p.uniforms[q0 + i];
+    const u64 below = (1ull << i) - 1, sees = p.masks ? static_cast<u64>(p.masks[q0 + i]) & below : below;
+    d.parent = sees ? 63 - __builtin_clzll(sees) : -1;
+    d.inside = d.parent >= 0 && d.token >= 0 && d.token < p.vocab;
+    if (d.inside) {
+      d.z = Chunk<T>::one(static_cast<const T*>(p.logits)[(q0 + d.parent) * p.row_stride + d.token]);
+      if (p.draft) d.y = Chunk<T>::one(static_cast<const T*>(p.draft)[(q0 + d.parent) * p.draft_stride + d.token]);
+    }
+  }
+  return d;
+}
+
+// The child of a row that stays, or -1, by a whole wave; `children` are the row's.
+__device__ __forceinline__ int child_that_stays(const VerifyParams& p, const Draft& d, u64 children, double scale,
+                                                const RowStats& sp, const RowStats& sq) {
+  if (children == 0) return -1;
+  if (scale == 0) {
+    const u64 same = __ballot(d.inside && d.token == token_of(sp.key)) & children;
+    return same ? __builtin_ctzll(same) : -1;
+  }
+  if (!sp.ok) return -1;
+  const double px = d.inside ? weight(d.z, sp.top, scale) / sp.sum : 0.0;
+  if (p.draft) {
+    if (!sq.ok) return -1;
+    const double qx = d.inside ? weight(d.y, sq.top, scale) / sq.sum : 0.0;
+    const u64 passes = __ballot(d.inside && d.u * qx < px) & children;
+    return passes ? __builtin_ctzll(passes) : -1;
+  }
+  const u64 inside = __ballot(d.inside);
+  double left = 1;
+  u64 refused = 0;
+  for (u64 rest = children & inside; rest; rest &= rest - 1) {  // siblings in turn
+    const int j = __builtin_ctzll(rest);
+    const u64 twins = __ballot(d.token == static_cast<int64_t>(lane_of(static_cast<u64>(d.token), j)));
+    if (twins & refused) continue;
+    const double pj = lane_of(px, j);
+    if (lane_of(d.u, j) * left < pj) return j;
+    refused |= 1ull << j;
+    left -= pj;
+  }
+  return -1;
+}
+
+__device__ __forceinline__ u64 children_of(const Draft& d, int node) { return __ballot(d.parent == node); }
+
+// Writes a sequence's results, by one wave, and gives what is left to draw.
+__device__ __forceinline__ Record finish(const VerifyParams& p, int b, int q0, int n, const Draft& d, u64 kept, int node,
+                                         double scale, const RowStats& sp, const RowStats& sq, bool write) {
+  const int i = threadIdx.x & 63, count = __popcll(kept);
+  const u64 gone = children_of(d, node);
+  Record rec{q0 + node, kDone, scale, sp.top, sq.top, sp.sum / sq.sum, gone};
+  if (n > 0 && scale != 0) {
+    if (!sp.ok) rec.mode = kUndefined;
+    else if (p.draft) rec.mode = gone && sq.ok ? kRest : kAll;
+    else rec.mode = gone ? kWithout : kAll;
+  }
+  if (write) {
+    int32_t* path = p.path + static_cast<int64_t>(b) * p.max_rows;
+    int64_t* out = p.out + static_cast<int64_t>(b) * p.max_rows;
+    if (kept >> i & 1) {
+      const int at = __popcll(kept & ((1ull << i) - 1));
+      path[at] = i;
+      out[at] = d.token;
+    }
+    if (i >= count && i < p.max_rows) {
       path[i] = -1;
-      out[i] = -1;
+      if (i > count || n == 0) out[i] = -1;
+      else if (scale == 0) out[i] = token_of(sp.key);  // others: when it is drawn
     }
     if (i == 0) {
-      p.accepted[b] = 0;
-      rec.mode = kDone;
+      p.accepted[b] = count;
+      p.records[b] = rec;
     }
-    return;
   }
-  const bool real = i < n;
+  return rec;
+}
+
+// Rows of a sequence that is none are 0.
+__device__ __forceinline__ int rows_of(const VerifyParams& p, int b, int& q0) {
+  q0 = p.cu[b];
+  const int n = p.cu[b + 1] - q0;
+  return n <= 0 || n > p.max_rows || q0 < 0 || q0 + n > p.total ? 0 : n;
+}
+
+// Behind row_stats_kernel: the way by one wave, a row's segments per 16 lanes.
+template <typename T>
+__device__ __forceinline__ Record way_of(const VerifyParams& p, int b, bool write) {
+  const int lane = threadIdx.x & 63;
+  int q0;
+  const int n = rows_of(p, b, q0);
   const double scale = scale_of(p.temps[b]);
-  const int64_t token = real ? p.tokens[q0 + i] : -1;
-  const double u = real ? p.uniforms[q0 + i] : 0.0;
-  const u64 below = (1ull << i) - 1;
-  const u64 sees = real ? (p.masks ? static_cast<u64>(p.masks[q0 + i]) & below : below) : 0;
-  const int parent = sees ? 63 - __builtin_clzll(sees) : -1;
-  // the row's own statistics, then those of the parent
-  const float4* stats = p.stats + ((static_cast<int64_t>(b) * p.max_rows + min(i, n - 1)) << 1) * p.segments;
-  bool test = false, fresh = true;
-  RowStats mine{0, 0, false}, mine_q{0, 0, false};
-  u64 best = 0, siblings = 0;
-  double px = 0;
-  const int up = max(parent, 0);
-  const bool inside = token >= 0 && token < p.vocab && parent >= 0;
-  if (scale == 0) {
-    for (int k = 0; k < p.segments; ++k) {
-      const u64 key = static_cast<u64>(__float_as_uint(stats[k].y)) << 32 | __float_as_uint(stats[k].x);
-      best = key > best ? key : best;
-    }
-    const u32 first = 0xffffffffu - __shfl(static_cast<u32>(best), up);
-    test = inside && token == first;
-  } else {
-    mine = join(stats, p.segments, scale);
-    if (p.draft && i < n - 1) mine_q = join(stats + p.segments, p.segments, scale);
-    const double top = shfl_f64(mine.top, up), sum = shfl_f64(mine.sum, up);
-    const bool ok = __shfl(static_cast<int>(mine.ok), up);
-    if (inside) px = weight(Chunk<T>::one(static_cast<const T*>(p.logits)[(q0 + up) * p.row_stride + token]), top, scale) / sum;
-    if (p.draft) {
-      const double top_q = shfl_f64(mine_q.top, up), sum_q = shfl_f64(mine_q.sum, up);
-      const bool ok_q = __shfl(static_cast<int>(mine_q.ok), up);
-      double qx = 0;
-      if (inside) qx = weight(Chunk<T>::one(static_cast<const T*>(p.draft)[(q0 + up) * p.draft_stride + token]), top_q, scale) / sum_q;
-      test = inside && ok && ok_q && u * qx < px;
-    } else {
-      test = inside && ok;
-    }
-  }
-  if (p.masks) {  // siblings in turn
-    double left = 1;
-    const int token_lo = static_cast<int>(token), token_hi = static_cast<int>(token >> 32);
-    for (int j = 1; j < n; ++j) {
-      const int parent_j = __builtin_amdgcn_readlane(parent, j);
-      const bool twin = __builtin_amdgcn_readlane(token_lo, j) == token_lo &&
-                        __builtin_amdgcn_readlane(token_hi, j) == token_hi;
-      const bool fresh_j = __builtin_amdgcn_readlane(static_cast<int>(fresh), j);
-      const double pj = lane_f64(px, j);
-      if (j < i && parent >= 0 && parent_j == parent) {
-        siblings |= 1ull << j;
-        if (twin) fresh = false;
-        else if (fresh_j) left -= pj;
+  RowStats sp{0.f, 1, false, 0}, sq{0.f, 1, false, 0};
+  Draft d{-1, 0.0, -1, false, 0.f, 0.f};
+  u64 kept = 0;
+  int node = 0;
+  if (n > 0) {
+    // lanes 0 to 15 have p's segments, 16 to 31 q's
+    auto parts = [&](int i) {
+      const int seg = lane & 15;
+      const bool there = seg < p.segments && (lane < 16 || (lane < 32 && p.draft && i < n - 1 && scale != 0));
+      const int64_t at = (((static_cast<int64_t>(b) * p.max_rows + i) << 1) + (lane >> 4 & 1)) * p.segments + seg;
+      return there ? p.stats[at] : make_float4(-INFINITY, 0.f, 0.f, 0.f);
+    };
+    float4 x = parts(0);
+    d = draft_of<T>(p, q0, n);
+    while (true) {
+      if (scale == 0) {
+        const u64 key = static_cast<u64>(__float_as_uint(x.y)) << 32 | __float_as_uint(x.x);
+        sp.key = lane_of(best_of<16>((lane & 15) < p.segments && lane < 16 ? key : 0), 0);
+      } else {
+        const float top = max_of<16>(x.x);
+        const double sum = sum_of<16>(static_cast<double>(rebased({x.x, x.y}, clamped(top), scale32(scale))));
+        sp = stats_of(lane_of(top, 0), lane_of(sum, 0));
+        sq = stats_of(lane_of(top, 16), lane_of(sum, 16));
       }
+      const int next = child_that_stays(p, d, children_of(d, node), scale, sp, sq);
+      if (next < 0) break;  // uniform
+      kept |= 1ull << next;
+      node = next;
+      x = parts(node);
     }
-    if (scale != 0 && !p.draft) test = test && fresh && u * left < px;
-  } else if (scale != 0 && !p.draft) {
-    test = test && u < px;
   }
-  const u64 tests = __ballot(test);
-  const u64 wins = __ballot(test && (tests & siblings) == 0);
-  const bool kept = (wins >> i & 1) && (sees & ~1ull & ~wins) == 0;
-  const u64 keeps = __ballot(kept);
-  const int count = __popcll(keeps), end = keeps ? 63 - __builtin_clzll(keeps) : 0;
-  const u64 gone = __ballot(real && parent == end);
-  if (kept) {
-    const int at = __popcll(keeps & below);
-    path[at] = i;
-    out[at] = token;
+  return finish(p, b, q0, n, d, kept, node, scale, sp, sq, write);
+}
+
+// The way without the first pass: a workgroup per sequence takes only the rows that it gets to.
+template <typename T>
+__global__ __launch_bounds__(kWalkThreads) void walk_kernel(const VerifyParams p) {
+  __shared__ Part s_part[2][kWalkWaves];
+  __shared__ u64 s_key[2][kWalkWaves];
+  const int b = blockIdx.x, wave = threadIdx.x >> 6, lane = threadIdx.x & 63;
+  int q0;
+  const int n = rows_of(p, b, q0);
+  const double scale = scale_of(p.temps[b]);
+  RowStats sp{0.f, 1, false, 0}, sq{0.f, 1, false, 0};
+  Draft d{-1, 0.0, -1, false, 0.f, 0.f};
+  u64 kept = 0;
+  int node = 0;
+  if (n > 0) {
+    d = draft_of<T>(p, q0, n);
+    for (int turn = 0;; turn ^= 1) {  // all waves go the same way
+      const Row<T> row(static_cast<const T*>(p.logits) + (q0 + node) * p.row_stride, p.vocab);
+      if (scale == 0) {
+        const u64 key = key_of(row, 64 * wave, kWalkWaves, row.chunks());
+        if (lane == 0) s_key[turn][wave] = key;
+        __syncthreads();
+        sp.key = best_of<16>(s_key[turn][lane & 15]);
+      } else {
+        // with a draft's row the first half of the waves has p's, the second q's
+        const bool both = p.draft && node < n - 1;
+        const bool of_draft = both && wave >= kWalkWaves / 2;
+        const Row<T> mine(of_draft ? static_cast<const T*>(p.draft) + (q0 + node) * p.draft_stride : row.at, p.vocab);
+        const int waves = both ? kWalkWaves / 2 : kWalkWaves;
+        const Part part = part_of(mine, 64 * (wave & (waves - 1)), waves, row.chunks(), scale32(scale));
+        if (lane == 0) s_part[turn][wave] = part;
+        __syncthreads();
+        // lanes 0 to 15 join p's, 16 to 31 q's
+        const int at = lane & 15;
+        const bool there = lane < 16 ? at < waves : both && at < waves;
+        Part x = there ? s_part[turn][(lane < 16 ? 0 : waves) + at] : Part{-INFINITY, 0.f};
+        const float top = max_of<16>(x.max);
+        const double sum = sum_of<16>(static_cast<double>(rebased(x, clamped(top), scale32(scale))));
+        sp = stats_of(lane_of(top, 0), lane_of(sum, 0));
+        sq = stats_of(lane_of(top, 16), lane_of(sum, 16));
+      }
+      const int next = child_that_stays(p, d, children_of(d, node), scale, sp, sq);
+      if (next < 0) break;  // uniform
+      kept |= 1ull << next;
+      node = next;
+    }
   }
-  if (i >= count && i < p.max_rows) path[i] = -1;
-  if (i > count && i < p.max_rows) out[i] = -1;
-  if (i == 0) p.accepted[b] = count;
-  if (i != end) return;
-  rec.row = q0 + end;
-  rec.scale = scale;
-  rec.top_p = mine.top;
-  rec.top_q = mine_q.top;
-  rec.lambda = mine.sum / mine_q.sum;
-  rec.gone = gone;
-  if (scale == 0) {
-    out[count] = 0xffffffffu - static_cast<u32>(best);
-    rec.mode = kDone;
-  } else if (!mine.ok) {
-    rec.mode = kUndefined;
-  } else if (p.draft) {
-    rec.mode = gone && mine_q.ok ? kRest : kAll;
-  } else {
-    rec.mode = gone ? kWithout : kAll;
-  }
+  if (wave == 0) finish(p, b, q0, n, d, kept, node, scale, sp, sq, true);
 }
 
 // ---------------------------------------------------------------- sums of the last row
 
-// The refused tokens of a sequence that lie in chunks [cbeg, cend), up to 64 of them, in LDS.
+// The refused tokens of a sequence that lie among values [vbeg, vend), in LDS.
 struct Refused {
   int count;
   int32_t token[kMaxRows];
@@ -407,54 +611,71 @@ __device__ __forceinline__ void find_refused(const VerifyParams& p, const Record
   if (lane == 0) r.count = __popcll(which);
 }
 
-// A range per wave.
-template <typename T>
+// A range per wave.  WALKED: walk_kernel left the records; otherwise every wave goes the way anew.
+template <typename T, bool WALKED>
 __global__ __launch_bounds__(kThreads) void range_sums_kernel(const VerifyParams p) {
   constexpr int E = Chunk<T>::kSize;
   __shared__ Refused s_refused[kWaves];
   const int b = blockIdx.y, wave = threadIdx.x >> 6, lane = threadIdx.x & 63;
   const int range = blockIdx.x * kWaves + wave;
-  const Record rec = p.records[b];
+  Record rec;
+  if constexpr (WALKED) rec = p.records[b];
+  else rec = way_of<T>(p, b, range == 0);
   if (rec.mode == kDone || rec.mode == kUndefined || range >= p.ranges) return;
-  const int chunks = (p.vocab + E - 1) / E;
-  const int cbeg = range * p.range_chunks, cend = min(cbeg + p.range_chunks, chunks);
-  Refused& refused = s_refused[wave];
-  if (rec.mode == kWithout) {
-    find_refused(p, rec, p.cu[b], E * cbeg, E * cend, refused);
-    wait_lds();
-  }
-  const T* row = static_cast<const T*>(p.logits) + rec.row * p.row_stride;
-  const T* row_q = rec.mode == kRest ? static_cast<const T*>(p.draft) + rec.row * p.draft_stride : row;
+  const Row<T> row(static_cast<const T*>(p.logits) + rec.row * p.row_stride, p.vocab);
+  const int cbeg = range * p.range_chunks, cend = min(cbeg + p.range_chunks, row.chunks());
+  const double scale = rec.scale, top_p = rec.top_p, top_q = rec.top_q;
   Sums s{0, 0, 0, 0};
-  for (int c = cbeg + lane; c < cend; c += 64) {
-    float f[E];
-    load_chunk(row, c, p.vocab, f);
-    if (rec.mode == kRest) {
-      float g[E];
-      load_chunk(row_q, c, p.vocab, g);
+  uint4 in = row.load(cbeg + lane);
+  if (rec.mode == kRest) {
+    const Row<T> row_q(static_cast<const T*>(p.draft) + rec.row * p.draft_stride, p.vocab);
+    uint4 in_q = row_q.load(cbeg + lane);
+    for (int c = cbeg + lane; c < cend; c += 64) {
+      float f[E], g[E];
+      row.values(c, in, f);
+      row_q.values(c, in_q, g);
+      in = row.load(c + 64);
+      in_q = row_q.load(c + 64);
 #pragma unroll
       for (int e = 0; e < E; ++e) {
-        const double x = weight(f[e], rec.top_p, rec.scale), y = weight(g[e], rec.top_q, rec.scale);
+        const double x = weight_floor(f[e], top_p, scale), y = weight_floor(g[e], top_q, scale);
         const bool over = x > rec.lambda * y;
         s.p += x;
         s.q += y;
         s.p_over += over ? x : 0.0;
         s.q_over += over ? y : 0.0;
       }
-    } else {
+    }
+    s.q = sum_of(s.q);
+    s.q_over = sum_of(s.q_over);
+  } else {
+    Refused& refused = s_refused[wave];
+    bool some = false;
+    if (rec.mode == kWithout) {
+      find_refused(p, rec, p.cu[b], E * cbeg, E * cend, refused);
+      wait_lds();
+      some = refused.count != 0;
+    }
+    for (int c = cbeg + lane; c < cend; c += 64) {
+      float f[E];
+      row.values(c, in, f);
+      in = row.load(c + 64);
+      if (some) {  // uniform
 #pragma unroll
-      for (int e = 0; e < E; ++e) {
-        const double x = weight(f[e], rec.top_p, rec.scale);
-        s.p += x;
-        if (rec.mode == kWithout && refused.count) s.p_over += is_refused(refused, E * c + e) ? 0.0 : x;
-        else s.p_over += x;
+        for (int e = 0; e < E; ++e) {
+          const double x = weight_floor(f[e], top_p, scale);
+          s.p += x;
+          s.p_over += is_refused(refused, E * c + e) ? 0.0 : x;
+        }
+      } else {
+#pragma unroll
+        for (int e = 0; e < E; ++e) s.p += weight_floor(f[e], top_p, scale);
       }
     }
+    if (!some) s.p_over = s.p;
   }
-  s.p = wave_sum_f64(s.p);
-  s.q = wave_sum_f64(s.q);
-  s.p_over = wave_sum_f64(s.p_over);
-  s.q_over = wave_sum_f64(s.q_over);
+  s.p = sum_of(s.p);
+  s.p_over = sum_of(s.p_over);
   if (lane == 0) p.sums[static_cast<int64_t>(b) * p.ranges + range] = s;
 }
 
@@ -473,68 +694,55 @@ __global__ __launch_bounds__(kThreads) void next_token_kernel(const VerifyParams
   if (rec.mode == kDone) return;
   const int q0 = p.cu[b];
   int64_t* out = p.out + static_cast<int64_t>(b) * p.max_rows + p.accepted[b];
-  const T* row = static_cast<const T*>(p.logits) + rec.row * p.row_stride;
-  const int chunks = (p.vocab + E - 1) / E;
+  const Row<T> row(static_cast<const T*>(p.logits) + rec.row * p.row_stride, p.vocab);
   if (rec.mode == kUndefined) {  // the greedy token
-    u64 key = 0;
-    for (int c = tid; c < chunks; c += kThreads) {
-      float f[E];
-      load_chunk(row, c, p.vocab, f);
-#pragma unroll
-      for (int e = 0; e < E; ++e) {
-        const u64 k = greedy_key(f[e], E * c + e);
-        if (E * c + e < p.vocab && k > key) key = k;
-      }
-    }
-    key = wave_max_key(key);
+    const u64 key = key_of(row, 64 * wave, kWaves, row.chunks());
     if (lane == 0) s_key[wave] = key;
     __syncthreads();
-    if (tid) return;
-    for (int w = 1; w < kWaves; ++w) key = s_key[w] > key ? s_key[w] : key;
-    *out = 0xffffffffu - static_cast<u32>(key);
+    const u64 best = best_of<16>(s_key[lane & (kWaves - 1)]);
+    if (tid == 0) *out = token_of(best);
     return;
   }
   const double u = p.uniforms[q0];
   if (wave == 0) {
     const Sums* sums = p.sums + static_cast<int64_t>(b) * p.ranges;
-    double all_p = 0, all_q = 0, over_p = 0, over_q = 0;
+    Sums all{0, 0, 0, 0};
     for (int r = lane; r < p.ranges; r += 64) {
-      all_p += sums[r].p;
-      all_q += sums[r].q;
-      over_p += sums[r].p_over;
-      over_q += sums[r].q_over;
+      const Sums s = sums[r];
+      all.p += s.p;
+      all.q += s.q;
+      all.p_over += s.p_over;
+      all.q_over += s.q_over;
     }
-    all_p = wave_sum_f64(all_p);
-    all_q = wave_sum_f64(all_q);
-    over_p = wave_sum_f64(over_p);
-    over_q = wave_sum_f64(over_q);
-    const double lambda = rec.mode == kRest ? all_p / all_q : 0.0;
+    all = {sum_of(all.p), sum_of(all.q), sum_of(all.p_over), sum_of(all.q_over)};
+    const double lambda = rec.mode == kRest ? all.p / all.q : 0.0;
     int mode = rec.mode;
-    double whole = mode == kRest ? over_p - lambda * over_q : over_p;
-    if (!(whole > 0)) {  // nothing is left: from p as it is
+    double whole = all.p_over - lambda * all.q_over;
+    if (!(whole > kNothing)) {  // nothing is left: from p as it is
       mode = kAll;
-      whole = all_p;
+      whole = all.p;
     }
     auto of_range = [&](int r) {
       if (r >= p.ranges) return 0.0;
       const Sums s = sums[r];
-      return mode == kAll ? s.p : mode == kRest ? fmax(s.p_over - lambda * s.q_over, 0.0) : s.p_over;
+      const double x = mode == kAll ? s.p : s.p_over - lambda * s.q_over;
+      return x > kNothing ? x : 0.0;
     };
     const double border = u * whole;
     double before = 0, left = border;
     int found = -1, last = 0;
     for (int r0 = 0; r0 < p.ranges && found < 0; r0 += 64) {
       const double mine = of_range(r0 + lane);
-      const double upto = before + wave_scan_f64(mine);
+      const double upto = before + scan_f64(mine);
       const u64 past = __ballot(mine > 0 && upto > border), some = __ballot(mine > 0);
       if (past) {
         const int at = __builtin_ctzll(past);
         found = r0 + at;
-        left = border - shfl_f64(upto - mine, at);
+        left = border - lane_of(upto - mine, at);
       } else if (some) {
         last = r0 + 63 - __builtin_clzll(some);
       }
-      before = shfl_f64(upto, 63);
+      before = lane_of(upto, 63);
     }
     if (lane == 0) {
       s_lambda = lambda;
@@ -546,39 +754,41 @@ __global__ __launch_bounds__(kThreads) void next_token_kernel(const VerifyParams
   __syncthreads();
   const int mode = s_mode, range = s_range;
   const double lambda = s_lambda, left = s_left;
-  const int cbeg = range * p.range_chunks, cend = min(cbeg + p.range_chunks, chunks);
-  if (mode == kWithout && wave == 0) find_refused(p, rec, q0, E * cbeg, E * cend, s_refused);
-  __syncthreads();
+  const int cbeg = range * p.range_chunks, cend = min(cbeg + p.range_chunks, row.chunks());
+  if (mode == kWithout) {
+    if (wave == 0) find_refused(p, rec, q0, E * cbeg, E * cend, s_refused);
+    __syncthreads();
+  }
   // the range again, a chunk per thread
   double w[E], mine = 0;
   const int c = cbeg + tid;
 #pragma unroll
   for (int e = 0; e < E; ++e) w[e] = 0;
   if (c < cend) {
+    const double scale = rec.scale;
     float f[E];
-    load_chunk(row, c, p.vocab, f);
+    row.values(c, row.load(c), f);
+#pragma unroll
+    for (int e = 0; e < E; ++e) {
+      w[e] = weight(f[e], rec.top_p, scale);
+      if (mode == kWithout && is_refused(s_refused, E * c + e)) w[e] = 0;
+    }
     if (mode == kRest) {
+      const Row<T> row_q(static_cast<const T*>(p.draft) + rec.row * p.draft_stride, p.vocab);
       float g[E];
-      load_chunk(static_cast<const T*>(p.draft) + rec.row * p.draft_stride, c, p.vocab, g);
+      row_q.values(c, row_q.load(c), g);
 #pragma unroll
-      for (int e = 0; e < E; ++e)
-        w[e] = fmax(weight(f[e], rec.top_p, rec.scale) - lambda * weight(g[e], rec.top_q, rec.scale), 0.0);
-    } else {
-#pragma unroll
-      for (int e = 0; e < E; ++e) {
-        w[e] = weight(f[e], rec.top_p, rec.scale);
-        if (mode == kWithout && is_refused(s_refused, E * c + e)) w[e] = 0;
-      }
+      for (int e = 0; e < E; ++e) w[e] = fmax(w[e] - lambda * weight(g[e], rec.top_q, scale), 0.0);
     }
 #pragma unroll
     for (int e = 0; e < E; ++e) mine += w[e];
   }
-  double upto = wave_scan_f64(mine);
+  const double upto = scan_f64(mine);
   if (lane == 63) s_wave[wave] = upto;
   __syncthreads();
   double before = 0;
   for (int k = 0; k < wave; ++k) before += s_wave[k];
-  // the first value whose running sum is past the border, or the last that has a weight: as keys, least index first
+  // the first value whose running sum is past the border, or the last that has a weight: as keys
   double run = before + upto - mine;
   u64 key = tid == 0 ? E * cbeg + 1 : 0;
 #pragma unroll
@@ -589,12 +799,11 @@ __global__ __launch_bounds__(kThreads) void next_token_kernel(const VerifyParams
     const u64 k = run > left ? 1ull << 32 | (0xffffffffu - v) : v + 1;
     key = k > key ? k : key;
   }
-  key = wave_max_key(key);
+  key = best_of(key);
   if (lane == 0) s_key[wave] = key;
   __syncthreads();
-  if (tid) return;
-  for (int k = 1; k < kWaves; ++k) key = s_key[k] > key ? s_key[k] : key;
-  *out = key >> 32 ? 0xffffffffu - static_cast<u32>(key) : static_cast<int64_t>(key) - 1;
+  const u64 best = best_of<16>(s_key[lane & (kWaves - 1)]);
+  if (tid == 0) *out = best >> 32 ? token_of(best) : static_cast<int64_t>(best) - 1;
 }
 
 // ---------------------------------------------------------------- sizes
@@ -602,7 +811,12 @@ __global__ __launch_bounds__(kThreads) void next_token_kernel(const VerifyParams
 int segments_of(int64_t rows) {
   return static_cast<int>(std::max<int64_t>(1, std::min<int64_t>(kMaxSegments, 512 / std::max<int64_t>(rows, 1))));
 }
-int range_chunks_of(int) { return kRangeChunks; }
+// Chunks of a range, whole 64s: a row has kMostRanges at most, and a batch no more than 4096 unless rows have 64.
+int range_chunks_of(int64_t num_seqs, int64_t chunks) {
+  const int64_t per_row = std::max<int64_t>(64, std::min<int64_t>(kMostRanges, 4096 / std::max<int64_t>(num_seqs, 1)));
+  const int64_t per = (chunks + per_row - 1) / per_row;
+  return static_cast<int>(std::min<int64_t>(kMaxRange, (per + 63) / 64 * 64));
+}
 int64_t round16(int64_t n) { return (n + 15) / 16 * 16; }
 
 struct Layout {
@@ -614,18 +828,31 @@ Layout layout_of(int64_t num_seqs, int64_t max_rows, int64_t vocab) {
   const int64_t rows = 2 * num_seqs * max_rows;
   l.records = round16(std::max(rows, std::min<int64_t>(rows * kMaxSegments, 1024)) * sizeof(float4));
   l.sums = l.records + round16(num_seqs * sizeof(Record));
-  const int64_t ranges = ((vocab + 3) / 4 + 63) / 64;  // the most that any type and range length has
+  const int64_t chunks = (vocab + 3) / 4;
+  const int64_t ranges = std::max<int64_t>(std::min<int64_t>(kMostRanges, (chunks + 63) / 64), (chunks + kMaxRange - 1) / kMaxRange);
   l.bytes = l.sums + num_seqs * ranges * sizeof(Sums);
   return l;
+}
+
+// Whether walk_kernel's fewer rows, with a workgroup each, are likely to take less time than all rows over all workgroups.
+bool walks(const VerifyParams& p, int item) {
+  const int64_t row = static_cast<int64_t>(p.vocab) * item;
+  const int64_t rows = static_cast<int64_t>(p.total) + (p.draft ? p.total - p.num_seqs : 0);
+  return static_cast<double>(rows) * row / 5.5e6 > 4 * ((p.draft ? 2 : 1) * row / 8e4 + 2);
 }
 
 template <typename T>
 int launch(const char* fn, const VerifyParams& p, hipStream_t s) {
   const LaunchOrder order;
-  const dim3 stats(p.segments, p.max_rows * (p.draft ? 2 : 1), p.num_seqs);
-  hipLaunchKernelGGL(row_stats_kernel<T>, stats, dim3(kThreads), 0, s, p);
-  hipLaunchKernelGGL(keep_kernel<T>, dim3(p.num_seqs), dim3(64), 0, s, p);
-  hipLaunchKernelGGL(range_sums_kernel<T>, dim3((p.ranges + kWaves - 1) / kWaves, p.num_seqs), dim3(kThreads), 0, s, p);
+  const dim3 sums((p.ranges + kWaves - 1) / kWaves, p.num_seqs);
+  if (walks(p, sizeof(T))) {
+    hipLaunchKernelGGL(walk_kernel<T>, dim3(p.num_seqs), dim3(kWalkThreads), 0, s, p);
+    hipLaunchKernelGGL((range_sums_kernel<T, true>), sums, dim3(kThreads), 0, s, p);
+  } else {
+    const dim3 stats(p.segments, p.max_rows * (p.draft ? 2 : 1), p.num_seqs);
+    hipLaunchKernelGGL(row_stats_kernel<T>, stats, dim3(kThreads), 0, s, p);
+    hipLaunchKernelGGL((range_sums_kernel<T, false>), sums, dim3(kThreads), 0, s, p);
+  }
   hipLaunchKernelGGL(next_token_kernel<T>, dim3(p.num_seqs), dim3(kThreads), 0, s, p);
   return launch_status(fn);
 }
@@ -696,8 +923,8 @@ extern "C" int kvp_verify_drafts(const void* logits, int32_t logits_fp32, int64_
   p.path = path;
   p.out = out_tokens;
   p.segments = segments_of(2ll * num_seqs * max_seqlen_q);
-  p.range_chunks = range_chunks_of(num_seqs);
   const int chunks = (vocab + per16 - 1) / per16;
+  p.range_chunks = range_chunks_of(num_seqs, chunks);
   p.ranges = (chunks + p.range_chunks - 1) / p.range_chunks;
   p.stats = reinterpret_cast<float4*>(ws + at.stats);
   p.records = reinterpret_cast<Record*>(ws + at.records);

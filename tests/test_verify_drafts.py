@@ -99,9 +99,30 @@ def same(got, want):
         assert x.dtype == y.dtype and torch.equal(x, y), f"{name}:\n{x}\n{y}"
 
 
+def many(a, want):
+    """The batch again and again, in one call of 100 MB of logits and more, which takes another way through the rows."""
+    rows, vocab = a["logits"].shape
+    times = -(-220_000_000 // (rows * vocab * a["logits"].element_size()))
+    seqs = len(a["temperatures"])
+    if times * seqs > 20_000:
+        return
+    wide = {name: t if not isinstance(t, torch.Tensor) else t.repeat(times, *[1] * (t.dim() - 1)) for name, t in a.items()}
+    for name in ("logits", "draft_logits"):
+        if wide[name] is not None:
+            room = torch.full((rows * times, -(-vocab // 8) * 8), math.nan, dtype=a[name].dtype, device="cuda")
+            room[:, :vocab] = wide[name]
+            wide[name] = room[:, :vocab]
+    cu = a["cu_seqlens_q"]
+    steps = torch.arange(times, device="cuda", dtype=torch.int32)[:, None] * rows
+    wide["cu_seqlens_q"] = torch.cat(((cu[:-1] + steps).view(-1), cu[-1:] + steps[-1]))
+    same(fused.verify_drafts(**wide), [w.repeat(times, *[1] * (w.dim() - 1)) for w in want])
+
+
 def check(batch):
     want, _ = batch.want()
-    same(fused.verify_drafts(**batch.on_gpu()), want)
+    a = batch.on_gpu()
+    same(fused.verify_drafts(**a), want)
+    many(a, want)
     return want
 
 
@@ -189,6 +210,7 @@ def test_temperatures_and_numbers_at_their_ends(cuda_device, form):
     x.uniforms[36:48] = BELOW_ONE
     *want, _ = oracle.verify_drafts(**x.args())
     same(fused.verify_drafts(**x.on_gpu()), want)
+    many(x.on_gpu(), want)
 
 
 @pytest.mark.gpu
@@ -203,7 +225,9 @@ def test_a_draft_model_that_is_the_target_keeps_everything(cuda_device, dtype):
     x.uniforms.view(20, 8)[:, 1:] = BELOW_ONE
     got = fused.verify_drafts(**x.on_gpu())
     assert (got[0] == 7).all()
-    same(got, oracle.verify_drafts(**x.args())[:3])
+    want = oracle.verify_drafts(**x.args())[:3]
+    same(got, want)
+    many(x.on_gpu(), want)
 
 
 @pytest.mark.gpu
