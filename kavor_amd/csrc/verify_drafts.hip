@@ -28,13 +28,14 @@ typedef unsigned long long u64;
 
 constexpr int kThreads = 512;
 constexpr int kWaves = kThreads / 64;
-constexpr int kWalkThreads = 1024;
-constexpr int kWalkWaves = kWalkThreads / 64;
 constexpr int kMaxRows = 64;  // rows of a sequence, as in kvp_tree_attention: one per lane
 constexpr int kMaxSegments = 16;   // of a row: one per lane of a 16-lane row where they are joined
 constexpr int kMaxRange = 512;     // chunks of a range, at most: one per thread where it is taken again
 constexpr int kMostRanges = 512;   // of a row, unless they would be longer than that
 constexpr int kBatch = 4;          // chunks in flight per lane
+constexpr int64_t kOnePass = 200 << 20;  // bytes of logits up to which all rows are taken at once
+constexpr int kMaxPasses = 8;
+constexpr int kKnown = 32;  // sequences from which the last rows are found by a kernel of its own
 constexpr float kReach = 16.f;     // binary orders that a value may lie above the reference
 constexpr float kHuge = 3.4028234e38f;
 // Weights relative to a row's largest: a single one below kTiny counts as 0.  Sums take them as 2^-1000 at least, so up to
@@ -71,8 +72,11 @@ struct VerifyParams {
   int32_t* path;    // [num_seqs][max_rows]
   int64_t* out;     // [num_seqs][max_rows]
   int32_t segments; // of a row in the first pass
-  int32_t range_chunks, ranges;
+  int32_t range_chunks, ranges, ranges_per_wave;
   float4* stats;    // [sequence][row][p, q][segment]: maximum and sum, or the greedy key
+  uint4* drafts;    // [2][sequence][row]: what leave_drafts() finds
+  u32* list;        // rows of a pass: sequence, row, p or q
+  u32* counts;      // of them, by pass
   Record* records;
   Sums* sums;       // [sequence][range]
 };
@@ -255,26 +259,43 @@ __device__ __forceinline__ float rebased(const Part& part, float to, float scale
   return part.sum * fast_exp2((clamped(part.max) - to) * scale);
 }
 
+// a b, rounded: fused into a subtraction it would differ from itself by that rounding.
+__device__ __forceinline__ float product(float a, float b) {
+#pragma clang fp contract(off)
+  return a * b;
+}
+
 // The chunks from c0 on that the waves of a group of `waves` take, 64 at a time, up to cend; c0 is the wave's own first one.
 template <typename T>
 __device__ __forceinline__ Part part_of(const Row<T>& row, int c0, int waves, int cend, float scale) {
   constexpr int E = Chunk<T>::kSize;
   const int lane = threadIdx.x & 63, step = 64 * waves;
   const int whole = min(cend, row.full);
-  float m = -INFINITY, s = 0.f, ref = -kHuge;
+  // s is the sum of 2^(x scale - shift), one fma a value, or of 2^((x - ref) scale) where `far`: shift is
+  // off by up to 2^-24 of itself, which a fma shows
+  float m = -INFINITY, s = 0.f, ref = -kHuge, shift = 0.f;
+  bool far = true;
   auto take = [&](auto count, const float* f) __attribute__((always_inline)) {
     constexpr int N = decltype(count)::value;
     float most = max3(f[0], f[1], f[2]);
 #pragma unroll
     for (int e = 3; e < N; e += 2) most = max3(most, f[e], f[min(e + 1, N - 1)]);
-    if (__any((most - ref) * scale > kReach)) {  // uniform
-      const float to = clamped(max_of(most));
-      s *= fast_exp2((ref - to) * scale);
+    if (__any((far ? (most - ref) * scale : fmaf(most, scale, -shift)) > kReach)) {  // uniform
+      const float to = clamped(max_of(most)), by = product(to, scale);
+      const bool now = !(fabsf(by) < 0x1p20f);
+      s *= fast_exp2(far || now ? (ref - to) * scale : shift - by);
       ref = to;
+      shift = by;
+      far = now;
     }
     m = max3(m, most, most);
+    if (far) {
 #pragma unroll
-    for (int e = 0; e < N; ++e) s += fast_exp2((f[e] - ref) * scale);
+      for (int e = 0; e < N; ++e) s += fast_exp2((f[e] - ref) * scale);
+    } else {
+#pragma unroll
+      for (int e = 0; e < N; ++e) s += fast_exp2(fmaf(f[e], scale, -shift));
+    }
   };
   uint4 in[kBatch];
   auto load_batch = [&](int c) {
@@ -302,7 +323,8 @@ __device__ __forceinline__ Part part_of(const Row<T>& row, int c0, int waves, in
     }
   }
   const float top = max_of(m);
-  return {top, sum_of(s) * fast_exp2((ref - clamped(top)) * scale)};
+  const float to_top = far ? (ref - clamped(top)) * scale : -fmaf(clamped(top), scale, -shift);
+  return {top, sum_of(s) * fast_exp2(to_top)};
 }
 
 // The greedy key of the same chunks.
@@ -352,42 +374,6 @@ __device__ __forceinline__ u64 key_of(const Row<T>& row, int c0, int waves, int 
   return best_of(key);
 }
 
-// A segment of a row per workgroup.
-template <typename T>
-__global__ __launch_bounds__(kThreads) void row_stats_kernel(const VerifyParams p) {
-  __shared__ Part s_part[kWaves];
-  __shared__ u64 s_key[kWaves];
-  const int seg = static_cast<int>(blockIdx.x), i = blockIdx.y >> (p.draft ? 1 : 0), b = blockIdx.z;
-  const bool of_draft = p.draft && (blockIdx.y & 1);
-  const int q0 = p.cu[b], n = p.cu[b + 1] - q0;
-  if (n > p.max_rows || q0 < 0 || q0 + n > p.total || i >= n - (of_draft ? 1 : 0)) return;
-  const double scale = scale_of(p.temps[b]);
-  if (of_draft && scale == 0) return;
-  const Row<T> row(of_draft ? static_cast<const T*>(p.draft) + (q0 + i) * p.draft_stride
-                            : static_cast<const T*>(p.logits) + (q0 + i) * p.row_stride, p.vocab);
-  const int chunks = row.chunks(), per = (chunks + p.segments - 1) / p.segments;
-  const int cbeg = min(seg * per, chunks), cend = min(cbeg + per, chunks);
-  const int wave = threadIdx.x >> 6, lane = threadIdx.x & 63;
-  float4& out = p.stats[(((static_cast<int64_t>(b) * p.max_rows + i) << 1) + of_draft) * p.segments + seg];
-  if (scale == 0) {  // uniform
-    const u64 key = key_of(row, cbeg + 64 * wave, kWaves, cend);
-    if (lane == 0) s_key[wave] = key;
-    __syncthreads();
-    if (wave != 0) return;
-    const u64 best = best_of<16>(s_key[lane & (kWaves - 1)]);
-    if (lane == 0) out = make_float4(__uint_as_float(static_cast<u32>(best)), __uint_as_float(static_cast<u32>(best >> 32)), 0.f, 0.f);
-    return;
-  }
-  const Part part = part_of(row, cbeg + 64 * wave, kWaves, cend, scale32(scale));
-  if (lane == 0) s_part[wave] = part;
-  __syncthreads();
-  if (wave != 0) return;
-  Part mine = s_part[lane & (kWaves - 1)];
-  const float top = max_of<16>(mine.max);
-  const float sum = sum_of<16>(lane < kWaves ? rebased(mine, clamped(top), scale32(scale)) : 0.f);
-  if (lane == 0) out = make_float4(top, sum, 0.f, 0.f);
-}
-
 // ---------------------------------------------------------------- the way through the drafts
 
 // What a row's parts come to.
@@ -404,49 +390,84 @@ __device__ __forceinline__ RowStats stats_of(float max, double sum) {
 // A row of the sequence per lane.
 struct Draft {
   int64_t token;
-  double u;
-  int parent;    // -1: none
-  bool inside;   // a draft with a parent and a token of the vocabulary
-  float z, y;    // its logits in its parent's rows
+  int parent;  // -1: none
+  u64 line;    // its ancestors and itself
+  float u;
+  float z, y;  // its logits in its parent's rows
+  __device__ __forceinline__ bool inside(int vocab) const { return parent >= 0 && token >= 0 && token < vocab; }
 };
-template <typename T>
-__device__ __forceinline__ Draft draft_of(const VerifyParams& p, int q0, int n) {
+// Parents and lines.
+__device__ __forceinline__ Draft lines_of(const VerifyParams& p, int q0, int n) {
   const int i = threadIdx.x & 63;
-  Draft d{-1, 0.0, -1, false, 0.f, 0.f};
+  Draft d{-1, -1, 0, 0.f, 0.f, 0.f};
   if (i < n) {
-    d.token = p.tokens[q0 + i];
-    d.u = p.uniforms[q0 + i];
     const u64 below = (1ull << i) - 1, sees = p.masks ? static_cast<u64>(p.masks[q0 + i]) & below : below;
     d.parent = sees ? 63 - __builtin_clzll(sees) : -1;
-    d.inside = d.parent >= 0 && d.token >= 0 && d.token < p.vocab;
-    if (d.inside) {
-      d.z = Chunk<T>::one(static_cast<const T*>(p.logits)[(q0 + d.parent) * p.row_stride + d.token]);
-      if (p.draft) d.y = Chunk<T>::one(static_cast<const T*>(p.draft)[(q0 + d.parent) * p.draft_stride + d.token]);
+    d.line = p.masks ? (d.parent >= 0 ? 1ull << d.parent : 0) | 1ull << i : below | 1ull << i;
+  }
+  if (p.masks) {  // each round doubles how far back a line goes
+    int back = d.parent;
+#pragma unroll
+    for (int round = 0; round < 6; ++round) {
+      const u64 older = static_cast<u64>(__shfl(static_cast<u32>(d.line >> 32), max(back, 0))) << 32 |
+                        __shfl(static_cast<u32>(d.line), max(back, 0));
+      const int further = __shfl(back, max(back, 0));
+      if (back >= 0) {
+        d.line |= older;
+        back = further;
+      }
     }
   }
   return d;
+}
+// All of it, found once and left for the kernels behind, which then have no chain of loads to wait for.
+template <typename T>
+__device__ __forceinline__ void leave_drafts(const VerifyParams& p, int b, int q0, int n) {
+  const int i = threadIdx.x & 63;
+  const bool real = i < n;
+  const int64_t token = real ? p.tokens[q0 + i] : -1;
+  const float u = real ? p.uniforms[q0 + i] : 0.f;
+  Draft d = lines_of(p, q0, n);
+  d.token = token;
+  if (d.inside(p.vocab)) {
+    d.z = Chunk<T>::one(static_cast<const T*>(p.logits)[(q0 + d.parent) * p.row_stride + token]);
+    if (p.draft) d.y = Chunk<T>::one(static_cast<const T*>(p.draft)[(q0 + d.parent) * p.draft_stride + token]);
+  }
+  if (!real) return;
+  uint4* at = p.drafts + static_cast<int64_t>(b) * p.max_rows + i;
+  at[0] = make_uint4(static_cast<u32>(token), static_cast<u32>(token >> 32), static_cast<u32>(d.line), static_cast<u32>(d.line >> 32));
+  at[static_cast<int64_t>(p.num_seqs) * p.max_rows] =
+      make_uint4(static_cast<u32>(d.parent), __float_as_uint(u), __float_as_uint(d.z), __float_as_uint(d.y));
+}
+__device__ __forceinline__ Draft left_drafts(const VerifyParams& p, int b, int n) {
+  const int i = threadIdx.x & 63;
+  const uint4* at = p.drafts + static_cast<int64_t>(b) * p.max_rows + min(i, p.max_rows - 1);
+  const uint4 x = at[0], y = at[static_cast<int64_t>(p.num_seqs) * p.max_rows];
+  if (i >= n) return {-1, -1, 0, 0.f, 0.f, 0.f};
+  return {static_cast<int64_t>(static_cast<u64>(x.y) << 32 | x.x), static_cast<int>(y.x), static_cast<u64>(x.w) << 32 | x.z,
+          __uint_as_float(y.y), __uint_as_float(y.z), __uint_as_float(y.w)};
 }
 
 // The child of a row that stays, or -1, by a whole wave; `children` are the row's.
 __device__ __forceinline__ int child_that_stays(const VerifyParams& p, const Draft& d, u64 children, double scale,
                                                 const RowStats& sp, const RowStats& sq) {
   if (children == 0) return -1;
+  const bool in = d.inside(p.vocab);
   if (scale == 0) {
-    const u64 same = __ballot(d.inside && d.token == token_of(sp.key)) & children;
+    const u64 same = __ballot(in && d.token == token_of(sp.key)) & children;
     return same ? __builtin_ctzll(same) : -1;
   }
   if (!sp.ok) return -1;
-  const double px = d.inside ? weight(d.z, sp.top, scale) / sp.sum : 0.0;
+  const double px = in ? weight(d.z, sp.top, scale) / sp.sum : 0.0;
   if (p.draft) {
     if (!sq.ok) return -1;
-    const double qx = d.inside ? weight(d.y, sq.top, scale) / sq.sum : 0.0;
-    const u64 passes = __ballot(d.inside && d.u * qx < px) & children;
+    const double qx = in ? weight(d.y, sq.top, scale) / sq.sum : 0.0;
+    const u64 passes = __ballot(in && d.u * qx < px) & children;
     return passes ? __builtin_ctzll(passes) : -1;
   }
-  const u64 inside = __ballot(d.inside);
   double left = 1;
   u64 refused = 0;
-  for (u64 rest = children & inside; rest; rest &= rest - 1) {  // siblings in turn
+  for (u64 rest = children & __ballot(in); rest; rest &= rest - 1) {  // siblings in turn
     const int j = __builtin_ctzll(rest);
     const u64 twins = __ballot(d.token == static_cast<int64_t>(lane_of(static_cast<u64>(d.token), j)));
     if (twins & refused) continue;
@@ -460,10 +481,19 @@ __device__ __forceinline__ int child_that_stays(const VerifyParams& p, const Dra
 
 __device__ __forceinline__ u64 children_of(const Draft& d, int node) { return __ballot(d.parent == node); }
 
+struct Way {
+  u64 kept;
+  int node;
+  bool ended;  // no child of node stays; otherwise it has not been asked
+  RowStats sp, sq;
+};
+
 // Writes a sequence's results, by one wave, and gives what is left to draw.
-__device__ __forceinline__ Record finish(const VerifyParams& p, int b, int q0, int n, const Draft& d, u64 kept, int node,
-                                         double scale, const RowStats& sp, const RowStats& sq, bool write) {
-  const int i = threadIdx.x & 63, count = __popcll(kept);
+__device__ __forceinline__ Record finish(const VerifyParams& p, int b, int q0, int n, const Draft& d, const Way& way,
+                                         double scale, bool write) {
+  const RowStats &sp = way.sp, &sq = way.sq;
+  const u64 kept = way.kept;
+  const int i = threadIdx.x & 63, count = __popcll(kept), node = way.node;
   const u64 gone = children_of(d, node);
   Record rec{q0 + node, kDone, scale, sp.top, sq.top, sp.sum / sq.sum, gone};
   if (n > 0 && scale != 0) {
@@ -499,95 +529,146 @@ __device__ __forceinline__ int rows_of(const VerifyParams& p, int b, int& q0) {
   return n <= 0 || n > p.max_rows || q0 < 0 || q0 + n > p.total ? 0 : n;
 }
 
-// Behind row_stats_kernel: the way by one wave, a row's segments per 16 lanes.
-template <typename T>
-__device__ __forceinline__ Record way_of(const VerifyParams& p, int b, bool write) {
+// A row's parts: lanes 0 to 15 have p's segments, 16 to 31 q's.
+__device__ __forceinline__ float4 parts_of(const VerifyParams& p, int b, int i) {
+  const int lane = threadIdx.x & 63, seg = min(lane & 15, p.segments - 1);
+  return p.stats[(((static_cast<int64_t>(b) * p.max_rows + i) << 1) + (p.draft ? lane >> 4 & 1 : 0)) * p.segments + seg];
+}
+// The way from row 0 by one wave, as far as row `depth` of it.  The statistics of the rows before that one are there; x are
+// row 0's parts.
+__device__ __forceinline__ Way way_to(const VerifyParams& p, int b, int n, const Draft& d, double scale, float4 x, int depth) {
+  Way way{0, 0, false, {0.f, 1, false, 0}, {0.f, 1, false, 0}};
   const int lane = threadIdx.x & 63;
-  int q0;
-  const int n = rows_of(p, b, q0);
-  const double scale = scale_of(p.temps[b]);
-  RowStats sp{0.f, 1, false, 0}, sq{0.f, 1, false, 0};
-  Draft d{-1, 0.0, -1, false, 0.f, 0.f};
-  u64 kept = 0;
-  int node = 0;
-  if (n > 0) {
-    // lanes 0 to 15 have p's segments, 16 to 31 q's
-    auto parts = [&](int i) {
-      const int seg = lane & 15;
-      const bool there = seg < p.segments && (lane < 16 || (lane < 32 && p.draft && i < n - 1 && scale != 0));
-      const int64_t at = (((static_cast<int64_t>(b) * p.max_rows + i) << 1) + (lane >> 4 & 1)) * p.segments + seg;
-      return there ? p.stats[at] : make_float4(-INFINITY, 0.f, 0.f, 0.f);
-    };
-    float4 x = parts(0);
-    d = draft_of<T>(p, q0, n);
-    while (true) {
-      if (scale == 0) {
-        const u64 key = static_cast<u64>(__float_as_uint(x.y)) << 32 | __float_as_uint(x.x);
-        sp.key = lane_of(best_of<16>((lane & 15) < p.segments && lane < 16 ? key : 0), 0);
-      } else {
-        const float top = max_of<16>(x.x);
-        const double sum = sum_of<16>(static_cast<double>(rebased({x.x, x.y}, clamped(top), scale32(scale))));
-        sp = stats_of(lane_of(top, 0), lane_of(sum, 0));
-        sq = stats_of(lane_of(top, 16), lane_of(sum, 16));
-      }
-      const int next = child_that_stays(p, d, children_of(d, node), scale, sp, sq);
-      if (next < 0) break;  // uniform
-      kept |= 1ull << next;
-      node = next;
-      x = parts(node);
+  while (depth-- > 0) {
+    const bool there = (lane & 15) < p.segments && (lane < 16 || (lane < 32 && p.draft && way.node < n - 1));
+    if (scale == 0) {
+      const u64 key = static_cast<u64>(__float_as_uint(x.y)) << 32 | __float_as_uint(x.x);
+      way.sp.key = lane_of(best_of<16>(there ? key : 0), 0);
+    } else {
+      const Part part{there ? x.x : -INFINITY, there ? x.y : 0.f};
+      const float top = max_of<16>(part.max);
+      const double sum = sum_of<16>(static_cast<double>(rebased(part, clamped(top), scale32(scale))));
+      way.sp = stats_of(lane_of(top, 0), lane_of(sum, 0));
+      way.sq = stats_of(lane_of(top, 16), lane_of(sum, 16));
     }
+    const int next = child_that_stays(p, d, children_of(d, way.node), scale, way.sp, way.sq);
+    if (next < 0) {  // uniform
+      way.ended = true;
+      break;
+    }
+    way.kept |= 1ull << next;
+    way.node = next;
+    if (depth > 0) x = parts_of(p, b, next);
   }
-  return finish(p, b, q0, n, d, kept, node, scale, sp, sq, write);
+  return way;
 }
 
-// The way without the first pass: a workgroup per sequence takes only the rows that it gets to.
+// Maximum and sum (or greedy key) of a segment of a row, by a workgroup.
 template <typename T>
-__global__ __launch_bounds__(kWalkThreads) void walk_kernel(const VerifyParams p) {
-  __shared__ Part s_part[2][kWalkWaves];
-  __shared__ u64 s_key[2][kWalkWaves];
-  const int b = blockIdx.x, wave = threadIdx.x >> 6, lane = threadIdx.x & 63;
+__device__ __forceinline__ void row_segment(const VerifyParams& p, int b, int q0, int i, bool of_draft, int seg, double scale,
+                                            Part* s_part, u64* s_key) {
+  const int wave = threadIdx.x >> 6, lane = threadIdx.x & 63;
+  const Row<T> row(of_draft ? static_cast<const T*>(p.draft) + (q0 + i) * p.draft_stride
+                            : static_cast<const T*>(p.logits) + (q0 + i) * p.row_stride, p.vocab);
+  const int chunks = row.chunks(), per = (chunks + p.segments - 1) / p.segments;
+  const int cbeg = min(seg * per, chunks), cend = min(cbeg + per, chunks);
+  float4& out = p.stats[(((static_cast<int64_t>(b) * p.max_rows + i) << 1) + of_draft) * p.segments + seg];
+  if (scale == 0) {  // uniform
+    const u64 key = key_of(row, cbeg + 64 * wave, kWaves, cend);
+    if (lane == 0) s_key[wave] = key;
+    __syncthreads();
+    if (wave != 0) return;
+    const u64 best = best_of<16>(s_key[lane & (kWaves - 1)]);
+    if (lane == 0)
+      out = make_float4(__uint_as_float(static_cast<u32>(best)), __uint_as_float(static_cast<u32>(best >> 32)), 0.f, 0.f);
+    return;
+  }
+  const Part part = part_of(row, cbeg + 64 * wave, kWaves, cend, scale32(scale));
+  if (lane == 0) s_part[wave] = part;
+  __syncthreads();
+  if (wave != 0) return;
+  const Part mine = s_part[lane & (kWaves - 1)];
+  const float top = max_of<16>(mine.max);
+  const float sum = sum_of<16>((lane & 15) < kWaves ? rebased(mine, clamped(top), scale32(scale)) : 0.f);
+  if (lane == 0) out = make_float4(top, sum, 0.f, 0.f);
+}
+
+// The first rows of every sequence, as many as the grid has: a segment per workgroup.  One more workgroup for each
+// sequence leaves what there is to know of its drafts, and clears the counters of the lists.
+template <typename T>
+__global__ __launch_bounds__(kThreads) void row_stats_kernel(const VerifyParams p) {
+  __shared__ Part s_part[kWaves];
+  __shared__ u64 s_key[kWaves];
+  const int b = blockIdx.z, item = blockIdx.y;
+  const int i = p.draft ? item >> 1 : item;
+  const bool of_draft = p.draft && (item & 1);
+  int q0;
+  const int n = rows_of(p, b, q0);
+  if (item == static_cast<int>(gridDim.y) - 1) {
+    if (blockIdx.x == 0 && threadIdx.x < 64) {
+      leave_drafts<T>(p, b, q0, n);
+      if (b == 0 && threadIdx.x < kMaxPasses) p.counts[threadIdx.x] = 0;
+    }
+    return;
+  }
+  if (i >= n - (of_draft ? 1 : 0)) return;
+  const double scale = scale_of(p.temps[b]);
+  if (of_draft && scale == 0) return;
+  row_segment<T>(p, b, q0, i, of_draft, blockIdx.x, scale, s_part, s_key);
+}
+
+// Lists the rows `from` .. `to` - 1 steps from row 0 that the sequences can still get to, given those before them: a wave
+// per sequence.
+__global__ __launch_bounds__(64) void list_rows_kernel(const VerifyParams p, const int from, const int to, const int pass) {
+  const int b = blockIdx.x, lane = threadIdx.x;
+  const float4 x = parts_of(p, b, 0);
   int q0;
   const int n = rows_of(p, b, q0);
   const double scale = scale_of(p.temps[b]);
-  RowStats sp{0.f, 1, false, 0}, sq{0.f, 1, false, 0};
-  Draft d{-1, 0.0, -1, false, 0.f, 0.f};
-  u64 kept = 0;
-  int node = 0;
-  if (n > 0) {
-    d = draft_of<T>(p, q0, n);
-    for (int turn = 0;; turn ^= 1) {  // all waves go the same way
-      const Row<T> row(static_cast<const T*>(p.logits) + (q0 + node) * p.row_stride, p.vocab);
-      if (scale == 0) {
-        const u64 key = key_of(row, 64 * wave, kWalkWaves, row.chunks());
-        if (lane == 0) s_key[turn][wave] = key;
-        __syncthreads();
-        sp.key = best_of<16>(s_key[turn][lane & 15]);
-      } else {
-        // with a draft's row the first half of the waves has p's, the second q's
-        const bool both = p.draft && node < n - 1;
-        const bool of_draft = both && wave >= kWalkWaves / 2;
-        const Row<T> mine(of_draft ? static_cast<const T*>(p.draft) + (q0 + node) * p.draft_stride : row.at, p.vocab);
-        const int waves = both ? kWalkWaves / 2 : kWalkWaves;
-        const Part part = part_of(mine, 64 * (wave & (waves - 1)), waves, row.chunks(), scale32(scale));
-        if (lane == 0) s_part[turn][wave] = part;
-        __syncthreads();
-        // lanes 0 to 15 join p's, 16 to 31 q's
-        const int at = lane & 15;
-        const bool there = lane < 16 ? at < waves : both && at < waves;
-        Part x = there ? s_part[turn][(lane < 16 ? 0 : waves) + at] : Part{-INFINITY, 0.f};
-        const float top = max_of<16>(x.max);
-        const double sum = sum_of<16>(static_cast<double>(rebased(x, clamped(top), scale32(scale))));
-        sp = stats_of(lane_of(top, 0), lane_of(sum, 0));
-        sq = stats_of(lane_of(top, 16), lane_of(sum, 16));
-      }
-      const int next = child_that_stays(p, d, children_of(d, node), scale, sp, sq);
-      if (next < 0) break;  // uniform
-      kept |= 1ull << next;
-      node = next;
-    }
-  }
-  if (wave == 0) finish(p, b, q0, n, d, kept, node, scale, sp, sq, true);
+  const Draft d = left_drafts(p, b, n);
+  if (n <= from) return;
+  const Way way = way_to(p, b, n, d, scale, x, from);
+  if (way.ended) return;  // uniform
+  const int steps = __popcll(d.line) - 1;
+  const u64 rows = __ballot((d.line >> way.node & 1) && (d.line & 1) && steps >= from && steps < to);
+  const u64 rows_q = p.draft && scale != 0 ? rows & ~(1ull << (n - 1)) : 0;
+  const int count = __popcll(rows), items = count + __popcll(rows_q);
+  u32 at = 0;
+  if (lane == 0) at = atomicAdd(&p.counts[pass], static_cast<u32>(items));  // their order changes no result
+  at = __builtin_amdgcn_readfirstlane(at);
+  const u64 below = (1ull << lane) - 1;
+  const u32 item = static_cast<u32>(b) << 8 | static_cast<u32>(lane) << 1;
+  if (rows >> lane & 1) p.list[at + __popcll(rows & below)] = item;
+  if (rows_q >> lane & 1) p.list[at + count + __popcll(rows_q & below)] = item | 1;
 }
+
+// The listed rows: a unit is a segment of one, and workgroups take them in turn.
+template <typename T>
+__global__ __launch_bounds__(kThreads) void listed_stats_kernel(const VerifyParams p, const int pass) {
+  __shared__ Part s_part[2][kWaves];
+  __shared__ u64 s_key[2][kWaves];
+  const int units = static_cast<int>(p.counts[pass]) * p.segments;
+  int turn = 0;
+  for (int unit = blockIdx.x; unit < units; unit += gridDim.x, turn ^= 1) {
+    const int at = unit / p.segments, seg = unit - at * p.segments;
+    const u32 item = p.list[at];
+    const int b = static_cast<int>(item >> 8);
+    row_segment<T>(p, b, p.cu[b], static_cast<int>(item >> 1 & 127), item & 1, seg, scale_of(p.temps[b]), s_part[turn],
+                   s_key[turn]);
+  }
+}
+
+// The whole way, by one wave.
+__device__ __forceinline__ Record last_row(const VerifyParams& p, int b, bool write) {
+  const float4 x = parts_of(p, b, 0);
+  int q0;
+  const int n = rows_of(p, b, q0);
+  const double scale = scale_of(p.temps[b]);
+  const Draft d = left_drafts(p, b, n);
+  const Way way = way_to(p, b, n, d, scale, x, n > 0 ? kMaxRows : 0);
+  return finish(p, b, q0, n, d, way, scale, write);
+}
+__global__ __launch_bounds__(64) void last_row_kernel(const VerifyParams p) { last_row(p, blockIdx.x, true); }
 
 // ---------------------------------------------------------------- sums of the last row
 
@@ -602,81 +683,131 @@ __device__ __forceinline__ bool is_refused(const Refused& r, int v) {
   return hit;
 }
 // By a whole wave; a row of the sequence per lane.
-__device__ __forceinline__ void find_refused(const VerifyParams& p, const Record& rec, int q0, int vbeg, int vend, Refused& r) {
+__device__ __forceinline__ void find_refused(const VerifyParams& p, const Record& rec, int b, int vbeg, int vend, Refused& r) {
   const int lane = threadIdx.x & 63;
-  const int64_t t = rec.gone >> lane & 1 ? p.tokens[q0 + lane] : -1;
+  const int64_t t = rec.gone >> lane & 1 ? p.tokens[p.cu[b] + lane] : -1;
   const bool in = t >= vbeg && t < vend;
   const u64 which = __ballot(in);
   if (in) r.token[__popcll(which & ((1ull << lane) - 1))] = static_cast<int32_t>(t);
   if (lane == 0) r.count = __popcll(which);
 }
 
-// A range per wave.  WALKED: walk_kernel left the records; otherwise every wave goes the way anew.
-template <typename T, bool WALKED>
+// x where `on`, otherwise a value below 2^-1022: its high word alone is cleared.
+__device__ __forceinline__ double only(bool on, double x) {
+  const u64 bits = static_cast<u64>(__double_as_longlong(x));
+  const u32 hi = on ? static_cast<u32>(bits >> 32) : 0;
+  return __longlong_as_double(static_cast<long long>(static_cast<u64>(hi) << 32 | static_cast<u32>(bits)));
+}
+
+// Neighbouring ranges per wave.  KNOWN: last_row_kernel left the records; otherwise every wave goes the way anew.
+//
+// Where 64 chunks have no weight of 2^-28 of the largest or more, as most have in a row that is sure of its token, weights
+// are taken in 32 bits: off by 2^-22 of themselves and 2^-50 of the largest, which is some 1e-13 of a row's sum.
+template <typename T, bool KNOWN>
 __global__ __launch_bounds__(kThreads) void range_sums_kernel(const VerifyParams p) {
   constexpr int E = Chunk<T>::kSize;
   __shared__ Refused s_refused[kWaves];
   const int b = blockIdx.y, wave = threadIdx.x >> 6, lane = threadIdx.x & 63;
-  const int range = blockIdx.x * kWaves + wave;
+  int range = (blockIdx.x * kWaves + wave) * p.ranges_per_wave;
+  if (range >= p.ranges) return;
   Record rec;
-  if constexpr (WALKED) rec = p.records[b];
-  else rec = way_of<T>(p, b, range == 0);
-  if (rec.mode == kDone || rec.mode == kUndefined || range >= p.ranges) return;
+  if constexpr (KNOWN) rec = p.records[b];
+  else rec = last_row(p, b, range == 0);
+  if (rec.mode == kDone || rec.mode == kUndefined) return;
   const Row<T> row(static_cast<const T*>(p.logits) + rec.row * p.row_stride, p.vocab);
-  const int cbeg = range * p.range_chunks, cend = min(cbeg + p.range_chunks, row.chunks());
-  const double scale = rec.scale, top_p = rec.top_p, top_q = rec.top_q;
-  Sums s{0, 0, 0, 0};
-  uint4 in = row.load(cbeg + lane);
-  if (rec.mode == kRest) {
-    const Row<T> row_q(static_cast<const T*>(p.draft) + rec.row * p.draft_stride, p.vocab);
-    uint4 in_q = row_q.load(cbeg + lane);
-    for (int c = cbeg + lane; c < cend; c += 64) {
-      float f[E], g[E];
-      row.values(c, in, f);
-      row_q.values(c, in_q, g);
-      in = row.load(c + 64);
-      in_q = row_q.load(c + 64);
+  const Row<T> row_q(rec.mode == kRest ? static_cast<const T*>(p.draft) + rec.row * p.draft_stride : row.at, p.vocab);
+  const double top_p = rec.top_p, top_q = rec.top_q, scale = rec.scale;
+  const float top_p32 = static_cast<float>(top_p), top_q32 = static_cast<float>(top_q), scale_f = scale32(scale);
+  const float lambda32 = static_cast<float>(rec.lambda);
+  const int last = min(range + p.ranges_per_wave, p.ranges);
+  int c = range * p.range_chunks + lane;
+  uint4 in = row.load(c), in_q = row_q.load(c);
+  auto small = [&](const float (&f)[E], float top) {  // of the wave's chunks
+    float most = max3(f[0], f[1], f[2]);
 #pragma unroll
-      for (int e = 0; e < E; ++e) {
-        const double x = weight_floor(f[e], top_p, scale), y = weight_floor(g[e], top_q, scale);
-        const bool over = x > rec.lambda * y;
-        s.p += x;
-        s.q += y;
-        s.p_over += over ? x : 0.0;
-        s.q_over += over ? y : 0.0;
-      }
-    }
-    s.q = sum_of(s.q);
-    s.q_over = sum_of(s.q_over);
-  } else {
-    Refused& refused = s_refused[wave];
-    bool some = false;
-    if (rec.mode == kWithout) {
-      find_refused(p, rec, p.cu[b], E * cbeg, E * cend, refused);
-      wait_lds();
-      some = refused.count != 0;
-    }
-    for (int c = cbeg + lane; c < cend; c += 64) {
-      float f[E];
-      row.values(c, in, f);
-      in = row.load(c + 64);
-      if (some) {  // uniform
+    for (int e = 3; e < E; e += 2) most = max3(most, f[e], f[min(e + 1, E - 1)]);
+    return !__any((most - top) * scale_f > -28.f);
+  };
+  for (; range < last; ++range) {
+    const int cbeg = range * p.range_chunks, cend = min(cbeg + p.range_chunks, row.chunks());
+    Sums s{0, 0, 0, 0};
+    if (rec.mode == kRest) {
+      for (int c0 = cbeg; c0 < cend; c0 += 64, c += 64) {  // uniform
+        float f[E], g[E];
+#pragma unroll
+        for (int e = 0; e < E; ++e) f[e] = g[e] = -INFINITY;
+        if (c < cend) {
+          row.values(c, in, f);
+          row_q.values(c, in_q, g);
+        }
+        in = row.load(c + 64);
+        in_q = row_q.load(c + 64);
+        if (small(f, top_p32) && small(g, top_q32)) {  // uniform
+          float sp = 0.f, sq = 0.f, sp_over = 0.f, sq_over = 0.f;
+#pragma unroll
+          for (int e = 0; e < E; ++e) {
+            const float x = fast_exp2((f[e] - top_p32) * scale_f), y = fast_exp2((g[e] - top_q32) * scale_f);
+            const bool over = x > lambda32 * y;
+            sp += x;
+            sq += y;
+            sp_over += over ? x : 0.f;
+            sq_over += over ? y : 0.f;
+          }
+          s.p += sp;
+          s.q += sq;
+          s.p_over += sp_over;
+          s.q_over += sq_over;
+          continue;
+        }
 #pragma unroll
         for (int e = 0; e < E; ++e) {
-          const double x = weight_floor(f[e], top_p, scale);
+          const double x = weight_floor(f[e], top_p, scale), y = weight_floor(g[e], top_q, scale);
+          const bool over = x > rec.lambda * y;
           s.p += x;
-          s.p_over += is_refused(refused, E * c + e) ? 0.0 : x;
+          s.q += y;
+          s.p_over += only(over, x);
+          s.q_over += only(over, y);
         }
-      } else {
-#pragma unroll
-        for (int e = 0; e < E; ++e) s.p += weight_floor(f[e], top_p, scale);
       }
+      s.q = sum_of(s.q);
+      s.q_over = sum_of(s.q_over);
+    } else {
+      Refused& refused = s_refused[wave];
+      bool some = false;
+      if (rec.mode == kWithout) {
+        find_refused(p, rec, b, E * cbeg, E * cend, refused);
+        wait_lds();
+        some = refused.count != 0;
+      }
+      for (int c0 = cbeg; c0 < cend; c0 += 64, c += 64) {  // uniform
+        float f[E];
+#pragma unroll
+        for (int e = 0; e < E; ++e) f[e] = -INFINITY;
+        if (c < cend) row.values(c, in, f);
+        in = row.load(c + 64);
+        if (some) {
+#pragma unroll
+          for (int e = 0; e < E; ++e) {
+            const double x = weight_floor(f[e], top_p, scale);
+            s.p += x;
+            s.p_over += is_refused(refused, E * c + e) ? 0.0 : x;
+          }
+        } else if (small(f, top_p32)) {  // uniform
+          float sp = 0.f;
+#pragma unroll
+          for (int e = 0; e < E; ++e) sp += fast_exp2((f[e] - top_p32) * scale_f);
+          s.p += sp;
+        } else {
+#pragma unroll
+          for (int e = 0; e < E; ++e) s.p += weight_floor(f[e], top_p, scale);
+        }
+      }
+      if (!some) s.p_over = s.p;
     }
-    if (!some) s.p_over = s.p;
+    s.p = sum_of(s.p);
+    s.p_over = sum_of(s.p_over);
+    if (lane == 0) p.sums[static_cast<int64_t>(b) * p.ranges + range] = s;
   }
-  s.p = sum_of(s.p);
-  s.p_over = sum_of(s.p_over);
-  if (lane == 0) p.sums[static_cast<int64_t>(b) * p.ranges + range] = s;
 }
 
 // ---------------------------------------------------------------- the next token
@@ -692,7 +823,6 @@ __global__ __launch_bounds__(kThreads) void next_token_kernel(const VerifyParams
   const int b = blockIdx.x, tid = threadIdx.x, wave = tid >> 6, lane = tid & 63;
   const Record rec = p.records[b];
   if (rec.mode == kDone) return;
-  const int q0 = p.cu[b];
   int64_t* out = p.out + static_cast<int64_t>(b) * p.max_rows + p.accepted[b];
   const Row<T> row(static_cast<const T*>(p.logits) + rec.row * p.row_stride, p.vocab);
   if (rec.mode == kUndefined) {  // the greedy token
@@ -703,7 +833,7 @@ __global__ __launch_bounds__(kThreads) void next_token_kernel(const VerifyParams
     if (tid == 0) *out = token_of(best);
     return;
   }
-  const double u = p.uniforms[q0];
+  const double u = p.uniforms[p.cu[b]];
   if (wave == 0) {
     const Sums* sums = p.sums + static_cast<int64_t>(b) * p.ranges;
     Sums all{0, 0, 0, 0};
@@ -756,7 +886,7 @@ __global__ __launch_bounds__(kThreads) void next_token_kernel(const VerifyParams
   const double lambda = s_lambda, left = s_left;
   const int cbeg = range * p.range_chunks, cend = min(cbeg + p.range_chunks, row.chunks());
   if (mode == kWithout) {
-    if (wave == 0) find_refused(p, rec, q0, E * cbeg, E * cend, s_refused);
+    if (wave == 0) find_refused(p, rec, b, E * cbeg, E * cend, s_refused);
     __syncthreads();
   }
   // the range again, a chunk per thread
@@ -808,8 +938,11 @@ __global__ __launch_bounds__(kThreads) void next_token_kernel(const VerifyParams
 
 // ---------------------------------------------------------------- sizes
 
+// Segments of a row: some 2048 workgroups for the rows of a pass, or their next power of two below.
 int segments_of(int64_t rows) {
-  return static_cast<int>(std::max<int64_t>(1, std::min<int64_t>(kMaxSegments, 512 / std::max<int64_t>(rows, 1))));
+  int segments = 1;
+  while (segments < kMaxSegments && 2 * segments * rows <= 2048) segments *= 2;
+  return segments;
 }
 // Chunks of a range, whole 64s: a row has kMostRanges at most, and a batch no more than 4096 unless rows have 64.
 int range_chunks_of(int64_t num_seqs, int64_t chunks) {
@@ -820,13 +953,16 @@ int range_chunks_of(int64_t num_seqs, int64_t chunks) {
 int64_t round16(int64_t n) { return (n + 15) / 16 * 16; }
 
 struct Layout {
-  int64_t stats, records, sums, bytes;
+  int64_t stats, drafts, list, counts, records, sums, bytes;
 };
 Layout layout_of(int64_t num_seqs, int64_t max_rows, int64_t vocab) {
   Layout l{};
-  // the stats of every row in one segment, or of up to 512 segments and a row
-  const int64_t rows = 2 * num_seqs * max_rows;
-  l.records = round16(std::max(rows, std::min<int64_t>(rows * kMaxSegments, 1024)) * sizeof(float4));
+  // of every row one segment, or up to 16 in batches that have no more than 2048 of them
+  const int64_t lists = std::max(num_seqs, std::min<int64_t>(num_seqs * kMaxSegments, 2048));
+  l.drafts = round16(2 * max_rows * lists * sizeof(float4));
+  l.list = l.drafts + round16(2 * num_seqs * max_rows * sizeof(uint4));
+  l.counts = l.list + round16(2 * num_seqs * max_rows * sizeof(u32));
+  l.records = l.counts + round16(kMaxPasses * sizeof(u32));
   l.sums = l.records + round16(num_seqs * sizeof(Record));
   const int64_t chunks = (vocab + 3) / 4;
   const int64_t ranges = std::max<int64_t>(std::min<int64_t>(kMostRanges, (chunks + 63) / 64), (chunks + kMaxRange - 1) / kMaxRange);
@@ -834,23 +970,30 @@ Layout layout_of(int64_t num_seqs, int64_t max_rows, int64_t vocab) {
   return l;
 }
 
-// Whether walk_kernel's fewer rows, with a workgroup each, are likely to take less time than all rows over all workgroups.
-bool walks(const VerifyParams& p, int item) {
-  const int64_t row = static_cast<int64_t>(p.vocab) * item;
-  const int64_t rows = static_cast<int64_t>(p.total) + (p.draft ? p.total - p.num_seqs : 0);
-  return static_cast<double>(rows) * row / 5.5e6 > 4 * ((p.draft ? 2 : 1) * row / 8e4 + 2);
-}
-
 template <typename T>
-int launch(const char* fn, const VerifyParams& p, hipStream_t s) {
+int launch(const char* fn, VerifyParams p, hipStream_t s) {
   const LaunchOrder order;
-  const dim3 sums((p.ranges + kWaves - 1) / kWaves, p.num_seqs);
-  if (walks(p, sizeof(T))) {
-    hipLaunchKernelGGL(walk_kernel<T>, dim3(p.num_seqs), dim3(kWalkThreads), 0, s, p);
+  // All rows in one pass; or, in a large batch, row 0 first, then those 1 and 2 steps behind it that sequences get to,
+  // then 3 to 6, .. and in the last pass the rest.  About half of what is left is expected to be got to each time.
+  const int per_row = p.draft ? 2 : 1;
+  const int64_t rows = std::max<int64_t>(p.total * per_row, p.num_seqs);
+  int64_t bytes = rows * p.vocab * static_cast<int64_t>(sizeof(T));
+  const bool one = bytes < kOnePass || p.max_rows == 1;
+  p.segments = segments_of(one ? rows : p.num_seqs * per_row);
+  hipLaunchKernelGGL(row_stats_kernel<T>, dim3(p.segments, (one ? p.max_rows : 1) * per_row + 1, p.num_seqs), dim3(kThreads),
+                     0, s, p);
+  for (int from = 1, to, pass = 0; !one && from < p.max_rows; from = to, ++pass) {
+    bytes /= 2;
+    to = bytes < kOnePass ? kMaxRows : 2 * from + 1;
+    hipLaunchKernelGGL(list_rows_kernel, dim3(p.num_seqs), dim3(64), 0, s, p, from, to, pass);
+    hipLaunchKernelGGL(listed_stats_kernel<T>, dim3(2048), dim3(kThreads), 0, s, p, pass);
+  }
+  const int per_wg = kWaves * p.ranges_per_wave;
+  const dim3 sums((p.ranges + per_wg - 1) / per_wg, p.num_seqs);
+  if (p.num_seqs >= kKnown) {
+    hipLaunchKernelGGL(last_row_kernel, dim3(p.num_seqs), dim3(64), 0, s, p);
     hipLaunchKernelGGL((range_sums_kernel<T, true>), sums, dim3(kThreads), 0, s, p);
   } else {
-    const dim3 stats(p.segments, p.max_rows * (p.draft ? 2 : 1), p.num_seqs);
-    hipLaunchKernelGGL(row_stats_kernel<T>, stats, dim3(kThreads), 0, s, p);
     hipLaunchKernelGGL((range_sums_kernel<T, false>), sums, dim3(kThreads), 0, s, p);
   }
   hipLaunchKernelGGL(next_token_kernel<T>, dim3(p.num_seqs), dim3(kThreads), 0, s, p);
@@ -922,11 +1065,14 @@ extern "C" int kvp_verify_drafts(const void* logits, int32_t logits_fp32, int64_
   p.accepted = accepted;
   p.path = path;
   p.out = out_tokens;
-  p.segments = segments_of(2ll * num_seqs * max_seqlen_q);
   const int chunks = (vocab + per16 - 1) / per16;
   p.range_chunks = range_chunks_of(num_seqs, chunks);
   p.ranges = (chunks + p.range_chunks - 1) / p.range_chunks;
+  p.ranges_per_wave = 1;
   p.stats = reinterpret_cast<float4*>(ws + at.stats);
+  p.drafts = reinterpret_cast<uint4*>(ws + at.drafts);
+  p.list = reinterpret_cast<u32*>(ws + at.list);
+  p.counts = reinterpret_cast<u32*>(ws + at.counts);
   p.records = reinterpret_cast<Record*>(ws + at.records);
   p.sums = reinterpret_cast<Sums*>(ws + at.sums);
   const auto s = static_cast<hipStream_t>(stream);
