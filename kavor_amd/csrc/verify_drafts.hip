@@ -28,14 +28,16 @@ typedef unsigned long long u64;
 
 constexpr int kThreads = 512;
 constexpr int kWaves = kThreads / 64;
+constexpr int kRowThreads = 256;  // where rows are streamed
+constexpr int kRowWaves = kRowThreads / 64;
 constexpr int kMaxRows = 64;  // rows of a sequence, as in kvp_tree_attention: one per lane
 constexpr int kMaxSegments = 16;   // of a row: one per lane of a 16-lane row where they are joined
 constexpr int kMaxRange = 512;     // chunks of a range, at most: one per thread where it is taken again
 constexpr int kMostRanges = 512;   // of a row, unless they would be longer than that
-constexpr int kBatch = 4;          // chunks in flight per lane
-constexpr int64_t kOnePass = 200 << 20;  // bytes of logits up to which all rows are taken at once
+constexpr int kBatch = 2;          // chunks in flight per lane
+constexpr int64_t kOnePass = 200 << 20;  // bytes of logits that are read in one pass, whether all of them are got to or not
 constexpr int kMaxPasses = 8;
-constexpr int kKnown = 32;  // sequences from which the last rows are found by a kernel of its own
+constexpr int kKnown = 64;              // sequences from which the last rows are found by a kernel of its own
 constexpr float kReach = 16.f;     // binary orders that a value may lie above the reference
 constexpr float kHuge = 3.4028234e38f;
 // Weights relative to a row's largest: a single one below kTiny counts as 0.  Sums take them as 2^-1000 at least, so up to
@@ -109,8 +111,12 @@ struct Row {
   int vocab, full;  // full chunks
   __device__ __forceinline__ Row(const T* base, int vocab) : at(base), vocab(vocab), full(vocab / E) {}
   __device__ __forceinline__ int chunks() const { return (vocab + E - 1) / E; }
-  __device__ __forceinline__ uint4 load(int c) const {  // of a whole chunk; another one if c is none
+  // A whole chunk; another one if c is none.
+  __device__ __forceinline__ uint4 load(int c) const {
     return full > 0 ? *reinterpret_cast<const uint4*>(at + static_cast<int64_t>(E) * min(c, full - 1)) : make_uint4(0, 0, 0, 0);
+  }
+  __device__ __forceinline__ uint4 load_nt(int c) const {
+    return full > 0 ? load16_nt(at + static_cast<int64_t>(E) * min(c, full - 1)) : make_uint4(0, 0, 0, 0);
   }
   // Chunk c, of which load() gave w.
   __device__ __forceinline__ void values(int c, uint4 w, float (&f)[E]) const {
@@ -228,15 +234,13 @@ __device__ __forceinline__ double shfl_f64(double x, int from) {
   return __longlong_as_double(static_cast<long long>(static_cast<u64>(__shfl(static_cast<u32>(v >> 32), from)) << 32 |
                                                      __shfl(static_cast<u32>(v), from)));
 }
-// Sum of x over the lanes up to this one.
-__device__ __forceinline__ double scan_f64(double x) {
-  const int lane = threadIdx.x & 63;
-#pragma unroll
-  for (int s = 1; s < 64; s <<= 1) {
-    const double o = shfl_f64(x, max(lane - s, 0));
-    x += lane >= s ? o : 0.0;
-  }
-  return x;
+// x moved CTRL (row_shr) lanes up in each row of 16, 0 where there is none.
+template <int CTRL>
+__device__ __forceinline__ double shifted(double x) {
+  const u64 v = static_cast<u64>(__double_as_longlong(x));
+  const u32 lo = __builtin_amdgcn_update_dpp(0, static_cast<int>(v), CTRL, 0xf, 0xf, false);
+  const u32 hi = __builtin_amdgcn_update_dpp(0, static_cast<int>(v >> 32), CTRL, 0xf, 0xf, false);
+  return __longlong_as_double(static_cast<long long>(static_cast<u64>(hi) << 32 | lo));
 }
 // x of one lane, the same for all.
 __device__ __forceinline__ float lane_of(float x, int lane) {
@@ -248,6 +252,16 @@ __device__ __forceinline__ u64 lane_of(u64 x, int lane) {
 }
 __device__ __forceinline__ double lane_of(double x, int lane) {
   return __longlong_as_double(static_cast<long long>(lane_of(static_cast<u64>(__double_as_longlong(x)), lane)));
+}
+// Sum of x over the lanes up to this one.
+__device__ __forceinline__ double scan_f64(double x) {
+  x += shifted<0x111>(x);
+  x += shifted<0x112>(x);
+  x += shifted<0x114>(x);
+  x += shifted<0x118>(x);
+  const double r0 = lane_of(x, 15), r1 = r0 + lane_of(x, 31), r2 = r1 + lane_of(x, 47);
+  const int row = (threadIdx.x & 63) >> 4;
+  return x + (row == 0 ? 0.0 : row == 1 ? r0 : row == 2 ? r1 : r2);
 }
 
 // ---------------------------------------------------------------- maximum and sum of a row
@@ -300,7 +314,7 @@ __device__ __forceinline__ Part part_of(const Row<T>& row, int c0, int waves, in
   uint4 in[kBatch];
   auto load_batch = [&](int c) {
 #pragma unroll
-    for (int u = 0; u < kBatch; ++u) in[u] = row.load(c + u * step + lane);
+    for (int u = 0; u < kBatch; ++u) in[u] = row.load_nt(c + u * step + lane);
   };
   load_batch(c0);
 #pragma unroll 1
@@ -338,7 +352,7 @@ __device__ __forceinline__ u64 key_of(const Row<T>& row, int c0, int waves, int 
   uint4 in[kBatch];
   auto load_batch = [&](int c) {
 #pragma unroll
-    for (int u = 0; u < kBatch; ++u) in[u] = row.load(c + u * step + lane);
+    for (int u = 0; u < kBatch; ++u) in[u] = row.load_nt(c + u * step + lane);
   };
   load_batch(c0);
 #pragma unroll 1
@@ -534,9 +548,10 @@ __device__ __forceinline__ float4 parts_of(const VerifyParams& p, int b, int i) 
   const int lane = threadIdx.x & 63, seg = min(lane & 15, p.segments - 1);
   return p.stats[(((static_cast<int64_t>(b) * p.max_rows + i) << 1) + (p.draft ? lane >> 4 & 1 : 0)) * p.segments + seg];
 }
-// The way from row 0 by one wave, as far as row `depth` of it.  The statistics of the rows before that one are there; x are
-// row 0's parts.
-__device__ __forceinline__ Way way_to(const VerifyParams& p, int b, int n, const Draft& d, double scale, float4 x, int depth) {
+// The way from row 0 by one wave, as far as row `depth` of it.  The statistics of the rows before that one are there; x and
+// ahead are rows 0's and 1's parts, loaded together: a way that goes on mostly does so to row 1.
+__device__ __forceinline__ Way way_to(const VerifyParams& p, int b, int n, const Draft& d, double scale, float4 x,
+                                      float4 ahead, int depth) {
   Way way{0, 0, false, {0.f, 1, false, 0}, {0.f, 1, false, 0}};
   const int lane = threadIdx.x & 63;
   while (depth-- > 0) {
@@ -558,7 +573,7 @@ __device__ __forceinline__ Way way_to(const VerifyParams& p, int b, int n, const
     }
     way.kept |= 1ull << next;
     way.node = next;
-    if (depth > 0) x = parts_of(p, b, next);
+    if (depth > 0) x = next == 1 ? ahead : parts_of(p, b, next);
   }
   return way;
 }
@@ -574,31 +589,31 @@ __device__ __forceinline__ void row_segment(const VerifyParams& p, int b, int q0
   const int cbeg = min(seg * per, chunks), cend = min(cbeg + per, chunks);
   float4& out = p.stats[(((static_cast<int64_t>(b) * p.max_rows + i) << 1) + of_draft) * p.segments + seg];
   if (scale == 0) {  // uniform
-    const u64 key = key_of(row, cbeg + 64 * wave, kWaves, cend);
+    const u64 key = key_of(row, cbeg + 64 * wave, kRowWaves, cend);
     if (lane == 0) s_key[wave] = key;
     __syncthreads();
     if (wave != 0) return;
-    const u64 best = best_of<16>(s_key[lane & (kWaves - 1)]);
+    const u64 best = best_of<16>(s_key[lane & (kRowWaves - 1)]);
     if (lane == 0)
       out = make_float4(__uint_as_float(static_cast<u32>(best)), __uint_as_float(static_cast<u32>(best >> 32)), 0.f, 0.f);
     return;
   }
-  const Part part = part_of(row, cbeg + 64 * wave, kWaves, cend, scale32(scale));
+  const Part part = part_of(row, cbeg + 64 * wave, kRowWaves, cend, scale32(scale));
   if (lane == 0) s_part[wave] = part;
   __syncthreads();
   if (wave != 0) return;
-  const Part mine = s_part[lane & (kWaves - 1)];
+  const Part mine = s_part[lane & (kRowWaves - 1)];
   const float top = max_of<16>(mine.max);
-  const float sum = sum_of<16>((lane & 15) < kWaves ? rebased(mine, clamped(top), scale32(scale)) : 0.f);
+  const float sum = sum_of<16>((lane & 15) < kRowWaves ? rebased(mine, clamped(top), scale32(scale)) : 0.f);
   if (lane == 0) out = make_float4(top, sum, 0.f, 0.f);
 }
 
 // The first rows of every sequence, as many as the grid has: a segment per workgroup.  One more workgroup for each
 // sequence leaves what there is to know of its drafts, and clears the counters of the lists.
 template <typename T>
-__global__ __launch_bounds__(kThreads) void row_stats_kernel(const VerifyParams p) {
-  __shared__ Part s_part[kWaves];
-  __shared__ u64 s_key[kWaves];
+__global__ __launch_bounds__(kRowThreads) void row_stats_kernel(const VerifyParams p) {
+  __shared__ Part s_part[kRowWaves];
+  __shared__ u64 s_key[kRowWaves];
   const int b = blockIdx.z, item = blockIdx.y;
   const int i = p.draft ? item >> 1 : item;
   const bool of_draft = p.draft && (item & 1);
@@ -621,13 +636,13 @@ __global__ __launch_bounds__(kThreads) void row_stats_kernel(const VerifyParams 
 // per sequence.
 __global__ __launch_bounds__(64) void list_rows_kernel(const VerifyParams p, const int from, const int to, const int pass) {
   const int b = blockIdx.x, lane = threadIdx.x;
-  const float4 x = parts_of(p, b, 0);
+  const float4 x = parts_of(p, b, 0), ahead = parts_of(p, b, min(1, p.max_rows - 1));
   int q0;
   const int n = rows_of(p, b, q0);
   const double scale = scale_of(p.temps[b]);
   const Draft d = left_drafts(p, b, n);
   if (n <= from) return;
-  const Way way = way_to(p, b, n, d, scale, x, from);
+  const Way way = way_to(p, b, n, d, scale, x, ahead, from);
   if (way.ended) return;  // uniform
   const int steps = __popcll(d.line) - 1;
   const u64 rows = __ballot((d.line >> way.node & 1) && (d.line & 1) && steps >= from && steps < to);
@@ -644,9 +659,9 @@ __global__ __launch_bounds__(64) void list_rows_kernel(const VerifyParams p, con
 
 // The listed rows: a unit is a segment of one, and workgroups take them in turn.
 template <typename T>
-__global__ __launch_bounds__(kThreads) void listed_stats_kernel(const VerifyParams p, const int pass) {
-  __shared__ Part s_part[2][kWaves];
-  __shared__ u64 s_key[2][kWaves];
+__global__ __launch_bounds__(kRowThreads) void listed_stats_kernel(const VerifyParams p, const int pass) {
+  __shared__ Part s_part[2][kRowWaves];
+  __shared__ u64 s_key[2][kRowWaves];
   const int units = static_cast<int>(p.counts[pass]) * p.segments;
   int turn = 0;
   for (int unit = blockIdx.x; unit < units; unit += gridDim.x, turn ^= 1) {
@@ -660,12 +675,12 @@ __global__ __launch_bounds__(kThreads) void listed_stats_kernel(const VerifyPara
 
 // The whole way, by one wave.
 __device__ __forceinline__ Record last_row(const VerifyParams& p, int b, bool write) {
-  const float4 x = parts_of(p, b, 0);
+  const float4 x = parts_of(p, b, 0), ahead = parts_of(p, b, min(1, p.max_rows - 1));
   int q0;
   const int n = rows_of(p, b, q0);
   const double scale = scale_of(p.temps[b]);
   const Draft d = left_drafts(p, b, n);
-  const Way way = way_to(p, b, n, d, scale, x, n > 0 ? kMaxRows : 0);
+  const Way way = way_to(p, b, n, d, scale, x, ahead, n > 0 ? kMaxRows : 0);
   return finish(p, b, q0, n, d, way, scale, write);
 }
 __global__ __launch_bounds__(64) void last_row_kernel(const VerifyParams p) { last_row(p, blockIdx.x, true); }
@@ -938,10 +953,10 @@ __global__ __launch_bounds__(kThreads) void next_token_kernel(const VerifyParams
 
 // ---------------------------------------------------------------- sizes
 
-// Segments of a row: some 2048 workgroups for the rows of a pass, or their next power of two below.
+// Segments of a row: some 4096 workgroups for the rows of a pass, or their next power of two below.
 int segments_of(int64_t rows) {
   int segments = 1;
-  while (segments < kMaxSegments && 2 * segments * rows <= 2048) segments *= 2;
+  while (segments < kMaxSegments && 2 * segments * rows <= 4096) segments *= 2;
   return segments;
 }
 // Chunks of a range, whole 64s: a row has kMostRanges at most, and a batch no more than 4096 unless rows have 64.
@@ -957,8 +972,8 @@ struct Layout {
 };
 Layout layout_of(int64_t num_seqs, int64_t max_rows, int64_t vocab) {
   Layout l{};
-  // of every row one segment, or up to 16 in batches that have no more than 2048 of them
-  const int64_t lists = std::max(num_seqs, std::min<int64_t>(num_seqs * kMaxSegments, 2048));
+  // of every row one segment, or up to 16 in batches that have no more than 4096 of them
+  const int64_t lists = std::max(num_seqs, std::min<int64_t>(num_seqs * kMaxSegments, 4096));
   l.drafts = round16(2 * max_rows * lists * sizeof(float4));
   l.list = l.drafts + round16(2 * num_seqs * max_rows * sizeof(uint4));
   l.counts = l.list + round16(2 * num_seqs * max_rows * sizeof(u32));
@@ -974,19 +989,21 @@ template <typename T>
 int launch(const char* fn, VerifyParams p, hipStream_t s) {
   const LaunchOrder order;
   // All rows in one pass; or, in a large batch, row 0 first, then those 1 and 2 steps behind it that sequences get to,
-  // then 3 to 6, .. and in the last pass the rest.  About half of what is left is expected to be got to each time.
+  // then 3 to 6, .. and in the last pass the rest.  About half of what is left is expected to be got to each time; the
+  // first cut pays earlier where drafts were chosen, of which fewer stay (8 trees of 60 rows, 139 MB: 35 us with one,
+  // 45 without; 64 sampled chains of 5, 166 MB: 70 and 66), one more each 200 MB.
   const int per_row = p.draft ? 2 : 1;
   const int64_t rows = std::max<int64_t>(p.total * per_row, p.num_seqs);
   int64_t bytes = rows * p.vocab * static_cast<int64_t>(sizeof(T));
-  const bool one = bytes < kOnePass || p.max_rows == 1;
+  const bool one = bytes < kOnePass / (p.draft ? 1 : 2) || p.max_rows == 1;
   p.segments = segments_of(one ? rows : p.num_seqs * per_row);
-  hipLaunchKernelGGL(row_stats_kernel<T>, dim3(p.segments, (one ? p.max_rows : 1) * per_row + 1, p.num_seqs), dim3(kThreads),
+  hipLaunchKernelGGL(row_stats_kernel<T>, dim3(p.segments, (one ? p.max_rows : 1) * per_row + 1, p.num_seqs), dim3(kRowThreads),
                      0, s, p);
   for (int from = 1, to, pass = 0; !one && from < p.max_rows; from = to, ++pass) {
     bytes /= 2;
     to = bytes < kOnePass ? kMaxRows : 2 * from + 1;
     hipLaunchKernelGGL(list_rows_kernel, dim3(p.num_seqs), dim3(64), 0, s, p, from, to, pass);
-    hipLaunchKernelGGL(listed_stats_kernel<T>, dim3(2048), dim3(kThreads), 0, s, p, pass);
+    hipLaunchKernelGGL(listed_stats_kernel<T>, dim3(4096), dim3(kRowThreads), 0, s, p, pass);
   }
   const int per_wg = kWaves * p.ranges_per_wave;
   const dim3 sums((p.ranges + per_wg - 1) / per_wg, p.num_seqs);

@@ -102,7 +102,7 @@ def same(got, want):
 def many(a, want):
     """The batch again and again, in one call of 100 MB of logits and more, which takes another way through the rows."""
     rows, vocab = a["logits"].shape
-    times = -(-220_000_000 // (rows * vocab * a["logits"].element_size()))
+    times = -(-230_000_000 // (rows * vocab * a["logits"].element_size()))
     seqs = len(a["temperatures"])
     if times * seqs > 20_000:
         return
