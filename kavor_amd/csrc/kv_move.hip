@@ -16,6 +16,7 @@ namespace {
 constexpr int kThreads = 256;
 constexpr int kMaxRows = 64;  // rows of a sequence, as in kvp_tree_attention
 constexpr int kBatch = 8;     // rows in flight per thread
+constexpr int kMostGroups = 2048;  // workgroups from which one takes several layers
 
 // ---------------------------------------------------------------- drafts kept
 
@@ -39,19 +40,54 @@ struct KeepParams {
   Divisor div_block, div_units;
 };
 
+__device__ __forceinline__ int64_t of_lane(int64_t x, int lane) {
+  const uint64_t v = static_cast<uint64_t>(x);
+  return static_cast<int64_t>(static_cast<uint64_t>(static_cast<u32>(__builtin_amdgcn_readlane(static_cast<int>(v >> 32), lane))) << 32 |
+                              static_cast<u32>(__builtin_amdgcn_readlane(static_cast<int>(v), lane)));
+}
+
+// Moves a unit of each row in `which`, a row's offsets per lane, in layers first .. last - 1.
+template <typename V, typename Load, typename Store>
+__device__ __forceinline__ void move_rows(unsigned long long which, int64_t src, int64_t dst, uint8_t* base, int first, int last,
+                                          int64_t layer_stride, Load load, Store store) {
+  unsigned long long rest = which;
+  int layer = first;
+#pragma unroll 1
+  while (layer < last) {  // uniform, as all that follows but the data
+    V v[kBatch];
+    int64_t to[kBatch];
+    int count = 0;
+#pragma unroll
+    for (int j = 0; j < kBatch; ++j) {
+      if (layer >= last) continue;
+      const int row = __builtin_ctzll(rest);
+      v[j] = load(base + layer * layer_stride + of_lane(src, row));
+      to[j] = layer * layer_stride + of_lane(dst, row);
+      ++count;
+      rest &= rest - 1;
+      if (rest == 0) {
+        rest = which;
+        ++layer;
+      }
+    }
+#pragma unroll
+    for (int j = 0; j < kBatch; ++j)
+      if (j < count) store(base + to[j], v[j]);
+  }
+}
+
 // A sequence's tokens base + path[j] go to base + 1 + j.  A path rises, so path[j] > j and what is written
 // was read before: in the batch of the same thread, or an earlier one.
 __global__ __launch_bounds__(kThreads) void keep_drafts_kernel(const KeepParams p) {
-  __shared__ int64_t s_src[kMaxRows], s_dst[kMaxRows];              // byte offsets of the rows
-  __shared__ int64_t s_scale_src[kMaxRows], s_scale_dst[kMaxRows];  // and of their scales, head 0
   const int b = blockIdx.y;
   const int lane = threadIdx.x & 63;
   const int n = p.cu[b + 1] - p.cu[b], len = p.lens[b], kept = p.accepted[b];
+  const int entry = lane < p.width ? p.path[b * p.path_stride + lane] : 0;  // with the others: a round trip less
   const bool ok = n > 0 && n <= len && kept >= 0 && kept < n && kept <= p.width;
   if (blockIdx.x == 0 && blockIdx.z == 0 && threadIdx.x == 0) p.new_lens[b] = ok ? len - n + 1 + kept : len;
   if (!ok || kept == 0) return;  // uniform
   // every wave finds the moves, one per lane: up to the first entry that does not rise or has no page
-  const int row = lane < kept ? p.path[b * p.path_stride + lane] : n;
+  const int row = lane < kept ? entry : n;
   const int before = __shfl_up(row, 1);
   bool good = lane < kept && row < n && row > (lane == 0 ? 0 : before);
   const int from = len - n + row, to = len - n + 1 + lane;
@@ -62,53 +98,27 @@ __global__ __launch_bounds__(kThreads) void keep_drafts_kernel(const KeepParams 
   good = good && from_blk >= 0 && from_blk < p.num_cache_blocks && to_blk >= 0 && to_blk < p.num_cache_blocks;
   const unsigned long long bad = ~__ballot(good);
   const unsigned long long run = bad ? (1ull << __builtin_ctzll(bad)) - 1 : ~0ull;  // lanes before the first bad one
-  const bool moves = (run >> lane & 1) && from != to;  // what is in its place stays there
-  const unsigned long long which = __ballot(moves);
-  const int count = __popcll(which);
-  if (count == 0) return;  // uniform
-  if (threadIdx.x < 64 && moves) {
-    const int at = __popcll(which & ((1ull << lane) - 1));
-    const int from_off = from - from_page * p.block_size, to_off = to - to_page * p.block_size;
-    s_src[at] = from_blk * p.blk_stride + from_off * p.slot_stride;
-    s_dst[at] = to_blk * p.blk_stride + to_off * p.slot_stride;
-    s_scale_src[at] = from_blk * p.scale_blk_stride + from_off;
-    s_scale_dst[at] = to_blk * p.scale_blk_stride + to_off;
-  }
-  __syncthreads();
-  const int unit = blockIdx.x * kThreads + threadIdx.x;
-  const int per_side = p.heads * p.row_units;
+  const unsigned long long which = __ballot((run >> lane & 1) && from != to);        // what is in its place stays there
+  if (which == 0) return;  // uniform
+  const int from_off = from - from_page * p.block_size, to_off = to - to_page * p.block_size;
+  const int unit = blockIdx.x * blockDim.x + threadIdx.x, per_side = p.heads * p.row_units;
   const int first = blockIdx.z * p.layers_per_wg, last = min(first + p.layers_per_wg, p.layers);
-  if (unit < 2 * per_side) {
-    const int side = unit >= per_side, in_side = unit - side * per_side;
+  // the whole wave goes both ways: the rows' offsets are its lanes'
+  const bool of_rows = unit < 2 * per_side, of_scales = !of_rows && unit < p.units;
+  if (__any(of_rows)) {
+    const int64_t src = from_blk * p.blk_stride + from_off * p.slot_stride, dst = to_blk * p.blk_stride + to_off * p.slot_stride;
+    const int side = unit >= per_side, in_side = of_rows ? unit - side * per_side : 0;
     const int h = div_by(in_side, p.div_units), c = in_side - h * p.row_units;
-    uint8_t* base = p.cache[side] + h * p.head_stride + 16 * c;
-    for (int l = first; l < last; ++l) {
-      uint8_t* layer = base + l * p.layer_stride;
-      for (int m0 = 0; m0 < count; m0 += kBatch) {
-        uint4 v[kBatch];
-#pragma unroll
-        for (int j = 0; j < kBatch; ++j)
-          if (m0 + j < count) v[j] = load16_nt(layer + s_src[m0 + j]);
-#pragma unroll
-        for (int j = 0; j < kBatch; ++j)
-          if (m0 + j < count) store16_nt(layer + s_dst[m0 + j], v[j]);
-      }
-    }
-  } else if (unit < p.units) {  // a head's scales: one byte a token
-    const int i = unit - 2 * per_side, side = i >= p.heads, h = i - side * p.heads;
-    uint8_t* base = p.scale[side] + h * p.scale_head_stride;
-    for (int l = first; l < last; ++l) {
-      uint8_t* layer = base + l * p.scale_layer_stride;
-      for (int m0 = 0; m0 < count; m0 += kBatch) {
-        uint8_t v[kBatch];
-#pragma unroll
-        for (int j = 0; j < kBatch; ++j)
-          if (m0 + j < count) v[j] = layer[s_scale_src[m0 + j]];
-#pragma unroll
-        for (int j = 0; j < kBatch; ++j)
-          if (m0 + j < count) layer[s_scale_dst[m0 + j]] = v[j];
-      }
-    }
+    move_rows<uint4>(which, src, dst, p.cache[side] + h * p.head_stride + 16 * c, first, last, p.layer_stride,
+                     [&](const uint8_t* at) { return of_rows ? *reinterpret_cast<const uint4*>(at) : make_uint4(0, 0, 0, 0); },
+                     [&](uint8_t* at, uint4 v) { if (of_rows) store16_nt(at, v); });
+  }
+  if (__any(of_scales)) {  // a head's scales: one byte a token
+    const int64_t src = from_blk * p.scale_blk_stride + from_off, dst = to_blk * p.scale_blk_stride + to_off;
+    const int i = of_scales ? unit - 2 * per_side : 0, side = i >= p.heads, h = i - side * p.heads;
+    move_rows<uint8_t>(which, src, dst, p.scale[side] + h * p.scale_head_stride, first, last, p.scale_layer_stride,
+                       [&](const uint8_t* at) { return of_scales ? *at : uint8_t{0}; },
+                       [&](uint8_t* at, uint8_t v) { if (of_scales) *at = v; });
   }
 }
 
@@ -371,12 +381,13 @@ extern "C" int kvp_keep_drafts(void* k_cache, void* v_cache, int64_t cache_layer
   p.units = 2 * num_kv_heads * (p.row_units + (k_scale ? 1 : 0));
   p.div_block = divisor(static_cast<uint32_t>(block_size));
   p.div_units = divisor(static_cast<uint32_t>(p.row_units));
-  const int parts = (p.units + kThreads - 1) / kThreads;
+  // workgroups of as many waves as the units have, four at most
+  const int threads = std::min(kThreads, (p.units + 63) / 64 * 64), parts = (p.units + threads - 1) / threads;
   const int64_t all = static_cast<int64_t>(parts) * num_seqs * num_layers;
-  p.layers_per_wg = static_cast<int>(std::min<int64_t>(num_layers, std::max<int64_t>(1, all / 4096)));
+  p.layers_per_wg = static_cast<int>(std::min<int64_t>(num_layers, std::max<int64_t>(1, all / kMostGroups)));
   const int z = (num_layers + p.layers_per_wg - 1) / p.layers_per_wg;
   if (z > 65535) return fail(KVP_EUNSUPPORTED, "%s: too many layers", fn);
-  hipLaunchKernelGGL(keep_drafts_kernel, dim3(parts, num_seqs, z), dim3(kThreads), 0, static_cast<hipStream_t>(stream), p);
+  hipLaunchKernelGGL(keep_drafts_kernel, dim3(parts, num_seqs, z), dim3(threads), 0, static_cast<hipStream_t>(stream), p);
   return launch_status(fn);
 }
 

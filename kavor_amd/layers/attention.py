@@ -492,6 +492,12 @@ def _ints(name: str, t: torch.Tensor, like: torch.Tensor) -> None:
         _require_int32(name, t, like.device)
 
 
+def _all_ints(index: int, a: torch.Tensor, b: torch.Tensor, c: torch.Tensor) -> bool:
+    i32 = torch.int32
+    return (a.dtype is i32 and b.dtype is i32 and c.dtype is i32 and a.get_device() == index and b.get_device() == index
+            and c.get_device() == index and a.is_contiguous() and b.is_contiguous() and c.is_contiguous())
+
+
 def _table(block_table: torch.Tensor, rows: int, like: torch.Tensor):
     if not _is(block_table, torch.int32, like.get_device(), 2):
         _refuse("block_table", block_table, torch.int32, 2, like.device)
@@ -709,22 +715,25 @@ def keep_drafts(k_cache: torch.Tensor, v_cache: torch.Tensor, path: torch.Tensor
         if scales != (*shape[:-3], heads, block_size):
             raise ValueError(f"the scales must be {(*shape[:-3], heads, block_size)}, got {tuple(scales)}")
         scale = (k_scale.data_ptr(), v_scale.data_ptr(), ss[0] if dim == 5 else 0, ss[-3], ss[-2])
-    for name, t in (("cu_seqlens_q", cu_seqlens_q), ("cache_seqlens", cache_seqlens), ("accepted", accepted)):
-        _ints(name, t, k_cache)
-    _require("path", path, torch.int32, k_cache, 2)
-    batch = cu_seqlens_q.numel() - 1
-    if batch < 0 or cache_seqlens.numel() < batch or accepted.numel() < batch or path.shape[0] < batch:
+    index = k_cache.get_device()
+    if not _all_ints(index, cu_seqlens_q, cache_seqlens, accepted):
+        for name, t in (("cu_seqlens_q", cu_seqlens_q), ("cache_seqlens", cache_seqlens), ("accepted", accepted)):
+            _ints(name, t, k_cache)
+    if not _is(path, torch.int32, index, 2):
+        _refuse("path", path, torch.int32, 2, k_cache.device)
+    batch, (path_rows, path_width) = cu_seqlens_q.numel() - 1, path.shape
+    if batch < 0 or cache_seqlens.numel() < batch or accepted.numel() < batch or path_rows < batch:
         raise ValueError("cu_seqlens_q must have an entry more than sequences, and cache_seqlens, accepted and path one "
                          "for each")
-    bt, bt_stride, width = _table(block_table, batch, k_cache)
-    new_lens = cache_seqlens.new_empty((batch,))
     if layers == 0:
         raise ValueError("the caches have no layers")
-    _launch("kvp_keep_drafts", k_cache.get_device(), k_cache.data_ptr(), v_cache.data_ptr(), cs[0] if dim == 5 else 0,
+    bt, bt_stride, width = _table(block_table, batch, k_cache)
+    new_lens = cache_seqlens.new_empty((batch,))
+    _launch("kvp_keep_drafts", index, k_cache.data_ptr(), v_cache.data_ptr(), cs[0] if dim == 5 else 0,
             cs[-4], cs[-3], cs[-2], *scale, layers, num_blocks, bt, bt_stride, path.data_ptr(),
-            path.stride(0) if path.shape[0] > 1 else path.shape[1], path.shape[1], accepted.data_ptr(),
+            path.stride(0) if path_rows > 1 else path_width, path_width, accepted.data_ptr(),
             cu_seqlens_q.data_ptr(), cache_seqlens.data_ptr(), batch, heads, head_dim, block_size, width,
-            new_lens.data_ptr(), _stream(k_cache))
+            new_lens.data_ptr(), torch._C._cuda_getCurrentRawStream(index))
     return new_lens
 
 

@@ -349,9 +349,11 @@ def verify_drafts(logits: torch.Tensor, tokens: torch.Tensor, uniforms: torch.Te
     n, vocab = logits.shape
     if logits.stride(1) != 1 and vocab > 1:
         raise ValueError("logits must have a contiguous last dimension")
-    for name, t, kind, count in (("tokens", tokens, torch.int64, n), ("uniforms", uniforms, torch.float32, n)):
-        if not (t.dtype is kind and t.get_device() == index and t.is_contiguous() and t.numel() == count):
-            raise ValueError(f"{name} must be a contiguous {kind} tensor on the logits' device, one per row")
+    if not (tokens.dtype is torch.int64 and tokens.get_device() == index and tokens.is_contiguous() and tokens.numel() == n):
+        raise ValueError("tokens must be a contiguous int64 tensor on the logits' device, one per row")
+    if not (uniforms.dtype is torch.float32 and uniforms.get_device() == index and uniforms.is_contiguous()
+            and uniforms.numel() == n):
+        raise ValueError("uniforms must be a contiguous fp32 tensor on the logits' device, one per row")
     if not (cu_seqlens_q.dtype is torch.int32 and cu_seqlens_q.get_device() == index and cu_seqlens_q.is_contiguous()
             and cu_seqlens_q.numel() > 0):
         raise ValueError("cu_seqlens_q must be a contiguous int32 tensor on the logits' device with an entry more "
@@ -371,10 +373,11 @@ def verify_drafts(logits: torch.Tensor, tokens: torch.Tensor, uniforms: torch.Te
                 and (draft_logits.stride(1) == 1 or vocab <= 1)):
             raise ValueError("draft_logits must have the logits' type, shape and device and a contiguous last dimension")
         draft, draft_stride = draft_logits.data_ptr(), draft_logits.stride(0) if n > 1 else -(-vocab // 8) * 8
-    accepted = cu_seqlens_q.new_empty((batch,))
-    path = cu_seqlens_q.new_empty((batch, max(rows, 0)))
-    out = tokens.new_empty((batch, max(rows, 0)))
-    stream = _stream(logits)
+    width = rows if rows > 0 else 0
+    accepted = cu_seqlens_q.new_empty(batch)
+    path = cu_seqlens_q.new_empty(batch, width)
+    out = tokens.new_empty(batch, width)
+    stream = torch._C._cuda_getCurrentRawStream(index)
     need = verify_workspace_bytes(batch, rows, vocab)
     ws = _verify_pool.ready(index, stream, need)
     if ws is None:
