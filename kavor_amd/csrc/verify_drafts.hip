@@ -6,14 +6,19 @@
 // chosen (no q) is kept where u (1 - what its refused siblings have of p) < p(x); behind refused ones the next
 // token follows p without them.  Either way a token of the output is distributed as p.
 //
-// What a row decides about its drafts is independent of what other rows decide, so all of it is computed at
-// once, a row of a sequence per lane: a row is kept where it and all that its mask sees have won, which is
-// one test of 64-bit words.
+// In a few launches:
+//   - maximum and sum of the rows of logits, in 32 bits, a segment of a row per workgroup.  Rows behind a refused draft
+//     decide nothing: large batches take row 0 of every sequence first, then the rows that each can still get to.
+//   - the way through the drafts, by a wave per sequence with a row per lane: siblings are ballots.
+//   - the next token: the least index whose running sum of weights passes u times their sum.  A vocabulary's
+//     borders lie down to 1e-9 of the sum apart, closer than 32-bit sums tell, so the weights of the one row that
+//     a sequence ends at are added in 64 bits, range by range; the range with the border is taken again value by value.
 //
-// The next token is the least index whose running sum of weights passes u times their sum.  A vocabulary's
-// borders lie down to 1e-9 of the sum apart, closer than 32-bit sums tell, so the weights of the one row that
-// a sequence ends at are computed and added in 64 bits, in ranges; the range that holds the border is taken
-// again value by value.  All other rows need their maximum and sum in 32 bits only.
+// What bounds it: few rows, the latency of three launches and their chains of loads (a tree of 12 rows of 151936 bf16
+// values: 17 us); many, HBM for the rows, then the vector ALUs for the last ones.  256 chains of 5 with a draft
+// model's logits take 157 us: 34, 40 and 22 for the rows (450 of 760 MB, 4.7 TB/s), 38 for the last ones' sums, 7 for the
+// tokens, and 5 or 6 for each of the three kernels between them.  With all rows read they took 223 us, with a
+// workgroup per sequence that goes its way row by row 173: its longest ways were the end of the launch.
 #include <math.h>
 
 #include <algorithm>
@@ -30,10 +35,12 @@ constexpr int kThreads = 512;
 constexpr int kWaves = kThreads / 64;
 constexpr int kRowThreads = 256;  // where rows are streamed
 constexpr int kRowWaves = kRowThreads / 64;
+constexpr int kSumThreads = 256;  // where ranges are summed, each by a wave
+constexpr int kSumWaves = kSumThreads / 64;
 constexpr int kMaxRows = 64;  // rows of a sequence, as in kvp_tree_attention: one per lane
 constexpr int kMaxSegments = 16;   // of a row: one per lane of a 16-lane row where they are joined
 constexpr int kMaxRange = 512;     // chunks of a range, at most: one per thread where it is taken again
-constexpr int kMostRanges = 512;   // of a row, unless they would be longer than that
+constexpr int kMostRanges = 512, kLeastRanges = 128;  // of a row, unless they would be longer or shorter than that
 constexpr int kBatch = 2;          // chunks in flight per lane
 constexpr int64_t kOnePass = 200 << 20;  // bytes of logits that are read in one pass, whether all of them are got to or not
 constexpr int kMaxPasses = 8;
@@ -74,7 +81,7 @@ struct VerifyParams {
   int32_t* path;    // [num_seqs][max_rows]
   int64_t* out;     // [num_seqs][max_rows]
   int32_t segments; // of a row in the first pass
-  int32_t range_chunks, ranges, ranges_per_wave;
+  int32_t range_chunks, ranges;
   float4* stats;    // [sequence][row][p, q][segment]: maximum and sum, or the greedy key
   uint4* drafts;    // [2][sequence][row]: what leave_drafts() finds
   u32* list;        // rows of a pass: sequence, row, p or q
@@ -539,8 +546,8 @@ __device__ __forceinline__ Record finish(const VerifyParams& p, int b, int q0, i
 // Rows of a sequence that is none are 0.
 __device__ __forceinline__ int rows_of(const VerifyParams& p, int b, int& q0) {
   q0 = p.cu[b];
-  const int n = p.cu[b + 1] - q0;
-  return n <= 0 || n > p.max_rows || q0 < 0 || q0 + n > p.total ? 0 : n;
+  const int end = p.cu[b + 1];
+  return q0 < 0 || end <= q0 || end > p.total || end - q0 > p.max_rows ? 0 : end - q0;
 }
 
 // A row's parts: lanes 0 to 15 have p's segments, 16 to 31 q's.
@@ -714,16 +721,16 @@ __device__ __forceinline__ double only(bool on, double x) {
   return __longlong_as_double(static_cast<long long>(static_cast<u64>(hi) << 32 | static_cast<u32>(bits)));
 }
 
-// Neighbouring ranges per wave.  KNOWN: last_row_kernel left the records; otherwise every wave goes the way anew.
+// A range per wave.  KNOWN: last_row_kernel left the records; otherwise every wave goes the way anew.
 //
 // Where 64 chunks have no weight of 2^-28 of the largest or more, as most have in a row that is sure of its token, weights
 // are taken in 32 bits: off by 2^-22 of themselves and 2^-50 of the largest, which is some 1e-13 of a row's sum.
 template <typename T, bool KNOWN>
-__global__ __launch_bounds__(kThreads) void range_sums_kernel(const VerifyParams p) {
+__global__ __launch_bounds__(kSumThreads) void range_sums_kernel(const VerifyParams p) {
   constexpr int E = Chunk<T>::kSize;
-  __shared__ Refused s_refused[kWaves];
+  __shared__ Refused s_refused[kSumWaves];
   const int b = blockIdx.y, wave = threadIdx.x >> 6, lane = threadIdx.x & 63;
-  int range = (blockIdx.x * kWaves + wave) * p.ranges_per_wave;
+  const int range = blockIdx.x * kSumWaves + wave;
   if (range >= p.ranges) return;
   Record rec;
   if constexpr (KNOWN) rec = p.records[b];
@@ -734,8 +741,8 @@ __global__ __launch_bounds__(kThreads) void range_sums_kernel(const VerifyParams
   const double top_p = rec.top_p, top_q = rec.top_q, scale = rec.scale;
   const float top_p32 = static_cast<float>(top_p), top_q32 = static_cast<float>(top_q), scale_f = scale32(scale);
   const float lambda32 = static_cast<float>(rec.lambda);
-  const int last = min(range + p.ranges_per_wave, p.ranges);
-  int c = range * p.range_chunks + lane;
+  const int cbeg = range * p.range_chunks, cend = min(cbeg + p.range_chunks, row.chunks());
+  int c = cbeg + lane;
   uint4 in = row.load(c), in_q = row_q.load(c);
   auto small = [&](const float (&f)[E], float top) {  // of the wave's chunks
     float most = max3(f[0], f[1], f[2]);
@@ -743,86 +750,83 @@ __global__ __launch_bounds__(kThreads) void range_sums_kernel(const VerifyParams
     for (int e = 3; e < E; e += 2) most = max3(most, f[e], f[min(e + 1, E - 1)]);
     return !__any((most - top) * scale_f > -28.f);
   };
-  for (; range < last; ++range) {
-    const int cbeg = range * p.range_chunks, cend = min(cbeg + p.range_chunks, row.chunks());
-    Sums s{0, 0, 0, 0};
-    if (rec.mode == kRest) {
-      for (int c0 = cbeg; c0 < cend; c0 += 64, c += 64) {  // uniform
-        float f[E], g[E];
+  Sums s{0, 0, 0, 0};
+  if (rec.mode == kRest) {
+    for (int c0 = cbeg; c0 < cend; c0 += 64, c += 64) {  // uniform
+      float f[E], g[E];
 #pragma unroll
-        for (int e = 0; e < E; ++e) f[e] = g[e] = -INFINITY;
-        if (c < cend) {
-          row.values(c, in, f);
-          row_q.values(c, in_q, g);
-        }
-        in = row.load(c + 64);
-        in_q = row_q.load(c + 64);
-        if (small(f, top_p32) && small(g, top_q32)) {  // uniform
-          float sp = 0.f, sq = 0.f, sp_over = 0.f, sq_over = 0.f;
-#pragma unroll
-          for (int e = 0; e < E; ++e) {
-            const float x = fast_exp2((f[e] - top_p32) * scale_f), y = fast_exp2((g[e] - top_q32) * scale_f);
-            const bool over = x > lambda32 * y;
-            sp += x;
-            sq += y;
-            sp_over += over ? x : 0.f;
-            sq_over += over ? y : 0.f;
-          }
-          s.p += sp;
-          s.q += sq;
-          s.p_over += sp_over;
-          s.q_over += sq_over;
-          continue;
-        }
+      for (int e = 0; e < E; ++e) f[e] = g[e] = -INFINITY;
+      if (c < cend) {
+        row.values(c, in, f);
+        row_q.values(c, in_q, g);
+      }
+      in = row.load(c + 64);
+      in_q = row_q.load(c + 64);
+      if (small(f, top_p32) && small(g, top_q32)) {  // uniform
+        float sp = 0.f, sq = 0.f, sp_over = 0.f, sq_over = 0.f;
 #pragma unroll
         for (int e = 0; e < E; ++e) {
-          const double x = weight_floor(f[e], top_p, scale), y = weight_floor(g[e], top_q, scale);
-          const bool over = x > rec.lambda * y;
-          s.p += x;
-          s.q += y;
-          s.p_over += only(over, x);
-          s.q_over += only(over, y);
+          const float x = fast_exp2((f[e] - top_p32) * scale_f), y = fast_exp2((g[e] - top_q32) * scale_f);
+          const bool over = x > lambda32 * y;
+          sp += x;
+          sq += y;
+          sp_over += over ? x : 0.f;
+          sq_over += over ? y : 0.f;
         }
+        s.p += sp;
+        s.q += sq;
+        s.p_over += sp_over;
+        s.q_over += sq_over;
+        continue;
       }
-      s.q = sum_of(s.q);
-      s.q_over = sum_of(s.q_over);
-    } else {
-      Refused& refused = s_refused[wave];
-      bool some = false;
-      if (rec.mode == kWithout) {
-        find_refused(p, rec, b, E * cbeg, E * cend, refused);
-        wait_lds();
-        some = refused.count != 0;
+#pragma unroll
+      for (int e = 0; e < E; ++e) {
+        const double x = weight_floor(f[e], top_p, scale), y = weight_floor(g[e], top_q, scale);
+        const bool over = x > rec.lambda * y;
+        s.p += x;
+        s.q += y;
+        s.p_over += only(over, x);
+        s.q_over += only(over, y);
       }
-      for (int c0 = cbeg; c0 < cend; c0 += 64, c += 64) {  // uniform
-        float f[E];
-#pragma unroll
-        for (int e = 0; e < E; ++e) f[e] = -INFINITY;
-        if (c < cend) row.values(c, in, f);
-        in = row.load(c + 64);
-        if (some) {
-#pragma unroll
-          for (int e = 0; e < E; ++e) {
-            const double x = weight_floor(f[e], top_p, scale);
-            s.p += x;
-            s.p_over += is_refused(refused, E * c + e) ? 0.0 : x;
-          }
-        } else if (small(f, top_p32)) {  // uniform
-          float sp = 0.f;
-#pragma unroll
-          for (int e = 0; e < E; ++e) sp += fast_exp2((f[e] - top_p32) * scale_f);
-          s.p += sp;
-        } else {
-#pragma unroll
-          for (int e = 0; e < E; ++e) s.p += weight_floor(f[e], top_p, scale);
-        }
-      }
-      if (!some) s.p_over = s.p;
     }
-    s.p = sum_of(s.p);
-    s.p_over = sum_of(s.p_over);
-    if (lane == 0) p.sums[static_cast<int64_t>(b) * p.ranges + range] = s;
+    s.q = sum_of(s.q);
+    s.q_over = sum_of(s.q_over);
+  } else {
+    Refused& refused = s_refused[wave];
+    bool some = false;
+    if (rec.mode == kWithout) {
+      find_refused(p, rec, b, E * cbeg, E * cend, refused);
+      wait_lds();
+      some = refused.count != 0;
+    }
+    for (int c0 = cbeg; c0 < cend; c0 += 64, c += 64) {  // uniform
+      float f[E];
+#pragma unroll
+      for (int e = 0; e < E; ++e) f[e] = -INFINITY;
+      if (c < cend) row.values(c, in, f);
+      in = row.load(c + 64);
+      if (some) {
+#pragma unroll
+        for (int e = 0; e < E; ++e) {
+          const double x = weight_floor(f[e], top_p, scale);
+          s.p += x;
+          s.p_over += is_refused(refused, E * c + e) ? 0.0 : x;
+        }
+      } else if (small(f, top_p32)) {  // uniform
+        float sp = 0.f;
+#pragma unroll
+        for (int e = 0; e < E; ++e) sp += fast_exp2((f[e] - top_p32) * scale_f);
+        s.p += sp;
+      } else {
+#pragma unroll
+        for (int e = 0; e < E; ++e) s.p += weight_floor(f[e], top_p, scale);
+      }
+    }
+    if (!some) s.p_over = s.p;
   }
+  s.p = sum_of(s.p);
+  s.p_over = sum_of(s.p_over);
+  if (lane == 0) p.sums[static_cast<int64_t>(b) * p.ranges + range] = s;
 }
 
 // ---------------------------------------------------------------- the next token
@@ -959,9 +963,10 @@ int segments_of(int64_t rows) {
   while (segments < kMaxSegments && 2 * segments * rows <= 4096) segments *= 2;
   return segments;
 }
-// Chunks of a range, whole 64s: a row has kMostRanges at most, and a batch no more than 4096 unless rows have 64.
+// Chunks of a range, whole 64s: a batch has no more than 4096 ranges, which fill the GPU once, unless rows would have fewer
+// than kLeastRanges, and a row no more than kMostRanges.
 int range_chunks_of(int64_t num_seqs, int64_t chunks) {
-  const int64_t per_row = std::max<int64_t>(64, std::min<int64_t>(kMostRanges, 4096 / std::max<int64_t>(num_seqs, 1)));
+  const int64_t per_row = std::max<int64_t>(kLeastRanges, std::min<int64_t>(kMostRanges, 4096 / std::max<int64_t>(num_seqs, 1)));
   const int64_t per = (chunks + per_row - 1) / per_row;
   return static_cast<int>(std::min<int64_t>(kMaxRange, (per + 63) / 64 * 64));
 }
@@ -979,9 +984,11 @@ Layout layout_of(int64_t num_seqs, int64_t max_rows, int64_t vocab) {
   l.counts = l.list + round16(2 * num_seqs * max_rows * sizeof(u32));
   l.records = l.counts + round16(kMaxPasses * sizeof(u32));
   l.sums = l.records + round16(num_seqs * sizeof(Record));
+  // ranges of all rows, by the type with the most chunks; as range_chunks_of() has them, and growing with both arguments
   const int64_t chunks = (vocab + 3) / 4;
-  const int64_t ranges = std::max<int64_t>(std::min<int64_t>(kMostRanges, (chunks + 63) / 64), (chunks + kMaxRange - 1) / kMaxRange);
-  l.bytes = l.sums + num_seqs * ranges * sizeof(Sums);
+  const int64_t wanted = std::max(std::min<int64_t>(num_seqs * kMostRanges, 4096), num_seqs * kLeastRanges);
+  const int64_t ranges = std::max(std::min(wanted, num_seqs * ((chunks + 63) / 64)), num_seqs * ((chunks + kMaxRange - 1) / kMaxRange));
+  l.bytes = l.sums + ranges * sizeof(Sums);
   return l;
 }
 
@@ -993,7 +1000,7 @@ int launch(const char* fn, VerifyParams p, hipStream_t s) {
   // first cut pays earlier where drafts were chosen, of which fewer stay (8 trees of 60 rows, 139 MB: 35 us with one,
   // 45 without; 64 sampled chains of 5, 166 MB: 70 and 66), one more each 200 MB.
   const int per_row = p.draft ? 2 : 1;
-  const int64_t rows = std::max<int64_t>(p.total * per_row, p.num_seqs);
+  const int64_t rows = std::max<int64_t>(static_cast<int64_t>(p.total) * per_row, p.num_seqs);
   int64_t bytes = rows * p.vocab * static_cast<int64_t>(sizeof(T));
   const bool one = bytes < kOnePass / (p.draft ? 1 : 2) || p.max_rows == 1;
   p.segments = segments_of(one ? rows : p.num_seqs * per_row);
@@ -1005,13 +1012,12 @@ int launch(const char* fn, VerifyParams p, hipStream_t s) {
     hipLaunchKernelGGL(list_rows_kernel, dim3(p.num_seqs), dim3(64), 0, s, p, from, to, pass);
     hipLaunchKernelGGL(listed_stats_kernel<T>, dim3(4096), dim3(kRowThreads), 0, s, p, pass);
   }
-  const int per_wg = kWaves * p.ranges_per_wave;
-  const dim3 sums((p.ranges + per_wg - 1) / per_wg, p.num_seqs);
+  const dim3 sums((p.ranges + kSumWaves - 1) / kSumWaves, p.num_seqs);
   if (p.num_seqs >= kKnown) {
     hipLaunchKernelGGL(last_row_kernel, dim3(p.num_seqs), dim3(64), 0, s, p);
-    hipLaunchKernelGGL((range_sums_kernel<T, true>), sums, dim3(kThreads), 0, s, p);
+    hipLaunchKernelGGL((range_sums_kernel<T, true>), sums, dim3(kSumThreads), 0, s, p);
   } else {
-    hipLaunchKernelGGL((range_sums_kernel<T, false>), sums, dim3(kThreads), 0, s, p);
+    hipLaunchKernelGGL((range_sums_kernel<T, false>), sums, dim3(kSumThreads), 0, s, p);
   }
   hipLaunchKernelGGL(next_token_kernel<T>, dim3(p.num_seqs), dim3(kThreads), 0, s, p);
   return launch_status(fn);
@@ -1085,7 +1091,6 @@ extern "C" int kvp_verify_drafts(const void* logits, int32_t logits_fp32, int64_
   const int chunks = (vocab + per16 - 1) / per16;
   p.range_chunks = range_chunks_of(num_seqs, chunks);
   p.ranges = (chunks + p.range_chunks - 1) / p.range_chunks;
-  p.ranges_per_wave = 1;
   p.stats = reinterpret_cast<float4*>(ws + at.stats);
   p.drafts = reinterpret_cast<uint4*>(ws + at.drafts);
   p.list = reinterpret_cast<u32*>(ws + at.list);

@@ -399,3 +399,54 @@ def test_refusals_of_wrong_tensors(cuda_device):
     for rows in (0, 65, -1):
         with pytest.raises(_lib.KVPathError, match="max_seqlen_q"):
             fused.verify_drafts(**{**good, "max_seqlen_q": rows})
+
+
+@pytest.mark.gpu
+def test_offsets_that_wrap_are_no_rows(cuda_device):
+    """Ends past 2^31 that would make a short sequence of two far apart numbers."""
+    x = Batch([3, 2, 4], 100, torch.bfloat16, "chosen", seed=2)
+    x.cu = torch.tensor([2 ** 31 - 3, -2 ** 31 + 1, 2 ** 31 - 1, -2 ** 31], dtype=torch.int32)
+    got = fused.verify_drafts(**x.on_gpu())
+    assert (got[0] == 0).all() and (got[1] == -1).all() and (got[2] == -1).all()
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype,vocab", [(torch.bfloat16, 2_500_000), (torch.float32, 1_200_003)])
+@pytest.mark.parametrize("form", ["sampled", "chosen"])
+def test_vocabularies_of_more_ranges_than_threads(cuda_device, dtype, vocab, form):
+    check(Batch([3, 1], vocab, dtype, form, seed=9, greedy=0.0, width=3.0))
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("form", ["sampled", "chosen", "tree"])
+def test_results_do_not_depend_on_another_threads_calls(cuda_device, form):
+    """Two threads on one stream, whose calls share the workspace: one reads its rows in one pass, one in several."""
+    import threading
+
+    small, large = Batch([5, 9, 2], 4000, torch.bfloat16, form, seed=1), Batch([64] * 24, 1500, torch.float32, form, seed=2)
+    calls = [b.on_gpu() for b in (small, large)]
+    for k in ("logits", "draft_logits", "tokens", "uniforms", "tree_mask"):
+        if calls[1][k] is not None:
+            t = calls[1][k].repeat(14, *[1] * (calls[1][k].dim() - 1))
+            calls[1][k] = torch.nn.functional.pad(t, (0, 4))[:, :t.shape[1]] if t.dim() == 2 else t
+    calls[1]["cu_seqlens_q"] = torch.arange(0, 64 * 24 * 14 + 1, 64, dtype=torch.int32, device="cuda")
+    calls[1]["temperatures"] = calls[1]["temperatures"].repeat(14)
+    want = [[t.clone() for t in fused.verify_drafts(**a)] for a in calls]
+    got, errors, start = [[], []], [], threading.Barrier(2)
+
+    def work(i):
+        try:
+            start.wait()
+            for _ in range(60):
+                got[i].append(fused.verify_drafts(**calls[i]))
+        except Exception as e:  # reported by the test itself
+            errors.append(e)
+    threads = [threading.Thread(target=work, args=(i,)) for i in range(2)]
+    for t in threads:
+        t.start()
+    for t in threads:
+        t.join()
+    torch.cuda.synchronize()
+    assert not errors, errors
+    for i in range(2):
+        assert all(torch.equal(a, b) for r in got[i] for a, b in zip(r, want[i]))
