@@ -526,9 +526,9 @@ int kvp_token_logprobs(const void* logits, int32_t logits_fp32, int64_t row_stri
  * Where nothing is left to follow, it follows p.  Greedy otherwise (T <= 0 or NaN): a draft stays if it
  * is kvp_argmax_bf16's index of logits[r], and the next token is that index.
  *   The next token is the least index whose running sum of weights exceeds row 0's uniform number times
- * their sum.  Weights are relative to the row's largest; sums are in 64 bits, and so are weights, but for
- * some below 2^-28, which may be off by 2^-22 of themselves, and those below 2^-985, which are 0.  What decides
- * about drafts comes from sums in 32 bits.
+ * their sum.  Sums are in 64 bits, and so are weights, but for some below 2^-28 of the row's largest, which
+ * may be off by 2^-46 of that, and those below 2^-985 of it, which are 0.  What decides about drafts comes
+ * from sums in 32 bits.
  * accepted[b]: the number of drafts that stay; path[b, 0 .. accepted): their rows in the sequence,
  * rising; out_tokens[b, 0 .. accepted): their tokens, and the next token behind them; the rest of
  * both [num_seqs, max_seqlen_q] is -1.

@@ -724,7 +724,9 @@ __device__ __forceinline__ double only(bool on, double x) {
 // A range per wave.  KNOWN: last_row_kernel left the records; otherwise every wave goes the way anew.
 //
 // Where 64 chunks have no weight of 2^-28 of the largest or more, as most have in a row that is sure of its token, weights
-// are taken in 32 bits: off by 2^-22 of themselves and 2^-50 of the largest, which is some 1e-13 of a row's sum.
+// are taken in 32 bits: of 2^t the exponent is off by 2^-24 of itself, twice, and the exponential by 2^-23, so a weight by
+// less than (1.4 |t| + 2) 2^-24 of itself, which for t <= -28 is 2^-46 of the largest and less.  The signs differ: a row of
+// 151936 is off by some 1e-12 of its sum, 2e-9 at worst.  256 chains with a draft model's logits: 38 us, 63 without.
 template <typename T, bool KNOWN>
 __global__ __launch_bounds__(kSumThreads) void range_sums_kernel(const VerifyParams p) {
   constexpr int E = Chunk<T>::kSize;

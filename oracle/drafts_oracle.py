@@ -36,14 +36,14 @@ def draw(weights: torch.Tensor, u: float) -> int:
 
 
 def verify_drafts(logits, tokens, uniforms, temperatures, cu_seqlens_q, max_seqlen_q, tree_mask=None, draft_logits=None):
-    """(accepted, path, out_tokens), and the least distance of a decision from its border: of u times what it is held
-    against, relative, and of the drawn number from the neighbouring borders, of the sum."""
+    """(accepted, path, out_tokens), and how near they come to be others: the least distance of the two sides of a
+    decision, of the larger one, and that of a drawn number from a border, of the sum."""
     T, vocab = logits.shape
     B = len(cu_seqlens_q) - 1
     accepted = torch.zeros(B, dtype=torch.int32)
     path = torch.full((B, max_seqlen_q), -1, dtype=torch.int32)
     out = torch.full((B, max_seqlen_q), -1, dtype=torch.int64)
-    margin = math.inf
+    decided = drawn = math.inf
     for b in range(B):
         q0, n = int(cu_seqlens_q[b]), int(cu_seqlens_q[b + 1] - cu_seqlens_q[b])
         if not (0 < n <= max_seqlen_q and q0 >= 0 and q0 + n <= T):
@@ -69,11 +69,11 @@ def verify_drafts(logits, tokens, uniforms, temperatures, cu_seqlens_q, max_seql
                     q = softmax(draft_logits[q0 + node], temp)
                     a, c = (u * float(q[x]), float(p[x])) if inside and q is not None else (1.0, 0.0)
                     ok = a < c
-                    margin = min(margin, abs(a - c) / max(a, c, 1e-300))
+                    decided = min(decided, abs(a - c) / max(a, c, 1e-300))
                 else:
                     a, c = (u * float(left.sum()), float(left[x])) if inside else (1.0, 0.0)
                     ok = a < c
-                    margin = min(margin, abs(a - c) / max(a, c, 1e-300))
+                    decided = min(decided, abs(a - c) / max(a, c, 1e-300))
                 if ok:
                     found = i
                     break
@@ -94,11 +94,11 @@ def verify_drafts(logits, tokens, uniforms, temperatures, cu_seqlens_q, max_seql
             u = float(uniforms[q0])
             last = draw(left, u)
             sums = torch.cumsum(left, 0) / left.sum()
-            margin = min(margin, float((sums - u).abs().min())) if u > 0 else margin
+            drawn = min(drawn, float((sums - u).abs().min())) if u > 0 else drawn
         accepted[b] = len(rows)
         path[b, :len(rows)] = torch.tensor(rows, dtype=torch.int32)
         out[b, :len(rows) + 1] = torch.tensor(toks + [last])
-    return accepted, path, out, margin
+    return accepted, path, out, decided, drawn
 
 
 def keep_drafts(caches, path, accepted, cu_seqlens_q, cache_seqlens, block_table):

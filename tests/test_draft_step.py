@@ -16,7 +16,7 @@ from oracle import drafts_oracle, operators_oracle
 from tests.helpers import bits_equal, gen, randn_bf16
 from tests.test_kept_drafts import oracle_caches, pool_of, views
 from tests.test_tree_attention import close
-from tests.test_verify_drafts import same, trees
+from tests.test_verify_drafts import reach, same, trees
 
 L, H, HKV, D, BLOCK, PAGES, VOCAB = 3, 8, 2, 128, 64, 14, 1013
 SCALE = D ** -0.5
@@ -112,10 +112,11 @@ class Loop:
     def check(self, results):
         logits, got, before, lens, outs = results
         h, i = self.host, {n: t.cpu() for n, t in self.inputs.items()}
-        *want, margin = drafts_oracle.verify_drafts(
+        *want, decided, drawn = drafts_oracle.verify_drafts(
             logits.cpu(), i["tokens"], i["uniforms"], h["temps"], h["cu"], max(ROWS), h.get("mask"),
             i["draft"][:, :VOCAB] if self.chain else None)
-        assert margin > 1e-5
+        apart, off = reach(VOCAB)
+        assert decided > apart and drawn > off
         same(got, want)
         moved = before.cpu()
         new = drafts_oracle.keep_drafts(oracle_caches(*views(moved, BLOCK, HKV, D, self.quantised)), want[1], want[0], h["cu"],

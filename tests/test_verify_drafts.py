@@ -1,11 +1,12 @@
 """Verification of drafted tokens against the 64-bit oracle: equal counts, paths and tokens.
 
-Sums that decide about drafts are in 32 bits.  The exponent of 2^t is rounded to 2^-24 of itself, three times, the exponential is
-off by 2^-23, and a thread adds at most vocab / 512 + 8 values one after the other before a tree of twelve additions: a
-row's sum is off by at most (vocab / 512 + 24 + 3 |t|) 2^-24 of itself, with |t| <= 40 wherever 2^t matters, so a
-decision is the oracle's where its two sides are further apart than twice that.  Next tokens come from 64-bit
-sums, off by less than 1e-12 of the whole.  Inputs nearer than that to a border are no test (the oracle says how near
-they are, and the seeds are such that none are).
+Sums that decide about drafts are in 32 bits.  Of 2^t the exponent is rounded to 2^-24 of itself, three times, the
+exponential is off by 2^-23, and a thread adds at most vocab / 256 + 16 values one after the other before a tree of twelve
+additions: a row's sum is off by at most (vocab / 256 + 32 + 3 |t|) 2^-24 of itself, with |t| <= 40 wherever 2^t
+matters, so a decision is the oracle's where its two sides are further apart than twice that.  Next tokens come from 64-bit
+sums of weights that are off by 2^-46 of the largest one at most: the oracle's where the number lies more than vocab times
+that, and 1e-12 for the sums, from a border.  Inputs nearer to a border would be no test: the oracle says how near
+they come, and the seeds are such that none does.
 """
 
 import math
@@ -23,7 +24,8 @@ BELOW_ONE = 1 - 2.0 ** -24
 
 
 def reach(vocab):
-    return 2 * (vocab / 512 + 24 + 120) * 2.0 ** -24
+    """How far the two sides of a decision have to be apart, and the drawn number from a border."""
+    return 2 * (vocab / 256 + 32 + 120) * 2.0 ** -24, vocab * 2.0 ** -46 + 1e-12
 
 
 def trees(lens, rng):
@@ -88,9 +90,10 @@ class Batch:
         return a
 
     def want(self):
-        *want, margin = oracle.verify_drafts(**self.args())
-        assert margin > 1e-11
-        return want, margin
+        *want, decided, drawn = oracle.verify_drafts(**self.args())
+        apart, off = reach(self.logits.shape[1])
+        assert decided > apart and drawn > off, (decided, apart, drawn, off)
+        return want
 
 
 def same(got, want):
@@ -119,7 +122,7 @@ def many(a, want):
 
 
 def check(batch):
-    want, _ = batch.want()
+    want = batch.want()
     a = batch.on_gpu()
     same(fused.verify_drafts(**a), want)
     many(a, want)
@@ -208,7 +211,7 @@ def test_temperatures_and_numbers_at_their_ends(cuda_device, form):
     x.logits[18, 40] = x.logits[18].max()  # at a temperature near 0: the first of two equal ones, or both
     x.uniforms[24:36] = 0.0
     x.uniforms[36:48] = BELOW_ONE
-    *want, _ = oracle.verify_drafts(**x.args())
+    want = oracle.verify_drafts(**x.args())[:3]
     same(fused.verify_drafts(**x.on_gpu()), want)
     many(x.on_gpu(), want)
 
@@ -250,7 +253,10 @@ def test_siblings_and_what_is_left_of_them(cuda_device):
     x.temps[4] = 0.0
     x.mask[24:27] = torch.tensor([1, 3, 7])
     x.tokens[25], x.tokens[26] = x.logits[24].argmax(), x.logits[25].argmax()
-    want = check(x)
+    # the decisions with numbers just below 1 are 2^-24 from their borders, and exact: five weights of 1 among others of 1e-13
+    want = oracle.verify_drafts(**x.args())[:3]
+    same(fused.verify_drafts(**x.on_gpu()), want)
+    many(x.on_gpu(), want)
     assert want[1][3, 0] == 2 and want[0][4] == 2
 
 
@@ -267,7 +273,7 @@ def test_sequences_that_are_no_batch(cuda_device):
     """More rows than announced, rows outside the tensor, falling offsets: nothing kept, no token; the others as ever."""
     x = Batch([3, 5, 2, 4], 200, torch.bfloat16, "chosen", seed=6)
     x.max_q = 4
-    want, _ = x.want()
+    want = x.want()
     assert want[0][1] == 0 and (want[2][1] == -1).all()
     same(fused.verify_drafts(**x.on_gpu()), want)
     for ends in ([0, 3, 3, 20, 14], [-2, 3, 8, 10, 14], [0, 8, 3, 10, 14]):
@@ -287,7 +293,7 @@ def test_sequences_that_are_no_batch(cuda_device):
 def test_rows_far_apart(cuda_device, form):
     """Rows more than 2^32 bytes from the first one."""
     x = Batch([3], 400, torch.bfloat16, form, seed=4, greedy=0.0)
-    want, _ = x.want()
+    want = x.want()
     a = x.on_gpu()
     stride = (5 << 28) + 64
     for name in ("logits", "draft_logits"):
@@ -301,7 +307,7 @@ def test_rows_far_apart(cuda_device, form):
 def test_other_streams_and_captured_graphs(cuda_device):
     first, second = (Batch([5, 0, 9, 2], 3001, torch.bfloat16, "sampled", seed=s) for s in (1, 2))
     second.cu = first.cu
-    wants = [b.want()[0] for b in (first, second)]
+    wants = [b.want() for b in (first, second)]
     side = torch.cuda.Stream()
     a = first.on_gpu()
     torch.cuda.synchronize()
@@ -333,7 +339,7 @@ def test_two_graphs_in_turn(cuda_device):
         a, graph = b.on_gpu(), torch.cuda.CUDAGraph()
         with torch.cuda.graph(graph):
             got = fused.verify_drafts(**a)
-        made.append((graph, a, got, b.want()[0]))
+        made.append((graph, a, got, b.want()))
     for _ in range(3):
         for graph, _, got, want in made:
             for t in got:
