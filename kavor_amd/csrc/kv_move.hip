@@ -4,6 +4,10 @@
 // Both are bound by HBM (each byte read and written once) or by the latency of a launch and two or three
 // dependent loads.  Neither needs a temporary: a thread owns 16 bytes of every row (page) it moves and takes
 // them in an order in which nothing is overwritten before it is read, so no thread waits for another.
+// The drafts of 64 trees of 5 to 25 rows that stay, in 28 layers (41 MB): 17 us, 4.9 TB/s read and written; with nontemporal
+// loads 24, as they were written and attended to just before.  A page of 1 MiB in 28 layers: 11.4 us, 5.1 TB/s; 96
+// pages of 256 KiB from 32: 168 us, 5.6 TB/s; 300 of 129 KiB, half of which are also read: 407 us, 5.5 TB/s (cached
+// loads: 429).
 #include <algorithm>
 #include <new>
 #include <vector>

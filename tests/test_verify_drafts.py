@@ -456,3 +456,26 @@ def test_results_do_not_depend_on_another_threads_calls(cuda_device, form):
     assert not errors, errors
     for i in range(2):
         assert all(torch.equal(a, b) for r in got[i] for a, b in zip(r, want[i]))
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+@pytest.mark.parametrize("form", ["sampled", "chosen"])
+def test_numbers_that_fall_among_small_weights(cuda_device, dtype, form):
+    """Rows that are sure of one token, and numbers behind it, among weights of some 2^-28.3 that are taken in 32 bits: they
+    are 3e-9 wide, 200 times as much as the sum of 1000 of them may be off."""
+    n, vocab, g = 20, 1000, gen(6)
+    x = Batch([2] * n, vocab, dtype, "chosen", seed=7, greedy=0.0)
+    x.logits[:] = (-19.5 - 0.3 * torch.rand(2 * n, vocab, generator=g)).to(dtype)
+    x.logits[:, 123] = 0.0
+    x.temps[:] = 1.0
+    if form == "sampled":  # what is left of p behind a refused draft lies at the one token and among the others
+        x.draft = (-19.5 - 0.3 * torch.rand(2 * n, vocab, generator=g)).to(dtype)
+        x.draft[:, 123], x.draft[:, 900] = 0.0, 9.0
+        x.tokens[1::2] = 900
+    else:
+        x.tokens[1::2] = 124
+    x.uniforms.view(n, 2)[:, 1] = BELOW_ONE
+    x.uniforms.view(n, 2)[:, 0] = 1 - (1 + torch.arange(n)) * 2.0 ** -24
+    want = check(x)
+    assert (want[0] == 0).all() and len(set(want[2][:, 0].tolist())) > n / 2
