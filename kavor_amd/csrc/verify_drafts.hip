@@ -57,6 +57,8 @@ enum Mode : int32_t { kDone = 0, kAll = 1, kRest = 2, kWithout = 3, kUndefined =
 struct Record {   // of a sequence
   int32_t row;    // of logits
   int32_t mode;
+  int32_t count;  // drafts that stay
+  float u;        // row 0's number
   double scale;   // log2(e) / T
   double top_p, top_q;  // the rows' maxima
   double lambda;  // sum of exp(p's logits) over that of q's, from 32-bit sums
@@ -516,7 +518,7 @@ __device__ __forceinline__ Record finish(const VerifyParams& p, int b, int q0, i
   const u64 kept = way.kept;
   const int i = threadIdx.x & 63, count = __popcll(kept), node = way.node;
   const u64 gone = children_of(d, node);
-  Record rec{q0 + node, kDone, scale, sp.top, sq.top, sp.sum / sq.sum, gone};
+  Record rec{q0 + node, kDone, count, lane_of(d.u, 0), scale, sp.top, sq.top, sp.sum / sq.sum, gone};
   if (n > 0 && scale != 0) {
     if (!sp.ok) rec.mode = kUndefined;
     else if (p.draft) rec.mode = gone && sq.ok ? kRest : kAll;
@@ -842,9 +844,17 @@ __global__ __launch_bounds__(kThreads) void next_token_kernel(const VerifyParams
   __shared__ u64 s_key[kWaves];
   __shared__ Refused s_refused;
   const int b = blockIdx.x, tid = threadIdx.x, wave = tid >> 6, lane = tid & 63;
+  // the first wave's sums together with the record: a round trip less
+  constexpr int kHeld = 2;  // all 128 that a row has in a batch of 32 sequences and more
+  const Sums* sums = p.sums + static_cast<int64_t>(b) * p.ranges;
+  Sums held[kHeld];
+  if (wave == 0) {
+#pragma unroll
+    for (int k = 0; k < kHeld; ++k) held[k] = sums[min(lane + 64 * k, p.ranges - 1)];
+  }
   const Record rec = p.records[b];
   if (rec.mode == kDone) return;
-  int64_t* out = p.out + static_cast<int64_t>(b) * p.max_rows + p.accepted[b];
+  int64_t* out = p.out + static_cast<int64_t>(b) * p.max_rows + rec.count;
   const Row<T> row(static_cast<const T*>(p.logits) + rec.row * p.row_stride, p.vocab);
   if (rec.mode == kUndefined) {  // the greedy token
     const u64 key = key_of(row, 64 * wave, kWaves, row.chunks());
@@ -854,17 +864,15 @@ __global__ __launch_bounds__(kThreads) void next_token_kernel(const VerifyParams
     if (tid == 0) *out = token_of(best);
     return;
   }
-  const double u = p.uniforms[p.cu[b]];
   if (wave == 0) {
-    const Sums* sums = p.sums + static_cast<int64_t>(b) * p.ranges;
     Sums all{0, 0, 0, 0};
-    for (int r = lane; r < p.ranges; r += 64) {
-      const Sums s = sums[r];
-      all.p += s.p;
-      all.q += s.q;
-      all.p_over += s.p_over;
-      all.q_over += s.q_over;
-    }
+    auto add = [&](const Sums& x) {
+      all = {all.p + x.p, all.q + x.q, all.p_over + x.p_over, all.q_over + x.q_over};
+    };
+#pragma unroll
+    for (int k = 0; k < kHeld; ++k)
+      if (lane + 64 * k < p.ranges) add(held[k]);
+    for (int r = lane + 64 * kHeld; r < p.ranges; r += 64) add(sums[r]);
     all = {sum_of(all.p), sum_of(all.q), sum_of(all.p_over), sum_of(all.q_over)};
     const double lambda = rec.mode == kRest ? all.p / all.q : 0.0;
     int mode = rec.mode;
@@ -873,17 +881,15 @@ __global__ __launch_bounds__(kThreads) void next_token_kernel(const VerifyParams
       mode = kAll;
       whole = all.p;
     }
-    auto of_range = [&](int r) {
-      if (r >= p.ranges) return 0.0;
-      const Sums s = sums[r];
-      const double x = mode == kAll ? s.p : s.p_over - lambda * s.q_over;
-      return x > kNothing ? x : 0.0;
+    auto of_range = [&](const Sums& x) {
+      const double w = mode == kAll ? x.p : x.p_over - lambda * x.q_over;
+      return w > kNothing ? w : 0.0;
     };
-    const double border = u * whole;
+    const double border = rec.u * whole;
     double before = 0, left = border;
     int found = -1, last = 0;
-    for (int r0 = 0; r0 < p.ranges && found < 0; r0 += 64) {
-      const double mine = of_range(r0 + lane);
+    auto take = [&](int r0, const Sums& x) {
+      const double mine = r0 + lane < p.ranges ? of_range(x) : 0.0;
       const double upto = before + scan_f64(mine);
       const u64 past = __ballot(mine > 0 && upto > border), some = __ballot(mine > 0);
       if (past) {
@@ -894,7 +900,11 @@ __global__ __launch_bounds__(kThreads) void next_token_kernel(const VerifyParams
         last = r0 + 63 - __builtin_clzll(some);
       }
       before = lane_of(upto, 63);
-    }
+    };
+#pragma unroll
+    for (int k = 0; k < kHeld; ++k)
+      if (found < 0 && 64 * k < p.ranges) take(64 * k, held[k]);  // uniform
+    for (int r0 = 64 * kHeld; r0 < p.ranges && found < 0; r0 += 64) take(r0, sums[min(r0 + lane, p.ranges - 1)]);
     if (lane == 0) {
       s_lambda = lambda;
       s_mode = mode;
