@@ -885,9 +885,8 @@ __global__ __launch_bounds__(kThreads) void next_token_kernel(const VerifyParams
       const double w = mode == kAll ? x.p : x.p_over - lambda * x.q_over;
       return w > kNothing ? w : 0.0;
     };
-    const double border = rec.u * whole;
-    double before = 0, left = border;
-    int found = -1, last = 0;
+    double border, before, left;
+    int found, last;
     auto take = [&](int r0, const Sums& x) {
       const double mine = r0 + lane < p.ranges ? of_range(x) : 0.0;
       const double upto = before + scan_f64(mine);
@@ -901,14 +900,22 @@ __global__ __launch_bounds__(kThreads) void next_token_kernel(const VerifyParams
       }
       before = lane_of(upto, 63);
     };
+    for (;;) {  // uniform
+      border = rec.u * whole;
+      before = 0;
+      found = last = -1;
 #pragma unroll
-    for (int k = 0; k < kHeld; ++k)
-      if (found < 0 && 64 * k < p.ranges) take(64 * k, held[k]);  // uniform
-    for (int r0 = 64 * kHeld; r0 < p.ranges && found < 0; r0 += 64) take(r0, sums[min(r0 + lane, p.ranges - 1)]);
+      for (int k = 0; k < kHeld; ++k)
+        if (found < 0 && 64 * k < p.ranges) take(64 * k, held[k]);
+      for (int r0 = 64 * kHeld; r0 < p.ranges && found < 0; r0 += 64) take(r0, sums[min(r0 + lane, p.ranges - 1)]);
+      if (found >= 0 || last >= 0 || mode == kAll) break;
+      mode = kAll;  // the ranges have too little each
+      whole = all.p;
+    }
     if (lane == 0) {
       s_lambda = lambda;
       s_mode = mode;
-      s_range = found < 0 ? last : found;
+      s_range = found < 0 ? max(last, 0) : found;
       s_left = found < 0 ? INFINITY : left;
     }
   }
@@ -923,6 +930,7 @@ __global__ __launch_bounds__(kThreads) void next_token_kernel(const VerifyParams
   // the range again, a chunk per thread
   double w[E], mine = 0;
   const int c = cbeg + tid;
+  u32 end = 0;  // behind the last value with a weight in p
 #pragma unroll
   for (int e = 0; e < E; ++e) w[e] = 0;
   if (c < cend) {
@@ -933,6 +941,7 @@ __global__ __launch_bounds__(kThreads) void next_token_kernel(const VerifyParams
     for (int e = 0; e < E; ++e) {
       w[e] = weight(f[e], rec.top_p, scale);
       if (mode == kWithout && is_refused(s_refused, E * c + e)) w[e] = 0;
+      if (w[e] > 0) end = E * c + e + 1;
     }
     if (mode == kRest) {
       const Row<T> row_q(static_cast<const T*>(p.draft) + rec.row * p.draft_stride, p.vocab);
@@ -949,22 +958,23 @@ __global__ __launch_bounds__(kThreads) void next_token_kernel(const VerifyParams
   __syncthreads();
   double before = 0;
   for (int k = 0; k < wave; ++k) before += s_wave[k];
-  // the first value whose running sum is past the border, or the last that has a weight: as keys
+  // the first value whose running sum is past the border, or the last that has a weight, or, where the range's sum
+  // was a rounding of nothing, the last that has one in p: as keys
   double run = before + upto - mine;
-  u64 key = tid == 0 ? E * cbeg + 1 : 0;
+  u64 key = end;
 #pragma unroll
   for (int e = 0; e < E; ++e) {
     if (!(w[e] > 0)) continue;
     run += w[e];
     const u32 v = E * c + e;
-    const u64 k = run > left ? 1ull << 32 | (0xffffffffu - v) : v + 1;
+    const u64 k = run > left ? 2ull << 32 | (0xffffffffu - v) : 1ull << 32 | (v + 1);
     key = k > key ? k : key;
   }
   key = best_of(key);
   if (lane == 0) s_key[wave] = key;
   __syncthreads();
   const u64 best = best_of<16>(s_key[lane & (kWaves - 1)]);
-  if (tid == 0) *out = best >> 32 ? token_of(best) : static_cast<int64_t>(best) - 1;
+  if (tid == 0) *out = best >> 33 ? token_of(best) : static_cast<int64_t>(static_cast<u32>(best)) - 1;
 }
 
 // ---------------------------------------------------------------- sizes

@@ -234,6 +234,36 @@ def test_a_draft_model_that_is_the_target_keeps_everything(cuda_device, dtype):
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+@pytest.mark.parametrize("vocab", [37, 4099, 70_001])
+def test_what_is_left_between_equal_distributions_is_never_a_hidden_token(cuda_device, dtype, vocab):
+    """Drafts that neither model can give, from a draft model that is the target but for a shift, exact or rounded: what is
+    left of p - q is nothing, or roundings.  Whatever the number, the next token is one that the target can give."""
+    seqs, g = 130, gen(vocab)
+    logits = torch.randn(2 * seqs, vocab, generator=g)
+    logits[::4] *= 12  # rows with all but a few weights small
+    logits[:, ::2] = -math.inf
+    logits = logits.to(dtype)
+    shift = torch.where(torch.arange(2 * seqs) % 8 < 4, 0.0, 3.7)[:, None]
+    a = dict(logits=logits, draft_logits=(logits.float() + shift).to(dtype),
+             tokens=2 * torch.randint((vocab + 1) // 2, (2 * seqs,), generator=g),
+             uniforms=torch.linspace(0, 1, 2 * seqs).clamp(max=BELOW_ONE), temperatures=torch.ones(seqs),
+             cu_seqlens_q=2 * torch.arange(seqs + 1, dtype=torch.int32))
+    room = {}
+    for name, t in a.items():
+        room[name] = t.cuda()
+        if t.dim() == 2:
+            wide = torch.full((2 * seqs, -(-vocab // 8) * 8), math.nan, dtype=dtype, device="cuda")
+            wide[:, :vocab] = room[name]
+            room[name] = wide[:, :vocab]
+    for few in (seqs, 3):  # both ways to the sums
+        n = dict(room, cu_seqlens_q=room["cu_seqlens_q"][:few + 1])
+        accepted, path, out = fused.verify_drafts(**n, max_seqlen_q=2)
+        assert int(accepted.abs().sum()) == 0 and bool((path == -1).all()) and bool((out[:, 1] == -1).all())
+        assert bool((out[:, 0] % 2 == 1).all()), out[:, 0].tolist()
+
+
+@pytest.mark.gpu
 def test_siblings_and_what_is_left_of_them(cuda_device):
     """Siblings with one token, siblings that have nearly all of p, a row that sees no row, masks with bits above."""
     x = Batch([6, 6, 6, 6, 3], 64, torch.float32, "tree", seed=8, greedy=0.0)
