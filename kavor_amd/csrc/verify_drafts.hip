@@ -16,7 +16,7 @@
 //
 // What bounds it: few rows, the latency of three launches and their chains of loads (a tree of 12 rows of 151936 bf16
 // values: 17 us); many, HBM for the rows, then the vector ALUs for the last ones.  256 chains of 5 with a draft
-// model's logits take 157 us: 34, 40 and 22 for the rows (450 of 760 MB, 4.7 TB/s), 38 for the last ones' sums, 7 for the
+// model's logits take 155 us: 34, 40 and 22 for the rows (500 of 760 MB, 5.2 TB/s), 38 for the last ones' sums, 6 for the
 // tokens, and 5 or 6 for each of the three kernels between them.  With all rows read they took 223 us, with a
 // workgroup per sequence that goes its way row by row 173: its longest ways were the end of the launch.
 #include <math.h>
