@@ -30,6 +30,18 @@ struct LaunchOrder {
 inline bool aligned16(const void* ptr) { return (reinterpret_cast<uintptr_t>(ptr) & 15u) == 0; }
 inline bool mult8(int64_t stride) { return (stride & 7) == 0; }
 
+// Whether [a, a + bytes) has a byte of one of `rows` rows of `width` bytes, `stride` >= width bytes apart, the first at b.
+inline bool overlap(const void* a, int64_t bytes, const void* b, int64_t rows, int64_t stride, int64_t width) {
+  if (bytes <= 0 || rows <= 0 || width <= 0) return false;
+  const int64_t from = static_cast<int64_t>(reinterpret_cast<uintptr_t>(a) - reinterpret_cast<uintptr_t>(b));
+  if (from < 0) return from + bytes > 0;
+  const int64_t row = from / stride;
+  return row < rows && (from - row * stride < width || (row + 1 < rows && (row + 1) * stride < from + bytes));
+}
+inline bool overlap(const void* a, int64_t a_bytes, const void* b, int64_t b_bytes) {
+  return overlap(a, a_bytes, b, 1, b_bytes, b_bytes);
+}
+
 // ---------------------------------------------------------------- device side
 
 // bf16 halves of a packed 32-bit word, widened exactly to fp32.

@@ -355,6 +355,13 @@ extern "C" int kvp_keep_drafts(void* k_cache, void* v_cache, int64_t cache_layer
   if (off4(block_tables) || off4(path) || off4(accepted) || off4(cu_seqlens_q) || off4(cache_seqlens) ||
       off4(new_seqlens))
     return fail(KVP_EINVAL, "%s: misaligned integers", fn);
+  // a sequence's new length is written by one of its workgroups while the others read these
+  const int64_t seqs = num_seqs, bytes = 4 * seqs;
+  if (overlap(new_seqlens, bytes, cache_seqlens, bytes) || overlap(new_seqlens, bytes, accepted, bytes) ||
+      overlap(new_seqlens, bytes, cu_seqlens_q, bytes + 4) ||
+      overlap(new_seqlens, bytes, path, seqs, 4 * path_stride, 4 * path_width) ||
+      overlap(new_seqlens, bytes, block_tables, seqs, 4 * block_table_stride, 4 * static_cast<int64_t>(max_blocks_per_seq)))
+    return fail(KVP_EINVAL, "%s: new_seqlens overlaps an input", fn);
   KeepParams p{};
   p.cache[0] = static_cast<uint8_t*>(k_cache);
   p.cache[1] = static_cast<uint8_t*>(v_cache);

@@ -259,3 +259,41 @@ def test_refusals_of_wrong_tensors(cuda_device):
             attention.keep_drafts(**{**good, name: value})
     with pytest.raises(_lib.KVPathError, match="overlap"):
         attention.keep_drafts(**{**good, "k_cache": k[:1].expand(2, -1, -1, -1, -1), "v_cache": v[:1].expand(2, -1, -1, -1, -1)})
+
+
+def test_new_lengths_in_an_inputs_place_are_refused():
+    """Workgroups of one sequence read its length and its path while another of them writes the new length."""
+    lib = _lib.lib()
+    at = dict(bt=1 << 12, path=2 << 12, accepted=3 << 12, cu=4 << 12, lens=5 << 12, new=6 << 12)
+    sizes = dict(bt=4 * (2 * 7 + 4), path=4 * (2 * 9 + 8), accepted=12, cu=16, lens=12, new=12)  # three sequences
+
+    def call(**over):
+        p = dict(at, **over)
+        return lib.kvp_keep_drafts(16, 16, 1 << 20, 16384, 128, 64, None, None, 0, 0, 0, 2, 8, p["bt"], 7, p["path"], 9, 8,
+                                   p["accepted"], p["cu"], p["lens"], 3, 2, 64, 64, 4, p["new"], None)
+
+    for name in ("bt", "path", "accepted", "cu", "lens"):
+        for new in (at[name], at[name] + sizes[name] - 4, at[name] - sizes["new"] + 4):
+            assert call(new=new) == _lib.KVP_EINVAL, (name, new)
+            assert b"new_seqlens" in lib.kvp_last_error()
+
+
+@pytest.mark.gpu
+def test_new_lengths_between_an_inputs_rows(cuda_device):
+    """What lies between rows of the tables is no part of them."""
+    g, rng = gen(8), random.Random(8)
+    step = Step([90, 70], [6, 9], 64, 8, g, rng, kept=3)
+    pool = pool_of(2, 8, 64, 2, 128, False, g)
+    want, got = pool.clone(), pool.cuda()
+    lens = oracle.keep_drafts(oracle_caches(*views(want, 64, 2, 128, False)), *step.args())
+    path, accepted, cu, old, bt = step.args("cuda")
+    room = torch.full((2, 8), -1, dtype=torch.int32, device="cuda")
+    room[:, :bt.shape[1]] = bt
+    k, v, _, _ = views(got, 64, 2, 128, False)
+    s = k.stride()
+    rc = _lib.lib().kvp_keep_drafts(
+        k.data_ptr(), v.data_ptr(), s[0], s[1], s[2], s[3], None, None, 0, 0, 0, 2, 8, room.data_ptr(), 8, path.data_ptr(),
+        path.stride(0), path.shape[1], accepted.data_ptr(), cu.data_ptr(), old.data_ptr(), 2, 2, 128, 64, bt.shape[1],
+        room.data_ptr() + 4 * 5, torch.cuda.current_stream().cuda_stream)
+    assert rc == _lib.KVP_OK
+    assert torch.equal(room[0, 5:7].cpu(), lens) and torch.equal(got.cpu(), want)
