@@ -559,7 +559,8 @@ int kvp_verify_drafts(const void* logits, int32_t logits_fp32, int64_t row_strid
  * or whose block id (its own or its destination's) is outside [0, num_cache_blocks) or behind the table.
  * A sequence with n_b <= 0, n_b > cache_seqlens[b] or accepted[b] outside [0, min(n_b - 1, path_width)]
  * is left alone, with new_seqlens[b] = cache_seqlens[b].  Pages that hold rows of a sequence belong
- * to it alone.  A call whose new_seqlens shares memory with the integers that it reads is refused.
+ * to it alone.  A call whose new_seqlens shares memory with the integers that it reads is refused, and so
+ * is one whose K and V (or their scales) are the same memory.
  *   Caches are kvp_append_bf16's or, with k_scale and v_scale, quantised ones, in num_layers layers that
  * lie cache_layer_stride (scale_layer_stride) apart; any block_size.  path_width <= 64.
  */

@@ -362,6 +362,9 @@ extern "C" int kvp_keep_drafts(void* k_cache, void* v_cache, int64_t cache_layer
       overlap(new_seqlens, bytes, path, seqs, 4 * path_stride, 4 * path_width) ||
       overlap(new_seqlens, bytes, block_tables, seqs, 4 * block_table_stride, 4 * static_cast<int64_t>(max_blocks_per_seq)))
     return fail(KVP_EINVAL, "%s: new_seqlens overlaps an input", fn);
+  // a row is moved by threads of its own for K and for V
+  if (k_cache == v_cache || (k_scale && k_scale == v_scale))
+    return fail(KVP_EINVAL, "%s: k_cache and v_cache, k_scale and v_scale must not be the same memory", fn);
   KeepParams p{};
   p.cache[0] = static_cast<uint8_t*>(k_cache);
   p.cache[1] = static_cast<uint8_t*>(v_cache);

@@ -297,3 +297,15 @@ def test_new_lengths_between_an_inputs_rows(cuda_device):
         room.data_ptr() + 4 * 5, torch.cuda.current_stream().cuda_stream)
     assert rc == _lib.KVP_OK
     assert torch.equal(room[0, 5:7].cpu(), lens) and torch.equal(got.cpu(), want)
+
+
+def test_keys_and_values_in_one_place_are_refused():
+    """Two threads would move each row, one of them perhaps after the other has written over it."""
+    lib = _lib.lib()
+
+    def call(k, v, ks=None, vs=None):
+        return lib.kvp_keep_drafts(k, v, 1 << 20, 16384, 128, 64, ks, vs, 1 << 20, 128, 64, 2, 8, 1 << 12, 4, 2 << 12, 8, 8,
+                                   3 << 12, 4 << 12, 5 << 12, 3, 2, 64, 64, 4, 6 << 12, None)
+
+    assert call(1 << 24, 1 << 24) == _lib.KVP_EINVAL and b"k_cache" in lib.kvp_last_error()
+    assert call(1 << 24, 1 << 25, 1 << 26, 1 << 26) == _lib.KVP_EINVAL and b"k_scale" in lib.kvp_last_error()
