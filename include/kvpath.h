@@ -531,7 +531,8 @@ int kvp_token_logprobs(const void* logits, int32_t logits_fp32, int64_t row_stri
  * from sums in 32 bits.
  * accepted[b]: the number of drafts that stay; path[b, 0 .. accepted): their rows in the sequence,
  * rising; out_tokens[b, 0 .. accepted): their tokens, and the next token behind them; the rest of
- * both [num_seqs, max_seqlen_q] is -1.
+ * both [num_seqs, max_seqlen_q] is -1.  Results that share memory with logits, draft_logits, tokens,
+ * temperatures, cu_seqlens_q or each other are refused.
  *   A row of logits with a NaN or +inf, or of -inf alone, keeps no draft at T > 0, and its next token is
  * the greedy one; such a row of draft_logits keeps none either, and the next token follows p.  A draft
  * outside [0, vocab) is refused.  Rows of draft_logits without a draft behind them are not read.  A

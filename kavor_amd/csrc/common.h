@@ -35,8 +35,9 @@ inline bool overlap(const void* a, int64_t bytes, const void* b, int64_t rows, i
   if (bytes <= 0 || rows <= 0 || width <= 0) return false;
   const int64_t from = static_cast<int64_t>(reinterpret_cast<uintptr_t>(a) - reinterpret_cast<uintptr_t>(b));
   if (from < 0) return from + bytes > 0;
+  if (from >= (rows - 1) * stride + width) return false;
   const int64_t row = from / stride;
-  return row < rows && (from - row * stride < width || (row + 1 < rows && (row + 1) * stride < from + bytes));
+  return from - row * stride < width || (row + 1 < rows && (row + 1) * stride < from + bytes);
 }
 inline bool overlap(const void* a, int64_t a_bytes, const void* b, int64_t b_bytes) {
   return overlap(a, a_bytes, b, 1, b_bytes, b_bytes);

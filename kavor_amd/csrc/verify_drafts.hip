@@ -1091,6 +1091,18 @@ extern "C" int kvp_verify_drafts(const void* logits, int32_t logits_fp32, int64_
   if (!workspace || workspace_bytes < need)
     return fail(KVP_EWORKSPACE, "%s: workspace of %zu bytes, %zu needed", fn, workspace_bytes, need);
   if (!aligned16(workspace)) return fail(KVP_EINVAL, "%s: workspace must be 16-byte aligned", fn);
+  // the kernels that write a sequence's results still read these, or run beside others that do
+  const int64_t seqs = num_seqs, value = logits_fp32 ? 4 : 2;
+  const struct { const void* at; int64_t bytes; } results[] = {
+      {accepted, 4 * seqs}, {path, 4 * seqs * max_seqlen_q}, {out_tokens, 8 * seqs * max_seqlen_q}};
+  for (const auto& r : results) {
+    bool shared = overlap(r.at, r.bytes, tokens, 8 * static_cast<int64_t>(total_q)) ||
+                  overlap(r.at, r.bytes, temperatures, 4 * seqs) || overlap(r.at, r.bytes, cu_seqlens_q, 4 * (seqs + 1)) ||
+                  (total_q > 0 && overlap(r.at, r.bytes, logits, total_q, value * row_stride, value * vocab)) ||
+                  (draft_logits && overlap(r.at, r.bytes, draft_logits, total_q, value * draft_row_stride, value * vocab));
+    for (const auto& x : results) shared = shared || (&x != &r && overlap(r.at, r.bytes, x.at, x.bytes));
+    if (shared) return fail(KVP_EINVAL, "%s: the results must not share memory with the inputs or each other", fn);
+  }
   const Layout at = layout_of(num_seqs, max_seqlen_q, vocab);
   char* ws = static_cast<char*>(workspace);
   VerifyParams p{};

@@ -509,3 +509,24 @@ def test_numbers_that_fall_among_small_weights(cuda_device, dtype, form):
     x.uniforms.view(n, 2)[:, 0] = 1 - (1 + torch.arange(n)) * 2.0 ** -24
     want = check(x)
     assert (want[0] == 0).all() and len(set(want[2][:, 0].tolist())) > n / 2
+
+
+def test_results_in_an_inputs_place_are_refused():
+    """Some kernels write a sequence's results while others still read these."""
+    lib = _lib.lib()
+    at = dict(logits=1 << 24, draft=2 << 24, tokens=1 << 12, temps=2 << 12, cu=3 << 12, accepted=4 << 12, path=5 << 12, out=6 << 12)
+    sizes = dict(logits=2 * (9 * 1008 + 1000), draft=2 * (9 * 1008 + 1000), tokens=8 * 10, temps=8, cu=12, accepted=8,
+                 path=4 * 16, out=8 * 16)
+
+    def call(**over):  # 10 rows of 1000 values at a stride of 1008, two sequences of at most 8 rows
+        p = dict(at, **over)
+        return lib.kvp_verify_drafts(p["logits"], 0, 1008, 10, 1000, p["draft"], 1008, p["tokens"], 1 << 20, p["temps"], p["cu"],
+                                     2, 8, None, p["accepted"], p["path"], p["out"], 1 << 30, 1 << 30, None)
+
+    for result in ("accepted", "path", "out"):
+        for other in at:
+            if other == result:
+                continue
+            for place in (at[other], at[other] + (sizes[other] - 1) // 8 * 8, at[other] - sizes[result] + 8):
+                assert call(**{result: place}) == _lib.KVP_EINVAL, (result, other, place)
+                assert b"share" in lib.kvp_last_error(), (result, other, lib.kvp_last_error())
