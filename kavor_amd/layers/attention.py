@@ -739,6 +739,20 @@ def keep_drafts(k_cache: torch.Tensor, v_cache: torch.Tensor, path: torch.Tensor
 
 # ----------------------------------------------------------------------------- pages
 
+def _page_ids(src: list[int], dst: list[int]) -> array:
+    """Both lists one behind the other, as the library reads them."""
+    try:
+        ids = array("i", src) + array("i", dst)
+        count = len(src)
+        # bytes fill an array as they are, so that it holds fewer ids than they have
+        whole = len(dst) == count and len(ids) == 2 * count and not isinstance(src, (bytes, bytearray))
+    except (TypeError, OverflowError) as e:
+        raise ValueError(f"src and dst must be lists of page ids: {e}") from None
+    if not whole:
+        raise ValueError("src and dst must be lists of page ids of one length")
+    return ids
+
+
 def copy_pages(pages: torch.Tensor, src: list[int], dst: list[int]) -> None:
     """Copies page src[i] to page dst[i] in every layer, as if all pages were read before any is written.
 
@@ -751,13 +765,8 @@ def copy_pages(pages: torch.Tensor, src: list[int], dst: list[int]) -> None:
     if pages.dim() != 3 or (pages.stride(2) != 1 and pages.shape[2] > 1):
         raise ValueError(f"pages must be [layers, num_pages, page] with contiguous pages, got shape {tuple(pages.shape)} "
                          f"with strides {tuple(pages.stride())}")
+    ids = _page_ids(src, dst)
     count = len(src)
-    if len(dst) != count:
-        raise ValueError("src and dst differ in length")
-    try:
-        ids = array("i", src) + array("i", dst)
-    except (TypeError, OverflowError) as e:
-        raise ValueError(f"src and dst must be lists of page ids: {e}") from None
     layers, num_pages, size = pages.shape
     item = pages.element_size()
     at = ids.buffer_info()[0]

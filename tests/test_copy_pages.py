@@ -179,3 +179,14 @@ def test_refusals_of_wrong_arguments(cuda_device):
     for pages, src, dst in ((pool, [0], [4]), (pool, [0, 1], [2, 2]), (pool[:, :, :40], [0], [1]), (pool[:1].expand(3, -1, -1), [0], [1])):
         with pytest.raises(_lib.KVPathError):
             attention.copy_pages(pages, src, dst)
+
+
+def test_page_ids_that_are_no_list():
+    """Bytes are not page ids: four of them were taken as one id, and their count as four."""
+    assert list(attention._page_ids([3, 1], (4, 5))) == [3, 1, 4, 5]
+    for ids in (b"\0\0\0\0", bytearray(4), "0", None, [0.5], [1 << 40], ["0"], 7):
+        for src, dst in ((ids, [1]), ([1], ids), (ids, ids)):
+            with pytest.raises(ValueError):
+                attention._page_ids(src, dst)
+    with pytest.raises(ValueError, match="length"):
+        attention._page_ids([0, 1], [1])
