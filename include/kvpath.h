@@ -535,7 +535,8 @@ int kvp_token_logprobs(const void* logits, int32_t logits_fp32, int64_t row_stri
  * temperatures, cu_seqlens_q or each other are refused.
  *   A row of logits with a NaN or +inf, or of -inf alone, keeps no draft at T > 0, and its next token is
  * the greedy one; such a row of draft_logits keeps none either, and the next token follows p.  A draft
- * outside [0, vocab) is refused.  Rows of draft_logits without a draft behind them are not read.  A
+ * outside [0, vocab), a filler of rows of one length, is refused and takes nothing from p: it was not
+ * sampled from q, so the next token follows p with draft_logits too.  Rows of draft_logits without a draft behind them are not read.  A
  * sequence without rows, with more than max_seqlen_q, or with rows outside [0, total_q) has
  * accepted 0 and -1 alone.
  *   logits and draft_logits in bf16 (logits_fp32 0) or fp32 (1), 16-byte aligned, row strides

@@ -2,8 +2,8 @@
 // follows the last one kept (kvp_verify_drafts).
 //
 // With p = softmax(z / T) of a row of logits and q the draft's distribution, a draft x that was sampled from
-// q is kept where u q(x) < p(x); behind a refused one the next token follows max(p - q, 0).  A draft that was
-// chosen (no q) is kept where u (1 - what its refused siblings have of p) < p(x); behind refused ones the next
+// q is kept where u q(x) < p(x); behind a refused one the next token follows max(p - q, 0), behind a filler that is no
+// token p.  A draft that was chosen (no q) is kept where u (1 - what its refused siblings have of p) < p(x); behind refused ones the next
 // token follows p without them.  Either way a token of the output is distributed as p.
 //
 // In a few launches:
@@ -517,11 +517,11 @@ __device__ __forceinline__ Record finish(const VerifyParams& p, int b, int q0, i
   const RowStats &sp = way.sp, &sq = way.sq;
   const u64 kept = way.kept;
   const int i = threadIdx.x & 63, count = __popcll(kept), node = way.node;
-  const u64 gone = children_of(d, node);
+  const u64 gone = children_of(d, node), sampled = gone & __ballot(d.inside(p.vocab));  // what is no token was not sampled
   Record rec{q0 + node, kDone, count, lane_of(d.u, 0), scale, sp.top, sq.top, sp.sum / sq.sum, gone};
   if (n > 0 && scale != 0) {
     if (!sp.ok) rec.mode = kUndefined;
-    else if (p.draft) rec.mode = gone && sq.ok ? kRest : kAll;
+    else if (p.draft) rec.mode = sampled && sq.ok ? kRest : kAll;
     else rec.mode = gone ? kWithout : kAll;
   }
   if (write) {

@@ -339,7 +339,8 @@ def verify_drafts(logits: torch.Tensor, tokens: torch.Tensor, uniforms: torch.Te
       - otherwise where u (1 - p of its siblings refused before) < p(x), and behind refused ones the
         next token follows p without them.
     The next token is the least index whose running sum of weights, in 64 bits, exceeds row 0's number
-    times their sum.  Returns (accepted int32 [B], path int32 [B, max_seqlen_q]: the rows that stay,
+    times their sum.  A draft outside [0, vocab) (rows padded to one length) is refused and takes nothing from p.
+    Returns (accepted int32 [B], path int32 [B, max_seqlen_q]: the rows that stay,
     out_tokens int64 [B, max_seqlen_q]: their tokens and the next one), -1 behind these.  A row of logits with a NaN or
     +inf, or of -inf alone, keeps no draft and gives the greedy token (NaN counts as largest)."""
     index, dtype = logits.get_device(), logits.dtype

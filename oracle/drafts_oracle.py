@@ -87,7 +87,7 @@ def verify_drafts(logits, tokens, uniforms, temperatures, cu_seqlens_q, max_seql
         if p is None:
             last = greedy(row)
         else:
-            if draft_logits is not None and children and q is not None:
+            if draft_logits is not None and q is not None and 0 <= int(tokens[q0 + children[0]]) < vocab:
                 left = (p - q).clamp(min=0)
             if not left.sum() > 0:
                 left = p

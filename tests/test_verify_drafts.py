@@ -530,3 +530,39 @@ def test_results_in_an_inputs_place_are_refused():
             for place in (at[other], at[other] + (sizes[other] - 1) // 8 * 8, at[other] - sizes[result] + 8):
                 assert call(**{result: place}) == _lib.KVP_EINVAL, (result, other, place)
                 assert b"share" in lib.kvp_last_error(), (result, other, lib.kvp_last_error())
+
+
+def test_the_oracle_draws_from_the_target_where_no_draft_was_sampled():
+    """p = (.5, .3, .2), q = (.7, .2, .1): behind a row's filler the next token follows p, behind a refused draft
+    max(p - q, 0), which has nothing of the first token."""
+    p, q = torch.tensor([0.5, 0.3, 0.2]), torch.tensor([0.7, 0.2, 0.1])
+    args = dict(logits=p.log().repeat(2, 1), temperatures=torch.ones(1), cu_seqlens_q=torch.tensor([0, 2]), max_seqlen_q=2,
+                draft_logits=q.log().repeat(2, 1))
+    for u, filler, refused in ((0.0, 0, 1), (0.49, 0, 1), (0.51, 1, 2), (0.79, 1, 2), (0.81, 2, 2)):
+        for token, want in ((-1, filler), (3, filler), (1 << 40, filler), (0, refused)):
+            got = oracle.verify_drafts(tokens=torch.tensor([0, token]), uniforms=torch.tensor([u, 0.99]), **args)
+            assert got[0] == 0 and got[2].tolist() == [[want, -1]], (u, token)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("seqs", [40_000, 40])
+def test_rows_padded_with_tokens_that_are_none_follow_the_target(cuda_device, seqs):
+    """A draft model that stopped early: the next token is distributed as the target's, by the chi-squared statistic over 11
+    degrees of freedom (48 is passed once in 1e6), or as the oracle has it."""
+    n, vocab, g = seqs, 12, gen(11)
+    z, y = torch.randn(vocab, generator=g) * 1.5, torch.randn(vocab, generator=g) * 1.5
+    x = Batch([3], vocab, torch.bfloat16, "sampled", seed=1)
+    x.logits, x.draft = z.bfloat16().repeat(3 * n, 1), y.bfloat16().repeat(3 * n, 1)
+    x.temps, x.uniforms = torch.full((n,), 0.8), torch.rand(3 * n, generator=g)
+    x.cu, x.max_q = torch.arange(0, 3 * n + 1, 3, dtype=torch.int32), 3
+    x.tokens = torch.zeros(n, 3, dtype=torch.int64)
+    x.tokens[:, 1] = torch.where(torch.arange(n) % 2 == 0, -1, vocab)
+    x.tokens = x.tokens.view(-1)
+    got = fused.verify_drafts(**x.on_gpu())
+    assert int(got[0].abs().sum()) == 0
+    if n < 100:
+        same(got, x.want())
+        return
+    p = torch.softmax(z.bfloat16().double() / 0.8, 0)
+    seen = torch.bincount(got[2][:, 0].cpu(), minlength=vocab).double()
+    assert float(((seen - n * p) ** 2 / (n * p)).sum()) < 48
