@@ -528,7 +528,7 @@ int kvp_token_logprobs(const void* logits, int32_t logits_fp32, int64_t row_stri
  *   The next token is the least index whose running sum of weights exceeds row 0's uniform number times
  * their sum.  Sums are in 64 bits, and so are weights, but for some below 2^-28 of the row's largest, which
  * may be off by 2^-46 of that, and those below 2^-985 of it, which are 0.  What decides about drafts comes
- * from sums in 32 bits.
+ * from sums in 32 bits; a chosen draft that has all of p but 2^-25 stays whatever its number.
  * accepted[b]: the number of drafts that stay; path[b, 0 .. accepted): their rows in the sequence,
  * rising; out_tokens[b, 0 .. accepted): their tokens, and the next token behind them; the rest of
  * both [num_seqs, max_seqlen_q] is -1.  Results that share memory with logits, draft_logits, tokens,

@@ -345,9 +345,10 @@ __device__ __forceinline__ Part part_of(const Row<T>& row, int c0, int waves, in
       take(std::integral_constant<int, E>{}, f);
     }
   }
-  const float top = max_of(m);
-  const float to_top = far ? (ref - clamped(top)) * scale : -fmaf(clamped(top), scale, -shift);
-  return {top, sum_of(s) * fast_exp2(to_top)};
+  // divided by the weight that the largest value was added with: a sum that is this weight alone gives 1.  Times its
+  // reciprocal's exponential it gave up to 2^-23 more, and a draft that has all of p could be refused.
+  const float top = max_of(m), at = clamped(top);
+  return {top, sum_of(s) / fast_exp2(far ? (at - ref) * scale : fmaf(at, scale, -shift))};
 }
 
 // The greedy key of the same chunks.

@@ -566,3 +566,42 @@ def test_rows_padded_with_tokens_that_are_none_follow_the_target(cuda_device, se
     p = torch.softmax(z.bfloat16().double() / 0.8, 0)
     seen = torch.bincount(got[2][:, 0].cpu(), minlength=vocab).double()
     assert float(((seen - n * p) ** 2 / (n * p)).sum()) < 48
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+@pytest.mark.parametrize("form", ["sampled", "chosen", "tree"])
+@pytest.mark.parametrize("rest,cold", [(0.0, 1.0), (2.0 ** -27, 1.0), (0.0, 1e-2), (0.0, 5e-4)])
+def test_rows_that_are_sure_of_their_token(cuda_device, dtype, form, rest, cold):
+    """p of a token is 1 but for 2^-26, or much less, and its number the last one below 1: it stays.
+
+    Sums of weights relative to the largest: an addition to 1 and more is rounded by no more than what is added, be it
+    that it is lost or rounded up, so the sum lies between 1 and 1 + 2^-25, and p of the token above 1 - 2^-24.  At low
+    temperatures the largest logit over T is large, and a rounding of it no longer small."""
+    n, vocab, g = 48, 20_011, gen(12)
+    x = Batch([3] * n, 32, dtype, form, seed=12, greedy=0.0)
+    x.temps = (torch.rand(n, generator=g) + 0.4) * cold
+    heat = x.temps.repeat_interleave(3)[:, None]
+    top = torch.randint(0, vocab, (3 * n,), generator=g)
+    at = torch.rand(3 * n, 1, generator=g) * 300 - 100  # where a row's largest value lies
+    low = math.log(rest / vocab) if rest else -95.0
+    fall = heat / cold * (low - 3 * torch.rand(3 * n, vocab, generator=g))
+    x.logits = (at.to(dtype) + fall).to(dtype)
+    x.logits.scatter_(1, top[:, None], at.to(dtype))
+    weights = ((x.logits.double() - at.to(dtype).double()) / heat).exp().sum(1) - 1
+    assert float(weights.max()) < (2.0 ** -26 if rest else 1e-30)
+    if form == "sampled":
+        x.draft = x.logits.clone()
+    row = torch.arange(3 * n).view(n, 3)
+    parents = torch.tensor([-1, 0, 1]) if form != "tree" else torch.tensor([-1, 0, 0])
+    x.tokens = torch.zeros(n, 3, dtype=torch.int64)
+    for i in (1, 2):
+        x.tokens[:, i] = top[row[:, int(parents[i])]]
+    x.tokens = x.tokens.view(-1)
+    x.mask = torch.tensor([1, 3, 5]).repeat(n) if form == "tree" else None
+    x.uniforms = torch.full((3 * n,), BELOW_ONE)
+    x.uniforms[::3] = torch.rand(n, generator=g)
+    want = oracle.verify_drafts(**x.args())[:3]
+    assert bool((want[0] == (1 if form == "tree" else 2)).all())
+    same(fused.verify_drafts(**x.on_gpu()), want)
+    many(x.on_gpu(), want)
