@@ -523,8 +523,8 @@ int kvp_token_logprobs(const void* logits, int32_t logits_fp32, int64_t row_stri
  *   - without (drafts that were chosen, in a chain or a tree), its siblings taken in order of their
  *     rows, where u (1 - p of the siblings refused before) < p(x); a token that a sibling had is refused.
  *     Behind refused ones the next token follows p without their tokens.
- * Where nothing is left to follow, it follows p.  Greedy otherwise (T <= 0 or NaN): a draft stays if it
- * is kvp_argmax_bf16's index of logits[r], and the next token is that index.
+ * Where 2^-46 of p or less is left to follow, it follows p.  Greedy otherwise (T <= 0 or NaN): a draft
+ * stays if it is kvp_argmax_bf16's index of logits[r], and the next token is that index.
  *   The next token is the least index whose running sum of weights exceeds row 0's uniform number times
  * their sum.  Sums are in 64 bits, and so are weights, but for some below 2^-28 of the row's largest, which
  * may be off by 2^-46 of that, and those below 2^-985 of it, which are 0.  What decides about drafts comes

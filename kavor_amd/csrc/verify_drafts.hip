@@ -50,6 +50,10 @@ constexpr float kHuge = 3.4028234e38f;
 // Weights relative to a row's largest: a single one below kTiny counts as 0.  Sums take them as 2^-1000 at least, so up to
 // 2^30 hidden values add up to less than kNothing, and one of the 2^12 of a range that has more is no less than kTiny.
 constexpr double kTiny = 0x1p-985, kNothing = 0x1p-969;
+// Of p's weights: if less is left behind refused drafts, it is nothing.  It is as much as a weight may be off by, and a sequence
+// gets to so little as rarely, but for decisions that 32-bit sums miss: what follows would be a token that p all but
+// excludes (two siblings with all of p, the second with the last number below 1: one time in ten).
+constexpr double kLeft = 0x1p-46;
 
 // What a sequence has left to draw.
 enum Mode : int32_t { kDone = 0, kAll = 1, kRest = 2, kWithout = 3, kUndefined = 4 };
@@ -878,7 +882,7 @@ __global__ __launch_bounds__(kThreads) void next_token_kernel(const VerifyParams
     const double lambda = rec.mode == kRest ? all.p / all.q : 0.0;
     int mode = rec.mode;
     double whole = all.p_over - lambda * all.q_over;
-    if (!(whole > kNothing)) {  // nothing is left: from p as it is
+    if (!(whole > kLeft * all.p)) {  // nothing is left: from p as it is
       mode = kAll;
       whole = all.p;
     }

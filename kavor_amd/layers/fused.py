@@ -338,11 +338,11 @@ def verify_drafts(logits: torch.Tensor, tokens: torch.Tensor, uniforms: torch.Te
         one the next token follows max(p - q, 0);
       - otherwise where u (1 - p of its siblings refused before) < p(x), and behind refused ones the
         next token follows p without them.
-    The next token is the least index whose running sum of weights, in 64 bits, exceeds row 0's number
-    times their sum.  A draft outside [0, vocab) (rows padded to one length) is refused and takes nothing from p.
-    Returns (accepted int32 [B], path int32 [B, max_seqlen_q]: the rows that stay,
-    out_tokens int64 [B, max_seqlen_q]: their tokens and the next one), -1 behind these.  A row of logits with a NaN or
-    +inf, or of -inf alone, keeps no draft and gives the greedy token (NaN counts as largest)."""
+    Where no more than 2^-46 of p is left, the next token follows p.  It is the least index whose running sum of
+    weights, in 64 bits, exceeds row 0's number times their sum.  A draft outside [0, vocab) (rows padded to one
+    length) is refused and takes nothing from p.  Returns (accepted int32 [B], path int32 [B, max_seqlen_q]: the
+    rows that stay, out_tokens int64 [B, max_seqlen_q]: their tokens and the next one), -1 behind these.  A row of
+    logits with a NaN or +inf, or of -inf alone, keeps no draft and gives the greedy token (NaN counts as largest)."""
     index, dtype = logits.get_device(), logits.dtype
     if index < 0 or (dtype is not torch.bfloat16 and dtype is not torch.float32) or logits.dim() != 2:
         raise ValueError(f"logits must be a bf16 or fp32 [T, vocab] GPU tensor (got {dtype} of shape "

@@ -89,7 +89,7 @@ def verify_drafts(logits, tokens, uniforms, temperatures, cu_seqlens_q, max_seql
         else:
             if draft_logits is not None and q is not None and 0 <= int(tokens[q0 + children[0]]) < vocab:
                 left = (p - q).clamp(min=0)
-            if not left.sum() > 0:
+            if not left.sum() > 2.0 ** -46:
                 left = p
             u = float(uniforms[q0])
             last = draw(left, u)

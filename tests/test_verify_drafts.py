@@ -605,3 +605,33 @@ def test_rows_that_are_sure_of_their_token(cuda_device, dtype, form, rest, cold)
     assert bool((want[0] == (1 if form == "tree" else 2)).all())
     same(fused.verify_drafts(**x.on_gpu()), want)
     many(x.on_gpu(), want)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+@pytest.mark.parametrize("few", [False, True])
+def test_where_siblings_have_all_of_p_nothing_else_is_drawn(cuda_device, dtype, few):
+    """Two siblings with all of p but 2^-100: the first is refused, the second has the last number below 1.  Its share of
+    what is left is 1, which sums in 32 bits may miss by 2^-24 and more: where it is refused the next token follows p, and
+    is one of the two."""
+    n, vocab, g = 2000, 1500, gen(13)
+    logits = -80.0 - 20.0 * torch.rand(n, vocab, generator=g)
+    pair = torch.stack([torch.randperm(vocab, generator=g)[:2] for _ in range(n)])
+    logits.scatter_(1, pair, torch.stack([torch.zeros(n), -2.0 * torch.rand(n, generator=g)], 1))
+    logits = torch.nn.functional.pad(logits, (0, -vocab % 8), value=math.nan).to(dtype).repeat_interleave(3, 0)
+    uniforms = torch.tensor([0.0, 0.95, BELOW_ONE]).repeat(n)
+    uniforms[::3] = torch.linspace(0, 1, n).clamp(max=BELOW_ONE)
+    tokens = torch.zeros(n, 3, dtype=torch.int64)
+    tokens[:, 1:] = pair
+    cu = torch.arange(0, 3 * n + 1, 3, dtype=torch.int32)
+    mask = torch.tensor([1, 3, 5]).repeat(n)
+    step = 20 if few else n  # sequences of a call: both ways to the sums
+    for b in range(0, 400 if few else n, step):
+        r = slice(3 * b, 3 * (b + step))
+        accepted, path, out = (t.cpu() for t in fused.verify_drafts(
+            logits[r].cuda()[:, :vocab], tokens.view(-1)[r].cuda(), uniforms[r].cuda(), torch.ones(step, device="cuda"),
+            cu[:step + 1].cuda(), 3, mask[r].cuda()))
+        first = out[:, :1]
+        assert bool((first == pair[b:b + step]).any(1).all()), (b, first[~(first == pair[b:b + step]).any(1)].view(-1).tolist())
+        kept = accepted == 1
+        assert bool((kept | (accepted == 0)).all()) and bool((path[kept, 0] == 2).all())
