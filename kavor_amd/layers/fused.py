@@ -305,6 +305,7 @@ def token_logprobs(logits: torch.Tensor, tokens: torch.Tensor, top: int = 0):
     return logprobs, entropy, rank, top_logprobs, top_tokens
 
 
+_INT_MAX = 2 ** 31 - 1  # sizes are passed as 32-bit integers
 _verify_pool = Workspaces("verify_drafts", "reserve_verify_workspace")
 
 
@@ -360,6 +361,8 @@ def verify_drafts(logits: torch.Tensor, tokens: torch.Tensor, uniforms: torch.Te
         raise ValueError("cu_seqlens_q must be a contiguous int32 tensor on the logits' device with an entry more "
                          "than sequences")
     batch, rows = cu_seqlens_q.numel() - 1, int(max_seqlen_q)
+    if n > _INT_MAX or vocab > _INT_MAX or not -_INT_MAX <= rows <= _INT_MAX:
+        raise ValueError(f"{n} rows of {vocab} values, max_seqlen_q {rows}: sizes must be below 2^31")
     if not (temperatures.dtype is torch.float32 and temperatures.get_device() == index and temperatures.is_contiguous()
             and temperatures.numel() >= batch):
         raise ValueError("temperatures must be a contiguous fp32 tensor on the logits' device, one per sequence")

@@ -635,3 +635,16 @@ def test_where_siblings_have_all_of_p_nothing_else_is_drawn(cuda_device, dtype, 
         assert bool((first == pair[b:b + step]).any(1).all()), (b, first[~(first == pair[b:b + step]).any(1)].view(-1).tolist())
         kept = accepted == 1
         assert bool((kept | (accepted == 0)).all()) and bool((path[kept, 0] == 2).all())
+
+
+@pytest.mark.gpu
+def test_sizes_that_pass_32_bits_are_refused(cuda_device):
+    """Not taken as what is left of them."""
+    good = Batch([3, 2], 64, torch.bfloat16, "chosen", seed=1).on_gpu()
+    with pytest.raises(ValueError, match="2\\^31"):
+        fused.verify_drafts(**{**good, "max_seqlen_q": (1 << 32) + 8})
+    row = torch.empty(1, (1 << 32) + 8, dtype=torch.bfloat16, device="cuda")
+    one = dict(logits=row, tokens=good["tokens"][:1], uniforms=good["uniforms"][:1], temperatures=good["temperatures"][:1],
+               cu_seqlens_q=torch.tensor([0, 1], dtype=torch.int32, device="cuda"), max_seqlen_q=1)
+    with pytest.raises(ValueError, match="2\\^31"):
+        fused.verify_drafts(**one)
