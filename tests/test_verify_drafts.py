@@ -648,3 +648,41 @@ def test_sizes_that_pass_32_bits_are_refused(cuda_device):
                cu_seqlens_q=torch.tensor([0, 1], dtype=torch.int32, device="cuda"), max_seqlen_q=1)
     with pytest.raises(ValueError, match="2\\^31"):
         fused.verify_drafts(**one)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype,form,lens,vocab,times,steps", [
+    (torch.bfloat16, "tree", [62] * 20, 4000, 45, 3),       # 446 MB: rows 0, 1 and 2 steps behind, the rest
+    (torch.bfloat16, "tree", [62] * 20, 4000, 87, 7),       # 863 MB: 3 to 6 steps behind as well
+    (torch.bfloat16, "chosen", [12] * 20, 4000, 450, 7),    # 864 MB
+    (torch.bfloat16, "sampled", [12] * 20, 4000, 230, 7),   # 442 MB and as much of the draft model's
+    (torch.float32, "sampled", [9] * 20, 4001, 160, 7),     # 461 MB and as much
+    (torch.bfloat16, "tree", [62, 61, 64, 60], 151_936, 6, 3),  # 450 MB in 24 sequences, whose ways the sums' kernel finds
+    (torch.float32, "tree", [64] * 8, 7, 7400, 1)])         # 106 MB of the shortest rows that get to several passes
+def test_batches_that_take_their_rows_in_several_passes(cuda_device, dtype, form, lens, vocab, times, steps):
+    """Limits of 200 MB (100 MB without a draft model's logits) for the last pass, each taking half of what was left."""
+    x = Batch(lens, vocab, dtype, form, seed=vocab + len(lens), greedy=0.2, width=9.0)
+    x.uniforms *= 0.2  # ways of some length
+    x.uniforms[x.cu[:-1].long()] *= 5.0
+    rng = random.Random(vocab)
+    for q0, n in zip(x.cu.tolist(), lens):
+        for i in range(1, n):
+            up = q0 + (i - 1 if x.mask is None else (int(x.mask[q0 + i]) & (1 << i) - 1).bit_length() - 1)
+            if form != "sampled" and rng.random() < 0.85:  # most drafts are the best behind their rows, but for later siblings
+                x.logits[up, x.tokens[q0 + i]] = x.logits[up].max() + 4.0
+    want = x.want()
+    rows, width = len(x.tokens), -(-vocab // 8) * 8
+    passes = 1 + sum(rows * times * vocab * x.logits.element_size() * (2 if form == "sampled" else 1) >= at << 20
+                     for at in ((200, 400, 800) if form == "sampled" else (100, 400, 800)))
+    assert passes >= {1: 2, 3: 3, 7: 4}[steps] and bool((want[0] >= steps).any()), (passes, want[0])
+    a = x.on_gpu()
+    for name in ("logits", "draft_logits"):
+        if a[name] is not None:
+            room = torch.full((rows * times, width), math.nan, dtype=dtype, device="cuda")
+            room[:, :vocab] = a[name].repeat(times, 1)
+            a[name] = room[:, :vocab]
+    for name in ("tokens", "uniforms", "temperatures", "tree_mask"):
+        a[name] = a[name].repeat(times) if a[name] is not None else None
+    cu, steps_of = a["cu_seqlens_q"], torch.arange(times, device="cuda", dtype=torch.int32)[:, None] * rows
+    a["cu_seqlens_q"] = torch.cat(((cu[:-1] + steps_of).view(-1), cu[-1:] + steps_of[-1]))
+    same(fused.verify_drafts(**a), [w.repeat(times, *[1] * (w.dim() - 1)) for w in want])
