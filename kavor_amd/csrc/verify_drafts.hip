@@ -242,11 +242,6 @@ template <int LANES = 64>
 __device__ __forceinline__ u64 best_of(u64 x) {
   return combine<LANES>(x, [](u64 a, u64 b) { return a > b ? a : b; });
 }
-__device__ __forceinline__ double shfl_f64(double x, int from) {
-  const u64 v = static_cast<u64>(__double_as_longlong(x));
-  return __longlong_as_double(static_cast<long long>(static_cast<u64>(__shfl(static_cast<u32>(v >> 32), from)) << 32 |
-                                                     __shfl(static_cast<u32>(v), from)));
-}
 // x moved CTRL (row_shr) lanes up in each row of 16, 0 where there is none.
 template <int CTRL>
 __device__ __forceinline__ double shifted(double x) {
