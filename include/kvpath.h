@@ -527,8 +527,10 @@ int kvp_token_logprobs(const void* logits, int32_t logits_fp32, int64_t row_stri
  * stays if it is kvp_argmax_bf16's index of logits[r], and the next token is that index.
  *   The next token is the least index whose running sum of weights exceeds row 0's uniform number times
  * their sum.  Sums are in 64 bits, and so are weights, but for some below 2^-28 of the row's largest, which
- * may be off by 2^-46 of that, and those below 2^-985 of it, which are 0.  What decides about drafts comes
- * from sums in 32 bits; a chosen draft that has all of p but 2^-25 stays whatever its number.
+ * may be off by 2^-46 of that, and those below 2^-985 of it, which are 0.  What decides about drafts, and
+ * whether a value's p counts as above its q, comes from sums in 32 bits (a p and a q that are nearer to each
+ * other than these are off count with their difference of either sign, or not at all); a draft that has
+ * all of p but 2^-25 stays whatever its number.
  * accepted[b]: the number of drafts that stay; path[b, 0 .. accepted): their rows in the sequence,
  * rising; out_tokens[b, 0 .. accepted): their tokens, and the next token behind them; the rest of
  * both [num_seqs, max_seqlen_q] is -1.  Results that share memory with logits, draft_logits, tokens,
@@ -536,9 +538,9 @@ int kvp_token_logprobs(const void* logits, int32_t logits_fp32, int64_t row_stri
  *   A row of logits with a NaN or +inf, or of -inf alone, keeps no draft at T > 0, and its next token is
  * the greedy one; such a row of draft_logits keeps none either, and the next token follows p.  A draft
  * outside [0, vocab), a filler of rows of one length, is refused and takes nothing from p: it was not
- * sampled from q, so the next token follows p with draft_logits too.  Rows of draft_logits without a draft behind them are not read.  A
- * sequence without rows, with more than max_seqlen_q, or with rows outside [0, total_q) has
- * accepted 0 and -1 alone.
+ * sampled from q, so the next token follows p with draft_logits too.  Rows of draft_logits without a
+ * draft behind them are not read.  A sequence without rows, with more than max_seqlen_q, or with rows
+ * outside [0, total_q) has accepted 0 and -1 alone.
  *   logits and draft_logits in bf16 (logits_fp32 0) or fp32 (1), 16-byte aligned, row strides
  * (elements) multiples of 16 bytes.  The workspace is 16-byte aligned and needs no initialisation;
  * its size falls with no argument that grows.

@@ -70,7 +70,9 @@ struct Record {   // of a sequence
 };
 
 struct Sums {  // of a range, relative to the maxima: of p's and q's weights, and of those where p's is larger
-  double p, q, p_over, q_over;  // kWithout: p_over is p's without the refused tokens
+  // Larger by the ratio of 32-bit sums: of values that are closer to each other than it is off, p_over and q_over give the
+  // difference with either sign, or nothing.  kWithout: p_over is p's without the refused tokens.
+  double p, q, p_over, q_over;
 };
 
 struct VerifyParams {
@@ -726,9 +728,12 @@ __device__ __forceinline__ double only(bool on, double x) {
 // A range per wave.  KNOWN: last_row_kernel left the records; otherwise every wave goes the way anew.
 //
 // Where 64 chunks have no weight of 2^-28 of the largest or more, as most have in a row that is sure of its token, weights
-// are taken in 32 bits: of 2^t the exponent is off by 2^-24 of itself, twice, and the exponential by 2^-23, so a weight by
-// less than (1.4 |t| + 2) 2^-24 of itself, which for t <= -28 is 2^-46 of the largest and less.  The signs differ: a row of
-// 151936 is off by some 1e-12 of its sum, 2e-9 at worst.  256 chains with a draft model's logits: 38 us, 63 without.
+// are taken in 32 bits and a chunk's 4 or 8 added there, before they go to the 64-bit sums.  The exponent t of 2^t is rounded
+// three times, as a difference, in the scale and as their product, each time by 2^-24 of itself over its mantissa.  At -28,
+// where the product's is 1.75, that is 2.2 * 2^-24 of t at most (1 + 1/1.75 + 1/1.75), or 42 * 2^-24 of the weight; with 2 for
+// the exponential and 7 for the additions 51 * 2^-24, less than 2^-46 of the largest weight, and the less the smaller t.
+// The signs differ: a row of 151936 is off by some 1e-12 of its sum, 2e-9 at worst.  256 chains with a draft model's logits:
+// 38 us, 63 without.
 template <typename T, bool KNOWN>
 __global__ __launch_bounds__(kSumThreads) void range_sums_kernel(const VerifyParams p) {
   constexpr int E = Chunk<T>::kSize;
