@@ -2,9 +2,10 @@
 // follows the last one kept (kvp_verify_drafts).
 //
 // With p = softmax(z / T) of a row of logits and q the draft's distribution, a draft x that was sampled from
-// q is kept where u q(x) < p(x); behind a refused one the next token follows max(p - q, 0), behind a filler that is no
-// token p.  A draft that was chosen (no q) is kept where u (1 - what its refused siblings have of p) < p(x); behind refused ones the next
-// token follows p without them.  Either way a token of the output is distributed as p.
+// q is kept where u q(x) < p(x); behind a refused one the next token follows max(p - q, 0), and p behind a filler, which
+// is no token and was not sampled.  A draft that was chosen (no q) is kept where u (1 - what its refused siblings have of
+// p) < p(x); behind refused ones the next token follows p without them.  Either way a token of the output is
+// distributed as p.
 //
 // In a few launches:
 //   - maximum and sum of the rows of logits, in 32 bits, a segment of a row per workgroup.  Rows behind a refused draft
